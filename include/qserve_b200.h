@@ -125,6 +125,43 @@ QS_API int qs_prefill_attention(const void* q, const void* k, const void* v, int
                          int64_t out_stride, const int32_t* cu_seqlens, int batch, int num_tokens, int max_seqlen, int num_heads,
                          int num_kv_heads, int head_dim, float softmax_scale, void* stream);
 
+/* Portions of sequences in the paged cache (csrc/paged_cache.cu, csrc/paged_attention.cu; extensions, the reference appends whole prompts only and
+ * attends over keys of the same call).  A flat batch of num_tokens rows holds the LAST cu_seqlens[b + 1] - cu_seqlens[b] positions of sequence b, whose
+ * pages (kv_pointers int64 [batch, 2, max_blocks], K and V, each 16-byte aligned) hold lengths[b] positions with them: row t of it has position
+ * lengths[b] - (cu_seqlens[b + 1] - t).  cu_seqlens int32 [batch + 1], ascending; NULL: one row per sequence.  Rows behind the last sequence are
+ * neither read nor written; positions outside a sequence's max_blocks pages are never touched.  head_dim 128, tokens_per_block 64,
+ * kv_cache_with_zeros 1, size_per_token = num_kv_heads * 128 * bits / 8; row strides in halfs, multiples of 8, heads contiguous; 16-byte aligned.
+ * Unlike the operators above, these read all of their tables behind the wait for the kernel before them. */
+/* q_out <- q rotated, pages <- quantised rotated k and v (q, k, v are not written; q_out may be q).  NeoX rotation in place position, angle
+ * position * rotary_base^(-2i/128), sine and cosine correct to fp32 at any position.  Codes, scale and zero per (token, kv head) as
+ * qs_apply_bias_rope_update_kv_cache stores them, except that a code is never more than 15 (INT4), that a row whose values are equal, or too near
+ * to one another for a zero in fp16, is held as its middle value, and that a row with an infinity or NaN reads as NaN. */
+QS_API int qs_append_kv_cache(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out,
+                              int64_t q_out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch,
+                              int num_tokens, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block,
+                              int size_per_token, int rotary_embedding_dim, float rotary_base, int int4_kv_cache, int kv_cache_with_zeros, void* stream);
+/* k_out, v_out fp16 [num_tokens, num_kv_heads, 128] <- what the pages stand for: half(s u + half(-s z)) (INT4), half(s (u - z)) (INT8) */
+QS_API int qs_read_kv_cache(void* k_out, void* v_out, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch,
+                            int num_tokens, int max_blocks_per_seq, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token,
+                            int int4_kv_cache, int kv_cache_with_zeros, void* stream);
+/* out [T, num_heads, 128]: causal attention of every row over positions 0 .. its own of its sequence, all out of the pages (also the portion's own:
+ * append first).  q rotated; softmax_scale > 0.  max_seqlen >= the longest portion (rows behind it are left as they are), max_length >= the
+ * longest sequence (decides how the keys are split, nothing else).  A row without a position (lengths[b] smaller than the portion) gets zeros.
+ * workspace: qs_paged_prompt_attention_workspace_bytes(...) of the same numbers, any contents, not shared by calls that run at the same time. */
+QS_API size_t qs_paged_prompt_attention_workspace_bytes(int batch, int num_tokens, int max_seqlen, int max_length, int num_heads, int num_kv_heads);
+QS_API int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
+                                     const int32_t* lengths, int batch, int num_tokens, int max_seqlen, int max_length, int max_blocks_per_seq,
+                                     int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache,
+                                     int kv_cache_with_zeros, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+/* out [batch, num_heads, 128]: attention of one row per sequence over its lengths[b] positions, all out of the pages, where the first shared_blocks
+ * pages of all sequences are the same ones (they are taken from kv_pointers[0]): their keys are read and unpacked once for all rows.  A
+ * sequence may be shorter than the shared pages; lengths[b] 0 gets zeros.  workspace: qs_shared_prefix_attention_workspace_bytes(...). */
+QS_API size_t qs_shared_prefix_attention_workspace_bytes(int batch, int shared_blocks, int num_heads, int num_kv_heads);
+QS_API int qs_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* lengths,
+                                      int batch, int shared_blocks, int max_length, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim,
+                                      int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros, float softmax_scale,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
 /* qserve_backend.fused_attention.compute_padding_offsets         kernels/csrc/fused_attention/input_metadata_helper.cu:33-45 */
 QS_API int qs_compute_padding_offsets(int32_t* padding_offsets, const int32_t* cu_seqlens, int batch, int max_seqlen, void* stream);
 

@@ -32,6 +32,13 @@ SIGNATURES = {
     "qs_apply_bias_rope_update_kv_cache": (c_int, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _I, _I, _P]),
     "qs_compute_padding_offsets": (c_int, [_P, _P, _I, _I, _P]),
     "qs_prefill_attention": (c_int, [_P, _P, _P, _L, _L, _L, _P, _L, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    # portions of sequences in the paged cache (csrc/paged_cache.cu, csrc/paged_attention.cu)
+    "qs_append_kv_cache": (c_int, [_P, _P, _P, _L, _L, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
+    "qs_read_kv_cache": (c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "qs_paged_prompt_attention_workspace_bytes": (c_size_t, [_I, _I, _I, _I, _I, _I]),
+    "qs_paged_prompt_attention": (c_int, [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
+    "qs_shared_prefix_attention_workspace_bytes": (c_size_t, [_I, _I, _I, _I]),
+    "qs_shared_prefix_attention": (c_int, [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
     "qs_rms_norm": (c_int, [_P, _P, _P, _F, _I, _I, _I, _P]),
     "qs_rms_norm_general": (c_int, [_P, _P, _P, _P, _F, _I, _I, _I, _P]),
     "qs_rms_norm_general_fuse_sum": (c_int, [_P, _P, _P, _P, _P, _F, _I, _I, _I, _P]),

@@ -337,6 +337,51 @@ def single_query_attention_quant(q, k, v, kv_pointers, length_per_sample, memory
                                        rotary_embedding_dim, rotary_base, int4_kv_cache, kv_cache_with_zeros, out_q, out_scale, out_sum)
 
 
+# --------------------------------------------------------------------------------------------------
+# portions of sequences in the paged cache (extensions: the reference appends whole prompts only, and attends over keys of the same call)
+#
+# A flat batch of rows holds the last cu_seqlens[b + 1] - cu_seqlens[b] positions of sequence b (cu_seqlens int32 [B + 1]; None: one row per sequence);
+# lengths int32 [B] counts what the sequence's pages hold with them, kv_pointers int64 [B, 2, blocks] as for single_query_attention, pages 16-byte aligned.
+# Heads are 128 wide and contiguous, rows start on 16-byte boundaries.  Rows behind the last sequence (a padded batch) are neither read nor written:
+# those of a given `out` stay as they are, those of a new result are unset.
+# --------------------------------------------------------------------------------------------------
+
+
+def append_kv_cache(q, k, v, kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, tokens_per_block: int, size_per_token: int, rotary_embedding_dim: int,
+                    rotary_base: float, int4_kv_cache: bool, kv_cache_with_zeros: bool, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """RoPE of q [T,Hq,128] and k [T,Hkv,128] at the rows' positions, per-token-per-head quantisation of k and v into the pages: what
+    apply_bias_rope_update_kv_cache does for whole prompts, for portions that continue sequences (single tokens among them).  Returns the rotated q (`out`
+    may be q itself); q, k and v are not changed.  A row of equal values is held as that value; one with an infinity or NaN reads as NaN."""
+    return _bind.append_kv_cache(q, k, v, kv_pointers, cu_seqlens, lengths, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4_kv_cache,
+                                 kv_cache_with_zeros, out)
+
+
+def read_kv_cache(kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, num_tokens: int, tokens_per_block: int, size_per_token: int, int4_kv_cache: bool,
+                  kv_cache_with_zeros: bool):
+    """What the pages stand for at the last positions of the sequences: two new tensors k, v fp16 [num_tokens,Hkv,128] (num_tokens >= cu_seqlens[-1]).
+    A whole sequence is read with cu_seqlens over its length."""
+    return _bind.read_kv_cache(kv_pointers, cu_seqlens, lengths, num_tokens, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros)
+
+
+def paged_prompt_attention(q, kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, max_seqlen: int, max_length: int, tokens_per_block: int,
+                           size_per_token: int, int4_kv_cache: bool, kv_cache_with_zeros: bool, softmax_scale: Optional[float] = None,
+                           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of the rotated q [T,Hq,128] of portions over positions 0 .. its own of each row's sequence, keys and values out of the pages (those of the
+    portion too: append_kv_cache first).  max_seqlen >= the longest portion, max_length >= the longest sequence.  Returns fp16 [T,Hq,128]; a row without a position
+    (lengths[b] smaller than the portion) gets zeros.  softmax_scale > 0, default 128 ** -0.5."""
+    return _bind.paged_prompt_attention(q, kv_pointers, cu_seqlens, lengths, max_seqlen, max_length, tokens_per_block, size_per_token, int4_kv_cache,
+                                        kv_cache_with_zeros, softmax_scale, out)
+
+
+def shared_prefix_attention(q, kv_pointers, lengths, shared_blocks: int, max_length: int, tokens_per_block: int, size_per_token: int, int4_kv_cache: bool,
+                            kv_cache_with_zeros: bool, softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one rotated row per sequence, q [B,Hq,128], over its lengths[b] positions, all out of the pages (the new token's too: append_kv_cache first),
+    where the first `shared_blocks` pages of all sequences are the same pages (they are taken from kv_pointers[0]): those are read and unpacked once for the
+    whole batch.  A sequence may end within the shared pages; lengths[b] = 0 gets zeros.  max_length >= the longest sequence."""
+    return _bind.shared_prefix_attention(q, kv_pointers, lengths, shared_blocks, max_length, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros,
+                                         softmax_scale, out)
+
+
 class PeerContext:
     """Peer-mapped buffers of a tensor-parallel group for the fused all-reduce (qs_add_rms_norm_general_peer): built once from
     torch.distributed._symmetric_memory (device memory + NVLink peer mappings are torch's plumbing; the kernel is ours).

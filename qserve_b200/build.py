@@ -17,9 +17,9 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libqserve_b200.so")
 BIND = os.path.join(HERE, "_bind.so")  # CPython binding of the hot operators (bind.cpp): the one part that is built against torch
-SOURCES = ["capi.cu", "gemm.cu", "attention.cu", "prefill_attention.cu", "elementwise.cu", "hybrid.cu", "hybrid_blocks.cu", "hybrid_linear.cu", "hybrid_latent.cu",
+SOURCES = ["capi.cu", "gemm.cu", "attention.cu", "prefill_attention.cu", "paged_cache.cu", "paged_attention.cu", "elementwise.cu", "hybrid.cu", "hybrid_blocks.cu", "hybrid_linear.cu", "hybrid_latent.cu",
            "hybrid_recurrent.cu", "hybrid_scan.cu", "hybrid_tile.cu"]
-HEADERS = ["common.cuh", "hybrid_common.cuh", "hybrid_conv.cuh", "launch.h", os.path.join("..", "..", "include", "qserve_b200.h")]
+HEADERS = ["common.cuh", "hybrid_common.cuh", "hybrid_conv.cuh", "launch.h", "paged_common.cuh", os.path.join("..", "..", "include", "qserve_b200.h")]
 
 NVCC_FLAGS = [
     "-std=c++17", "-O3", "-lineinfo",

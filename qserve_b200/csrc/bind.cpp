@@ -245,6 +245,139 @@ PyObject* single_query_attention_quant(const Args& a) {  // the 16 arguments of 
   return none();
 }
 
+// ---- portions of sequences in the paged cache ----
+// what the operators share: tables of a batch, page geometry, rows of heads
+struct Cache {
+  const int64_t* kvp;
+  const int32_t *cu, *lens;
+  int batch, max_blocks, heads_kv, size, tpb, int4, zeros;
+};
+void same_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  require_cuda(t, name);
+  if (t.get_device() != like.get_device()) throw std::runtime_error(std::string(name) + " must be on the device of the other tensors");
+}
+const int32_t* int32_vector(const at::Tensor& t, int64_t n, const at::Tensor& like, const char* name) {
+  same_device(t, like, name);
+  if (t.scalar_type() != at::kInt || t.dim() != 1 || t.size(0) != n || !t.is_contiguous()) throw std::runtime_error(std::string(name) + " must be contiguous int32 [" + std::to_string(n) + "]");
+  return static_cast<const int32_t*>(t.data_ptr());
+}
+// arguments kvp, cu (-1: there is none), lens, and from `at` on tokens_per_block, size_per_token; then int4 and zeros at `flags`
+Cache cache_of(const Args& a, const at::Tensor& like, int kvp, int cu, int lens, int at, int flags) {
+  const at::Tensor& t = a.tensor(kvp);
+  same_device(t, like, "kv_pointers");
+  require(t.scalar_type() == at::kLong && t.is_contiguous() && t.dim() == 3 && t.size(1) == 2, "kv_pointers must be contiguous int64 [batch, 2, blocks]");
+  require(t.size(0) <= 0x3fffffff && t.size(2) <= 0x3fffffff, "kv_pointers: too many sequences or blocks");
+  Cache c;
+  c.kvp = static_cast<const int64_t*>(t.data_ptr());
+  c.batch = static_cast<int>(t.size(0));
+  c.max_blocks = static_cast<int>(t.size(2));
+  c.cu = cu < 0 || a.none(cu) ? nullptr : int32_vector(a.tensor(cu), t.size(0) + 1, like, "cu_seqlens");
+  c.lens = int32_vector(a.tensor(lens), t.size(0), like, "lengths");
+  c.tpb = a.small(at);
+  c.size = a.small(at + 1);
+  c.int4 = a.truth(flags);
+  c.zeros = a.truth(flags + 1);
+  c.heads_kv = static_cast<int>(static_cast<int64_t>(c.size) * 8 / (128 * (c.int4 ? 4 : 8)));
+  return c;
+}
+struct Heads {
+  void* p;
+  int64_t stride;
+  int rows, heads;
+};
+Heads heads_of(const at::Tensor& t, const at::Tensor& like, const char* name) {
+  same_device(t, like, name);
+  const std::string n(name);
+  if (t.scalar_type() != at::kHalf || t.dim() != 3 || t.size(2) != 128) throw std::runtime_error(n + " must be float16 [tokens, heads, 128]");
+  if (t.size(0) > 0 && (t.stride(2) != 1 || (t.size(1) > 1 && t.stride(1) != 128))) throw std::runtime_error(n + ": heads must be contiguous rows of 128 halfs");
+  if (t.size(0) > 0x7fffffff || t.size(1) > 0xffff) throw std::runtime_error(n + ": too many rows or heads");
+  // (a single row has no stride to speak of)
+  return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : t.size(1) * 128, static_cast<int>(t.size(0)), static_cast<int>(t.size(1))};
+}
+// the result's tensor: argument i, or a new one of q's sizes where it is None
+at::Tensor result_of(const Args& a, int i, const at::Tensor& q) {
+  if (a.none(i)) return at::empty({q.size(0), q.size(1), q.size(2)}, q.options().requires_grad(false));
+  const at::Tensor& t = a.tensor(i);
+  require(t.dim() == 3 && t.size(0) == q.size(0) && t.size(1) == q.size(1) && t.size(2) == q.size(2), "out must have the sizes of q");
+  return t;
+}
+// A work space of the call's own: calls on several streams and captured graphs never share one
+at::Tensor scratch(const at::Tensor& q, size_t bytes) { return at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).requires_grad(false)); }
+float scale_of(const Args& a, int i) { return a.none(i) ? 0.08838834764831845f : a.real(i); }
+
+// q, k, v, kv_pointers, cu_seqlens or None, lengths, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4, zeros, out or None
+PyObject* append_kv_cache(const Args& a) {
+  const at::Tensor &qt = a.tensor(0), &kt = a.tensor(1), &vt = a.tensor(2);
+  const Heads q = heads_of(qt, qt, "q"), k = heads_of(kt, qt, "k"), v = heads_of(vt, qt, "v");
+  require(q.rows == k.rows && q.rows == v.rows && k.heads == v.heads, "q, k, v must cover the same tokens; k and v the same heads");
+  const Cache c = cache_of(a, qt, 3, 4, 5, 6, 10);
+  at::Tensor out = result_of(a, 12, qt);
+  const Heads o = heads_of(out, qt, "out");
+  const int rot = a.small(8);
+  const float base = a.real(9);
+  launch(qt, [&](void* s) {
+    return qs_append_kv_cache(q.p, k.p, v.p, q.stride, k.stride, v.stride, o.p, o.stride, c.kvp, c.cu, c.lens, c.batch, q.rows, c.max_blocks, q.heads, k.heads, 128,
+                              c.tpb, c.size, rot, base, c.int4, c.zeros, s);
+  });
+  return THPVariable_Wrap(std::move(out));
+}
+// kv_pointers, cu_seqlens or None, lengths, num_tokens, tokens_per_block, size_per_token, int4, zeros
+PyObject* read_kv_cache(const Args& a) {
+  const at::Tensor& t = a.tensor(0);
+  const Cache c = cache_of(a, t, 0, 1, 2, 4, 6);
+  const int tokens = a.small(3);
+  require(tokens >= 0, "num_tokens must not be negative");
+  const at::TensorOptions options = t.options().dtype(at::kHalf).requires_grad(false);
+  at::Tensor k = at::empty({tokens, c.heads_kv, 128}, options), v = at::empty({tokens, c.heads_kv, 128}, options);
+  void *kp = k.data_ptr(), *vp = v.data_ptr();
+  launch(t, [&](void* s) { return qs_read_kv_cache(kp, vp, c.kvp, c.cu, c.lens, c.batch, tokens, c.max_blocks, c.heads_kv, 128, c.tpb, c.size, c.int4, c.zeros, s); });
+  PyObject* const ko = THPVariable_Wrap(std::move(k));
+  PyObject* const vo = THPVariable_Wrap(std::move(v));
+  PyObject* const both = ko && vo ? PyTuple_Pack(2, ko, vo) : nullptr;
+  Py_XDECREF(ko);
+  Py_XDECREF(vo);
+  return both;
+}
+// q, kv_pointers, cu_seqlens or None, lengths, max_seqlen, max_length, tokens_per_block, size_per_token, int4, zeros, softmax_scale or None, out or None
+PyObject* paged_prompt_attention(const Args& a) {
+  const at::Tensor& qt = a.tensor(0);
+  const Heads q = heads_of(qt, qt, "q");
+  const Cache c = cache_of(a, qt, 1, 2, 3, 6, 8);
+  at::Tensor out = result_of(a, 11, qt);
+  const Heads o = heads_of(out, qt, "out");
+  const int max_seqlen = a.small(4), max_length = a.small(5);
+  const float scale = scale_of(a, 10);
+  const size_t need = qs_paged_prompt_attention_workspace_bytes(c.batch, q.rows, max_seqlen < q.rows ? max_seqlen : q.rows, max_length, q.heads, c.heads_kv);
+  at::Tensor ws;
+  if (need > 0) ws = scratch(qt, need);
+  void* const wp = need > 0 ? ws.data_ptr() : nullptr;
+  launch(qt, [&](void* s) {
+    return qs_paged_prompt_attention(q.p, q.stride, o.p, o.stride, c.kvp, c.cu, c.lens, c.batch, q.rows, max_seqlen, max_length, c.max_blocks, q.heads, c.heads_kv, 128,
+                                     c.tpb, c.size, c.int4, c.zeros, scale, wp, need, s);
+  });
+  return THPVariable_Wrap(std::move(out));
+}
+// q, kv_pointers, lengths, shared_blocks, max_length, tokens_per_block, size_per_token, int4, zeros, softmax_scale or None, out or None
+PyObject* shared_prefix_attention(const Args& a) {
+  const at::Tensor& qt = a.tensor(0);
+  const Heads q = heads_of(qt, qt, "q");
+  const Cache c = cache_of(a, qt, 1, -1, 2, 5, 7);
+  require(q.rows == c.batch, "q must have one row per sequence");
+  at::Tensor out = result_of(a, 10, qt);
+  const Heads o = heads_of(out, qt, "out");
+  const int shared = a.small(3), max_length = a.small(4);
+  const float scale = scale_of(a, 9);
+  const size_t need = qs_shared_prefix_attention_workspace_bytes(c.batch, shared, q.heads, c.heads_kv);
+  at::Tensor ws;
+  if (need > 0) ws = scratch(qt, need);
+  void* const wp = need > 0 ? ws.data_ptr() : nullptr;
+  launch(qt, [&](void* s) {
+    return qs_shared_prefix_attention(q.p, q.stride, o.p, o.stride, c.kvp, c.lens, c.batch, shared, max_length, c.max_blocks, q.heads, c.heads_kv, 128, c.tpb, c.size,
+                                      c.int4, c.zeros, scale, wp, need, s);
+  });
+  return THPVariable_Wrap(std::move(out));
+}
+
 // ---- row operators ----
 struct Rows {
   int tokens, width;
@@ -408,6 +541,10 @@ PyMethodDef methods[] = {QS_ENTRY(w4a8_per_chn, 8),
                          QS_ENTRY(w8a8, 6),
                          QS_ENTRY(single_query_attention, 15),
                          QS_ENTRY(single_query_attention_quant, 16),
+                         QS_ENTRY(append_kv_cache, 13),
+                         QS_ENTRY(read_kv_cache, 8),
+                         QS_ENTRY(paged_prompt_attention, 12),
+                         QS_ENTRY(shared_prefix_attention, 11),
                          QS_ENTRY(rms_norm_general, 6),
                          QS_ENTRY(rms_norm_general_fuse_sum, 7),
                          QS_ENTRY(invoke_quant, 3),

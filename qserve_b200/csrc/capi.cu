@@ -169,6 +169,116 @@ int qs_apply_bias_rope_update_kv_cache(void* qkv, const int32_t* seq_lens, const
   return prefill_rope_append(a);
 }
 
+// what every operator over portions in the paged cache asks of its arguments
+static int paged_cache(PagedCache& c, const char* op, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens,
+                       int max_blocks, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4, int zeros) {
+  QS_REQUIRE(batch >= 0 && num_tokens >= 0 && max_blocks >= 0, "%s: negative size", op);
+  QS_REQUIRE(head_dim == 128, "%s: head_dim=%d, only 128 is supported", op, head_dim);
+  QS_REQUIRE(zeros, "%s: only kv_cache_with_zeros=True is supported", op);
+  QS_REQUIRE(tokens_per_block == 64, "%s: tokens_per_block=%d, only 64 is supported", op, tokens_per_block);
+  QS_REQUIRE(num_kv_heads > 0 && size_per_token == static_cast<long long>(num_kv_heads) * 128 * (int4 ? 4 : 8) / 8,
+             "%s: size_per_token=%d does not match %d kv heads x %d bits", op, size_per_token, num_kv_heads, int4 ? 4 : 8);
+  QS_REQUIRE(max_blocks <= (1 << 24), "%s: %d pages per sequence", op, max_blocks);
+  if (batch > 0 && num_tokens > 0) QS_REQUIRE(kv_pointers && lengths, "%s: null tensor", op);
+  c.kv_pointers = reinterpret_cast<const long long*>(kv_pointers);
+  c.cu_seqlens = cu_seqlens;
+  c.lengths = lengths;
+  c.max_blocks = max_blocks;
+  c.num_kv_heads = num_kv_heads;
+  c.int4 = int4 != 0;
+  return qs::QS_OK;
+}
+static int paged_rows(const char* op, const char* name, const void* t, int64_t stride, int heads) {
+  QS_REQUIRE(t != nullptr, "%s: %s is null", op, name);
+  QS_REQUIRE(aligned16(t) && stride % 8 == 0, "%s: rows of %s must start on 16-byte boundaries", op, name);
+  QS_REQUIRE(stride >= static_cast<int64_t>(heads) * 128, "%s: row stride of %s smaller than the row", op, name);
+  return qs::QS_OK;
+}
+
+int qs_append_kv_cache(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out, int64_t q_out_stride,
+                       const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens, int max_blocks_per_seq,
+                       int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int rotary_embedding_dim, float rotary_base,
+                       int int4_kv_cache, int kv_cache_with_zeros, void* stream) {
+  const char* op = "append_kv_cache";
+  AppendArgs a;
+  int rc = paged_cache(a.cache, op, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
+                       int4_kv_cache, kv_cache_with_zeros);
+  if (rc) return rc;
+  QS_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0, "%s: heads %d / kv heads %d", op, num_heads, num_kv_heads);
+  QS_REQUIRE(rotary_embedding_dim == head_dim, "%s: rotary_embedding_dim=%d must equal head_dim", op, rotary_embedding_dim);
+  QS_REQUIRE(rotary_base > 0.f && rotary_base < 3.0e38f, "%s: rotary_base must be positive and finite", op);
+  if (batch == 0 || num_tokens == 0) return qs::QS_OK;
+  if ((rc = paged_rows(op, "q", q, q_stride, num_heads)) || (rc = paged_rows(op, "k", k, k_stride, num_kv_heads)) ||
+      (rc = paged_rows(op, "v", v, v_stride, num_kv_heads)) || (rc = paged_rows(op, "out", q_out, q_out_stride, num_heads)))
+    return rc;
+  a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.q_out_stride = q_out_stride;
+  a.batch = batch; a.num_tokens = num_tokens; a.num_heads = num_heads; a.rotary_base = rotary_base; a.stream = stream;
+  return append_kv_cache(a);
+}
+
+int qs_read_kv_cache(void* k_out, void* v_out, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens,
+                     int max_blocks_per_seq, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros,
+                     void* stream) {
+  const char* op = "read_kv_cache";
+  PagedCache c;
+  int rc = paged_cache(c, op, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
+                       int4_kv_cache, kv_cache_with_zeros);
+  if (rc || batch == 0 || num_tokens == 0) return rc;
+  if ((rc = paged_rows(op, "k", k_out, num_kv_heads * 128, num_kv_heads)) || (rc = paged_rows(op, "v", v_out, num_kv_heads * 128, num_kv_heads))) return rc;
+  return read_kv_cache(k_out, v_out, c, batch, num_tokens, stream);
+}
+
+size_t qs_paged_prompt_attention_workspace_bytes(int batch, int num_tokens, int max_seqlen, int max_length, int num_heads, int num_kv_heads) {
+  return paged_prompt_workspace(batch, num_tokens, max_seqlen, max_length, num_heads, num_kv_heads);
+}
+
+int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
+                              const int32_t* lengths, int batch, int num_tokens, int max_seqlen, int max_length, int max_blocks_per_seq, int num_heads,
+                              int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros,
+                              float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "paged_prompt_attention";
+  PagedAttnArgs a;
+  int rc = paged_cache(a.cache, op, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
+                       int4_kv_cache, kv_cache_with_zeros);
+  if (rc) return rc;
+  QS_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0, "%s: heads %d / kv heads %d", op, num_heads, num_kv_heads);
+  QS_REQUIRE(max_seqlen >= 0 && max_length >= 0, "%s: negative size", op);
+  QS_REQUIRE(softmax_scale > 0.f && softmax_scale < 3.0e38f, "%s: softmax_scale must be positive and finite", op);
+  if (batch == 0 || num_tokens == 0 || max_seqlen == 0) return qs::QS_OK;
+  if ((rc = paged_rows(op, "q", q, q_stride, num_heads)) || (rc = paged_rows(op, "out", out, out_stride, num_heads))) return rc;
+  QS_REQUIRE(aligned16(workspace), "%s: workspace must be 16-byte aligned", op);
+  a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.batch = batch; a.num_tokens = num_tokens; a.num_heads = num_heads;
+  a.max_seqlen = max_seqlen < num_tokens ? max_seqlen : num_tokens; a.max_length = max_length; a.softmax_scale = softmax_scale;
+  a.workspace = workspace; a.workspace_bytes = workspace_bytes; a.stream = stream;
+  return paged_prompt_attention(a);
+}
+
+size_t qs_shared_prefix_attention_workspace_bytes(int batch, int shared_blocks, int num_heads, int num_kv_heads) {
+  return shared_prefix_workspace(batch, shared_blocks, num_heads, num_kv_heads);
+}
+
+int qs_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* lengths, int batch,
+                               int shared_blocks, int max_length, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block,
+                               int size_per_token, int int4_kv_cache, int kv_cache_with_zeros, float softmax_scale, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+  const char* op = "shared_prefix_attention";
+  PagedAttnArgs a;
+  int rc = paged_cache(a.cache, op, kv_pointers, nullptr, lengths, batch, batch, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
+                       int4_kv_cache, kv_cache_with_zeros);
+  if (rc) return rc;
+  QS_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0, "%s: heads %d / kv heads %d", op, num_heads, num_kv_heads);
+  QS_REQUIRE(shared_blocks >= 0 && shared_blocks <= max_blocks_per_seq, "%s: shared_blocks=%d of %d pages per sequence", op, shared_blocks, max_blocks_per_seq);
+  QS_REQUIRE(max_length >= 0, "%s: negative size", op);
+  QS_REQUIRE(softmax_scale > 0.f && softmax_scale < 3.0e38f, "%s: softmax_scale must be positive and finite", op);
+  QS_REQUIRE(batch <= 65535 && num_heads <= 65535, "%s: batch=%d / heads=%d exceed the grid limits", op, batch, num_heads);
+  if (batch == 0) return qs::QS_OK;
+  if ((rc = paged_rows(op, "q", q, q_stride, num_heads)) || (rc = paged_rows(op, "out", out, out_stride, num_heads))) return rc;
+  QS_REQUIRE(aligned16(workspace), "%s: workspace must be 16-byte aligned", op);
+  a.q = q; a.out = out; a.q_stride = q_stride; a.out_stride = out_stride; a.batch = batch; a.num_tokens = batch; a.num_heads = num_heads; a.max_seqlen = 1;
+  a.max_length = max_length; a.softmax_scale = softmax_scale; a.workspace = workspace; a.workspace_bytes = workspace_bytes; a.stream = stream;
+  return shared_prefix_attention(a, shared_blocks);
+}
+
 int qs_prefill_attention(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* out,
                          int64_t out_stride, const int32_t* cu_seqlens, int batch, int num_tokens, int max_seqlen, int num_heads, int num_kv_heads,
                          int head_dim, float softmax_scale, void* stream) {

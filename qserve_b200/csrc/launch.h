@@ -125,4 +125,39 @@ struct PrefillAttnArgs {
 };
 int prefill_attention(const PrefillAttnArgs& a);
 
+// paged_cache.cu, paged_attention.cu: portions of sequences in the paged INT4 / INT8 cache
+struct PagedCache {
+  const long long* kv_pointers = nullptr;  // [B, 2, max_blocks] absolute device addresses
+  const int* cu_seqlens = nullptr;         // [B + 1] rows of the sequences' portions; null: one row each
+  const int* lengths = nullptr;            // [B] positions that a sequence holds, its portion included
+  int max_blocks = 0, num_kv_heads = 0;
+  bool int4 = true;
+};
+struct AppendArgs {
+  const void *q = nullptr, *k = nullptr, *v = nullptr;  // fp16 [T, H, 128], rows of *_stride halfs
+  void* q_out = nullptr;
+  long long q_stride = 0, k_stride = 0, v_stride = 0, q_out_stride = 0;
+  PagedCache cache;
+  int batch = 0, num_tokens = 0, num_heads = 0;
+  float rotary_base = 10000.f;
+  void* stream = nullptr;
+};
+int append_kv_cache(const AppendArgs& a);
+int read_kv_cache(void* k_out, void* v_out, const PagedCache& c, int batch, int num_tokens, void* stream);
+struct PagedAttnArgs {
+  const void* q = nullptr;  // fp16 [T, Hq, 128], rotated
+  void* out = nullptr;
+  long long q_stride = 0, out_stride = 0;
+  PagedCache cache;
+  int batch = 0, num_tokens = 0, num_heads = 0, max_seqlen = 0, max_length = 0;
+  float softmax_scale = 0.f;
+  void* workspace = nullptr;
+  size_t workspace_bytes = 0;
+  void* stream = nullptr;
+};
+size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads);
+int paged_prompt_attention(const PagedAttnArgs& a);
+size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_heads);
+int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks);
+
 }  // namespace qs

@@ -1,0 +1,1017 @@
+// qserve_b200 -- attention over the paged INT4 / INT8 cache of many query rows per key: portions of prompts (qs_paged_prompt_attention), and single tokens of a
+// batch whose sequences share their first pages (qs_shared_prefix_attention).
+//
+// Tile kernel.  The rows of a tile are (token, query head) pairs of one kv head: 128 rows see the same keys, whose codes are unpacked once for all of them.  Per
+// page of 64 keys:
+//     bulk copies     the head's codes, scales and zeros of K and V into a ring of raw slots
+//     unpack          4 warps: codes -> fp16 numbers in the swizzled shared-memory form that the products take (keys past the last row's limit: zeros)
+//     S = Q K^T       8 x tcgen05.mma 128 x 64 x 16, accumulators in tensor memory
+//     softmax         4 warps, thread = row (tensor memory lane): running maximum and sum in 32 bits, P = exp2(..) rounded to fp16, into tensor memory
+//     O += P V        4 x tcgen05.mma 128 x 128 x 16, A from tensor memory
+// A long axis of keys is split over blocks where the rows alone do not fill the device; their partial rows (O, maximum, sum, all fp32) are joined by
+// join_kernel (prompts) or by the tail kernel (shared prefix).
+//
+// Tail kernel (shared prefix): the pages behind the shared ones, one block of a cluster per (sequence, kv head, share of its pages), on mma.sync; joins its
+// warps', its cluster's and the prefix's partial rows and writes the result.
+#include <math_constants.h>
+
+#include <type_traits>
+
+#include "paged_common.cuh"
+
+namespace qs {
+namespace {
+
+using namespace paged;
+
+// ------------------------------------------------------------------------------------------------------------------------
+// PTX
+// ------------------------------------------------------------------------------------------------------------------------
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, uint32_t b_mn_major) {
+  // D = f32 (bits 4..5 = 1), A = B = f16, A K-major, B K-major or MN-major (bit 16), N >> 3 at bit 17, M >> 4 at bit 24
+  return (1u << 4) | (b_mn_major << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      :
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      :
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// rows of 128 bytes = 64 neighbours along N, one row per K index, 128-byte swizzle; lbo: from one 64-column group to the next, 1024 bytes from 8 K rows to the next 8
+__device__ __forceinline__ uint64_t desc_sw128_mn(uint32_t smem_addr, uint32_t lbo_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>(lbo_bytes >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
+      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// tile kernel
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int kRows = 128;                   // rows of a tile
+constexpr int kQBytes = kRows * kD * 2;      // two swizzled halves of 64 columns
+constexpr int kKvBytes = kPage * kD * 2;     // a page's K or V as fp16, two halves
+constexpr int kKvHalf = kKvBytes / 2;
+constexpr float kRescale = 8.f;              // log2 units that a row's maximum may grow before O is rescaled
+constexpr uint32_t kTileCols = 256, kColP = 64, kColO = 128;  // of a tile's tensor memory columns: S [0, 64), P [64, 96), O [128, 256)
+
+template <int BITS, int TILES>
+struct TileCfg {
+  static constexpr int kSoftmaxWarps = 4 * TILES;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4 + 1);  // softmax, unpack, issue
+  static constexpr int kBlocksPerSm = TILES == 1 ? 2 : 1;
+  static constexpr int kKStages = TILES == 1 ? 1 : 2;
+  static constexpr int kVStages = TILES == 1 && BITS == 8 ? 1 : 2;
+  static constexpr int kSlots = TILES == 1 ? (BITS == 4 ? 3 : 2) : (BITS == 4 ? 8 : 5);  // raw ring
+  static constexpr int kCodes = Geom<BITS>::kCodes;
+  static constexpr int kMeta = 2 * kCodes;               // K scales, K zeros, V scales, V zeros: 128 bytes each
+  static constexpr int kSlotBytes = 2 * kCodes + 512;
+  static constexpr int kOffK = TILES * kQBytes, kOffV = kOffK + kKStages * kKvBytes, kOffRaw = kOffV + kVStages * kKvBytes;
+  static constexpr int kOffBar = kOffRaw + kSlots * kSlotBytes;
+  static constexpr int kSmem = kOffBar + 256;
+  static_assert(kSmem * kBlocksPerSm + 1024 * kBlocksPerSm <= 228 * 1024, "shared memory of a multiprocessor");
+};
+
+struct TileParams {
+  const __half* q;
+  __half* out;
+  long long q_stride, out_stride;
+  const long long* kv_pointers;
+  const int *cu, *lengths;
+  int batch, num_tokens, max_blocks, num_heads, num_kv_heads;
+  int row_blocks, nsplit, shared_blocks;  // shared_blocks > 0: the rows of all sequences over the first sequence's first pages
+  float scale_log2;
+  float* part;                            // nsplit > 1: O [rows][nsplit][128], rows = token * num_heads + head
+  float2* part_ml;                        // (maximum, sum) [rows][nsplit]
+};
+
+template <int BITS, int TILES, bool PARTIAL>
+__global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, TILES>::kBlocksPerSm) tile_kernel(const __grid_constant__ TileParams p) {
+  using C = TileCfg<BITS, TILES>;
+  using G = Geom<BITS>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* bar_q = bar;             // the queries lie in shared memory
+  uint64_t* bar_s = bar + 1;         // [2] a page's S complete
+  uint64_t* bar_read = bar + 3;      // [2] S read: the next one may follow
+  uint64_t* bar_p = bar + 5;         // [2] P written
+  uint64_t* bar_o = bar + 7;         // [2] O += P V retired
+  uint64_t* bar_kfull = bar + 9;     // [2] K unpacked
+  uint64_t* bar_kfree = bar + 11;    // [2] S = Q K^T of all tiles retired
+  uint64_t* bar_vfull = bar + 13;    // [2]
+  uint64_t* bar_vfree = bar + 15;    // [2]
+  uint64_t* bar_raw = bar + 17;      // [kSlots] raw slot landed
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + 26);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4;
+  if (threadIdx.x == 0) {
+    mbar_init(bar_q, C::kSoftmaxWarps);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&bar_s[t], 1);
+      mbar_init(&bar_read[t], 4);
+      mbar_init(&bar_p[t], 4);
+      mbar_init(&bar_o[t], 1);
+      mbar_init(&bar_kfull[t], 4);
+      mbar_init(&bar_kfree[t], 1);
+      mbar_init(&bar_vfull[t], 4);
+      mbar_init(&bar_vfree[t], 1);
+    }
+    for (int i = 0; i < C::kSlots; ++i) mbar_init(&bar_raw[i], 1);
+    fence_barrier_init();
+  }
+  if (warp == kIssueWarp) tmem_alloc<TILES * kTileCols>(s_tmem);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  pdl_wait();
+  // Only now: what is launched next may read what this kernel's predecessors wrote (the tail kernel does, ahead of its own wait)
+  pdl_launch_dependents();
+
+  // ---- this block's rows and pages ----
+  int idx = blockIdx.x;
+  const int hk = idx % p.num_kv_heads;
+  idx /= p.num_kv_heads;
+  const int split = idx % p.nsplit;
+  idx /= p.nsplit;
+  const int b = idx % p.batch, rb = p.row_blocks - 1 - idx / p.batch;  // the last rows see most keys: they are first
+  const int group = p.num_heads / p.num_kv_heads;
+  const Portion portion = p.shared_blocks > 0 ? Portion{0, p.num_tokens, 0} : portion_of(p.cu, p.lengths, b, p.num_tokens);
+  const int n_rows = portion.count * group;
+  const int row_base = rb * (TILES * kRows);
+  const bool any = row_base < n_rows;
+  int n_keys;  // that the block's last row sees
+  if (p.shared_blocks > 0) {
+    n_keys = p.shared_blocks * kPage;
+  } else {
+    const int last = min(n_rows, row_base + TILES * kRows) - 1;
+    n_keys = any ? min(max(portion.first + last / group + 1, 0), p.max_blocks * kPage) : 0;
+  }
+  const int n_pages = (n_keys + kPage - 1) / kPage;
+  const int page0 = static_cast<int>(static_cast<long long>(split) * n_pages / p.nsplit);
+  const int n_mine = any ? static_cast<int>(static_cast<long long>(split + 1) * n_pages / p.nsplit) - page0 : 0;
+
+  if (warp >= kUnpackWarp && warp < kIssueWarp) {
+    // ===================================== copies and unpacking =====================================
+    const int t = threadIdx.x - 32 * kUnpackWarp;
+    const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks;
+    const long long* vptrs = kptrs + p.max_blocks;
+    long long kp = 0, vp = 0;  // lane i of the first of these warps: the pages 32 n + i
+    auto issue = [&](int j) {  // (first warp) page j of this block's into its slot
+      if ((j & 31) == 0 && j + lane < n_mine) {
+        kp = __ldg(kptrs + page0 + j + lane);
+        vp = __ldg(vptrs + page0 + j + lane);
+      }
+      const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp, j & 31));
+      const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp, j & 31));
+      if (lane == 0) {
+        uint8_t* slot = smem + C::kOffRaw + (j % C::kSlots) * C::kSlotBytes;
+        uint64_t* full = &bar_raw[j % C::kSlots];
+        mbar_expect_tx(full, C::kSlotBytes);
+        bulk_copy_g2s(slot, k + G::codes_at(hk), C::kCodes, full);
+        bulk_copy_g2s(slot + C::kCodes, v + G::codes_at(hk), C::kCodes, full);
+        bulk_copy_g2s(slot + C::kMeta, k + G::scales_at(hk, p.num_kv_heads), 128, full);
+        bulk_copy_g2s(slot + C::kMeta + 128, k + G::zeros_at(hk, p.num_kv_heads), 128, full);
+        bulk_copy_g2s(slot + C::kMeta + 256, v + G::scales_at(hk, p.num_kv_heads), 128, full);
+        bulk_copy_g2s(slot + C::kMeta + 384, v + G::zeros_at(hk, p.num_kv_heads), 128, full);
+      }
+      __syncwarp();
+    };
+    if (warp == kUnpackWarp)
+      for (int j = 0; j < min(n_mine, C::kSlots); ++j) issue(j);
+    // thread: key t / 2, dims 64 (t % 2) .. + 63.  The odd threads take their words in the other order, so that eight neighbours meet every bank once.
+    const int key = t >> 1, part = t & 1;
+    const uint32_t row_at = part * kKvHalf + key * 128, swizzle = key & 7;
+    for (int j = 0; j < n_mine; ++j) {
+      const int slot = j % C::kSlots;
+      const uint8_t* raw = smem + C::kOffRaw + slot * C::kSlotBytes;
+      mbar_wait(&bar_raw[slot], static_cast<uint32_t>(j / C::kSlots) & 1u);
+      // A row of K or V whose scale or zero is no finite number stands for NaN: the key's score is NaN then (and goes where the key is masked), its value 0, so
+      // that a weight of 0 in a row that does not see it stays 0.
+      const bool live = (page0 + j) * kPage + key < n_keys;
+      const __half* meta = reinterpret_cast<const __half*>(raw + C::kMeta) + key;
+      __half ks = meta[0], kz = meta[64], vs = meta[128], vz = meta[192];
+      auto endless = [](__half h) { return (__half_as_ushort(h) & 0x7c00u) == 0x7c00u; };
+      bool bad = endless(ks) || endless(kz) || endless(vs) || endless(vz);
+      __half kc = BITS == 4 ? __hmul(__hneg(ks), kz) : kz, vc = BITS == 4 ? __hmul(__hneg(vs), vz) : vz;
+      bad = bad || endless(kc) || endless(vc);
+      if (!live || bad) {
+        vs = vc = __ushort_as_half(0);
+        ks = kc = __ushort_as_half(live ? 0x7fffu : 0);
+      }
+      auto unpack = [&](const uint8_t* codes, __half s, __half c, uint8_t* dst) {
+        const __half2 s2 = __half2half2(s), c2 = __half2half2(c);
+        auto put = [&](int chunk, const __half2 (&x)[4]) {
+          *reinterpret_cast<uint4*>(dst + row_at + ((chunk ^ swizzle) << 4)) = make_uint4(as_u32(x[0]), as_u32(x[1]), as_u32(x[2]), as_u32(x[3]));
+        };
+        const uint4* src = reinterpret_cast<const uint4*>(codes + t * (G::kRow / 2));
+        if constexpr (BITS == 4) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 w = src[i ^ part];
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              __half2 u[4];
+              codes_of_word4(words[k], u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) u[e] = __hfma2(u[e], s2, c2);
+              put(4 * (i ^ part) + k, u);  // dims 0 4 1 5 2 6 3 7 of eight: the queries lie in the same order, O's columns come out in it
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int at = i ^ (2 * part);
+            const uint4 w = src[at];
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              __half2 lo[2], hi[2];
+              codes_of_word8(words[2 * k], lo);
+              codes_of_word8(words[2 * k + 1], hi);
+              __half2 u[4] = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+              for (int e = 0; e < 4; ++e) u[e] = __hmul2(__hsub2(u[e], c2), s2);
+              put(2 * at + k, u);
+            }
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+      };
+      const int ks_at = j % C::kKStages, vs_at = j % C::kVStages;
+      mbar_wait(&bar_kfree[ks_at], (static_cast<uint32_t>(j / C::kKStages) & 1u) ^ 1u);
+      unpack(raw, ks, kc, smem + C::kOffK + ks_at * kKvBytes);
+      if (lane == 0) mbar_arrive(&bar_kfull[ks_at]);
+      mbar_wait(&bar_vfree[vs_at], (static_cast<uint32_t>(j / C::kVStages) & 1u) ^ 1u);
+      unpack(raw + C::kCodes, vs, vc, smem + C::kOffV + vs_at * kKvBytes);
+      if (lane == 0) mbar_arrive(&bar_vfull[vs_at]);
+      named_bar_sync(1, 128);  // all four warps are done with the slot
+      if (warp == kUnpackWarp && j + C::kSlots < n_mine) issue(j + C::kSlots);
+    }
+  } else if (warp == kIssueWarp) {
+    // ===================================== products =====================================
+    if (lane == 0 && n_mine > 0) {
+      constexpr uint32_t idesc_qk = idesc_f16(kRows, kPage, 0u), idesc_pv = idesc_f16(kRows, kD, 1u);
+      auto scores = [&](int j, int t) {
+        const int st = j % C::kKStages;
+#pragma unroll
+        for (int ks = 0; ks < kD / 16; ++ks) {
+          const uint64_t a = umma_desc_sw128(smem_u32(smem + t * kQBytes + (ks >> 2) * (kQBytes / 2))) + (ks & 3) * 2;
+          const uint64_t bd = umma_desc_sw128(smem_u32(smem + C::kOffK + st * kKvBytes + (ks >> 2) * kKvHalf)) + (ks & 3) * 2;
+          mma_f16_ss(tmem + t * kTileCols, a, bd, idesc_qk, ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&bar_s[t]);
+        if (t == TILES - 1) umma_commit(&bar_kfree[st]);
+      };
+      auto k_ready = [&](int j) {
+        mbar_wait(&bar_kfull[j % C::kKStages], static_cast<uint32_t>(j / C::kKStages) & 1u);
+        tc_fence_after();
+      };
+      mbar_wait(bar_q, 0);
+      k_ready(0);
+      for (int t = 0; t < TILES; ++t) scores(0, t);
+      for (int j = 0; j < n_mine; ++j) {
+        if (j + 1 < n_mine) {  // the next page's S, while this one's softmax goes on
+          k_ready(j + 1);
+          for (int t = 0; t < TILES; ++t) {
+            mbar_wait(&bar_read[t], static_cast<uint32_t>(j) & 1u);
+            tc_fence_after();
+            scores(j + 1, t);
+          }
+        }
+        const int st = j % C::kVStages;
+        mbar_wait(&bar_vfull[st], static_cast<uint32_t>(j / C::kVStages) & 1u);
+        for (int t = 0; t < TILES; ++t) {
+          mbar_wait(&bar_p[t], static_cast<uint32_t>(j) & 1u);
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < kPage / 16; ++kk) {
+            const uint64_t bd = desc_sw128_mn(smem_u32(smem + C::kOffV + st * kKvBytes + kk * 2048), kKvHalf);
+            mma_f16_ts(tmem + t * kTileCols + kColO, tmem + t * kTileCols + kColP + kk * 8, bd, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          }
+          umma_commit(&bar_o[t]);
+          if (t == TILES - 1) umma_commit(&bar_vfree[st]);
+        }
+      }
+    }
+  } else if (any) {
+    // ===================================== queries, softmax, results: thread = row =====================================
+    const int tile = warp >> 2, quarter = warp & 3;
+    const int first_row = row_base + tile * kRows + quarter * 32;
+    {
+      // half a warp a row, 16 bytes a lane
+      uint8_t* dst = smem + tile * kQBytes;
+      const int c = lane & 15;
+#pragma unroll 4
+      for (int k = 0; k < 32; k += 2) {
+        const int in_tile = quarter * 32 + k + (lane >> 4), r = first_row + k + (lane >> 4);
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (r < n_rows) {
+          const int tok = r / group, head = hk * group + (r - tok * group);
+          x = __ldg(reinterpret_cast<const uint4*>(p.q + (portion.start + tok) * p.q_stride + static_cast<long long>(head) * kD) + c);
+        }
+        if constexpr (BITS == 4)  // the order in which the keys' dims are unpacked
+          x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kQBytes / 2) + in_tile * 128 + (((c & 7) ^ (in_tile & 7)) << 4)) = x;
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q);
+    }
+    const int r = first_row + lane;
+    const int tok = r / group, head = hk * group + (r - tok * group);
+    int limit = -1;  // the last position that the row sees
+    if (r < n_rows) limit = p.shared_blocks > 0 ? min(__ldg(p.lengths + tok), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
+    int lowest = limit;  // of the warp's rows
+#pragma unroll
+    for (int m = 16; m >= 1; m >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, m));
+    const uint32_t t_s = tmem + tile * kTileCols + (static_cast<uint32_t>(quarter * 32) << 16), t_p = t_s + kColP, t_o = t_s + kColO;
+    float m_used = -CUDART_INF_F, l = 0.f;  // what O and the sum are expressed against (log2 units)
+    for (int j = 0; j < n_mine; ++j) {
+      const uint32_t ph = static_cast<uint32_t>(j) & 1u;
+      uint32_t x[2][32], w[32];
+      mbar_wait(&bar_s[tile], ph);
+      tc_fence_after();
+      tmem_ld_32x32b_x32(t_s, x[0]);
+      tmem_ld_32x32b_x32(t_s + 32, x[1]);
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_read[tile]);
+      const int key0 = (page0 + j) * kPage;
+      if (key0 + kPage - 1 > lowest) {  // warp-uniform
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (key0 + c * 32 + i > limit) x[c][i] = 0xff800000u;  // -inf
+      }
+      float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
+      const float m_page = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
+      auto retired = [&]() {  // the O += P V before
+        mbar_wait(&bar_o[tile], ph ^ 1u);
+        tc_fence_after();
+      };
+      if (j == 0) {
+        m_used = m_page;
+      } else {
+        const bool grow = m_page - m_used > kRescale;  // also from -inf; a row that has seen nothing yet and sees nothing here: NaN, no
+        if (__any_sync(0xffffffffu, grow)) {
+          retired();
+          const float m_new = grow ? m_page : m_used;
+          const float alpha = grow ? ex2(m_used - m_new) : 1.f;
+#pragma unroll 1
+          for (int c = 0; c < kD / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(t_o + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st_x32(t_o + c * 32, o);
+          }
+          l *= alpha;
+          m_used = m_new;
+        }
+      }
+      const float m_ref = m_used == -CUDART_INF_F ? 0.f : m_used;  // a row without any key so far: its weights are exp2(-inf) = 0
+#pragma unroll
+      for (int i = 0; i < 64; i += 2) {
+        const float p0 = ex2(fmaf(__uint_as_float(x[i >> 5][i & 31]), p.scale_log2, -m_ref));
+        const float p1 = ex2(fmaf(__uint_as_float(x[i >> 5][(i & 31) + 1]), p.scale_log2, -m_ref));
+        const __half2 h = __floats2half2_rn(p0, p1);
+        const float2 f = __half22float2(h);  // the sum is that of the rounded weights: numerator and denominator agree
+        l += f.x + f.y;
+        w[i >> 1] = as_u32(h);
+      }
+      if (j > 0) retired();
+      tmem_st_x32(t_p, w);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_p[tile]);
+    }
+    if (n_mine > 0) {
+      mbar_wait(&bar_o[tile], static_cast<uint32_t>(n_mine - 1) & 1u);
+      tc_fence_after();
+    }
+    const bool store = r < n_rows;
+    const long long token = portion.start + tok;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
+    const long long at = (token * p.num_heads + head) * p.nsplit + split;
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+      uint32_t o[32];
+      if (n_mine > 0) {
+        tmem_ld_32x32b_x32(t_o + c * 32, o);
+        tmem_wait_ld();
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = 0u;
+      }
+      if (!store) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]);
+        if constexpr (PARTIAL) {
+          float4* dst = reinterpret_cast<float4*>(p.part + at * kD + c * 32 + e * 8);
+          dst[0] = make_float4(f[0], f[1], f[2], f[3]);
+          dst[1] = make_float4(f[4], f[5], f[6], f[7]);
+        } else {
+          uint4 y;
+          y.x = as_u32(__floats2half2_rn(f[0] * inv, f[1] * inv));
+          y.y = as_u32(__floats2half2_rn(f[2] * inv, f[3] * inv));
+          y.z = as_u32(__floats2half2_rn(f[4] * inv, f[5] * inv));
+          y.w = as_u32(__floats2half2_rn(f[6] * inv, f[7] * inv));
+          *reinterpret_cast<uint4*>(p.out + token * p.out_stride + static_cast<long long>(head) * kD + c * 32 + e * 8) = y;
+        }
+      }
+    }
+    if (PARTIAL && store) p.part_ml[at] = make_float2(m_used, l);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssueWarp) tmem_dealloc<TILES * kTileCols>(tmem);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// partial rows of a split joined: a warp, lane = 4 dims.  Returns the sum and the maximum that acc is expressed against.
+// ------------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void join_rows(const float* part, const float2* ml, int nsplit, float& M, float& L, float4& acc) {
+  const int lane = threadIdx.x & 31;
+  for (int s0 = 0; s0 < nsplit; s0 += 32) {
+    const float2 mine = s0 + lane < nsplit ? __ldcg(ml + s0 + lane) : make_float2(-CUDART_INF_F, 0.f);
+    float m = mine.x;
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+    const float m_new = fmaxf(M, m), ref = m_new == -CUDART_INF_F ? 0.f : m_new;
+    const float old = ex2(M - ref), w = ex2(mine.x - ref);
+    float sum = mine.y * w;
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+    L = fmaf(L, old, sum);
+    acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
+    M = m_new;
+    const int n = min(32, nsplit - s0);
+#pragma unroll 8
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(part + static_cast<long long>(s0 + s) * kD) + lane);
+      acc.x = fmaf(x.x, ws, acc.x); acc.y = fmaf(x.y, ws, acc.y); acc.z = fmaf(x.z, ws, acc.z); acc.w = fmaf(x.w, ws, acc.w);
+    }
+  }
+}
+__device__ __forceinline__ uint2 scaled_h4(const float4& a, float L) {
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  return make_uint2(as_u32(__floats2half2_rn(a.x * inv, a.y * inv)), as_u32(__floats2half2_rn(a.z * inv, a.w * inv)));
+}
+
+// a warp per row of the result; rows behind the last sequence are left as they are
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileParams p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (row >= static_cast<long long>(p.num_tokens) * p.num_heads) return;
+  const int token = static_cast<int>(row / p.num_heads), head = static_cast<int>(row - static_cast<long long>(token) * p.num_heads);
+  if (sequence_of(p.cu, p.batch, token) < 0) return;
+  float M = -CUDART_INF_F, L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  join_rows(p.part + row * p.nsplit * kD, p.part_ml + row * p.nsplit, p.nsplit, M, L, acc);
+  reinterpret_cast<uint2*>(p.out + token * p.out_stride + static_cast<long long>(head) * kD)[lane] = scaled_h4(acc, L);
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// tail kernel: the pages behind the shared ones
+//
+// Warp w of a block takes every fourth half page (32 keys) of its share.  Codes go into the products as they lie: a nibble or byte in the low bits of an fp16 word
+// is the subnormal number u 2^-24, exact as an operand, so there is no conversion and nothing to take off again; scales, zeros and 2^24 are applied to scores and
+// weights in fp32:  q.k = s 2^24 (q.u 2^-24) + c sum(q),  sum p v = 2^24 sum (p s) u 2^-24 + sum p c.
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int kTailWarps = 4, kMaxG = 8, kSlice = 32, kMaxCluster = 8;
+constexpr int kOPitch = kD + 4;
+
+template <int BITS>
+struct SliceCfg {
+  static constexpr int kRow = Geom<BITS>::kRow;
+  static constexpr int kCodes = kSlice * kRow;
+  static constexpr int kOffV = kCodes, kOffMeta = 2 * kCodes;  // K scales, K zeros, V scales, V zeros: 64 bytes each
+  static constexpr int kBytes = 2 * kCodes + 256;
+  static constexpr int kSlots = 2;
+  static constexpr int kWarpBytes = kSlots * kBytes;
+  static_assert(kWarpBytes >= kMaxG * kOPitch * 4, "a warp's ring holds its partial rows at the end");
+  static constexpr int kSmem = kTailWarps * kWarpBytes;
+  // where 16-byte word c of a key's row lies: reads of K (rows p and p + 4) and transposing reads of V (one word of eight rows) meet every bank once
+  static __device__ __forceinline__ uint32_t place(int row, int c) {
+    if constexpr (BITS == 4) return (row >> 1) * 128 + (((row ^ (row >> 2)) & 1) * 4 + (c ^ ((row >> 1) & 3))) * 16;
+    else return row * 128 + (c ^ (((row >> 2) & 1) | ((row & 3) << 1))) * 16;
+  }
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t smem) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
+}
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float peer_f32(const float* mine, uint32_t rank) {
+  uint32_t a;
+  float f;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+  return f;
+}
+__device__ __forceinline__ float4 peer_f32x4(const float* mine, uint32_t rank) {
+  uint32_t a;
+  float4 f;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
+  return f;
+}
+
+struct TailParams {
+  const __half* q;
+  __half* out;
+  long long q_stride, out_stride;
+  const long long* kv_pointers;
+  const int* lengths;
+  int max_blocks, num_heads, num_kv_heads, shared_blocks, nsplit, cluster;
+  float scale_log2;
+  const float* part;
+  const float2* part_ml;
+};
+
+template <int BITS>
+__global__ void __launch_bounds__(32 * kTailWarps, BITS == 4 ? 4 : 3) tail_kernel(const __grid_constant__ TailParams p) {
+  using SC = SliceCfg<BITS>;
+  using G = Geom<BITS>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ __align__(16) __half s_q[kMaxG * kD];
+  __shared__ float s_m[kTailWarps][kMaxG], s_l[kTailWarps][kMaxG];
+  __shared__ float2 s_meta[kTailWarps][2][kSlice];
+  __shared__ __align__(16) float s_o[kMaxG * kD];        // the block's rows
+  __shared__ float s_bm[kMaxG], s_bl[kMaxG];
+  const int group = p.num_heads / p.num_kv_heads, parts = (group + kMaxG - 1) / kMaxG;
+  const int rank = blockIdx.x, b = blockIdx.z, hk = blockIdx.y / parts, part = blockIdx.y - hk * parts;
+  const int h0 = hk * group + part * kMaxG, heads = min(kMaxG, group - part * kMaxG);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  pdl_launch_dependents();
+  // The tile kernel before this one started this one after its own wait: everything ahead of the tile kernel is there.  Without one, this kernel waits itself.
+  if (p.nsplit == 0) pdl_wait();
+
+  const int len = min(__ldcg(p.lengths + b), p.max_blocks * kPage);
+  const int slices = max((len - p.shared_blocks * kPage + kSlice - 1) / kSlice, 0);
+  // the cluster's blocks and their warps take turns over the slices
+  const int stride = p.cluster * kTailWarps, mine = rank * kTailWarps + warp;
+  const int n_my = slices > mine ? (slices - mine + stride - 1) / stride : 0;
+  const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + p.shared_blocks;
+  const long long* vptrs = kptrs + p.max_blocks;
+  uint8_t* ring = smem + warp * SC::kWarpBytes;
+  const uint32_t ring_at = smem_u32(ring);
+  const uint32_t lane_at = SC::place(lane * 16 / SC::kRow, lane * 16 % SC::kRow / 16);
+  long long kp_l = 0, vp_l = 0;  // lane i: the pages of slices 32 n + i
+  auto issue = [&](int u) {
+    if ((u & 31) == 0 && u + lane < n_my) {
+      const int page = (mine + (u + lane) * stride) >> 1;
+      kp_l = __ldcg(kptrs + page);
+      vp_l = __ldcg(vptrs + page);
+    }
+    const int half = (mine + u * stride) & 1;
+    const uint8_t* kp = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp_l, u & 31));
+    const uint8_t* vp = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp_l, u & 31));
+    const uint32_t dst = ring_at + (u % SC::kSlots) * SC::kBytes;
+    const long long codes = G::codes_at(hk) + half * SC::kCodes + lane * 16;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int i = 0; i < SC::kCodes / 512; ++i)
+        cp_async16(dst + w * SC::kOffV + i * 512 + (BITS == 8 && (i & 1) ? lane_at ^ 16u : lane_at), (w ? vp : kp) + codes + i * 512);
+    if (lane < 16) {
+      const uint8_t* page_at = lane < 8 ? kp : vp;
+      const long long meta = (lane & 4) ? G::zeros_at(hk, p.num_kv_heads) : G::scales_at(hk, p.num_kv_heads);
+      cp_async16(dst + SC::kOffMeta + lane * 16, page_at + meta + half * 64 + (lane & 3) * 16);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < SC::kSlots; ++u) {
+    if (u < n_my) issue(u);
+    cp_async_commit();
+  }
+  // ---- the queries: 16 lanes a row ----
+  for (int i = threadIdx.x; i < kMaxG * 16; i += 32 * kTailWarps) {
+    const int r = i >> 4;
+    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+    if (r < heads) x = __ldcg(reinterpret_cast<const uint4*>(p.q + b * p.q_stride + static_cast<long long>(h0 + r) * kD) + (i & 15));
+    reinterpret_cast<uint4*>(s_q)[i] = x;
+  }
+  __syncthreads();
+  // Q as the B operand (n = head g) in the order of the codes: INT4 word w of a lane's 32 dims has nibbles (0, 4 | 1, 5), (2, 6 | 3, 7); INT8 (0, 1 | 2, 3)
+  uint32_t qb0[8], qb1[8];
+  float sumq0, sumq1;
+  {
+    uint32_t qw[16];
+    const uint4* qv = reinterpret_cast<const uint4*>(s_q + g * kD + 32 * q4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint4 t = qv[k];
+      qw[4 * k] = t.x; qw[4 * k + 1] = t.y; qw[4 * k + 2] = t.z; qw[4 * k + 3] = t.w;
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float2 f = __half22float2(as_h2(qw[k]));
+      sum += f.x + f.y;
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    sumq0 = __shfl_sync(0xffffffffu, sum, 8 * q4);
+    sumq1 = __shfl_sync(0xffffffffu, sum, 8 * q4 + 4);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if constexpr (BITS == 4) {
+        const int k0 = 4 * (s >> 1) + (s & 1);
+        qb0[s] = __byte_perm(qw[k0], qw[k0 + 2], 0x5410);
+        qb1[s] = as_u32(__hmul2(as_h2(__byte_perm(qw[k0], qw[k0 + 2], 0x7632)), __float2half2_rn(0.0625f)));  // high nibbles are 16 u
+      } else {
+        qb0[s] = qw[2 * s];
+        qb1[s] = qw[2 * s + 1];
+      }
+    }
+  }
+  constexpr float kUp = 16777216.f;  // 2^24
+  float o[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f, c0 = 0.f, c1 = 0.f;
+  const int tokA = (g & 1) * 4 + (g >> 1);
+  const uint32_t k_at = SC::place(tokA, BITS == 4 ? q4 : 2 * q4);
+  const uint32_t v_at = SC::place((lane & 1) * 4 + ((lane >> 1) & 3) + (lane & 8), lane >> 4) + SC::kOffV;
+  for (int u = 0; u < n_my; ++u) {
+    cp_async_wait<SC::kSlots - 1>();
+    __syncwarp();
+    const uint32_t slot = (u % SC::kSlots) * SC::kBytes;
+    const uint8_t* st = ring + slot;
+    const int t0 = p.shared_blocks * kPage + (mine + u * stride) * kSlice;
+    // (scale, c) per key in fp32, the scores' with the softmax scale; keys past the end: zeros
+    {
+      const __half* mp = reinterpret_cast<const __half*>(st + SC::kOffMeta) + lane;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const __half s = mp[64 * w], z = mp[64 * w + 32];
+        float2 f = make_float2(__half2float(s), BITS == 4 ? __half2float(__hmul(__hneg(s), z)) : -__half2float(s) * __half2float(z));
+        if (w == 0) f = make_float2(f.x * (p.scale_log2 * kUp), f.y * p.scale_log2);
+        if (t0 + lane >= len) f = make_float2(0.f, 0.f);
+        s_meta[warp][w][lane] = f;
+      }
+    }
+    __syncwarp();
+    float sc[2][4] = {};
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint8_t* krow = st + c * 16 * SC::kRow + k_at;
+      if constexpr (BITS == 4) {
+        const uint4 ka = *reinterpret_cast<const uint4*>(krow), kb = *reinterpret_cast<const uint4*>(krow + 8 * SC::kRow);
+        const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t xa = wa[w], xb = wb[w], ta = xa >> 8, tb = xb >> 8;
+          mma_16816(sc[c], xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, qb0[2 * w], qb1[2 * w]);
+          mma_16816(sc[c], ta & 0x000f000fu, tb & 0x000f000fu, ta & 0x00f000f0u, tb & 0x00f000f0u, qb0[2 * w + 1], qb1[2 * w + 1]);
+        }
+      } else {
+        const uint8_t* krow1 = st + c * 16 * SC::kRow + (k_at ^ 16u);
+        const uint4 ka0 = *reinterpret_cast<const uint4*>(krow), ka1 = *reinterpret_cast<const uint4*>(krow1);
+        const uint4 kb0 = *reinterpret_cast<const uint4*>(krow + 8 * SC::kRow), kb1 = *reinterpret_cast<const uint4*>(krow1 + 8 * SC::kRow);
+        const uint32_t wa[8] = {ka0.x, ka0.y, ka0.z, ka0.w, ka1.x, ka1.y, ka1.z, ka1.w};
+        const uint32_t wb[8] = {kb0.x, kb0.y, kb0.z, kb0.w, kb1.x, kb1.y, kb1.z, kb1.w};
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          mma_16816(sc[c], __byte_perm(wa[w], 0u, 0x4140), __byte_perm(wb[w], 0u, 0x4140), __byte_perm(wa[w], 0u, 0x4342), __byte_perm(wb[w], 0u, 0x4342),
+                    qb0[w], qb1[w]);
+      }
+    }
+    float tl[2][4], vs[2][2], vc[2][2];
+    const bool partial = t0 + kSlice > len;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float2 kA = s_meta[warp][0][c * 16 + tokA], kB = s_meta[warp][0][c * 16 + 8 + tokA];
+      const float2 vA = s_meta[warp][1][c * 16 + tokA], vB = s_meta[warp][1][c * 16 + 8 + tokA];
+      vs[c][0] = vA.x; vs[c][1] = vB.x; vc[c][0] = vA.y; vc[c][1] = vB.y;
+      tl[c][0] = fmaf(kA.x, sc[c][0], kA.y * sumq0);
+      tl[c][1] = fmaf(kA.x, sc[c][1], kA.y * sumq1);
+      tl[c][2] = fmaf(kB.x, sc[c][2], kB.y * sumq0);
+      tl[c][3] = fmaf(kB.x, sc[c][3], kB.y * sumq1);
+      if (partial) {
+        if (t0 + c * 16 + tokA >= len) tl[c][0] = tl[c][1] = -CUDART_INF_F;
+        if (t0 + c * 16 + 8 + tokA >= len) tl[c][2] = tl[c][3] = -CUDART_INF_F;
+      }
+    }
+    // A weight is at most 1 (a slice always has a key, so the maxima are numbers): p s stays in the range of fp16 whatever a value's scale is
+    float mh0 = fmaxf(fmaxf(tl[0][0], tl[0][2]), fmaxf(tl[1][0], tl[1][2])), mh1 = fmaxf(fmaxf(tl[0][1], tl[0][3]), fmaxf(tl[1][1], tl[1][3]));
+    if (__any_sync(0xffffffffu, mh0 > m0 || mh1 > m1)) {
+#pragma unroll
+      for (int m = 4; m <= 16; m <<= 1) {
+        mh0 = fmaxf(mh0, __shfl_xor_sync(0xffffffffu, mh0, m));
+        mh1 = fmaxf(mh1, __shfl_xor_sync(0xffffffffu, mh1, m));
+      }
+      const bool n0 = mh0 > m0, n1 = mh1 > m1;
+      const float a0 = n0 ? ex2(m0 - mh0) : 1.f, a1 = n1 ? ex2(m1 - mh1) : 1.f;
+      if (n0) m0 = mh0;
+      if (n1) m1 = mh1;
+      l0 *= a0; c0 *= a0; l1 *= a1; c1 *= a1;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        o[i][0] *= a0; o[i][2] *= a0;
+        o[i][1] *= a1; o[i][3] *= a1;
+      }
+    }
+    uint32_t bp[2][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float pA0 = ex2(tl[c][0] - m0), pA1 = ex2(tl[c][1] - m1), pB0 = ex2(tl[c][2] - m0), pB1 = ex2(tl[c][3] - m1);
+      l0 += pA0 + pB0; l1 += pA1 + pB1;
+      c0 = fmaf(pA0, vc[c][0], fmaf(pB0, vc[c][1], c0));
+      c1 = fmaf(pA1, vc[c][0], fmaf(pB1, vc[c][1], c1));
+      // the products' operand: p s rounded to fp16
+      bp[c][0] = movmatrix_trans(as_u32(__floats2half2_rn(pA0 * vs[c][0], pA1 * vs[c][0])));
+      bp[c][1] = movmatrix_trans(as_u32(__floats2half2_rn(pB0 * vs[c][1], pB1 * vs[c][1])));
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int h = 0; h < kD / (256 / BITS); ++h) {
+        uint32_t w[4];
+        ldmatrix_x4_trans(w, ring_at + slot + c * 16 * SC::kRow + (v_at ^ (h * 32u)));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t lo = w[2 * e], hi = w[2 * e + 1];
+          if constexpr (BITS == 4) {
+            const int i = 4 * h + 2 * e;
+            mma_16816(o[i], lo & 0x000f000fu, lo & 0x00f000f0u, hi & 0x000f000fu, hi & 0x00f000f0u, bp[c][0], bp[c][1]);
+            const uint32_t lo8 = lo >> 8, hi8 = hi >> 8;
+            mma_16816(o[i + 1], lo8 & 0x000f000fu, lo8 & 0x00f000f0u, hi8 & 0x000f000fu, hi8 & 0x00f000f0u, bp[c][0], bp[c][1]);
+          } else {
+            const int i = 2 * h + e;
+            mma_16816(o[i], __byte_perm(lo, 0u, 0x4240), __byte_perm(lo, 0u, 0x4341), __byte_perm(hi, 0u, 0x4240), __byte_perm(hi, 0u, 0x4341), bp[c][0],
+                      bp[c][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (u + SC::kSlots < n_my) issue(u + SC::kSlots);
+    cp_async_commit();
+  }
+  // ---- a warp's partial rows into its ring: [head][place of the dim] ----
+#pragma unroll
+  for (int m = 4; m <= 16; m <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, m);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, m);
+    c0 += __shfl_xor_sync(0xffffffffu, c0, m);
+    c1 += __shfl_xor_sync(0xffffffffu, c1, m);
+  }
+  if (g == 0) {
+    s_m[warp][2 * q4] = m0; s_m[warp][2 * q4 + 1] = m1;
+    s_l[warp][2 * q4] = l0; s_l[warp][2 * q4 + 1] = l1;
+  }
+  {
+    __syncwarp();
+    float* so0 = reinterpret_cast<float*>(ring) + (2 * q4) * kOPitch + g;
+    float* so1 = so0 + kOPitch;
+    constexpr float kOdd = BITS == 4 ? kUp * 0.0625f : kUp;  // INT4: odd dims are the high nibbles, 16 u
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      so0[16 * i] = fmaf(o[i][0], kUp, c0); so0[16 * i + 8] = fmaf(o[i][2], kOdd, c0);
+      so1[16 * i] = fmaf(o[i][1], kUp, c1); so1[16 * i + 8] = fmaf(o[i][3], kOdd, c1);
+    }
+  }
+  __syncthreads();
+  // ---- the block's rows ----
+  {
+    // the dim whose partial sums lie at this thread's place
+    const int t = threadIdx.x, d = BITS == 4 ? 32 * (t >> 5) + 4 * (t & 7) + 2 * ((t >> 4) & 1) + ((t >> 3) & 1) : 16 * (t >> 4) + 2 * (t & 7) + ((t >> 3) & 1);
+    for (int r = 0; r < heads; ++r) {
+      float M = -CUDART_INF_F;
+#pragma unroll
+      for (int w = 0; w < kTailWarps; ++w) M = fmaxf(M, s_m[w][r]);
+      const float ref = M == -CUDART_INF_F ? 0.f : M;
+      float acc = 0.f, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < kTailWarps; ++w) {
+        const float e = ex2(s_m[w][r] - ref);
+        acc = fmaf(reinterpret_cast<const float*>(smem + w * SC::kWarpBytes)[r * kOPitch + t], e, acc);
+        L = fmaf(s_l[w][r], e, L);
+      }
+      s_o[r * kD + d] = acc;
+      if (t == 0) {
+        s_bm[r] = M;
+        s_bl[r] = L;
+      }
+    }
+  }
+  if (p.cluster > 1) cluster_sync();
+  else __syncthreads();
+  if (p.nsplit > 0) pdl_wait();  // the prefix's partial rows
+  // ---- the cluster's blocks take turns over the heads, a block's warps too ----
+  for (int r = rank + p.cluster * warp; r < heads; r += p.cluster * kTailWarps) {
+    float M = -CUDART_INF_F, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < p.cluster; ++k) {
+      const float m = p.cluster > 1 ? peer_f32(s_bm + r, k) : s_bm[r], sum = p.cluster > 1 ? peer_f32(s_bl + r, k) : s_bl[r];
+      const float4 x = p.cluster > 1 ? peer_f32x4(s_o + r * kD + 4 * lane, k) : *reinterpret_cast<const float4*>(s_o + r * kD + 4 * lane);
+      const float m_new = fmaxf(M, m), ref = m_new == -CUDART_INF_F ? 0.f : m_new;
+      const float old = ex2(M - ref), w = ex2(m - ref);
+      L = L * old + sum * w;
+      acc.x = fmaf(x.x, w, acc.x * old); acc.y = fmaf(x.y, w, acc.y * old); acc.z = fmaf(x.z, w, acc.z * old); acc.w = fmaf(x.w, w, acc.w * old);
+      M = m_new;
+    }
+    const long long row = static_cast<long long>(b) * p.num_heads + h0 + r;
+    if (p.nsplit > 0) join_rows(p.part + row * p.nsplit * kD, p.part_ml + row * p.nsplit, p.nsplit, M, L, acc);
+    reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<long long>(h0 + r) * kD)[lane] = scaled_h4(acc, L);
+  }
+  if (p.cluster > 1) cluster_sync();  // no block leaves while another reads its rows
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
+// host side
+// ------------------------------------------------------------------------------------------------------------------------
+template <auto Kern>
+int allow_smem(int bytes, const char* what) {
+  static bool done[kMaxDevices] = {};  // of this kernel
+  bool& d = done[device_ordinal()];
+  if (d) return QS_OK;
+  const int rc = check_cuda(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
+  if (rc == QS_OK) d = true;
+  return rc;
+}
+
+// How a call over `rows` rows per kv head and sequence and at most `pages` pages is cut: tiles per block and splits of the pages
+struct Plan {
+  int tiles, row_blocks, nsplit;
+};
+Plan plan_tiles(long long rows, long long items, long long pages) {
+  Plan pl;
+  pl.tiles = rows <= kRows ? 1 : 2;
+  pl.row_blocks = static_cast<int>((rows + pl.tiles * kRows - 1) / (pl.tiles * kRows));
+  const long long blocks = items * pl.row_blocks, slots = static_cast<long long>(num_sms()) * (pl.tiles == 1 ? 2 : 1);
+  long long n = blocks > 0 ? slots / blocks : 1;
+  const long long most = pages / 4;  // a split has at least four pages
+  if (n > most) n = most;
+  if (n < 1) n = 1;
+  if (n > 128) n = 128;
+  pl.nsplit = static_cast<int>(n);
+  return pl;
+}
+size_t part_bytes(long long rows, int nsplit) { return static_cast<size_t>(rows) * nsplit * (kD * sizeof(float) + sizeof(float2)); }
+
+template <int BITS, int TILES, bool PARTIAL>
+int run_tiles(const TileParams& p, int batch_items, void* stream) {
+  using C = TileCfg<BITS, TILES>;
+  const int rc = allow_smem<tile_kernel<BITS, TILES, PARTIAL>>(C::kSmem, "paged attention: shared memory");
+  if (rc) return rc;
+  const long long blocks = static_cast<long long>(p.row_blocks) * batch_items * p.nsplit * p.num_kv_heads;
+  QS_REQUIRE(blocks <= 0x7fffffffll, "paged attention: %lld blocks", blocks);
+  return launch(tile_kernel<BITS, TILES, PARTIAL>, dim3(static_cast<unsigned>(blocks)), C::kThreads, C::kSmem, stream, "paged attention", 1, p);
+}
+int tiles(const TileParams& p, bool int4, int tiles_per_block, bool partial, int items, void* stream) {
+  auto pick = [&](auto bits, auto per, auto part) { return run_tiles<decltype(bits)::value, decltype(per)::value, decltype(part)::value>(p, items, stream); };
+  auto with = [&](auto bits, auto per) { return partial ? pick(bits, per, std::true_type{}) : pick(bits, per, std::false_type{}); };
+  auto sized = [&](auto bits) {
+    return tiles_per_block == 1 ? with(bits, std::integral_constant<int, 1>{}) : with(bits, std::integral_constant<int, 2>{});
+  };
+  return int4 ? sized(std::integral_constant<int, 4>{}) : sized(std::integral_constant<int, 8>{});
+}
+
+Plan plan_prompt(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
+  return plan_tiles(static_cast<long long>(max_seqlen) * (heads / kv_heads), static_cast<long long>(batch) * kv_heads, (static_cast<long long>(max_length) + kPage - 1) / kPage);
+}
+Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
+  return plan_tiles(static_cast<long long>(batch) * (heads / kv_heads), kv_heads, shared_blocks);
+}
+
+}  // namespace
+
+size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
+  if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  const Plan pl = plan_prompt(batch, max_seqlen, max_length, heads, kv_heads);
+  return pl.nsplit > 1 ? part_bytes(static_cast<long long>(num_tokens) * heads, pl.nsplit) : 0;
+}
+
+int paged_prompt_attention(const PagedAttnArgs& a) {
+  if (a.batch == 0 || a.num_tokens == 0 || a.max_seqlen == 0) return QS_OK;
+  const Plan pl = plan_prompt(a.batch, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
+  TileParams p{};
+  p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
+  p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths;
+  p.batch = a.batch; p.num_tokens = a.num_tokens; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
+  p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const long long rows = static_cast<long long>(a.num_tokens) * a.num_heads;
+  if (pl.nsplit > 1) {
+    QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.nsplit), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
+               part_bytes(rows, pl.nsplit));
+    p.part = static_cast<float*>(a.workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.nsplit * kD);
+  }
+  const int rc = tiles(p, a.cache.int4, pl.tiles, pl.nsplit > 1, a.batch, a.stream);
+  if (rc || pl.nsplit == 1) return rc;
+  return launch(join_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a.stream, "paged_prompt_attention: join", 1, p);
+}
+
+size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_heads) {
+  if (batch <= 0 || shared_blocks <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  return part_bytes(static_cast<long long>(batch) * heads, plan_shared(batch, shared_blocks, heads, kv_heads).nsplit);
+}
+
+int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
+  if (a.batch == 0) return QS_OK;
+  const long long rows = static_cast<long long>(a.batch) * a.num_heads;
+  TailParams t{};
+  t.q = static_cast<const __half*>(a.q); t.out = static_cast<__half*>(a.out); t.q_stride = a.q_stride; t.out_stride = a.out_stride;
+  t.kv_pointers = a.cache.kv_pointers; t.lengths = a.cache.lengths; t.max_blocks = a.cache.max_blocks; t.num_heads = a.num_heads;
+  t.num_kv_heads = a.cache.num_kv_heads; t.shared_blocks = shared_blocks; t.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  if (shared_blocks > 0) {
+    const Plan pl = plan_shared(a.batch, shared_blocks, a.num_heads, a.cache.num_kv_heads);
+    QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.nsplit), "shared_prefix_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
+               part_bytes(rows, pl.nsplit));
+    TileParams p{};
+    p.q = t.q; p.q_stride = t.q_stride; p.kv_pointers = t.kv_pointers; p.lengths = t.lengths;
+    p.batch = 1; p.num_tokens = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
+    p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.shared_blocks = shared_blocks; p.scale_log2 = t.scale_log2;
+    p.part = static_cast<float*>(a.workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.nsplit * kD);
+    t.nsplit = pl.nsplit; t.part = p.part; t.part_ml = p.part_ml;
+    const int rc = tiles(p, a.cache.int4, pl.tiles, true, 1, a.stream);
+    if (rc) return rc;
+  }
+  const int group = a.num_heads / t.num_kv_heads, heads_y = t.num_kv_heads * ((group + kMaxG - 1) / kMaxG);
+  // shares of a sequence's pages: as many blocks as the device holds at a time, a page for each warp pair at least
+  const long long slots = static_cast<long long>(num_sms()) * (a.cache.int4 ? 4 : 3), blocks = static_cast<long long>(heads_y) * a.batch;
+  const long long tail_pages = (static_cast<long long>(a.max_length) + kPage - 1) / kPage - shared_blocks;
+  t.cluster = 1;
+  while (t.cluster < kMaxCluster && blocks * t.cluster * 2 <= slots && tail_pages >= 2 * kTailWarps * t.cluster) t.cluster *= 2;
+  const dim3 grid(t.cluster, heads_y, a.batch);
+  auto run = [&](auto bits) {
+    constexpr int kBits = decltype(bits)::value;
+    const int rc = allow_smem<tail_kernel<kBits>>(SliceCfg<kBits>::kSmem, "shared_prefix_attention: shared memory");
+    if (rc) return rc;
+    return launch(tail_kernel<kBits>, grid, 32 * kTailWarps, SliceCfg<kBits>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
+  };
+  return a.cache.int4 ? run(std::integral_constant<int, 4>{}) : run(std::integral_constant<int, 8>{});
+}
+
+}  // namespace qs

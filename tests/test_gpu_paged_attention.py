@@ -1,0 +1,225 @@
+"""Prompt attention over the paged cache and attention behind a shared prefix against the definition in 64 bits."""
+import pytest
+import torch
+
+from qserve_b200 import backend
+from tests.paged_util import D, F64, HALF, PAGE, Cache, attention64, check_attention
+
+pytestmark = pytest.mark.gpu
+SCALE = D ** -0.5
+
+
+def starts(counts, dev):
+    return torch.tensor([sum(counts[:i]) for i in range(len(counts) + 1)], dtype=torch.int32, device=dev)
+
+
+def queries(T, hq, dev, seed=1):
+    return torch.randn(T, hq, D, generator=torch.Generator().manual_seed(seed)).half().to(dev)
+
+
+def prompt64(c, q, new, lens, scale=SCALE):
+    parts, at = [], 0
+    for b, (n, m) in enumerate(zip(new, lens)):
+        limit = torch.arange(m - n, m, device=c.dev)
+        parts.append(attention64(q[at:at + n], c.values(0, b, max(m, 0)), c.values(1, b, max(m, 0)), limit, scale))
+        at += n
+    return [torch.cat(x) for x in zip(*parts)]
+
+
+def run_prompt(c, q, new, **more):
+    return backend.paged_prompt_attention(q, c.table, starts(new, c.dev), c.lengths, max(new), max(c.lens), *c.args, **more)
+
+
+PROMPTS = [  # query heads, key/value heads, new tokens, positions held ahead of them
+    (4, 1, [1], [0]),
+    (8, 2, [1, 1, 1], [0, 63, 64]),
+    (32, 8, [5, 0, 17], [300, 12, 0]),           # a sequence that brings nothing
+    (8, 8, [64, 65, 127], [0, 1, 63]),           # one query head a key/value head
+    (10, 2, [31, 40], [100, 0]),                 # five heads: tiles that end inside a token
+    (16, 1, [9, 20], [511, 77]),
+    (14, 2, [33], [129]),                        # seven heads
+    (32, 8, [200, 129, 3], [70, 0, 640]),        # two tiles a block
+    (4, 4, [257], [0]),
+    (32, 8, [3], [5000]),                        # few rows: the keys are split
+    (8, 2, [40, 7], [4000, 3001]),
+    (8, 2, [300], [2000]),                       # two tiles a block, split
+]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,new,ahead", PROMPTS)
+def test_prompt(dev, bits, hq, hkv, new, ahead):
+    lens = [n + m for n, m in zip(new, ahead)]
+    c = Cache(lens, hkv, bits, dev, seed=sum(lens) + hq)
+    q = queries(sum(new), hq, dev)
+    check_attention(run_prompt(c, q, new), prompt64(c, q, new, lens), SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_prompt_sharp_scores(dev, bits):
+    """Queries ten times as large: a few keys take all the weight, maxima grow along the walk."""
+    new, lens = [70, 20], [1500, 333]
+    c = Cache(lens, 2, bits, dev, seed=5)
+    q = queries(90, 8, dev) * 10
+    check_attention(run_prompt(c, q, new, softmax_scale=0.05), prompt64(c, q, new, lens, 0.05), 0.05)
+
+
+def shared64(c, q, lens, scale=SCALE):
+    parts = [attention64(q[b:b + 1], c.values(0, b, m), c.values(1, b, m), torch.tensor([m - 1], device=c.dev), scale) for b, m in enumerate(lens)]
+    return [torch.cat(x) for x in zip(*parts)]
+
+
+SHARED = [  # query heads, key/value heads, shared pages, positions of the sequences
+    (4, 1, 1, [65]),
+    (8, 2, 0, [1, 64, 65, 200]),                 # nothing shared
+    (32, 8, 4, [300, 257, 256, 700]),            # one sequence that ends with the prefix
+    (8, 8, 16, [1025, 1100, 1024 + 640]),
+    (10, 2, 7, [449, 500, 460, 451, 470]),
+    (40, 2, 3, [200, 300]),                      # twenty heads a key/value head: three groups of the tail kernel
+    (32, 8, 10, [700] * 20 + [641] * 20),        # two tiles a block
+    (64, 64, 2, [130, 5000]),                    # long pages of one's own: clusters
+    (4, 1, 33, [2113, 9000]),
+    (32, 8, 5, [0, 100, 320, 321, 7, 400]),      # empty, and shorter than the prefix
+    (16, 1, 300, [19201, 19300]),                # many splits
+]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,shared,lens", SHARED)
+def test_shared(dev, bits, hq, hkv, shared, lens):
+    c = Cache(lens, hkv, bits, dev, shared=shared, seed=sum(lens) + hq)
+    q = queries(len(lens), hq, dev)
+    out = backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args)
+    check_attention(out, shared64(c, q, lens), SCALE)
+    assert all(bool((out[b] == 0).all()) for b, n in enumerate(lens) if n == 0)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_shared_is_the_prompt_operator_of_single_tokens(dev, bits):
+    """The same batch through both operators; where the whole prefix lies in a sequence's table nothing has to be said about it."""
+    lens = [900, 1030, 961, 1500]
+    c = Cache(lens, 2, bits, dev, shared=14, seed=3)
+    q = queries(4, 8, dev)
+    want = shared64(c, q, lens)
+    for out in (backend.shared_prefix_attention(q, c.table, c.lengths, 14, max(lens), *c.args),
+                backend.shared_prefix_attention(q, c.table, c.lengths, 3, max(lens), *c.args),
+                backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, max(lens), *c.args)):
+        check_attention(out, want, SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("new,ahead", [([70], [10]), ([6], [2600])])
+def test_a_key_that_is_no_number_reaches_the_rows_that_see_it(dev, bits, new, ahead):
+    """The keys of three positions of the portion get a scale that is no number, or a value's: rows ahead of them are as they were, the others are no numbers."""
+    lens = [n + m for n, m in zip(new, ahead)]
+    for which, at in ((0, 4), (1, 3), (1, 5)):
+        c = Cache(lens, 2, bits, dev, seed=8)
+        q = queries(new[0], 8, dev)
+        want = prompt64(c, q, new, lens)
+        pos = ahead[0] + at
+        c.meta(which)[c.pages[0, pos // PAGE], which ^ 1, :, pos % PAGE] = float("inf") if at == 3 else float("nan")
+        out = run_prompt(c, q, new)
+        check_attention(out[:at], [x[:at] for x in want], SCALE)
+        assert bool(torch.isnan(out[at:]).all())
+
+
+def test_rows_behind_the_batch_and_rows_without_a_position(dev):
+    c = Cache([40, 90], 2, 4, dev, seed=2)
+    new = [10, 20]
+    q = queries(50, 8, dev)
+    out = torch.full((50, 8, D), 7.0, dtype=HALF, device=dev)
+    got = backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, 20, 90, *c.args, out=out)
+    assert got.data_ptr() == out.data_ptr() and bool((out[30:] == 7).all())
+    check_attention(out[:30], prompt64(c, q[:30], new, [40, 90]), SCALE)
+    # split keys: the same
+    out.fill_(7.0)
+    backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, 20, 9000, *c.args, out=out)
+    assert bool((out[30:] == 7).all())
+    check_attention(out[:30], prompt64(c, q[:30], new, [40, 90]), SCALE)
+    # a length smaller than the portion: its first rows have no position
+    c.lengths[0] = 4
+    out = backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, 20, 90, *c.args)
+    assert bool((out[:6] == 0).all())
+    check_attention(out[6:10], prompt64(c, q[6:10], [4], [4]), SCALE)
+
+
+def test_lengths_past_the_tables_stay_inside(dev):
+    """A length that says more than a sequence has pages: the pages are the limit."""
+    c = Cache([128, 128], 2, 8, dev, shared=1, seed=2)
+    q = queries(2, 8, dev)
+    want = shared64(c, q, [128, 128])
+    c.lengths.fill_(100000)
+    check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, 1, 100000, *c.args), want, SCALE)
+    check_attention(backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 100000, *c.args), want, SCALE)
+
+
+def test_strides_and_results_in_place(dev):
+    lens = [300, 180, 700]
+    c = Cache(lens, 2, 4, dev, shared=2, seed=11)
+    rows = torch.randn(3, 5 + 8 + 3, D, generator=torch.Generator().manual_seed(2)).half().to(dev)
+    q = rows[:, 5:13]
+    want = shared64(c, q, lens)
+    wide = torch.zeros(3, 11, D, dtype=HALF, device=dev)
+    backend.shared_prefix_attention(q, c.table, c.lengths, 2, 700, *c.args, out=wide[:, 2:10])
+    check_attention(wide[:, 2:10], want, SCALE)
+    assert bool((wide[:, :2] == 0).all()) and bool((wide[:, 10:] == 0).all())
+    wide.zero_()
+    backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 700, *c.args, out=wide[:, 2:10])
+    check_attention(wide[:, 2:10], want, SCALE)
+    keep = rows.clone()
+    backend.shared_prefix_attention(q, c.table, c.lengths, 2, 700, *c.args, out=q)
+    check_attention(rows[:, 5:13], want, SCALE)
+    rows.copy_(keep)
+    backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 700, *c.args, out=q)
+    check_attention(rows[:, 5:13], want, SCALE)
+
+
+def test_two_graphs_at_once_and_again(dev):
+    """Two captured calls, replayed on two streams at a time, and the same bits every time."""
+    cases = []
+    for seed, lens in ((1, [3000, 2900, 3100]), (2, [2800, 3300])):
+        c = Cache(lens, 2, 4, dev, shared=30, seed=seed)
+        q = queries(len(lens), 8, dev, seed)
+        call = lambda c=c, q=q, lens=lens: (backend.shared_prefix_attention(q, c.table, c.lengths, 30, max(lens), *c.args),  # noqa: E731
+                                            backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, max(lens), *c.args))
+        eager = call()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = call()
+        cases.append((graph, stream, out, eager, call))  # with the call its inputs: a graph does not keep them
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for graph, stream, *_ in cases:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, out, eager, _ in cases:
+        assert all(torch.equal(a, b) for a, b in zip(out, eager))
+
+
+def test_lengths_change_between_replays(dev):
+    """A captured step whose lengths grow: what the tables say at the time of the replay counts."""
+    lens = [640, 700]
+    c = Cache([1000, 1000], 2, 8, dev, shared=9, seed=4)
+    c.lengths.copy_(torch.tensor(lens, dtype=torch.int32))
+    q = queries(2, 8, dev)
+    backend.shared_prefix_attention(q, c.table, c.lengths, 9, 1000, *c.args)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.lengths.add_(1)
+        out = backend.shared_prefix_attention(q, c.table, c.lengths, 9, 1000, *c.args)
+    for step in range(1, 4):
+        graph.replay()
+        check_attention(out, shared64(c, q, [n + step for n in lens]), SCALE)
+
+
+def test_empty_calls(dev):
+    c = Cache([64, 64], 2, 4, dev)
+    q = queries(0, 8, dev)
+    none = torch.zeros(0, 2, 1, dtype=torch.int64, device=dev)
+    zero = torch.zeros(0, dtype=torch.int32, device=dev)
+    assert backend.paged_prompt_attention(q, c.table, starts([0, 0], dev), c.lengths, 0, 64, *c.args).shape == (0, 8, D)
+    assert backend.shared_prefix_attention(q, none, zero, 0, 0, *c.args).shape == (0, 8, D)
+    assert backend.paged_prompt_attention(q, none, torch.zeros(1, dtype=torch.int32, device=dev), zero, 0, 0, *c.args).shape == (0, 8, D)
