@@ -35,19 +35,33 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uin
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
       :
-      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
       :
-      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool live) {  // 16 zeros where not live
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -83,12 +97,20 @@ constexpr int kQBytes = kRows * kD * 2;      // two swizzled halves of 64 column
 constexpr int kKvBytes = kPage * kD * 2;     // a page's K or V as fp16, two halves
 constexpr int kKvHalf = kKvBytes / 2;
 constexpr float kRescale = 8.f;              // log2 units that a row's maximum may grow before O is rescaled
-constexpr uint32_t kTileCols = 256, kColP = 64, kColO = 128;  // of a tile's tensor memory columns: S [0, 64), P [64, 96), O [128, 256)
+// Of a tile's tensor memory columns: S and then P of even pages [0, 64), of odd pages [64, 128), O [128, 256).  A page's P takes the place of its own S, so the next
+// page's S is there before this one's softmax ends, and P waits for no product.
+constexpr uint32_t kTileCols = 256, kColO = 128;
+
+// Registers per thread that the three warpgroups of a one-tile block trade for the launch's 80 (two blocks per multiprocessor): the softmax's increase waits until
+// its share is free, for good where the launch brought fewer than all shares together, so the host asks before the first launch.
+constexpr int kSoftmaxRegs = 112, kUnpackRegs = 72, kIssueRegs = 56;
+constexpr bool shares_suffice(int per_thread) { return 3 * per_thread >= kSoftmaxRegs + kUnpackRegs + kIssueRegs; }
 
 template <int BITS, int TILES>
 struct TileCfg {
+  static constexpr bool kShares = TILES == 1;
   static constexpr int kSoftmaxWarps = 4 * TILES;
-  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4 + 1);  // softmax, unpack, issue
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4 + 4);  // softmax, unpack, a warpgroup of which one warp issues products and one copies
   static constexpr int kBlocksPerSm = TILES == 1 ? 2 : 1;
   static constexpr int kKStages = TILES == 1 ? 1 : 2;
   static constexpr int kVStages = TILES == 1 && BITS == 8 ? 1 : 2;
@@ -98,7 +120,7 @@ struct TileCfg {
   static constexpr int kSlotBytes = 2 * kCodes + 512;
   static constexpr int kOffK = TILES * kQBytes, kOffV = kOffK + kKStages * kKvBytes, kOffRaw = kOffV + kVStages * kKvBytes;
   static constexpr int kOffBar = kOffRaw + kSlots * kSlotBytes;
-  static constexpr int kSmem = kOffBar + 256;
+  static constexpr int kSmem = kOffBar + 384;
   static_assert(kSmem * kBlocksPerSm + 1024 * kBlocksPerSm <= 228 * 1024, "shared memory of a multiprocessor");
 };
 
@@ -121,33 +143,40 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   using G = Geom<BITS>;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* bar_q = bar;             // the queries lie in shared memory
-  uint64_t* bar_s = bar + 1;         // [2] a page's S complete
-  uint64_t* bar_read = bar + 3;      // [2] S read: the next one may follow
-  uint64_t* bar_p = bar + 5;         // [2] P written
-  uint64_t* bar_o = bar + 7;         // [2] O += P V retired
-  uint64_t* bar_kfull = bar + 9;     // [2] K unpacked
-  uint64_t* bar_kfree = bar + 11;    // [2] S = Q K^T of all tiles retired
-  uint64_t* bar_vfull = bar + 13;    // [2]
-  uint64_t* bar_vfree = bar + 15;    // [2]
-  uint64_t* bar_raw = bar + 17;      // [kSlots] raw slot landed
-  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar + 26);
+  uint64_t* bar_q = bar;             // [2] a tile's queries lie in shared memory
+  uint64_t* bar_s = bar + 2;         // [2][2] tile, page parity: S complete
+  uint64_t* bar_p = bar + 6;         // [2][2] P written
+  // [2][2] O += P V retired.  Two, as for S and P: who waits for a page's product may be one page ahead of it or find the next one's done as well, and a barrier
+  // that went through two phases looks as if it had gone through none
+  uint64_t* bar_o = bar + 10;
+  uint64_t* bar_kfull = bar + 14;    // [2] K unpacked
+  uint64_t* bar_kfree = bar + 16;    // [2] S = Q K^T of all tiles retired
+  uint64_t* bar_vfull = bar + 18;    // [2]
+  uint64_t* bar_vfree = bar + 20;    // [2]
+  uint64_t* bar_raw = bar + 22;      // [kSlots] raw slot landed
+  uint64_t* bar_used = bar_raw + C::kSlots;  // [kSlots] raw slot unpacked
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar_used + C::kSlots);
+  static_assert((22 + 2 * C::kSlots) * 8 + 4 <= C::kSmem - C::kOffBar, "the barriers' place");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the shuffle: the same in all lanes, also to the compiler)
+  constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4, kCopyWarp = kIssueWarp + TILES;
   if (threadIdx.x == 0) {
-    mbar_init(bar_q, C::kSoftmaxWarps);
     for (int t = 0; t < 2; ++t) {
+      mbar_init(&bar_q[t], 4);
+      mbar_init(&bar_kfull[t], 4);
+      mbar_init(&bar_kfree[t], TILES);
+      mbar_init(&bar_vfull[t], 4);
+      mbar_init(&bar_vfree[t], TILES);
+    }
+    for (int t = 0; t < 4; ++t) {
       mbar_init(&bar_s[t], 1);
-      mbar_init(&bar_read[t], 4);
       mbar_init(&bar_p[t], 4);
       mbar_init(&bar_o[t], 1);
-      mbar_init(&bar_kfull[t], 4);
-      mbar_init(&bar_kfree[t], 1);
-      mbar_init(&bar_vfull[t], 4);
-      mbar_init(&bar_vfree[t], 1);
     }
-    for (int i = 0; i < C::kSlots; ++i) mbar_init(&bar_raw[i], 1);
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&bar_raw[i], 1);
+      mbar_init(&bar_used[i], 4);
+    }
     fence_barrier_init();
   }
   if (warp == kIssueWarp) tmem_alloc<TILES * kTileCols>(s_tmem);
@@ -155,18 +184,18 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  // ---- this block's share ----
+  unsigned idx = blockIdx.x;
+  const int hk = idx % static_cast<unsigned>(p.num_kv_heads);
+  idx /= static_cast<unsigned>(p.num_kv_heads);
+  const int split = idx % static_cast<unsigned>(p.nsplit);
+  idx /= static_cast<unsigned>(p.nsplit);
+  const int b = idx % static_cast<unsigned>(p.batch), rb = p.row_blocks - 1 - static_cast<int>(idx / static_cast<unsigned>(p.batch));  // the last rows see most keys: first
+  const int group = static_cast<unsigned>(p.num_heads) / static_cast<unsigned>(p.num_kv_heads);
   pdl_wait();
   // Only now: what is launched next may read what this kernel's predecessors wrote (the tail kernel does, ahead of its own wait)
   pdl_launch_dependents();
 
-  // ---- this block's rows and pages ----
-  int idx = blockIdx.x;
-  const int hk = idx % p.num_kv_heads;
-  idx /= p.num_kv_heads;
-  const int split = idx % p.nsplit;
-  idx /= p.nsplit;
-  const int b = idx % p.batch, rb = p.row_blocks - 1 - idx / p.batch;  // the last rows see most keys: they are first
-  const int group = p.num_heads / p.num_kv_heads;
   const Portion portion = p.shared_blocks > 0 ? Portion{0, p.num_tokens, 0} : portion_of(p.cu, p.lengths, b, p.num_tokens);
   const int n_rows = portion.count * group;
   const int row_base = rb * (TILES * kRows);
@@ -179,37 +208,14 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     n_keys = any ? min(max(portion.first + last / group + 1, 0), p.max_blocks * kPage) : 0;
   }
   const int n_pages = (n_keys + kPage - 1) / kPage;
-  const int page0 = static_cast<int>(static_cast<long long>(split) * n_pages / p.nsplit);
-  const int n_mine = any ? static_cast<int>(static_cast<long long>(split + 1) * n_pages / p.nsplit) - page0 : 0;
+  // (nsplit <= 128 splits of at most 2^24 pages: 32 bits hold the products)
+  const int page0 = static_cast<int>(static_cast<unsigned>(split) * n_pages / p.nsplit);
+  const int n_mine = any ? static_cast<int>(static_cast<unsigned>(split + 1) * n_pages / p.nsplit) - page0 : 0;
 
   if (warp >= kUnpackWarp && warp < kIssueWarp) {
-    // ===================================== copies and unpacking =====================================
+    // ===================================== unpacking =====================================
+    if constexpr (C::kShares) set_max_regs<false, kUnpackRegs>();
     const int t = threadIdx.x - 32 * kUnpackWarp;
-    const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks;
-    const long long* vptrs = kptrs + p.max_blocks;
-    long long kp = 0, vp = 0;  // lane i of the first of these warps: the pages 32 n + i
-    auto issue = [&](int j) {  // (first warp) page j of this block's into its slot
-      if ((j & 31) == 0 && j + lane < n_mine) {
-        kp = __ldg(kptrs + page0 + j + lane);
-        vp = __ldg(vptrs + page0 + j + lane);
-      }
-      const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp, j & 31));
-      const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp, j & 31));
-      if (lane == 0) {
-        uint8_t* slot = smem + C::kOffRaw + (j % C::kSlots) * C::kSlotBytes;
-        uint64_t* full = &bar_raw[j % C::kSlots];
-        mbar_expect_tx(full, C::kSlotBytes);
-        bulk_copy_g2s(slot, k + G::codes_at(hk), C::kCodes, full);
-        bulk_copy_g2s(slot + C::kCodes, v + G::codes_at(hk), C::kCodes, full);
-        bulk_copy_g2s(slot + C::kMeta, k + G::scales_at(hk, p.num_kv_heads), 128, full);
-        bulk_copy_g2s(slot + C::kMeta + 128, k + G::zeros_at(hk, p.num_kv_heads), 128, full);
-        bulk_copy_g2s(slot + C::kMeta + 256, v + G::scales_at(hk, p.num_kv_heads), 128, full);
-        bulk_copy_g2s(slot + C::kMeta + 384, v + G::zeros_at(hk, p.num_kv_heads), 128, full);
-      }
-      __syncwarp();
-    };
-    if (warp == kUnpackWarp)
-      for (int j = 0; j < min(n_mine, C::kSlots); ++j) issue(j);
     // thread: key t / 2, dims 64 (t % 2) .. + 63.  The odd threads take their words in the other order, so that eight neighbours meet every bank once.
     const int key = t >> 1, part = t & 1;
     const uint32_t row_at = part * kKvHalf + key * 128, swizzle = key & 7;
@@ -272,200 +278,237 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         __syncwarp();
       };
       const int ks_at = j % C::kKStages, vs_at = j % C::kVStages;
+      // (written out for K and for V: one body for both, 870 us became 930 with 4096 tokens behind 12000)
       mbar_wait(&bar_kfree[ks_at], (static_cast<uint32_t>(j / C::kKStages) & 1u) ^ 1u);
       unpack(raw, ks, kc, smem + C::kOffK + ks_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_kfull[ks_at]);
       mbar_wait(&bar_vfree[vs_at], (static_cast<uint32_t>(j / C::kVStages) & 1u) ^ 1u);
       unpack(raw + C::kCodes, vs, vc, smem + C::kOffV + vs_at * kKvBytes);
-      if (lane == 0) mbar_arrive(&bar_vfull[vs_at]);
-      named_bar_sync(1, 128);  // all four warps are done with the slot
-      if (warp == kUnpackWarp && j + C::kSlots < n_mine) issue(j + C::kSlots);
+      if (lane == 0) {
+        mbar_arrive(&bar_vfull[vs_at]);
+        mbar_arrive(&bar_used[slot]);
+      }
     }
-  } else if (warp == kIssueWarp) {
-    // ===================================== products =====================================
-    if (lane == 0 && n_mine > 0) {
-      constexpr uint32_t idesc_qk = idesc_f16(kRows, kPage, 0u), idesc_pv = idesc_f16(kRows, kD, 1u);
-      auto scores = [&](int j, int t) {
-        const int st = j % C::kKStages;
-#pragma unroll
-        for (int ks = 0; ks < kD / 16; ++ks) {
-          const uint64_t a = umma_desc_sw128(smem_u32(smem + t * kQBytes + (ks >> 2) * (kQBytes / 2))) + (ks & 3) * 2;
-          const uint64_t bd = umma_desc_sw128(smem_u32(smem + C::kOffK + st * kKvBytes + (ks >> 2) * kKvHalf)) + (ks & 3) * 2;
-          mma_f16_ss(tmem + t * kTileCols, a, bd, idesc_qk, ks > 0 ? 1u : 0u);
-        }
-        umma_commit(&bar_s[t]);
-        if (t == TILES - 1) umma_commit(&bar_kfree[st]);
-      };
-      auto k_ready = [&](int j) {
-        mbar_wait(&bar_kfull[j % C::kKStages], static_cast<uint32_t>(j / C::kKStages) & 1u);
-        tc_fence_after();
-      };
-      mbar_wait(bar_q, 0);
-      k_ready(0);
-      for (int t = 0; t < TILES; ++t) scores(0, t);
+  } else if (warp >= kIssueWarp) {
+    if constexpr (C::kShares) set_max_regs<false, kIssueRegs>();
+    if (warp == kCopyWarp) {
+      // ===================================== copies: six of a page, a lane each =====================================
+      const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + page0;
+      const long long* vptrs = kptrs + p.max_blocks;
+      long long kp = 0, vp = 0;  // lane i: page 32 n + i
+      // codes, scales, zeros of K (even lanes) and of V
+      const int what = lane >> 1, of_v = lane & 1;
+      const long long from = what == 0 ? G::codes_at(hk) : what == 1 ? G::scales_at(hk, p.num_kv_heads) : G::zeros_at(hk, p.num_kv_heads);
+      const int to = what == 0 ? of_v * C::kCodes : C::kMeta + of_v * 256 + (what - 1) * 128, bytes = what == 0 ? C::kCodes : 128;
       for (int j = 0; j < n_mine; ++j) {
-        if (j + 1 < n_mine) {  // the next page's S, while this one's softmax goes on
-          k_ready(j + 1);
-          for (int t = 0; t < TILES; ++t) {
-            mbar_wait(&bar_read[t], static_cast<uint32_t>(j) & 1u);
-            tc_fence_after();
-            scores(j + 1, t);
-          }
+        if ((j & 31) == 0 && j + lane < n_mine) {
+          kp = __ldg(kptrs + j + lane);
+          vp = __ldg(vptrs + j + lane);
         }
+        const long long k = __shfl_sync(0xffffffffu, kp, j & 31), v = __shfl_sync(0xffffffffu, vp, j & 31);
+        const int slot = j % C::kSlots;
+        mbar_wait(&bar_used[slot], (static_cast<uint32_t>(j / C::kSlots) & 1u) ^ 1u);
+        if (lane == 0) mbar_expect_tx(&bar_raw[slot], C::kSlotBytes);
+        __syncwarp();
+        if (lane < 6) bulk_copy_g2s(smem + C::kOffRaw + slot * C::kSlotBytes + to, reinterpret_cast<const uint8_t*>(of_v ? v : k) + from, bytes, &bar_raw[slot]);
+      }
+    } else if (warp < kCopyWarp && n_mine > 0) {
+      // ===================================== products: a warp per tile, all its lanes in step and one of them issuing =====================================
+      // (a lane that is alone in its branch takes 90 cycles for an instruction's descriptors, twelve of them a page and tile)
+      constexpr uint32_t idesc_qk = idesc_f16(kRows, kPage, 0u), idesc_pv = idesc_f16(kRows, kD, 1u);
+      const int t = warp - kIssueWarp;
+      const bool leader = elect_one();
+      const uint32_t base = smem_u32(smem), cols = tmem + t * kTileCols;
+      const uint64_t q_desc = umma_desc_sw128(base + t * kQBytes), k_desc = umma_desc_sw128(base + C::kOffK), v_desc = desc_sw128_mn(base + C::kOffV, kKvHalf);
+      auto scores = [&](int j) {
+        const int st = j % C::kKStages;
+        mbar_wait(&bar_kfull[st], static_cast<uint32_t>(j / C::kKStages) & 1u);
+        // over the P of the page before the one before, once that has been taken
+        if (j >= 2) mbar_wait(&bar_o[t * 2 + (j & 1)], static_cast<uint32_t>((j - 2) >> 1) & 1u);
+        tc_fence_after();
+        if (leader) {
+          const uint64_t kd = k_desc + static_cast<uint64_t>(st * (kKvBytes >> 4));
+          const uint32_t to = cols + (j & 1) * kPage;
+#pragma unroll
+          for (int ks = 0; ks < kD / 16; ++ks)
+            mma_f16_ss(to, q_desc + ((ks >> 2) * (kQBytes / 2 >> 4) + (ks & 3) * 2), kd + ((ks >> 2) * (kKvHalf >> 4) + (ks & 3) * 2), idesc_qk, ks > 0 ? 1u : 0u);
+          umma_commit(&bar_s[t * 2 + (j & 1)]);
+          umma_commit(&bar_kfree[st]);
+        }
+        __syncwarp();
+      };
+      mbar_wait(&bar_q[t], 0);
+      scores(0);
+      if (n_mine > 1) scores(1);
+      for (int j = 0; j < n_mine; ++j) {
         const int st = j % C::kVStages;
         mbar_wait(&bar_vfull[st], static_cast<uint32_t>(j / C::kVStages) & 1u);
-        for (int t = 0; t < TILES; ++t) {
-          mbar_wait(&bar_p[t], static_cast<uint32_t>(j) & 1u);
-          tc_fence_after();
+        mbar_wait(&bar_p[t * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u);
+        tc_fence_after();
+        if (leader) {
+          const uint64_t vd = v_desc + static_cast<uint64_t>(st * (kKvBytes >> 4));
+          const uint32_t from = cols + (j & 1) * kPage;
 #pragma unroll
-          for (int kk = 0; kk < kPage / 16; ++kk) {
-            const uint64_t bd = desc_sw128_mn(smem_u32(smem + C::kOffV + st * kKvBytes + kk * 2048), kKvHalf);
-            mma_f16_ts(tmem + t * kTileCols + kColO, tmem + t * kTileCols + kColP + kk * 8, bd, idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
-          }
-          umma_commit(&bar_o[t]);
-          if (t == TILES - 1) umma_commit(&bar_vfree[st]);
+          for (int kk = 0; kk < kPage / 16; ++kk) mma_f16_ts(cols + kColO, from + kk * 8, vd + kk * (2048 >> 4), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&bar_o[t * 2 + (j & 1)]);
+          umma_commit(&bar_vfree[st]);
         }
+        __syncwarp();
+        if (j + 2 < n_mine) scores(j + 2);
       }
     }
-  } else if (any) {
+  } else {
     // ===================================== queries, softmax, results: thread = row =====================================
+    if constexpr (C::kShares) set_max_regs<true, kSoftmaxRegs>();
     const int tile = warp >> 2, quarter = warp & 3;
     const int first_row = row_base + tile * kRows + quarter * 32;
-    {
-      // half a warp a row, 16 bytes a lane
+    const bool alive = first_row < n_rows;  // warp-uniform; a warp without rows lets its part of Q, S and P be what it is
+    const int r = first_row + lane, tok = r / group, head = hk * group + r - tok * group;
+    const bool row_is = r < n_rows;
+    if (alive) {
+      // half a warp a row, 16 bytes a lane, all rows on their way together; where a row begins is worked out by the lane whose row it is
       uint8_t* dst = smem + tile * kQBytes;
       const int c = lane & 15;
-#pragma unroll 4
-      for (int k = 0; k < 32; k += 2) {
-        const int in_tile = quarter * 32 + k + (lane >> 4), r = first_row + k + (lane >> 4);
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (r < n_rows) {
-          const int tok = r / group, head = hk * group + (r - tok * group);
-          x = __ldg(reinterpret_cast<const uint4*>(p.q + (portion.start + tok) * p.q_stride + static_cast<long long>(head) * kD) + c);
-        }
+      const unsigned long long mine = row_is ? reinterpret_cast<unsigned long long>(p.q + (portion.start + tok) * p.q_stride + static_cast<long long>(head) * kD) : 0ull;
+      uint4 x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const uint4* row = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, mine, 2 * k + (lane >> 4)));
+        x[k] = row ? __ldg(row + c) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int in_tile = quarter * 32 + 2 * k + (lane >> 4);
         if constexpr (BITS == 4)  // the order in which the keys' dims are unpacked
-          x = make_uint4(__byte_perm(x.x, x.z, 0x5410), __byte_perm(x.x, x.z, 0x7632), __byte_perm(x.y, x.w, 0x5410), __byte_perm(x.y, x.w, 0x7632));
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kQBytes / 2) + in_tile * 128 + (((c & 7) ^ (in_tile & 7)) << 4)) = x;
+          x[k] = make_uint4(__byte_perm(x[k].x, x[k].z, 0x5410), __byte_perm(x[k].x, x[k].z, 0x7632), __byte_perm(x[k].y, x[k].w, 0x5410),
+                            __byte_perm(x[k].y, x[k].w, 0x7632));
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (kQBytes / 2) + in_tile * 128 + (((c & 7) ^ (in_tile & 7)) << 4)) = x[k];
       }
       fence_proxy_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_q);
     }
-    const int r = first_row + lane;
-    const int tok = r / group, head = hk * group + (r - tok * group);
-    int limit = -1;  // the last position that the row sees
-    if (r < n_rows) limit = p.shared_blocks > 0 ? min(__ldg(p.lengths + tok), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
-    int lowest = limit;  // of the warp's rows
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar_q[tile]);
+    // the last position that the row sees, and the lowest of the warp's rows (one that is no row: its numbers go nowhere)
+    int limit = n_keys - 1;
+    if (row_is) limit = p.shared_blocks > 0 ? min(__ldg(p.lengths + tok), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
+    int lowest = limit;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, m));
-    const uint32_t t_s = tmem + tile * kTileCols + (static_cast<uint32_t>(quarter * 32) << 16), t_p = t_s + kColP, t_o = t_s + kColO;
+    const uint32_t t_s = tmem + tile * kTileCols + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + kColO;
     float m_used = -CUDART_INF_F, l = 0.f;  // what O and the sum are expressed against (log2 units)
     for (int j = 0; j < n_mine; ++j) {
-      const uint32_t ph = static_cast<uint32_t>(j) & 1u;
+      const uint32_t s_at = t_s + (j & 1) * kPage;
       uint32_t x[2][32], w[32];
-      mbar_wait(&bar_s[tile], ph);
+      mbar_wait(&bar_s[tile * 2 + (j & 1)], static_cast<uint32_t>(j >> 1) & 1u);
       tc_fence_after();
-      tmem_ld_32x32b_x32(t_s, x[0]);
-      tmem_ld_32x32b_x32(t_s + 32, x[1]);
-      tmem_wait_ld();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_read[tile]);
-      const int key0 = (page0 + j) * kPage;
-      if (key0 + kPage - 1 > lowest) {  // warp-uniform
+      if (alive) {
+        tmem_ld_32x32b_x32(s_at, x[0]);
+        tmem_ld_32x32b_x32(s_at + 32, x[1]);
+        tmem_wait_ld();
+        const int key0 = (page0 + j) * kPage;
+        if (key0 + kPage - 1 > lowest) {  // warp-uniform
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (key0 + c * 32 + i > limit) x[c][i] = 0xff800000u;  // -inf
+        }
+        float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (key0 + c * 32 + i > limit) x[c][i] = 0xff800000u;  // -inf
-      }
-      float top[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[c][i]));
-      const float m_page = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * p.scale_log2;
-      auto retired = [&]() {  // the O += P V before
-        mbar_wait(&bar_o[tile], ph ^ 1u);
-        tc_fence_after();
-      };
-      if (j == 0) {
-        m_used = m_page;
-      } else {
-        const bool grow = m_page - m_used > kRescale;  // also from -inf; a row that has seen nothing yet and sees nothing here: NaN, no
-        if (__any_sync(0xffffffffu, grow)) {
-          retired();
-          const float m_new = grow ? m_page : m_used;
-          const float alpha = grow ? ex2(m_used - m_new) : 1.f;
+          for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
+        const float m_page = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
+        if (j == 0) {
+          m_used = m_page;
+        } else {
+          const bool grow = m_page - m_used > kRescale;  // also from -inf; a row that has seen nothing yet and sees nothing here: NaN, no
+          if (__any_sync(0xffffffffu, grow)) {
+            mbar_wait(&bar_o[tile * 2 + ((j - 1) & 1)], static_cast<uint32_t>((j - 1) >> 1) & 1u);  // the O += P V before
+            tc_fence_after();
+            const float m_new = grow ? m_page : m_used;
+            const float alpha = grow ? ex2(m_used - m_new) : 1.f;
 #pragma unroll 1
-          for (int c = 0; c < kD / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(t_o + c * 32, o);
-            tmem_wait_ld();
+            for (int c = 0; c < kD / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32b_x32(t_o + c * 32, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st_x32(t_o + c * 32, o);
+              for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+              tmem_st_x32(t_o + c * 32, o);
+            }
+            l *= alpha;
+            m_used = m_new;
           }
-          l *= alpha;
-          m_used = m_new;
         }
-      }
-      const float m_ref = m_used == -CUDART_INF_F ? 0.f : m_used;  // a row without any key so far: its weights are exp2(-inf) = 0
+        const float m_ref = m_used == -CUDART_INF_F ? 0.f : m_used;  // a row without any key so far: its weights are exp2(-inf) = 0
+        const f2 scale2 = pack2(p.scale_log2, p.scale_log2), m2 = pack2(-m_ref, -m_ref);
+        f2 sum[2] = {pack2(l, 0.f), pack2(0.f, 0.f)};
 #pragma unroll
-      for (int i = 0; i < 64; i += 2) {
-        const float p0 = ex2(fmaf(__uint_as_float(x[i >> 5][i & 31]), p.scale_log2, -m_ref));
-        const float p1 = ex2(fmaf(__uint_as_float(x[i >> 5][(i & 31) + 1]), p.scale_log2, -m_ref));
-        const __half2 h = __floats2half2_rn(p0, p1);
-        const float2 f = __half22float2(h);  // the sum is that of the rounded weights: numerator and denominator agree
-        l += f.x + f.y;
-        w[i >> 1] = as_u32(h);
+        for (int i = 0; i < 64; i += 2) {
+          const float2 e = unpack2(fma2(pack2(__uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1])), scale2, m2));
+          const float p0 = ex2(e.x), p1 = ex2(e.y);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pack2(p0, p1));
+          w[i >> 1] = as_u32(__floats2half2_rn(p0, p1));
+        }
+        const float2 two = unpack2(add2(sum[0], sum[1]));
+        l = two.x + two.y;
+        tmem_st_x32(s_at, w);
+        tmem_wait_st();
       }
-      if (j > 0) retired();
-      tmem_st_x32(t_p, w);
-      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_p[tile]);
+      if (lane == 0) mbar_arrive(&bar_p[tile * 2 + (j & 1)]);
     }
-    if (n_mine > 0) {
-      mbar_wait(&bar_o[tile], static_cast<uint32_t>(n_mine - 1) & 1u);
+    if (alive) {
+      if (n_mine > 0) mbar_wait(&bar_o[tile * 2 + ((n_mine - 1) & 1)], static_cast<uint32_t>((n_mine - 1) >> 1) & 1u);
       tc_fence_after();
-    }
-    const bool store = r < n_rows;
-    const long long token = portion.start + tok;
-    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
-    const long long at = (token * p.num_heads + head) * p.nsplit + split;
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
+      // Through shared memory (the tile's queries are done with), so that half a warp stores 256 bytes of a row: a whole row of fp16, or half a partial one
+      uint8_t* mine = smem + tile * kQBytes + quarter * (kQBytes / 4);
+      const long long token = portion.start + tok, at = (token * p.num_heads + head) * p.nsplit + split;
+      unsigned long long to = 0ull;
+      if (row_is) to = PARTIAL ? reinterpret_cast<unsigned long long>(p.part + at * kD)
+                               : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
 #pragma unroll 1
-    for (int c = 0; c < kD / 32; ++c) {
-      uint32_t o[32];
-      if (n_mine > 0) {
-        tmem_ld_32x32b_x32(t_o + c * 32, o);
-        tmem_wait_ld();
-      } else {
+      for (int part = 0; part < (PARTIAL ? 2 : 1); ++part) {
+#pragma unroll 1
+        for (int c = 0; c < (PARTIAL ? 2 : 4); ++c) {
+          uint32_t o[32];
+          if (n_mine > 0) {
+            tmem_ld_32x32b_x32(t_o + part * 64 + c * 32, o);
+            tmem_wait_ld();
+          } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = 0u;
-      }
-      if (!store) continue;
+            for (int i = 0; i < 32; ++i) o[i] = 0u;
+          }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float f[8];
+          for (int e = 0; e < 4; ++e) {
+            float f[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]);
-        if constexpr (PARTIAL) {
-          float4* dst = reinterpret_cast<float4*>(p.part + at * kD + c * 32 + e * 8);
-          dst[0] = make_float4(f[0], f[1], f[2], f[3]);
-          dst[1] = make_float4(f[4], f[5], f[6], f[7]);
-        } else {
-          uint4 y;
-          y.x = as_u32(__floats2half2_rn(f[0] * inv, f[1] * inv));
-          y.y = as_u32(__floats2half2_rn(f[2] * inv, f[3] * inv));
-          y.z = as_u32(__floats2half2_rn(f[4] * inv, f[5] * inv));
-          y.w = as_u32(__floats2half2_rn(f[6] * inv, f[7] * inv));
-          *reinterpret_cast<uint4*>(p.out + token * p.out_stride + static_cast<long long>(head) * kD + c * 32 + e * 8) = y;
+            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]);
+            auto put = [&](int chunk, uint4 v) { *reinterpret_cast<uint4*>(mine + lane * 256 + ((chunk ^ (lane & 7)) << 4)) = v; };
+            if constexpr (PARTIAL) {
+              put(c * 8 + 2 * e, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
+              put(c * 8 + 2 * e + 1, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])));
+            } else {
+              put(c * 4 + e, make_uint4(as_u32(__floats2half2_rn(f[0] * inv, f[1] * inv)), as_u32(__floats2half2_rn(f[2] * inv, f[3] * inv)),
+                                        as_u32(__floats2half2_rn(f[4] * inv, f[5] * inv)), as_u32(__floats2half2_rn(f[6] * inv, f[7] * inv))));
+            }
+          }
         }
+        __syncwarp();
+#pragma unroll 4
+        for (int k = 0; k < 32; k += 2) {
+          const int in = k + (lane >> 4), chunk = lane & 15;
+          uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
+          if (row) row[part * 16 + chunk] = v;
+        }
+        __syncwarp();
       }
+      if (PARTIAL && row_is) p.part_ml[at] = make_float2(m_used, l);
     }
-    if (PARTIAL && store) p.part_ml[at] = make_float2(m_used, l);
   }
   tc_fence_before();
   __syncthreads();
@@ -546,12 +589,6 @@ struct SliceCfg {
   }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t smem) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(smem) : "memory");
 }
@@ -890,27 +927,33 @@ __global__ void __launch_bounds__(32 * kTailWarps, BITS == 4 ? 4 : 3) tail_kerne
 // ------------------------------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------------------------------
-template <auto Kern>
-int allow_smem(int bytes, const char* what) {
+template <auto Kern, typename Enough>
+int allow_smem(int bytes, const char* what, Enough enough) {
   static bool done[kMaxDevices] = {};  // of this kernel
   bool& d = done[device_ordinal()];
   if (d) return QS_OK;
+  cudaFuncAttributes attr{};
+  const int ra = check_cuda(cudaFuncGetAttributes(&attr, Kern), what);
+  if (ra) return ra;
+  QS_REQUIRE(enough(attr.numRegs), "%s: %d registers per thread are fewer than the warpgroups share out", what, attr.numRegs);
   const int rc = check_cuda(cudaFuncSetAttribute(Kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what);
   if (rc == QS_OK) d = true;
   return rc;
 }
 
-// How a call over `rows` rows per kv head and sequence and at most `pages` pages is cut: tiles per block and splits of the pages
+// How a call over `rows` rows per kv head and sequence and at most `pages` pages is cut: tiles per block and splits of the pages, as many as fit the device at a
+// time with `least` pages each.  One page where join_kernel follows (17 tokens behind 500 x 32 heads: four pages 13.3 us, two 12.4, one 11.2), two where the tail
+// kernel's few warps join (8 sequences, 1024 shared positions: four 12.0 us, two 9.8, one 10.4).
 struct Plan {
   int tiles, row_blocks, nsplit;
 };
-Plan plan_tiles(long long rows, long long items, long long pages) {
+Plan plan_tiles(long long rows, long long items, long long pages, int least) {
   Plan pl;
   pl.tiles = rows <= kRows ? 1 : 2;
   pl.row_blocks = static_cast<int>((rows + pl.tiles * kRows - 1) / (pl.tiles * kRows));
   const long long blocks = items * pl.row_blocks, slots = static_cast<long long>(num_sms()) * (pl.tiles == 1 ? 2 : 1);
   long long n = blocks > 0 ? slots / blocks : 1;
-  const long long most = pages / 4;  // a split has at least four pages
+  const long long most = pages / least;
   if (n > most) n = most;
   if (n < 1) n = 1;
   if (n > 128) n = 128;
@@ -922,7 +965,7 @@ size_t part_bytes(long long rows, int nsplit) { return static_cast<size_t>(rows)
 template <int BITS, int TILES, bool PARTIAL>
 int run_tiles(const TileParams& p, int batch_items, void* stream) {
   using C = TileCfg<BITS, TILES>;
-  const int rc = allow_smem<tile_kernel<BITS, TILES, PARTIAL>>(C::kSmem, "paged attention: shared memory");
+  const int rc = allow_smem<tile_kernel<BITS, TILES, PARTIAL>>(C::kSmem, "paged attention: shared memory", [](int regs) { return !C::kShares || shares_suffice(regs); });
   if (rc) return rc;
   const long long blocks = static_cast<long long>(p.row_blocks) * batch_items * p.nsplit * p.num_kv_heads;
   QS_REQUIRE(blocks <= 0x7fffffffll, "paged attention: %lld blocks", blocks);
@@ -938,10 +981,10 @@ int tiles(const TileParams& p, bool int4, int tiles_per_block, bool partial, int
 }
 
 Plan plan_prompt(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
-  return plan_tiles(static_cast<long long>(max_seqlen) * (heads / kv_heads), static_cast<long long>(batch) * kv_heads, (static_cast<long long>(max_length) + kPage - 1) / kPage);
+  return plan_tiles(static_cast<long long>(max_seqlen) * (heads / kv_heads), static_cast<long long>(batch) * kv_heads, (static_cast<long long>(max_length) + kPage - 1) / kPage, 1);
 }
 Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
-  return plan_tiles(static_cast<long long>(batch) * (heads / kv_heads), kv_heads, shared_blocks);
+  return plan_tiles(static_cast<long long>(batch) * (heads / kv_heads), kv_heads, shared_blocks, 2);
 }
 
 }  // namespace
@@ -1007,7 +1050,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   const dim3 grid(t.cluster, heads_y, a.batch);
   auto run = [&](auto bits) {
     constexpr int kBits = decltype(bits)::value;
-    const int rc = allow_smem<tail_kernel<kBits>>(SliceCfg<kBits>::kSmem, "shared_prefix_attention: shared memory");
+    const int rc = allow_smem<tail_kernel<kBits>>(SliceCfg<kBits>::kSmem, "shared_prefix_attention: shared memory", [](int) { return true; });
     if (rc) return rc;
     return launch(tail_kernel<kBits>, grid, 32 * kTailWarps, SliceCfg<kBits>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
   };
