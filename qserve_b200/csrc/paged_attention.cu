@@ -3,13 +3,14 @@
 //
 // Tile kernel.  The rows of a tile are (token, query head) pairs of one kv head: 128 rows see the same keys, whose codes are unpacked once for all of them.  Per
 // page of 64 keys:
-//     bulk copies     the head's codes, scales and zeros of K and V into a ring of raw slots
-//     unpack          4 warps: codes -> fp16 numbers in the swizzled shared-memory form that the products take (keys past the last row's limit: zeros)
+//     unpack          4 warps: codes, scales and zeros (one tile: from registers that they load a page ahead; two: from a ring of raw slots that bulk copies
+//                     fill) -> fp16 numbers in the swizzled shared-memory form that the products take (keys past the last row's limit: zeros)
 //     S = Q K^T       8 x tcgen05.mma 128 x 64 x 16, accumulators in tensor memory
 //     softmax         4 warps, thread = row (tensor memory lane): running maximum and sum in 32 bits, P = exp2(..) rounded to fp16, into tensor memory
 //     O += P V        4 x tcgen05.mma 128 x 128 x 16, A from tensor memory
-// A long axis of keys is split over blocks where the rows alone do not fill the device; their partial rows (O, maximum, sum, all fp32) are joined by
-// join_kernel (prompts) or by the tail kernel (shared prefix).
+// A long axis of keys is split over blocks where the rows alone do not fill the device.  A split leaves its rows' maximum and sum in fp32 and O / sum in fp16, rounded
+// as a result is (in fp32 they were most of what 64 sequences behind 8192 shared positions move: 32.2 us, now 30.8); join_kernel (prompts) or the tail
+// kernel (shared prefix) joins them in fp32.
 //
 // Tail kernel (shared prefix): the pages behind the shared ones, one block of a cluster per (sequence, kv head, share of its pages), on mma.sync; joins its
 // warps', its cluster's and the prefix's partial rows and writes the result.
@@ -102,21 +103,27 @@ constexpr float kRescale = 8.f;              // log2 units that a row's maximum 
 constexpr uint32_t kTileCols = 256, kColO = 128;
 
 // Registers per thread that the three warpgroups of a one-tile block trade for the launch's 80 (two blocks per multiprocessor): the softmax's increase waits until
-// its share is free, for good where the launch brought fewer than all shares together, so the host asks before the first launch.
-constexpr int kSoftmaxRegs = 112, kUnpackRegs = 72, kIssueRegs = 56;
-constexpr bool shares_suffice(int per_thread) { return 3 * per_thread >= kSoftmaxRegs + kUnpackRegs + kIssueRegs; }
+// its share is free, for good where the launch brought fewer than all shares together, and a decrease may not name more than there are, so the host asks before
+// the first launch.
+constexpr int kSoftmaxRegs = 112, kUnpackRegs = 80, kIssueRegs = 48;
+constexpr bool shares_suffice(int per_thread) {
+  return 3 * per_thread >= kSoftmaxRegs + kUnpackRegs + kIssueRegs && per_thread >= kUnpackRegs && per_thread >= kIssueRegs && per_thread <= kSoftmaxRegs;
+}
 
 template <int BITS, int TILES>
 struct TileCfg {
   static constexpr bool kShares = TILES == 1;
   static constexpr int kSoftmaxWarps = 4 * TILES;
-  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4 + 4);  // softmax, unpack, a warpgroup of which one warp issues products and one copies
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 4 + 4);  // softmax, unpack, a warpgroup of which a warp per tile issues products
   static constexpr int kBlocksPerSm = TILES == 1 ? 2 : 1;
-  static constexpr int kKStages = TILES == 1 ? 1 : 2;
-  static constexpr int kVStages = TILES == 1 && BITS == 8 ? 1 : 2;
-  static constexpr int kSlots = TILES == 1 ? (BITS == 4 ? 3 : 2) : (BITS == 4 ? 8 : 5);  // raw ring
+  static constexpr int kKStages = 2, kVStages = 2;
+  // One tile: the unpacking threads load codes, scales and zeros themselves, a page ahead in registers.  Two: a warp of its own has bulk copies bring them into a ring
+  // of raw slots.  us, ring / registers: 17 tokens behind 500 10.5 / 9.3, 8 sequences behind 1024 shared positions 9.8 / 8.3; 4096 tokens behind 12000 852 / 960 (two tiles
+  // leave the unpacking threads no time for loads).
+  static constexpr bool kRing = TILES == 2;
+  static constexpr int kSlots = kRing ? (BITS == 4 ? 8 : 5) : 0;
   static constexpr int kCodes = Geom<BITS>::kCodes;
-  static constexpr int kMeta = 2 * kCodes;               // K scales, K zeros, V scales, V zeros: 128 bytes each
+  static constexpr int kMeta = 2 * kCodes;               // of a slot: codes of K and V, then K scales, K zeros, V scales, V zeros, 128 bytes each
   static constexpr int kSlotBytes = 2 * kCodes + 512;
   static constexpr int kOffK = TILES * kQBytes, kOffV = kOffK + kKStages * kKvBytes, kOffRaw = kOffV + kVStages * kKvBytes;
   static constexpr int kOffBar = kOffRaw + kSlots * kSlotBytes;
@@ -133,7 +140,7 @@ struct TileParams {
   int batch, num_tokens, max_blocks, num_heads, num_kv_heads;
   int row_blocks, nsplit, shared_blocks;  // shared_blocks > 0: the rows of all sequences over the first sequence's first pages
   float scale_log2;
-  float* part;                            // nsplit > 1: O [rows][nsplit][128], rows = token * num_heads + head
+  __half* part;                           // nsplit > 1: O / sum [rows][nsplit][128], rows = token * num_heads + head
   float2* part_ml;                        // (maximum, sum) [rows][nsplit]
 };
 
@@ -149,33 +156,35 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   // [2][2] O += P V retired.  Two, as for S and P: who waits for a page's product may be one page ahead of it or find the next one's done as well, and a barrier
   // that went through two phases looks as if it had gone through none
   uint64_t* bar_o = bar + 10;
-  uint64_t* bar_kfull = bar + 14;    // [2] K unpacked
-  uint64_t* bar_kfree = bar + 16;    // [2] S = Q K^T of all tiles retired
-  uint64_t* bar_vfull = bar + 18;    // [2]
-  uint64_t* bar_vfree = bar + 20;    // [2]
-  uint64_t* bar_raw = bar + 22;      // [kSlots] raw slot landed
-  uint64_t* bar_used = bar_raw + C::kSlots;  // [kSlots] raw slot unpacked
+  uint64_t* bar_kfull = bar + 14;                     // [stages] K unpacked
+  uint64_t* bar_kfree = bar_kfull + C::kKStages;      // S = Q K^T of all tiles retired
+  uint64_t* bar_vfull = bar_kfree + C::kKStages;
+  uint64_t* bar_vfree = bar_vfull + C::kVStages;
+  uint64_t* bar_raw = bar_vfree + C::kVStages;        // [slots] raw slot landed
+  uint64_t* bar_used = bar_raw + C::kSlots;           // [slots] raw slot read
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar_used + C::kSlots);
-  static_assert((22 + 2 * C::kSlots) * 8 + 4 <= C::kSmem - C::kOffBar, "the barriers' place");
+  static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 4 <= C::kSmem - C::kOffBar, "the barriers' place");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the shuffle: the same in all lanes, also to the compiler)
   constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4, kCopyWarp = kIssueWarp + TILES;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&bar_q[t], 4);
-      mbar_init(&bar_kfull[t], 4);
-      mbar_init(&bar_kfree[t], TILES);
-      mbar_init(&bar_vfull[t], 4);
-      mbar_init(&bar_vfree[t], TILES);
+    }
+    for (int i = 0; i < C::kKStages; ++i) {
+      mbar_init(&bar_kfull[i], 4);
+      mbar_init(&bar_kfree[i], TILES);
+      mbar_init(&bar_vfull[i], 4);
+      mbar_init(&bar_vfree[i], TILES);
+    }
+    for (int i = 0; i < C::kSlots; ++i) {
+      mbar_init(&bar_raw[i], 1);
+      mbar_init(&bar_used[i], 4);
     }
     for (int t = 0; t < 4; ++t) {
       mbar_init(&bar_s[t], 1);
       mbar_init(&bar_p[t], 4);
       mbar_init(&bar_o[t], 1);
-    }
-    for (int i = 0; i < C::kSlots; ++i) {
-      mbar_init(&bar_raw[i], 1);
-      mbar_init(&bar_used[i], 4);
     }
     fence_barrier_init();
   }
@@ -219,15 +228,86 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     // thread: key t / 2, dims 64 (t % 2) .. + 63.  The odd threads take their words in the other order, so that eight neighbours meet every bank once.
     const int key = t >> 1, part = t & 1;
     const uint32_t row_at = part * kKvHalf + key * 128, swizzle = key & 7;
-    for (int j = 0; j < n_mine; ++j) {
+    const long long* ptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + page0;
+    constexpr int kWords = BITS / 2;  // 16-byte words of a thread's 64 codes
+    struct Raw {
+      uint4 k[kWords], v[kWords];
+      __half ks, kz, vs, vz;
+    };
+    // a page's codes, scales and zeros out of the pages ...
+    const long long codes = G::codes_at(hk) + t * (G::kRow / 2), scale = G::scales_at(hk, p.num_kv_heads) + key * 2, zero = G::zeros_at(hk, p.num_kv_heads) + key * 2;
+    long long kp = 0, vp = 0;  // lane i: page 32 n + i
+    auto fetch = [&](Raw& r, int j) {
+      if (j >= n_mine) return;
+      if ((j & 31) == 0 && j + lane < n_mine) {
+        kp = __ldcg(ptrs + j + lane);
+        vp = __ldcg(ptrs + p.max_blocks + j + lane);
+      }
+      const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp, j & 31));
+      const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp, j & 31));
+      r.ks = __ldcg(reinterpret_cast<const __half*>(k + scale));
+      r.kz = __ldcg(reinterpret_cast<const __half*>(k + zero));
+      r.vs = __ldcg(reinterpret_cast<const __half*>(v + scale));
+      r.vz = __ldcg(reinterpret_cast<const __half*>(v + zero));
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) r.k[i] = __ldcg(reinterpret_cast<const uint4*>(k + codes) + (i ^ (part * (kWords / 2))));
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) r.v[i] = __ldcg(reinterpret_cast<const uint4*>(v + codes) + (i ^ (part * (kWords / 2))));
+    };
+    // ... or out of their raw slot
+    auto take = [&](Raw& r, int j) {
       const int slot = j % C::kSlots;
-      const uint8_t* raw = smem + C::kOffRaw + slot * C::kSlotBytes;
+      const uint8_t* from = smem + C::kOffRaw + slot * C::kSlotBytes;
       mbar_wait(&bar_raw[slot], static_cast<uint32_t>(j / C::kSlots) & 1u);
+      const __half* meta = reinterpret_cast<const __half*>(from + C::kMeta) + key;
+      r.ks = meta[0]; r.kz = meta[64]; r.vs = meta[128]; r.vz = meta[192];
+      const uint4* k = reinterpret_cast<const uint4*>(from + t * (G::kRow / 2));
+      const uint4* v = reinterpret_cast<const uint4*>(from + C::kCodes + t * (G::kRow / 2));
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) r.k[i] = k[i ^ (part * (kWords / 2))];
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) r.v[i] = v[i ^ (part * (kWords / 2))];
+    };
+    auto unpack = [&](const uint4 (&raw)[kWords], __half s, __half c, uint8_t* dst) {
+      const __half2 s2 = __half2half2(s), c2 = __half2half2(c);
+      uint8_t* row = dst + row_at;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const int at = i ^ (part * (kWords / 2));
+        const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        auto put = [&](int chunk, const __half2 (&x)[4]) {
+          *reinterpret_cast<uint4*>(row + ((chunk ^ swizzle) << 4)) = make_uint4(as_u32(x[0]), as_u32(x[1]), as_u32(x[2]), as_u32(x[3]));
+        };
+        if constexpr (BITS == 4) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            __half2 u[4];
+            codes_of_word4(words[k], u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = __hfma2(u[e], s2, c2);
+            put(4 * at + k, u);  // dims 0 4 1 5 2 6 3 7 of eight: the queries lie in the same order, O's columns come out in it
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            __half2 lo[2], hi[2];
+            codes_of_word8(words[2 * k], lo);
+            codes_of_word8(words[2 * k + 1], hi);
+            __half2 u[4] = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) u[e] = __hmul2(__hsub2(u[e], c2), s2);
+            put(2 * at + k, u);
+          }
+        }
+      }
+      fence_proxy_async();
+      __syncwarp();
+    };
+    auto step = [&](Raw& raw, int j) {
       // A row of K or V whose scale or zero is no finite number stands for NaN: the key's score is NaN then (and goes where the key is masked), its value 0, so
       // that a weight of 0 in a row that does not see it stays 0.
       const bool live = (page0 + j) * kPage + key < n_keys;
-      const __half* meta = reinterpret_cast<const __half*>(raw + C::kMeta) + key;
-      __half ks = meta[0], kz = meta[64], vs = meta[128], vz = meta[192];
+      __half ks = raw.ks, kz = raw.kz, vs = raw.vs, vz = raw.vz;
       auto endless = [](__half h) { return (__half_as_ushort(h) & 0x7c00u) == 0x7c00u; };
       bool bad = endless(ks) || endless(kz) || endless(vs) || endless(vz);
       __half kc = BITS == 4 ? __hmul(__hneg(ks), kz) : kz, vc = BITS == 4 ? __hmul(__hneg(vs), vz) : vz;
@@ -236,62 +316,31 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         vs = vc = __ushort_as_half(0);
         ks = kc = __ushort_as_half(live ? 0x7fffu : 0);
       }
-      auto unpack = [&](const uint8_t* codes, __half s, __half c, uint8_t* dst) {
-        const __half2 s2 = __half2half2(s), c2 = __half2half2(c);
-        auto put = [&](int chunk, const __half2 (&x)[4]) {
-          *reinterpret_cast<uint4*>(dst + row_at + ((chunk ^ swizzle) << 4)) = make_uint4(as_u32(x[0]), as_u32(x[1]), as_u32(x[2]), as_u32(x[3]));
-        };
-        const uint4* src = reinterpret_cast<const uint4*>(codes + t * (G::kRow / 2));
-        if constexpr (BITS == 4) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 w = src[i ^ part];
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              __half2 u[4];
-              codes_of_word4(words[k], u);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) u[e] = __hfma2(u[e], s2, c2);
-              put(4 * (i ^ part) + k, u);  // dims 0 4 1 5 2 6 3 7 of eight: the queries lie in the same order, O's columns come out in it
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int at = i ^ (2 * part);
-            const uint4 w = src[at];
-            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              __half2 lo[2], hi[2];
-              codes_of_word8(words[2 * k], lo);
-              codes_of_word8(words[2 * k + 1], hi);
-              __half2 u[4] = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-              for (int e = 0; e < 4; ++e) u[e] = __hmul2(__hsub2(u[e], c2), s2);
-              put(2 * at + k, u);
-            }
-          }
-        }
-        fence_proxy_async();
-        __syncwarp();
-      };
       const int ks_at = j % C::kKStages, vs_at = j % C::kVStages;
-      // (written out for K and for V: one body for both, 870 us became 930 with 4096 tokens behind 12000)
       mbar_wait(&bar_kfree[ks_at], (static_cast<uint32_t>(j / C::kKStages) & 1u) ^ 1u);
-      unpack(raw, ks, kc, smem + C::kOffK + ks_at * kKvBytes);
+      unpack(raw.k, ks, kc, smem + C::kOffK + ks_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_kfull[ks_at]);
       mbar_wait(&bar_vfree[vs_at], (static_cast<uint32_t>(j / C::kVStages) & 1u) ^ 1u);
-      unpack(raw + C::kCodes, vs, vc, smem + C::kOffV + vs_at * kKvBytes);
-      if (lane == 0) {
-        mbar_arrive(&bar_vfull[vs_at]);
-        mbar_arrive(&bar_used[slot]);
+      unpack(raw.v, vs, vc, smem + C::kOffV + vs_at * kKvBytes);
+      if (lane == 0) mbar_arrive(&bar_vfull[vs_at]);
+    };
+    Raw raw;
+    if constexpr (C::kRing) {
+      for (int j = 0; j < n_mine; ++j) {
+        take(raw, j);
+        step(raw, j);
+        if (lane == 0) mbar_arrive(&bar_used[j % C::kSlots]);
+      }
+    } else {
+      fetch(raw, 0);
+      for (int j = 0; j < n_mine; ++j) {
+        step(raw, j);
+        fetch(raw, j + 1);
       }
     }
   } else if (warp >= kIssueWarp) {
     if constexpr (C::kShares) set_max_regs<false, kIssueRegs>();
-    if (warp == kCopyWarp) {
+    if (C::kRing && warp == kCopyWarp) {
       // ===================================== copies: six of a page, a lane each =====================================
       const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + page0;
       const long long* vptrs = kptrs + p.max_blocks;
@@ -300,7 +349,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       const int what = lane >> 1, of_v = lane & 1;
       const long long from = what == 0 ? G::codes_at(hk) : what == 1 ? G::scales_at(hk, p.num_kv_heads) : G::zeros_at(hk, p.num_kv_heads);
       const int to = what == 0 ? of_v * C::kCodes : C::kMeta + of_v * 256 + (what - 1) * 128, bytes = what == 0 ? C::kCodes : 128;
-      for (int j = 0; j < n_mine; ++j) {
+      if constexpr (C::kRing) for (int j = 0; j < n_mine; ++j) {
         if ((j & 31) == 0 && j + lane < n_mine) {
           kp = __ldg(kptrs + j + lane);
           vp = __ldg(vptrs + j + lane);
@@ -312,7 +361,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         __syncwarp();
         if (lane < 6) bulk_copy_g2s(smem + C::kOffRaw + slot * C::kSlotBytes + to, reinterpret_cast<const uint8_t*>(of_v ? v : k) + from, bytes, &bar_raw[slot]);
       }
-    } else if (warp < kCopyWarp && n_mine > 0) {
+    } else if (warp < kIssueWarp + TILES && n_mine > 0) {
       // ===================================== products: a warp per tile, all its lanes in step and one of them issuing =====================================
       // (a lane that is alone in its branch takes 90 cycles for an instruction's descriptors, twelve of them a page and tile)
       constexpr uint32_t idesc_qk = idesc_f16(kRows, kPage, 0u), idesc_pv = idesc_f16(kRows, kD, 1u);
@@ -464,48 +513,39 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       if (n_mine > 0) mbar_wait(&bar_o[tile * 2 + ((n_mine - 1) & 1)], static_cast<uint32_t>((n_mine - 1) >> 1) & 1u);
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
-      // Through shared memory (the tile's queries are done with), so that half a warp stores 256 bytes of a row: a whole row of fp16, or half a partial one
+      // Through shared memory (the tile's queries are done with), so that half a warp stores a whole row
       uint8_t* mine = smem + tile * kQBytes + quarter * (kQBytes / 4);
       const long long token = portion.start + tok, at = (token * p.num_heads + head) * p.nsplit + split;
       unsigned long long to = 0ull;
       if (row_is) to = PARTIAL ? reinterpret_cast<unsigned long long>(p.part + at * kD)
                                : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
 #pragma unroll 1
-      for (int part = 0; part < (PARTIAL ? 2 : 1); ++part) {
-#pragma unroll 1
-        for (int c = 0; c < (PARTIAL ? 2 : 4); ++c) {
-          uint32_t o[32];
-          if (n_mine > 0) {
-            tmem_ld_32x32b_x32(t_o + part * 64 + c * 32, o);
-            tmem_wait_ld();
-          } else {
+      for (int c = 0; c < 4; ++c) {
+        uint32_t o[32];
+        if (n_mine > 0) {
+          tmem_ld_32x32b_x32(t_o + c * 32, o);
+          tmem_wait_ld();
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] = 0u;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float f[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]);
-            auto put = [&](int chunk, uint4 v) { *reinterpret_cast<uint4*>(mine + lane * 256 + ((chunk ^ (lane & 7)) << 4)) = v; };
-            if constexpr (PARTIAL) {
-              put(c * 8 + 2 * e, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
-              put(c * 8 + 2 * e + 1, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])));
-            } else {
-              put(c * 4 + e, make_uint4(as_u32(__floats2half2_rn(f[0] * inv, f[1] * inv)), as_u32(__floats2half2_rn(f[2] * inv, f[3] * inv)),
-                                        as_u32(__floats2half2_rn(f[4] * inv, f[5] * inv)), as_u32(__floats2half2_rn(f[6] * inv, f[7] * inv))));
-            }
-          }
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float f[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]) * inv;
+          *reinterpret_cast<uint4*>(mine + lane * 256 + (((c * 4 + e) ^ (lane & 7)) << 4)) =
+              make_uint4(as_u32(__floats2half2_rn(f[0], f[1])), as_u32(__floats2half2_rn(f[2], f[3])), as_u32(__floats2half2_rn(f[4], f[5])),
+                         as_u32(__floats2half2_rn(f[6], f[7])));
+        }
+      }
+      __syncwarp();
 #pragma unroll 4
-        for (int k = 0; k < 32; k += 2) {
-          const int in = k + (lane >> 4), chunk = lane & 15;
-          uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
-          if (row) row[part * 16 + chunk] = v;
-        }
-        __syncwarp();
+      for (int k = 0; k < 32; k += 2) {
+        const int in = k + (lane >> 4), chunk = lane & 15;
+        uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
+        const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
+        if (row) row[chunk] = v;
       }
       if (PARTIAL && row_is) p.part_ml[at] = make_float2(m_used, l);
     }
@@ -518,7 +558,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 // ------------------------------------------------------------------------------------------------------------------------
 // partial rows of a split joined: a warp, lane = 4 dims.  Returns the sum and the maximum that acc is expressed against.
 // ------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void join_rows(const float* part, const float2* ml, int nsplit, float& M, float& L, float4& acc) {
+__device__ __forceinline__ void join_rows(const __half* part, const float2* ml, int nsplit, float& M, float& L, float4& acc) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < nsplit; s0 += 32) {
     const float2 mine = s0 + lane < nsplit ? __ldcg(ml + s0 + lane) : make_float2(-CUDART_INF_F, 0.f);
@@ -527,7 +567,8 @@ __device__ __forceinline__ void join_rows(const float* part, const float2* ml, i
     for (int k = 16; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     const float m_new = fmaxf(M, m), ref = m_new == -CUDART_INF_F ? 0.f : m_new;
     const float old = ex2(M - ref), w = ex2(mine.x - ref);
-    float sum = mine.y * w;
+    const float weight = mine.y * w;  // of O / sum
+    float sum = weight;
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
     L = fmaf(L, old, sum);
@@ -536,9 +577,10 @@ __device__ __forceinline__ void join_rows(const float* part, const float2* ml, i
     const int n = min(32, nsplit - s0);
 #pragma unroll 8
     for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w, s);
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(part + static_cast<long long>(s0 + s) * kD) + lane);
-      acc.x = fmaf(x.x, ws, acc.x); acc.y = fmaf(x.y, ws, acc.y); acc.z = fmaf(x.z, ws, acc.z); acc.w = fmaf(x.w, ws, acc.w);
+      const float ws = __shfl_sync(0xffffffffu, weight, s);
+      const uint2 x = __ldcg(reinterpret_cast<const uint2*>(part + static_cast<long long>(s0 + s) * kD) + lane);
+      const float2 a = __half22float2(as_h2(x.x)), b = __half22float2(as_h2(x.y));
+      acc.x = fmaf(a.x, ws, acc.x); acc.y = fmaf(a.y, ws, acc.y); acc.z = fmaf(b.x, ws, acc.z); acc.w = fmaf(b.y, ws, acc.w);
     }
   }
 }
@@ -547,19 +589,39 @@ __device__ __forceinline__ uint2 scaled_h4(const float4& a, float L) {
   return make_uint2(as_u32(__floats2half2_rn(a.x * inv, a.y * inv)), as_u32(__floats2half2_rn(a.z * inv, a.w * inv)));
 }
 
-// a warp per row of the result; rows behind the last sequence are left as they are
+// Rows of the result, WARPS warps each (they take turns over the splits); rows behind the last sequence are left as they are.
+template <int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileParams p) {
+  __shared__ __align__(16) float s_acc[4][kD];
+  __shared__ float2 s_ml[4];
   pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long row = static_cast<long long>(blockIdx.x) * (4 / WARPS) + warp / WARPS;
+  const bool in = row < static_cast<long long>(p.num_tokens) * p.num_heads;
+  const int token = in ? static_cast<int>(row / p.num_heads) : 0, head = in ? static_cast<int>(row - static_cast<long long>(token) * p.num_heads) : 0;
   pdl_wait();
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (row >= static_cast<long long>(p.num_tokens) * p.num_heads) return;
-  const int token = static_cast<int>(row / p.num_heads), head = static_cast<int>(row - static_cast<long long>(token) * p.num_heads);
-  if (sequence_of(p.cu, p.batch, token) < 0) return;
+  const bool mine = in && sequence_of(p.cu, p.batch, token) >= 0;
   float M = -CUDART_INF_F, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  join_rows(p.part + row * p.nsplit * kD, p.part_ml + row * p.nsplit, p.nsplit, M, L, acc);
-  reinterpret_cast<uint2*>(p.out + token * p.out_stride + static_cast<long long>(head) * kD)[lane] = scaled_h4(acc, L);
+  // this warp's run of the splits
+  const int part = warp % WARPS, s0 = p.nsplit * part / WARPS, s1 = p.nsplit * (part + 1) / WARPS;
+  if (mine) join_rows(p.part + (row * p.nsplit + s0) * kD, p.part_ml + row * p.nsplit + s0, s1 - s0, M, L, acc);
+  if constexpr (WARPS > 1) {
+    reinterpret_cast<float4*>(s_acc[warp])[lane] = acc;
+    if (lane == 0) s_ml[warp] = make_float2(M, L);
+    __syncthreads();
+    if (!mine || part != 0) return;
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) {
+      const float2 ml = s_ml[warp + w];
+      const float4 x = reinterpret_cast<const float4*>(s_acc[warp + w])[lane];
+      const float m_new = fmaxf(M, ml.x), ref = m_new == -CUDART_INF_F ? 0.f : m_new, old = ex2(M - ref), wt = ex2(ml.x - ref);
+      L = L * old + ml.y * wt;
+      acc.x = fmaf(x.x, wt, acc.x * old); acc.y = fmaf(x.y, wt, acc.y * old); acc.z = fmaf(x.z, wt, acc.z * old); acc.w = fmaf(x.w, wt, acc.w * old);
+      M = m_new;
+    }
+  }
+  if (mine) reinterpret_cast<uint2*>(p.out + token * p.out_stride + static_cast<long long>(head) * kD)[lane] = scaled_h4(acc, L);
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
@@ -627,34 +689,41 @@ struct TailParams {
   long long q_stride, out_stride;
   const long long* kv_pointers;
   const int* lengths;
-  int max_blocks, num_heads, num_kv_heads, shared_blocks, nsplit, cluster;
+  int batch, max_blocks, num_heads, num_kv_heads, shared_blocks, nsplit, cluster;
   float scale_log2;
-  const float* part;
+  const __half* part;
   const float2* part_ml;
 };
 
-template <int BITS>
+// SHARED: a block (and its cluster) per sequence and run of heads, the warps take turns over the slices; otherwise a warp for each of them, which saves the joining of
+// warps where there are enough to fill the device.
+template <int BITS, bool SHARED>
 __global__ void __launch_bounds__(32 * kTailWarps, BITS == 4 ? 4 : 3) tail_kernel(const __grid_constant__ TailParams p) {
   using SC = SliceCfg<BITS>;
   using G = Geom<BITS>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ __align__(16) __half s_q[kMaxG * kD];
+  __shared__ __align__(16) __half s_queries[(SHARED ? 1 : kTailWarps) * kMaxG * kD];
   __shared__ float s_m[kTailWarps][kMaxG], s_l[kTailWarps][kMaxG];
   __shared__ float2 s_meta[kTailWarps][2][kSlice];
-  __shared__ __align__(16) float s_o[kMaxG * kD];        // the block's rows
+  __shared__ __align__(16) float s_o[SHARED ? kMaxG * kD : 4];  // the block's rows
   __shared__ float s_bm[kMaxG], s_bl[kMaxG];
   const int group = p.num_heads / p.num_kv_heads, parts = (group + kMaxG - 1) / kMaxG;
-  const int rank = blockIdx.x, b = blockIdx.z, hk = blockIdx.y / parts, part = blockIdx.y - hk * parts;
-  const int h0 = hk * group + part * kMaxG, heads = min(kMaxG, group - part * kMaxG);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int rank = SHARED ? static_cast<int>(blockIdx.x) : 0;
+  const int run = SHARED ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.x) * kTailWarps + warp;  // not SHARED: of all sequences
+  const int runs = p.num_kv_heads * parts;
+  const int b = SHARED ? static_cast<int>(blockIdx.z) : min(run / runs, p.batch - 1), of_b = SHARED ? run : run % runs;
+  const bool live = SHARED || run < runs * p.batch;  // a warp past the last one walks an empty sequence
+  const int hk = of_b / parts, part = of_b - hk * parts;
+  const int h0 = hk * group + part * kMaxG, heads = live ? min(kMaxG, group - part * kMaxG) : 0;
   pdl_launch_dependents();
   // The tile kernel before this one started this one after its own wait: everything ahead of the tile kernel is there.  Without one, this kernel waits itself.
   if (p.nsplit == 0) pdl_wait();
 
-  const int len = min(__ldcg(p.lengths + b), p.max_blocks * kPage);
+  const int len = live ? min(__ldcg(p.lengths + b), p.max_blocks * kPage) : 0;
   const int slices = max((len - p.shared_blocks * kPage + kSlice - 1) / kSlice, 0);
   // the cluster's blocks and their warps take turns over the slices
-  const int stride = p.cluster * kTailWarps, mine = rank * kTailWarps + warp;
+  const int stride = SHARED ? p.cluster * kTailWarps : 1, mine = SHARED ? rank * kTailWarps + warp : 0;
   const int n_my = slices > mine ? (slices - mine + stride - 1) / stride : 0;
   const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + p.shared_blocks;
   const long long* vptrs = kptrs + p.max_blocks;
@@ -690,13 +759,15 @@ __global__ void __launch_bounds__(32 * kTailWarps, BITS == 4 ? 4 : 3) tail_kerne
     cp_async_commit();
   }
   // ---- the queries: 16 lanes a row ----
-  for (int i = threadIdx.x; i < kMaxG * 16; i += 32 * kTailWarps) {
+  __half* s_q = s_queries + (SHARED ? 0 : warp * kMaxG * kD);
+  for (int i = SHARED ? static_cast<int>(threadIdx.x) : lane; i < kMaxG * 16; i += SHARED ? 32 * kTailWarps : 32) {
     const int r = i >> 4;
     uint4 x = make_uint4(0u, 0u, 0u, 0u);
     if (r < heads) x = __ldcg(reinterpret_cast<const uint4*>(p.q + b * p.q_stride + static_cast<long long>(h0 + r) * kD) + (i & 15));
     reinterpret_cast<uint4*>(s_q)[i] = x;
   }
-  __syncthreads();
+  if constexpr (SHARED) __syncthreads();
+  else __syncwarp();
   // Q as the B operand (n = head g) in the order of the codes: INT4 word w of a lane's 32 dims has nibbles (0, 4 | 1, 5), (2, 6 | 3, 7); INT8 (0, 1 | 2, 3)
   uint32_t qb0[8], qb1[8];
   float sumq0, sumq1;
@@ -877,6 +948,25 @@ __global__ void __launch_bounds__(32 * kTailWarps, BITS == 4 ? 4 : 3) tail_kerne
       so1[16 * i] = fmaf(o[i][1], kUp, c1); so1[16 * i + 8] = fmaf(o[i][3], kOdd, c1);
     }
   }
+  if constexpr (!SHARED) {
+    __syncwarp();
+    if (p.nsplit > 0) pdl_wait();  // the prefix's partial rows
+    for (int r = 0; r < heads; ++r) {
+      const float* row = reinterpret_cast<const float*>(ring) + r * kOPitch;
+      float x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {  // dim 4 lane + k
+        const int d = 4 * lane + k;
+        x[k] = row[BITS == 4 ? (d & ~31) | ((d >> 1 & 1) << 4) | ((d & 1) << 3) | ((d >> 2) & 7) : (d & ~15) | ((d & 1) << 3) | ((d >> 1) & 7)];
+      }
+      float M = s_m[warp][r], L = s_l[warp][r];
+      float4 acc = make_float4(x[0], x[1], x[2], x[3]);
+      const long long at = static_cast<long long>(b) * p.num_heads + h0 + r;
+      if (p.nsplit > 0) join_rows(p.part + at * p.nsplit * kD, p.part_ml + at * p.nsplit, p.nsplit, M, L, acc);
+      reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<long long>(h0 + r) * kD)[lane] = scaled_h4(acc, L);
+    }
+    return;
+  }
   __syncthreads();
   // ---- the block's rows ----
   {
@@ -960,7 +1050,7 @@ Plan plan_tiles(long long rows, long long items, long long pages, int least) {
   pl.nsplit = static_cast<int>(n);
   return pl;
 }
-size_t part_bytes(long long rows, int nsplit) { return static_cast<size_t>(rows) * nsplit * (kD * sizeof(float) + sizeof(float2)); }
+size_t part_bytes(long long rows, int nsplit) { return static_cast<size_t>(rows) * nsplit * (kD * sizeof(__half) + sizeof(float2)); }
 
 template <int BITS, int TILES, bool PARTIAL>
 int run_tiles(const TileParams& p, int batch_items, void* stream) {
@@ -1007,12 +1097,13 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
   if (pl.nsplit > 1) {
     QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.nsplit), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
                part_bytes(rows, pl.nsplit));
-    p.part = static_cast<float*>(a.workspace);
+    p.part = static_cast<__half*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.nsplit * kD);
   }
   const int rc = tiles(p, a.cache.int4, pl.tiles, pl.nsplit > 1, a.batch, a.stream);
   if (rc || pl.nsplit == 1) return rc;
-  return launch(join_kernel, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, a.stream, "paged_prompt_attention: join", 1, p);
+  const bool wide = pl.nsplit >= 8;  // (24 tokens behind 60000, 37 splits: a warp a row 52.8 us, four 48.9; 17 behind 500, nine splits: 11.0 and 10.5)
+  return launch(wide ? join_kernel<4> : join_kernel<1>, dim3(static_cast<unsigned>(wide ? rows : (rows + 3) / 4)), 128, 0, a.stream, "paged_prompt_attention: join", 1, p);
 }
 
 size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_heads) {
@@ -1025,7 +1116,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   const long long rows = static_cast<long long>(a.batch) * a.num_heads;
   TailParams t{};
   t.q = static_cast<const __half*>(a.q); t.out = static_cast<__half*>(a.out); t.q_stride = a.q_stride; t.out_stride = a.out_stride;
-  t.kv_pointers = a.cache.kv_pointers; t.lengths = a.cache.lengths; t.max_blocks = a.cache.max_blocks; t.num_heads = a.num_heads;
+  t.batch = a.batch; t.kv_pointers = a.cache.kv_pointers; t.lengths = a.cache.lengths; t.max_blocks = a.cache.max_blocks; t.num_heads = a.num_heads;
   t.num_kv_heads = a.cache.num_kv_heads; t.shared_blocks = shared_blocks; t.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   if (shared_blocks > 0) {
     const Plan pl = plan_shared(a.batch, shared_blocks, a.num_heads, a.cache.num_kv_heads);
@@ -1035,7 +1126,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
     p.q = t.q; p.q_stride = t.q_stride; p.kv_pointers = t.kv_pointers; p.lengths = t.lengths;
     p.batch = 1; p.num_tokens = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
     p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.shared_blocks = shared_blocks; p.scale_log2 = t.scale_log2;
-    p.part = static_cast<float*>(a.workspace);
+    p.part = static_cast<__half*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.nsplit * kD);
     t.nsplit = pl.nsplit; t.part = p.part; t.part_ml = p.part_ml;
     const int rc = tiles(p, a.cache.int4, pl.tiles, true, 1, a.stream);
@@ -1047,14 +1138,18 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   const long long tail_pages = (static_cast<long long>(a.max_length) + kPage - 1) / kPage - shared_blocks;
   t.cluster = 1;
   while (t.cluster < kMaxCluster && blocks * t.cluster * 2 <= slots && tail_pages >= 2 * kTailWarps * t.cluster) t.cluster *= 2;
-  const dim3 grid(t.cluster, heads_y, a.batch);
-  auto run = [&](auto bits) {
+  const bool shared = blocks < 12 * num_sms();  // (a wave of warps; 128 sequences x 32 heads, INT8, 400 positions each behind 16384: 157 us by blocks, 142 by warps)
+  if (!shared) t.cluster = 1;
+  const dim3 grid = shared ? dim3(t.cluster, heads_y, a.batch) : dim3(static_cast<unsigned>((blocks + kTailWarps - 1) / kTailWarps));
+  auto run = [&](auto bits, auto by_block) {
     constexpr int kBits = decltype(bits)::value;
-    const int rc = allow_smem<tail_kernel<kBits>>(SliceCfg<kBits>::kSmem, "shared_prefix_attention: shared memory", [](int) { return true; });
+    constexpr bool kShared = decltype(by_block)::value;
+    const int rc = allow_smem<tail_kernel<kBits, kShared>>(SliceCfg<kBits>::kSmem, "shared_prefix_attention: shared memory", [](int) { return true; });
     if (rc) return rc;
-    return launch(tail_kernel<kBits>, grid, 32 * kTailWarps, SliceCfg<kBits>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
+    return launch(tail_kernel<kBits, kShared>, grid, 32 * kTailWarps, SliceCfg<kBits>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
   };
-  return a.cache.int4 ? run(std::integral_constant<int, 4>{}) : run(std::integral_constant<int, 8>{});
+  auto with = [&](auto bits) { return shared ? run(bits, std::true_type{}) : run(bits, std::false_type{}); };
+  return a.cache.int4 ? with(std::integral_constant<int, 4>{}) : with(std::integral_constant<int, 8>{});
 }
 
 }  // namespace qs

@@ -7,6 +7,7 @@
 #include <math_constants.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged_common.cuh"
 
@@ -23,52 +24,83 @@ struct Turns {
   double per_position[kD / 2];
 };
 
-// Eight lanes hold a row: lane l of them elements 8 l .. and 64 + 8 l .. as fp32 numbers.
+// Eight lanes hold a row: lane l of them elements 8 l .. and 64 + 8 l .. as fp32 pairs.
+constexpr uint32_t kMagic = 0x4b400000u;  // the bits of 1.5 x 2^23: a sum with it has a small whole number in its low bits, rounded to even
+__device__ __forceinline__ f2 both(float x) { return pack2(x, x); }
+// two products, each rounded: one by one, because the compiler makes a fused operation of a packed product and the sum after it, rounding modifiers or not (7 of 10^6
+// INT8 codes were others than the definition's)
+__device__ __forceinline__ f2 product(f2 a, f2 b) {
+  const float2 x = unpack2(a), y = unpack2(b);
+  return pack2(__fmul_rn(x.x, y.x), __fmul_rn(x.y, y.y));
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float min3_nan(float a, float b, float c) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+// the row's scale and zero and this lane's codes: INT4 word w of dims 64 w + 8 l .., INT8 words 2 w and 2 w + 1
+template <int BITS>
 struct Quantised {
   __half scale, zero;
-  uint32_t code[16];
+  uint32_t word[BITS / 2];
 };
 template <int BITS>
-__device__ __forceinline__ Quantised quantise_row(const float (&x)[16]) {
+__device__ __forceinline__ Quantised<BITS> quantise_row(const f2 (&x)[8]) {
   constexpr float kTop = BITS == 4 ? 15.f : 255.f;
-  float hi = x[0], lo = x[0], poison = 0.f;
+  float hi, lo;
+  {
+    const float2 a = unpack2(x[0]);
+    hi = max3_nan(a.x, a.y, a.y);
+    lo = min3_nan(a.x, a.y, a.y);
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    hi = fmaxf(hi, x[j]);
-    lo = fminf(lo, x[j]);
-    poison = fmaf(x[j], 0.f, poison);  // NaN where the row has a number that is none or has no end
+    for (int j = 1; j < 8; ++j) {
+      const float2 b = unpack2(x[j]);
+      hi = max3_nan(hi, b.x, b.y);
+      lo = min3_nan(lo, b.x, b.y);
+    }
   }
 #pragma unroll
   for (int m = 4; m >= 1; m >>= 1) {
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, m));
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, m));
-    poison += __shfl_xor_sync(0xffffffffu, poison, m);
+    const float h = __shfl_xor_sync(0xffffffffu, hi, m), w = __shfl_xor_sync(0xffffffffu, lo, m);
+    hi = max3_nan(hi, h, h);
+    lo = min3_nan(lo, w, w);
   }
-  Quantised r;
+  Quantised<BITS> r;
   const float span = __fsub_rn(hi, lo);
   r.scale = __float2half_rn(__fdiv_rn(span, kTop));
   r.zero = __float2half_rn(__fdiv_rn(__fmul_rn(-kTop, lo), span));
-  const float s = __half2float(r.scale);
-  float z = __half2float(r.zero);
-  if (poison != 0.f) {  // NaN: the whole row reads as NaN
+  float s = __half2float(r.scale), z = __half2float(r.zero), inv = __fdiv_rn(1.f, s);
+  if (!(span <= 131008.f)) {  // a number that is none, or has no end: the whole row reads as NaN
     r.scale = r.zero = __ushort_as_half(0x7fffu);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) r.code[j] = 0u;
+    inv = z = 0.f;
   } else if (s == 0.f || !(fabsf(z) <= 65504.f)) {
     // values of one kind, or so near to one another that their zero is none in fp16: the middle c of the row, held as 1 x |c| or as 0 - 1 x |c|
     const float c = __half2float(__float2half_rn((hi + lo) * 0.5f));
     r.scale = __float2half_rn(fabsf(c));
     r.zero = __float2half_rn(c < 0.f ? 1.f : 0.f);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) r.code[j] = c > 0.f ? 1u : 0u;
-  } else {
-    const float inv = __fdiv_rn(1.f, s);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      asm("cvt.rni.sat.u8.f32 %0, %1;" : "=r"(r.code[j]) : "f"(__fadd_rn(__fmul_rn(x[j], inv), z)));
-      if constexpr (BITS == 4) r.code[j] = min(r.code[j], 15u);
-    }
+    inv = 0.f;
+    z = c > 0.f ? 1.f : 0.f;
   }
+#pragma unroll
+  for (int k = 0; k < BITS / 2; ++k) r.word[k] = 0u;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    // x / s + z with both roundings, kept to 0 .. top, then to the nearest whole number
+    const float2 t = unpack2(add2(product(x[j], both(inv)), both(z)));
+    const float2 c = unpack2(add2(pack2(fminf(fmaxf(t.x, 0.f), kTop), fminf(fmaxf(t.y, 0.f), kTop)), both(__uint_as_float(kMagic))));
+    constexpr int kPer = 32 / BITS;  // codes of a word
+    uint32_t& w = r.word[2 * j / kPer];
+    w += (__float_as_uint(c.x) << (BITS * (2 * j % kPer))) + (__float_as_uint(c.y) << (BITS * (2 * j % kPer + 1)));
+  }
+  // the constant's bits, once for all codes of a word
+  constexpr uint32_t kBias = BITS == 4 ? kMagic * 0x11111111u : kMagic * 0x01010101u;
+#pragma unroll
+  for (int k = 0; k < BITS / 2; ++k) r.word[k] -= kBias;
   return r;
 }
 
@@ -92,10 +124,6 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, l = lane & 7;
   const int t = blockIdx.x * kWarps + warp;
   if (t >= p.num_tokens) return;
-  const int b = sequence_of(p.cu, p.batch, t);
-  if (b < 0) return;
-  const Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
-  const int pos = portion.first + t - portion.start;
   const int rows = p.num_heads + 2 * p.num_kv_heads, rotated = p.num_heads + p.num_kv_heads;
   const int begin = blockIdx.y * p.rows_per_warp, end = min(rows, begin + p.rows_per_warp);
   auto source = [&](int r) {
@@ -108,6 +136,7 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_consta
 #pragma unroll
     for (int e = 0; e < ROWS; ++e) {
       const int r = r0 + 4 * e + sub;
+      lo[e] = hi[e] = make_uint4(0u, 0u, 0u, 0u);
       if (r < end) {
         const uint4* x = reinterpret_cast<const uint4*>(source(r)) + l;
         lo[e] = x[0];
@@ -115,7 +144,19 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_consta
       }
     }
   };
-  fetch(begin);
+  fetch(begin);  // ahead of the tables: they come one after the other
+  const int b = sequence_of(p.cu, p.batch, t);
+  if (b < 0) return;
+  const Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
+  const int pos = portion.first + t - portion.start;
+  const int block = pos >> 6, slot = pos & (kPage - 1);
+  const bool held = pos >= 0 && block < p.max_blocks;  // a position outside the sequence's pages goes nowhere
+  uint8_t* pages[2] = {nullptr, nullptr};
+  if (held && end > p.num_heads) {
+    const long long* table = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + block;
+    pages[0] = reinterpret_cast<uint8_t*>(table[0]);
+    pages[1] = reinterpret_cast<uint8_t*>(table[p.max_blocks]);
+  }
   if (begin < rotated) {
 #pragma unroll
     for (int i = lane; i < kD / 2; i += 32) {
@@ -127,8 +168,6 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_consta
     }
     __syncwarp();
   }
-  const int block = pos >> 6, slot = pos & (kPage - 1);
-  const bool held = pos >= 0 && block < p.max_blocks;  // a position outside the sequence's pages goes nowhere
   for (int r0 = begin; r0 < end; r0 += 4 * ROWS) {
     if (r0 > begin) fetch(r0);
 #pragma unroll
@@ -136,65 +175,60 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_consta
       if (r0 + 4 * e >= end) break;
       const int r = r0 + 4 * e + sub;
       const bool live = r < end;
-      float x[16];
+      f2 x[8];
       {
         const __half2* a = reinterpret_cast<const __half2*>(&lo[e]);
         const __half2* c = reinterpret_cast<const __half2*>(&hi[e]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const float2 f = __half22float2(a[j]), g = __half22float2(c[j]);
-          x[2 * j] = live ? f.x : 0.f; x[2 * j + 1] = live ? f.y : 0.f;
-          x[8 + 2 * j] = live ? g.x : 0.f; x[8 + 2 * j + 1] = live ? g.y : 0.f;
+          x[j] = pack2(f.x, f.y);
+          x[4 + j] = pack2(g.x, g.y);
         }
       }
       if (live && r < rotated) {
-        float cs[8], sn[8];
-#pragma unroll
-        for (int j = 0; j < 8; j += 4) {
-          const float4 c = *reinterpret_cast<const float4*>(&s_cos[warp][8 * l + j]), s = *reinterpret_cast<const float4*>(&s_sin[warp][8 * l + j]);
-          cs[j] = c.x; cs[j + 1] = c.y; cs[j + 2] = c.z; cs[j + 3] = c.w;
-          sn[j] = s.x; sn[j + 1] = s.y; sn[j + 2] = s.z; sn[j + 3] = s.w;
-        }
         uint4 out[2];
         __half2* o = reinterpret_cast<__half2*>(out);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float f0 = x[j], f1 = x[8 + j];
-          x[j] = __fsub_rn(__fmul_rn(cs[j], f0), __fmul_rn(sn[j], f1));
-          x[8 + j] = __fadd_rn(__fmul_rn(cs[j], f1), __fmul_rn(sn[j], f0));
+        for (int j = 0; j < 4; j += 2) {
+          const ulonglong2 cs = *reinterpret_cast<const ulonglong2*>(&s_cos[warp][8 * l + 2 * j]), sn = *reinterpret_cast<const ulonglong2*>(&s_sin[warp][8 * l + 2 * j]);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const f2 c = k ? cs.y : cs.x, s = k ? sn.y : sn.x, f0 = x[j + k], f1 = x[4 + j + k];
+            x[j + k] = fma2(product(s, f1), both(-1.f), product(c, f0));
+            x[4 + j + k] = add2(product(c, f1), product(s, f0));
+          }
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          o[j] = __floats2half2_rn(x[2 * j], x[2 * j + 1]);
-          const float2 f = __half22float2(o[j]);  // keys are quantised as fp16 numbers
-          x[2 * j] = f.x;
-          x[2 * j + 1] = f.y;
+          const float2 f = unpack2(x[j]);
+          o[j] = __floats2half2_rn(f.x, f.y);
         }
         if (r < p.num_heads) {
           uint4* dst = reinterpret_cast<uint4*>(p.q_out + t * p.q_out_stride + r * kD) + l;
           dst[0] = out[0];
           dst[8] = out[1];
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {  // keys are quantised as fp16 numbers
+            const float2 f = __half22float2(o[j]);
+            x[j] = pack2(f.x, f.y);
+          }
         }
       }
       const bool mine = live && held && r >= p.num_heads;
       if (!__any_sync(0xffffffffu, mine)) continue;
-      const Quantised c = quantise_row<BITS>(x);
+      const Quantised<BITS> c = quantise_row<BITS>(x);
       if (!mine) continue;
       const int which = r >= rotated, head = r - p.num_heads - which * p.num_kv_heads;
-      uint8_t* page = reinterpret_cast<uint8_t*>(p.kv_pointers[(static_cast<long long>(b) * 2 + which) * p.max_blocks + block]);
+      uint8_t* page = which ? pages[1] : pages[0];
       uint8_t* row = page + G::codes_at(head) + slot * G::kRow;
       if constexpr (BITS == 4) {
-        uint32_t w[2] = {0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j >> 3] |= c.code[j] << (4 * (j & 7));
-        reinterpret_cast<uint32_t*>(row)[l] = w[0];
-        reinterpret_cast<uint32_t*>(row)[8 + l] = w[1];
+        reinterpret_cast<uint32_t*>(row)[l] = c.word[0];
+        reinterpret_cast<uint32_t*>(row)[8 + l] = c.word[1];
       } else {
-        uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[j >> 2] |= c.code[j] << (8 * (j & 3));
-        reinterpret_cast<uint2*>(row)[l] = make_uint2(w[0], w[1]);
-        reinterpret_cast<uint2*>(row)[8 + l] = make_uint2(w[2], w[3]);
+        reinterpret_cast<uint2*>(row)[l] = make_uint2(c.word[0], c.word[1]);
+        reinterpret_cast<uint2*>(row)[8 + l] = make_uint2(c.word[2], c.word[3]);
       }
       if (l == 0) {
         *reinterpret_cast<__half*>(page + G::scales_at(head, p.num_kv_heads) + slot * 2) = c.scale;
@@ -211,10 +245,12 @@ struct ReadParams {
   int batch, num_tokens, max_blocks, num_kv_heads;
 };
 
-// A warp per token, eight lanes per head row: 16 codes and 32 bytes of results a lane.
-template <int BITS>
+// A warp per token and run of 4 ROWS head rows, eight lanes a row: lane l has dims 8 l .. and 64 + 8 l .., so that a store takes whole sectors; everything that the
+// warp reads of the pages is on its way together.
+template <int BITS, int ROWS>
 __global__ void __launch_bounds__(32 * kWarps) read_kernel(const ReadParams p) {
   using G = Geom<BITS>;
+  using Word = std::conditional_t<BITS == 4, uint32_t, uint2>;  // eight codes
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane >> 3, l = lane & 7;
@@ -226,45 +262,53 @@ __global__ void __launch_bounds__(32 * kWarps) read_kernel(const ReadParams p) {
   const int pos = portion.first + t - portion.start;
   const int block = pos >> 6, slot = pos & (kPage - 1);
   if (pos < 0 || block >= p.max_blocks) return;
-  const uint8_t* pages[2];
+  const long long* table = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + block;
+  const uint8_t* const pages[2] = {reinterpret_cast<const uint8_t*>(table[0]), reinterpret_cast<const uint8_t*>(table[p.max_blocks])};
+  Word lo[ROWS], hi[ROWS];
+  __half s[ROWS], z[ROWS];
+  const int r0 = blockIdx.y * 4 * ROWS + sub;
 #pragma unroll
-  for (int w = 0; w < 2; ++w) pages[w] = reinterpret_cast<const uint8_t*>(p.kv_pointers[(static_cast<long long>(b) * 2 + w) * p.max_blocks + block]);
-#pragma unroll 4
-  for (int r = sub; r < 2 * p.num_kv_heads; r += 4) {
-    const int which = r >= p.num_kv_heads, head = r - which * p.num_kv_heads;
-    const uint8_t* page = which ? pages[1] : pages[0];
-    const uint8_t* row = page + G::codes_at(head) + slot * G::kRow;
-    const __half s = *reinterpret_cast<const __half*>(page + G::scales_at(head, p.num_kv_heads) + slot * 2);
-    const __half z = *reinterpret_cast<const __half*>(page + G::zeros_at(head, p.num_kv_heads) + slot * 2);
-    uint4 out[2];
-    __half2* o = reinterpret_cast<__half2*>(out);
-    if constexpr (BITS == 4) {
-      const uint2 w = reinterpret_cast<const uint2*>(row)[l];
-      const __half2 s2 = __half2half2(s), c2 = __half2half2(__hmul(__hneg(s), z));
+  for (int e = 0; e < ROWS; ++e) {
+    const int r = r0 + 4 * e, which = r >= p.num_kv_heads, head = r - which * p.num_kv_heads;
+    if (r < 2 * p.num_kv_heads) {
+      const uint8_t* page = which ? pages[1] : pages[0];
+      const Word* row = reinterpret_cast<const Word*>(page + G::codes_at(head) + slot * G::kRow);
+      lo[e] = row[l];
+      hi[e] = row[8 + l];
+      s[e] = *reinterpret_cast<const __half*>(page + G::scales_at(head, p.num_kv_heads) + slot * 2);
+      z[e] = *reinterpret_cast<const __half*>(page + G::zeros_at(head, p.num_kv_heads) + slot * 2);
+    }
+  }
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+  for (int e = 0; e < ROWS; ++e) {
+    const int r = r0 + 4 * e, which = r >= p.num_kv_heads, head = r - which * p.num_kv_heads;
+    if (r >= 2 * p.num_kv_heads) break;
+    uint4* dst = reinterpret_cast<uint4*>((which ? p.v : p.k) + (static_cast<long long>(t) * p.num_kv_heads + head) * kD);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const Word w = half ? hi[e] : lo[e];
+      uint4 out;
+      __half2* o = reinterpret_cast<__half2*>(&out);
+      if constexpr (BITS == 4) {
+        const __half2 s2 = __half2half2(s[e]), c2 = __half2half2(__hmul(__hneg(s[e]), z[e]));
         __half2 u[4], x[4];
-        codes_of_word4(i ? w.y : w.x, u);
+        codes_of_word4(w, u);
 #pragma unroll
         for (int j = 0; j < 4; ++j) x[j] = __hfma2(u[j], s2, c2);
-        o[4 * i] = __lows2half2(x[0], x[1]);
-        o[4 * i + 1] = __lows2half2(x[2], x[3]);
-        o[4 * i + 2] = __highs2half2(x[0], x[1]);
-        o[4 * i + 3] = __highs2half2(x[2], x[3]);
-      }
-    } else {
-      const uint4 w = reinterpret_cast<const uint4*>(row)[l];
-      const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-      const float sf = __half2float(s), zf = __half2float(z);
+        o[0] = __lows2half2(x[0], x[1]);
+        o[1] = __lows2half2(x[2], x[3]);
+        o[2] = __highs2half2(x[0], x[1]);
+        o[3] = __highs2half2(x[2], x[3]);
+      } else {
+        const float sf = __half2float(s[e]), zf = __half2float(z[e]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t x = words[i >> 1] >> (16 * (i & 1));
-        o[i] = __floats2half2_rn(sf * (static_cast<float>(x & 255u) - zf), sf * (static_cast<float>((x >> 8) & 255u) - zf));
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t x = (i < 2 ? w.x : w.y) >> (16 * (i & 1));
+          o[i] = __floats2half2_rn(sf * (static_cast<float>(x & 255u) - zf), sf * (static_cast<float>((x >> 8) & 255u) - zf));
+        }
       }
+      dst[8 * half + l] = out;
     }
-    __half* dst = (which ? p.v : p.k) + (static_cast<long long>(t) * p.num_kv_heads + head) * kD + 16 * l;
-    reinterpret_cast<uint4*>(dst)[0] = out[0];
-    reinterpret_cast<uint4*>(dst)[1] = out[1];
   }
 }
 
@@ -281,12 +325,13 @@ int append_kv_cache(const AppendArgs& a) {
   double f = 0.15915494309189533577;  // 1 / (2 pi)
   for (int i = 0; i < kD / 2; ++i, f *= step) p.turns.per_position[i] = f;
   const int rows = p.num_heads + 2 * p.num_kv_heads, blocks = (a.num_tokens + kWarps - 1) / kWarps;
-  const bool few = blocks < 2 * num_sms();  // a token's rows are shared out over several warps
-  p.rows_per_warp = few ? 8 : rows;
+  // A token's rows are shared out over several warps, eight rows each at least, as long as that makes no more than 48 warps per multiprocessor: every one of them
+  // works out the position's sines
+  const long long fair = static_cast<long long>(rows) * a.num_tokens / (48 * num_sms());
+  p.rows_per_warp = static_cast<int>(fair >= rows ? rows : 8 * (fair / 8 + 1));
   const dim3 grid(blocks, (rows + p.rows_per_warp - 1) / p.rows_per_warp);
   auto run = [&](auto kern) { return launch(kern, grid, 32 * kWarps, 0, a.stream, "append_kv_cache", 1, p); };
-  if (a.cache.int4) return few ? run(append_kernel<4, 2>) : run(append_kernel<4, 4>);
-  return few ? run(append_kernel<8, 2>) : run(append_kernel<8, 4>);
+  return a.cache.int4 ? run(append_kernel<4, 2>) : run(append_kernel<8, 2>);
 }
 
 int read_kv_cache(void* k_out, void* v_out, const PagedCache& c, int batch, int num_tokens, void* stream) {
@@ -294,9 +339,10 @@ int read_kv_cache(void* k_out, void* v_out, const PagedCache& c, int batch, int 
   ReadParams p{};
   p.k = static_cast<__half*>(k_out); p.v = static_cast<__half*>(v_out); p.kv_pointers = c.kv_pointers; p.cu = c.cu_seqlens; p.lengths = c.lengths;
   p.batch = batch; p.num_tokens = num_tokens; p.max_blocks = c.max_blocks; p.num_kv_heads = c.num_kv_heads;
-  const dim3 grid((num_tokens + kWarps - 1) / kWarps);
+  constexpr int kRows = 4;
+  const dim3 grid((num_tokens + kWarps - 1) / kWarps, (2 * c.num_kv_heads + 4 * kRows - 1) / (4 * kRows));
   auto run = [&](auto kern) { return launch(kern, grid, 32 * kWarps, 0, stream, "read_kv_cache", 1, p); };
-  return c.int4 ? run(read_kernel<4>) : run(read_kernel<8>);
+  return c.int4 ? run(read_kernel<4, kRows>) : run(read_kernel<8, kRows>);
 }
 
 }  // namespace qs

@@ -87,8 +87,9 @@ def check_attention(out, want, scale):
     """Roundings to fp16 of the kernels' operands, each by at most H relative: every key (its score is off by at most d = H scale sum |q k|, its weight by 2 d with
     the denominator's), every weight (and the sum), every value (the weight times the scale, in the kernel that applies scales to weights; its product with codes
     up to three times the value's spread), the result.  A number is off by no more than all of them at their worst.  They are independent, so the rows
-    together are off by about H / sqrt(3) of sqrt(sum w^2 v^2) for each of key, weight and value (the products with codes: 2.7 times), and of the result:
-    2 H in all, and no more than 4 H."""
+    together are off by about H / sqrt(3) of sqrt(sum w^2 v^2) for each of key, weight and value (the products with codes: 2.7 times), of the result, and of
+    the results of the splits of a long axis (sqrt(sum of their squares) is that of w^2 v^2 again): 2 H in all, and no more than 4 H.  At their worst the splits add
+    H sum w |v|, which is in the 6 H (2 for the weight and the sum, 1 for the value, 1 for a split; 3 in the tail kernel, which has no splits)."""
     o, absolute, spread, mass = want
     off = (out.to(F64) - o).abs()
     d = H * scale * mass[..., None]
