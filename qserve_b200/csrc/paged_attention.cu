@@ -59,6 +59,24 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 __device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool live) {  // 16 zeros where not live
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(live ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// eight bytes at this place of the shared memory of block `rank` of the cluster
+__device__ __forceinline__ uint2 peer_u2(const void* mine, uint32_t rank) {
+  uint32_t a;
+  uint2 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint4 peer_u4(const void* mine, uint32_t rank) {
+  uint32_t a;
+  uint4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
@@ -97,6 +115,7 @@ constexpr int kRows = 128;                   // rows of a tile
 constexpr int kQBytes = kRows * kD * 2;      // two swizzled halves of 64 columns
 constexpr int kKvBytes = kPage * kD * 2;     // a page's K or V as fp16, two halves
 constexpr int kKvHalf = kKvBytes / 2;
+constexpr int kMostCluster = 8;
 constexpr float kRescale = 8.f;              // log2 units that a row's maximum may grow before O is rescaled
 // Of a tile's tensor memory columns: S and then P of even pages [0, 64), of odd pages [64, 128), O [128, 256).  A page's P takes the place of its own S, so the next
 // page's S is there before this one's softmax ends, and P waits for no product.
@@ -139,12 +158,20 @@ struct TileParams {
   const int *cu, *lengths;
   int batch, num_tokens, max_blocks, num_heads, num_kv_heads;
   int row_blocks, nsplit, shared_blocks;  // shared_blocks > 0: the rows of all sequences over the first sequence's first pages
+  int cluster, parts;                     // blocks that join their splits through one another's shared memory; partial rows that are left: nsplit / cluster
   float scale_log2;
-  __half* part;                           // nsplit > 1: O / sum [rows][nsplit][128], rows = token * num_heads + head
-  float2* part_ml;                        // (maximum, sum) [rows][nsplit]
+  __half* part;                           // parts > 1: O / sum [rows][parts][128], rows = token * num_heads + head
+  float2* part_ml;                        // (maximum, sum) [rows][parts]
 };
 
-template <int BITS, int TILES, bool PARTIAL>
+__device__ __forceinline__ uint2 scaled_h4(const float4& a, float L) {
+  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
+  return make_uint2(as_u32(__floats2half2_rn(a.x * inv, a.y * inv)), as_u32(__floats2half2_rn(a.z * inv, a.w * inv)));
+}
+
+// What a block does with its rows: the result; a partial result; or its cluster's, joined first.
+enum : int { kWhole = 0, kPartial = 1, kCluster = 2 };
+template <int BITS, int TILES, int MODE>
 __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, TILES>::kBlocksPerSm) tile_kernel(const __grid_constant__ TileParams p) {
   using C = TileCfg<BITS, TILES>;
   using G = Geom<BITS>;
@@ -163,7 +190,10 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   uint64_t* bar_raw = bar_vfree + C::kVStages;        // [slots] raw slot landed
   uint64_t* bar_used = bar_raw + C::kSlots;           // [slots] raw slot read
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar_used + C::kSlots);
-  static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 4 <= C::kSmem - C::kOffBar, "the barriers' place");
+  // [128] rows' maximum and sum, for the cluster: over K, at the end.  (Shared memory of their own would leave L1 32 KB less: two blocks' 196 KB are a step of its
+  // size.  128 INT8 sequences behind 16384: 137 us, 158 so)
+  float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffK);
+  static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 4 <= 384, "the barriers' place");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the shuffle: the same in all lanes, also to the compiler)
   constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4, kCopyWarp = kIssueWarp + TILES;
@@ -194,11 +224,15 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   // ---- this block's share ----
-  unsigned idx = blockIdx.x;
+  unsigned idx = blockIdx.x, rank = 0;
+  if constexpr (MODE == kCluster) {
+    rank = idx & (p.cluster - 1);  // a power of two
+    idx /= static_cast<unsigned>(p.cluster);
+  }
   const int hk = idx % static_cast<unsigned>(p.num_kv_heads);
   idx /= static_cast<unsigned>(p.num_kv_heads);
-  const int split = idx % static_cast<unsigned>(p.nsplit);
-  idx /= static_cast<unsigned>(p.nsplit);
+  const int part = idx % static_cast<unsigned>(p.parts), split = MODE == kCluster ? part * p.cluster + rank : part;
+  idx /= static_cast<unsigned>(p.parts);
   const int b = idx % static_cast<unsigned>(p.batch), rb = p.row_blocks - 1 - static_cast<int>(idx / static_cast<unsigned>(p.batch));  // the last rows see most keys: first
   const int group = static_cast<unsigned>(p.num_heads) / static_cast<unsigned>(p.num_kv_heads);
   pdl_wait();
@@ -515,10 +549,10 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
       // Through shared memory (the tile's queries are done with), so that half a warp stores a whole row
       uint8_t* mine = smem + tile * kQBytes + quarter * (kQBytes / 4);
-      const long long token = portion.start + tok, at = (token * p.num_heads + head) * p.nsplit + split;
+      const long long token = portion.start + tok, at = (token * p.num_heads + head) * p.parts + part;
       unsigned long long to = 0ull;
-      if (row_is) to = PARTIAL ? reinterpret_cast<unsigned long long>(p.part + at * kD)
-                               : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
+      if (row_is) to = MODE == kPartial ? reinterpret_cast<unsigned long long>(p.part + at * kD)
+                                        : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
         uint32_t o[32];
@@ -539,15 +573,67 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
                          as_u32(__floats2half2_rn(f[6], f[7])));
         }
       }
-      __syncwarp();
+      if constexpr (MODE != kCluster) {
+        __syncwarp();
 #pragma unroll 4
-      for (int k = 0; k < 32; k += 2) {
-        const int in = k + (lane >> 4), chunk = lane & 15;
-        uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
-        const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
-        if (row) row[chunk] = v;
+        for (int k = 0; k < 32; k += 2) {
+          const int in = k + (lane >> 4), chunk = lane & 15;
+          uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
+          if (row) row[chunk] = v;
+        }
+        if (MODE == kPartial && row_is) p.part_ml[at] = make_float2(m_used, l);
+      } else {
+        s_ml[quarter * 32 + lane] = make_float2(m_used, l);
       }
-      if (PARTIAL && row_is) p.part_ml[at] = make_float2(m_used, l);
+    }
+    if constexpr (MODE == kCluster) {
+      // The blocks of the cluster take turns over the rows, the halves of their softmax warps too: lane = eight dims
+      cluster_sync();
+      const int rows = min(n_rows - row_base, kRows), chunk = lane & 15;
+#pragma unroll 1
+      for (int i = static_cast<int>(rank) + p.cluster * (2 * warp + (lane >> 4)); i < rows; i += p.cluster * 8) {
+        const uint8_t* at = smem + i * 256 + ((chunk ^ (i & 7)) << 4);
+        uint4 x[kMostCluster];
+        float2 ml[kMostCluster];
+#pragma unroll
+        for (int k = 0; k < kMostCluster; ++k) {
+          x[k] = make_uint4(0u, 0u, 0u, 0u);
+          ml[k] = make_float2(-CUDART_INF_F, 0.f);
+          if (k < p.cluster) {
+            const uint2 w = peer_u2(s_ml + i, k);
+            ml[k] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+            x[k] = peer_u4(at, k);
+          }
+        }
+        float M = -CUDART_INF_F, L = 0.f, acc[8] = {};
+#pragma unroll
+        for (int k = 0; k < kMostCluster; ++k) M = fmaxf(M, ml[k].x);
+        const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll
+        for (int k = 0; k < kMostCluster; ++k) {
+          const float w = ml[k].y * ex2(ml[k].x - ref);
+          L += w;
+          const uint32_t words[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 a = __half22float2(as_h2(words[e]));
+            acc[2 * e] = fmaf(a.x, w, acc[2 * e]);
+            acc[2 * e + 1] = fmaf(a.y, w, acc[2 * e + 1]);
+          }
+        }
+        const uint2 lo = scaled_h4(make_float4(acc[0], acc[1], acc[2], acc[3]), L), hi = scaled_h4(make_float4(acc[4], acc[5], acc[6], acc[7]), L);
+        const int row = row_base + i, t = row / group, h = hk * group + row - t * group;
+        const long long token = portion.start + t;
+        reinterpret_cast<uint4*>(p.out + token * p.out_stride + static_cast<long long>(h) * kD)[chunk] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      }
+      cluster_sync();  // no block leaves while another reads its rows
+    }
+  }
+  if constexpr (MODE == kCluster) {
+    if (warp >= kUnpackWarp) {  // the softmax warps' two waits
+      cluster_sync();
+      cluster_sync();
     }
   }
   tc_fence_before();
@@ -561,32 +647,36 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 __device__ __forceinline__ void join_rows(const __half* part, const float2* ml, int nsplit, float& M, float& L, float4& acc) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < nsplit; s0 += 32) {
-    const float2 mine = s0 + lane < nsplit ? __ldcg(ml + s0 + lane) : make_float2(-CUDART_INF_F, 0.f);
+    const int n = min(32, nsplit - s0);
+    const uint2* rows = reinterpret_cast<const uint2*>(part + static_cast<long long>(s0) * kD) + lane;
+    uint2 x[8];
+    auto fetch = [&](int s) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = s + k < n ? __ldcg(rows + (s + k) * (kD / 4)) : make_uint2(0u, 0u);
+    };
+    fetch(0);  // on their way together with the maxima and sums
+    const float2 mine = lane < n ? __ldcg(ml + s0 + lane) : make_float2(-CUDART_INF_F, 0.f);
     float m = mine.x;
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
     const float m_new = fmaxf(M, m), ref = m_new == -CUDART_INF_F ? 0.f : m_new;
-    const float old = ex2(M - ref), w = ex2(mine.x - ref);
-    const float weight = mine.y * w;  // of O / sum
+    const float old = ex2(M - ref), weight = mine.y * ex2(mine.x - ref);  // of O / sum
     float sum = weight;
 #pragma unroll
     for (int k = 16; k >= 1; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
     L = fmaf(L, old, sum);
     acc.x *= old; acc.y *= old; acc.z *= old; acc.w *= old;
     M = m_new;
-    const int n = min(32, nsplit - s0);
-#pragma unroll 8
-    for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, weight, s);
-      const uint2 x = __ldcg(reinterpret_cast<const uint2*>(part + static_cast<long long>(s0 + s) * kD) + lane);
-      const float2 a = __half22float2(as_h2(x.x)), b = __half22float2(as_h2(x.y));
-      acc.x = fmaf(a.x, ws, acc.x); acc.y = fmaf(a.y, ws, acc.y); acc.z = fmaf(b.x, ws, acc.z); acc.w = fmaf(b.y, ws, acc.w);
+    for (int s = 0; s < n; s += 8) {
+      if (s > 0) fetch(s);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {  // (behind the last split: zeros with a weight of zero)
+        const float ws = __shfl_sync(0xffffffffu, weight, (s + k) & 31);
+        const float2 a = __half22float2(as_h2(x[k].x)), b = __half22float2(as_h2(x[k].y));
+        acc.x = fmaf(a.x, ws, acc.x); acc.y = fmaf(a.y, ws, acc.y); acc.z = fmaf(b.x, ws, acc.z); acc.w = fmaf(b.y, ws, acc.w);
+      }
     }
   }
-}
-__device__ __forceinline__ uint2 scaled_h4(const float4& a, float L) {
-  const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-  return make_uint2(as_u32(__floats2half2_rn(a.x * inv, a.y * inv)), as_u32(__floats2half2_rn(a.z * inv, a.w * inv)));
 }
 
 // Rows of the result, WARPS warps each (they take turns over the splits); rows behind the last sequence are left as they are.
@@ -604,8 +694,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileP
   float M = -CUDART_INF_F, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   // this warp's run of the splits
-  const int part = warp % WARPS, s0 = p.nsplit * part / WARPS, s1 = p.nsplit * (part + 1) / WARPS;
-  if (mine) join_rows(p.part + (row * p.nsplit + s0) * kD, p.part_ml + row * p.nsplit + s0, s1 - s0, M, L, acc);
+  const int part = warp % WARPS, s0 = p.parts * part / WARPS, s1 = p.parts * (part + 1) / WARPS;
+  if (mine) join_rows(p.part + (row * p.parts + s0) * kD, p.part_ml + row * p.parts + s0, s1 - s0, M, L, acc);
   if constexpr (WARPS > 1) {
     reinterpret_cast<float4*>(s_acc[warp])[lane] = acc;
     if (lane == 0) s_ml[warp] = make_float2(M, L);
@@ -664,9 +754,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float peer_f32(const float* mine, uint32_t rank) {
   uint32_t a;
@@ -1031,88 +1118,115 @@ int allow_smem(int bytes, const char* what, Enough enough) {
   return rc;
 }
 
-// How a call over `rows` rows per kv head and sequence and at most `pages` pages is cut: tiles per block and splits of the pages, as many as fit the device at a
-// time with `least` pages each.  One page where join_kernel follows (17 tokens behind 500 x 32 heads: four pages 13.3 us, two 12.4, one 11.2), two where the tail
-// kernel's few warps join (8 sequences, 1024 shared positions: four 12.0 us, two 9.8, one 10.4).
+// How a call over `rows` rows per kv head and sequence (`outputs` result rows in all) and at most `pages` pages is cut: tiles per block, and splits of the pages.  The
+// cut whose time is estimated lowest: rounds of blocks over the device, each its pages and what comes ahead of the first and behind the last, and the joining of
+// the splits: by a cluster of up to eight blocks (one tile of a prompt), by join_kernel, or in the tail kernel.  The figures, in us, are those of the kernels' own
+// timelines; one or two one-tile blocks share a multiprocessor.  Measured, us: 17 tokens behind 500 in a cluster 7.8, with join_kernel 8.5; 4 behind 4000 9.2 and
+// 12.3; 24 behind 60000 one block per multiprocessor 54, two 46; 8 sequences behind 4096 shared positions two 13.9, one 11.6.  Splits that make more than one round
+// did not pay (4096 tokens behind 12000, three and a half rounds of blocks: 830, in two splits 865; six portions of 250: 64.5 and 81.8), nor clusters of two blocks
+// per multiprocessor (four of 20 behind 8000, INT8: 37.4, join_kernel 34.5).
 struct Plan {
-  int tiles, row_blocks, nsplit;
+  int tiles, row_blocks, nsplit, cluster, parts;
 };
-Plan plan_tiles(long long rows, long long items, long long pages, int least) {
+Plan plan_tiles(long long rows, long long items, long long outputs, long long pages, bool prompt) {
+  constexpr float kFixed = 3.5f, kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 5e6f;
   Plan pl;
   pl.tiles = rows <= kRows ? 1 : 2;
   pl.row_blocks = static_cast<int>((rows + pl.tiles * kRows - 1) / (pl.tiles * kRows));
-  const long long blocks = items * pl.row_blocks, slots = static_cast<long long>(num_sms()) * (pl.tiles == 1 ? 2 : 1);
-  long long n = blocks > 0 ? slots / blocks : 1;
-  const long long most = pages / least;
-  if (n > most) n = most;
-  if (n < 1) n = 1;
-  if (n > 128) n = 128;
-  pl.nsplit = static_cast<int>(n);
+  const long long blocks = items * pl.row_blocks, sms = num_sms();
+  float best = 3.0e38f;
+  pl.nsplit = pl.cluster = 1;
+  for (int per_sm = 1; per_sm <= (pl.tiles == 1 ? 2 : 1); ++per_sm) {
+    const float page = pl.tiles == 2 ? 0.92f : per_sm == 1 ? (rows <= 64 ? 0.7f : 0.95f) : (rows <= 64 ? 1.f : 1.2f);
+    for (int n = 1; n <= 128 && n <= (pages > 1 ? pages : 1); ++n) {
+      if (per_sm == 2 && blocks * n <= sms) continue;
+      if (n > 1 && blocks * n > sms * per_sm) break;
+      const bool cluster = prompt && pl.tiles == 1 && per_sm == 1 && n > 1 && n <= kMostCluster && (n & (n - 1)) == 0;
+      const long long rounds = (blocks * n + sms * per_sm - 1) / (sms * per_sm), each = (pages + n - 1) / n;
+      float t = rounds * (each * page + kFixed);
+      if (n > 1) t += !prompt ? kJoinTail * n : cluster ? kJoinCluster : kJoinKernel + outputs * n * (2.f * (kD * 2 + 8)) / kPartBytesPerUs;
+      if (t < best) {
+        best = t;
+        pl.nsplit = n;
+        pl.cluster = cluster ? n : 1;
+      }
+    }
+  }
+  pl.parts = pl.nsplit / pl.cluster;
   return pl;
 }
-size_t part_bytes(long long rows, int nsplit) { return static_cast<size_t>(rows) * nsplit * (kD * sizeof(__half) + sizeof(float2)); }
+size_t part_bytes(long long rows, int parts) { return static_cast<size_t>(rows) * parts * (kD * sizeof(__half) + sizeof(float2)); }
 
-template <int BITS, int TILES, bool PARTIAL>
+template <int BITS, int TILES, int MODE>
 int run_tiles(const TileParams& p, int batch_items, void* stream) {
   using C = TileCfg<BITS, TILES>;
-  const int rc = allow_smem<tile_kernel<BITS, TILES, PARTIAL>>(C::kSmem, "paged attention: shared memory", [](int regs) { return !C::kShares || shares_suffice(regs); });
+  const int rc = allow_smem<tile_kernel<BITS, TILES, MODE>>(C::kSmem, "paged attention: shared memory", [](int regs) { return !C::kShares || shares_suffice(regs); });
   if (rc) return rc;
   const long long blocks = static_cast<long long>(p.row_blocks) * batch_items * p.nsplit * p.num_kv_heads;
   QS_REQUIRE(blocks <= 0x7fffffffll, "paged attention: %lld blocks", blocks);
-  return launch(tile_kernel<BITS, TILES, PARTIAL>, dim3(static_cast<unsigned>(blocks)), C::kThreads, C::kSmem, stream, "paged attention", 1, p);
+  return launch(tile_kernel<BITS, TILES, MODE>, dim3(static_cast<unsigned>(blocks)), C::kThreads, C::kSmem, stream, "paged attention", p.cluster, p);
 }
-int tiles(const TileParams& p, bool int4, int tiles_per_block, bool partial, int items, void* stream) {
-  auto pick = [&](auto bits, auto per, auto part) { return run_tiles<decltype(bits)::value, decltype(per)::value, decltype(part)::value>(p, items, stream); };
-  auto with = [&](auto bits, auto per) { return partial ? pick(bits, per, std::true_type{}) : pick(bits, per, std::false_type{}); };
+int tiles(TileParams& p, const Plan& pl, bool int4, int items, void* stream) {
+  p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.cluster = pl.cluster; p.parts = pl.parts;
   auto sized = [&](auto bits) {
-    return tiles_per_block == 1 ? with(bits, std::integral_constant<int, 1>{}) : with(bits, std::integral_constant<int, 2>{});
+    constexpr int kBits = decltype(bits)::value;
+    if (pl.tiles == 2) return p.part ? run_tiles<kBits, 2, kPartial>(p, items, stream) : run_tiles<kBits, 2, kWhole>(p, items, stream);
+    if (pl.cluster > 1) return run_tiles<kBits, 1, kCluster>(p, items, stream);
+    return p.part ? run_tiles<kBits, 1, kPartial>(p, items, stream) : run_tiles<kBits, 1, kWhole>(p, items, stream);
   };
   return int4 ? sized(std::integral_constant<int, 4>{}) : sized(std::integral_constant<int, 8>{});
 }
 
-Plan plan_prompt(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
-  return plan_tiles(static_cast<long long>(max_seqlen) * (heads / kv_heads), static_cast<long long>(batch) * kv_heads, (static_cast<long long>(max_length) + kPage - 1) / kPage, 1);
+Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
+  return plan_tiles(static_cast<long long>(max_seqlen) * (heads / kv_heads), static_cast<long long>(batch) * kv_heads, static_cast<long long>(num_tokens) * heads,
+                    (static_cast<long long>(max_length) + kPage - 1) / kPage, true);
 }
+// Few sequences or few shared pages: the tail kernel reads every sequence's whole table, one launch instead of two.  us, both kernels / the tail alone (INT4, 32 heads
+// over 8, 100 positions behind): one sequence behind 512 6.5 / 6.0, behind 4096 9.5 / 8.2; two behind 512 6.7 / 6.3, behind 2048 7.9 / 9.0; eight behind 128 6.4 /
+// 4.9, behind 512 6.6 / 8.7.
+bool tail_alone(int batch, int shared_blocks) { return batch == 1 || static_cast<long long>(batch) * shared_blocks <= 16; }
 Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
-  return plan_tiles(static_cast<long long>(batch) * (heads / kv_heads), kv_heads, shared_blocks, 2);
+  return plan_tiles(static_cast<long long>(batch) * (heads / kv_heads), kv_heads, static_cast<long long>(batch) * heads, shared_blocks, false);
 }
 
 }  // namespace
 
 size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
   if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  const Plan pl = plan_prompt(batch, max_seqlen, max_length, heads, kv_heads);
-  return pl.nsplit > 1 ? part_bytes(static_cast<long long>(num_tokens) * heads, pl.nsplit) : 0;
+  const Plan pl = plan_prompt(batch, num_tokens, max_seqlen, max_length, heads, kv_heads);
+  return pl.parts > 1 ? part_bytes(static_cast<long long>(num_tokens) * heads, pl.parts) : 0;
 }
 
 int paged_prompt_attention(const PagedAttnArgs& a) {
   if (a.batch == 0 || a.num_tokens == 0 || a.max_seqlen == 0) return QS_OK;
-  const Plan pl = plan_prompt(a.batch, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
+  const Plan pl = plan_prompt(a.batch, a.num_tokens, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
   TileParams p{};
   p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths;
   p.batch = a.batch; p.num_tokens = a.num_tokens; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
-  p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   const long long rows = static_cast<long long>(a.num_tokens) * a.num_heads;
-  if (pl.nsplit > 1) {
-    QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.nsplit), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
-               part_bytes(rows, pl.nsplit));
+  if (pl.parts > 1) {
+    QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.parts), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
+               part_bytes(rows, pl.parts));
+    QS_REQUIRE(rows <= 0x7fffffffll, "paged_prompt_attention: %lld rows", rows);
     p.part = static_cast<__half*>(a.workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.nsplit * kD);
+    p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
   }
-  const int rc = tiles(p, a.cache.int4, pl.tiles, pl.nsplit > 1, a.batch, a.stream);
-  if (rc || pl.nsplit == 1) return rc;
-  const bool wide = pl.nsplit >= 8;  // (24 tokens behind 60000, 37 splits: a warp a row 52.8 us, four 48.9; 17 behind 500, nine splits: 11.0 and 10.5)
+  const int rc = tiles(p, pl, a.cache.int4, a.batch, a.stream);
+  if (rc || pl.parts == 1) return rc;
+  const bool wide = pl.parts >= 8;  // (24 tokens behind 60000, 37 parts: a warp a row 52.8 us, four 48.9; 17 behind 500, nine: 11.0 and 10.5)
   return launch(wide ? join_kernel<4> : join_kernel<1>, dim3(static_cast<unsigned>(wide ? rows : (rows + 3) / 4)), 128, 0, a.stream, "paged_prompt_attention: join", 1, p);
 }
 
 size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_heads) {
-  if (batch <= 0 || shared_blocks <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  return part_bytes(static_cast<long long>(batch) * heads, plan_shared(batch, shared_blocks, heads, kv_heads).nsplit);
+  if (batch <= 0 || shared_blocks <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || tail_alone(batch, shared_blocks)) return 0;
+  return part_bytes(static_cast<long long>(batch) * heads, plan_shared(batch, shared_blocks, heads, kv_heads).parts);
 }
 
 int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   if (a.batch == 0) return QS_OK;
+  if (tail_alone(a.batch, shared_blocks)) shared_blocks = 0;
   const long long rows = static_cast<long long>(a.batch) * a.num_heads;
   TailParams t{};
   t.q = static_cast<const __half*>(a.q); t.out = static_cast<__half*>(a.out); t.q_stride = a.q_stride; t.out_stride = a.out_stride;
@@ -1120,16 +1234,16 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   t.num_kv_heads = a.cache.num_kv_heads; t.shared_blocks = shared_blocks; t.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   if (shared_blocks > 0) {
     const Plan pl = plan_shared(a.batch, shared_blocks, a.num_heads, a.cache.num_kv_heads);
-    QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.nsplit), "shared_prefix_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
-               part_bytes(rows, pl.nsplit));
+    QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.parts), "shared_prefix_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
+               part_bytes(rows, pl.parts));
     TileParams p{};
     p.q = t.q; p.q_stride = t.q_stride; p.kv_pointers = t.kv_pointers; p.lengths = t.lengths;
     p.batch = 1; p.num_tokens = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
-    p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.shared_blocks = shared_blocks; p.scale_log2 = t.scale_log2;
+    p.shared_blocks = shared_blocks; p.scale_log2 = t.scale_log2;
     p.part = static_cast<__half*>(a.workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.nsplit * kD);
-    t.nsplit = pl.nsplit; t.part = p.part; t.part_ml = p.part_ml;
-    const int rc = tiles(p, a.cache.int4, pl.tiles, true, 1, a.stream);
+    p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
+    t.nsplit = pl.parts; t.part = p.part; t.part_ml = p.part_ml;
+    const int rc = tiles(p, pl, a.cache.int4, 1, a.stream);
     if (rc) return rc;
   }
   const int group = a.num_heads / t.num_kv_heads, heads_y = t.num_kv_heads * ((group + kMaxG - 1) / kMaxG);
