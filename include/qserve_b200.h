@@ -129,7 +129,7 @@ QS_API int qs_prefill_attention(const void* q, const void* k, const void* v, int
  * attends over keys of the same call).  A flat batch of num_tokens rows holds the LAST cu_seqlens[b + 1] - cu_seqlens[b] positions of sequence b, whose
  * pages (kv_pointers int64 [batch, 2, max_blocks], K and V, each 16-byte aligned) hold lengths[b] positions with them: row t of it has position
  * lengths[b] - (cu_seqlens[b + 1] - t).  cu_seqlens int32 [batch + 1], ascending; NULL: one row per sequence.  Rows behind the last sequence are
- * neither read nor written; positions outside a sequence's max_blocks pages are never touched.  head_dim 128, tokens_per_block 64,
+ * not written; positions outside a sequence's max_blocks pages are never touched.  head_dim 128, tokens_per_block 64,
  * kv_cache_with_zeros 1, size_per_token = num_kv_heads * 128 * bits / 8; row strides in halfs, multiples of 8, heads contiguous; 16-byte aligned.
  * Unlike the operators above, these read all of their tables behind the wait for the kernel before them. */
 /* q_out <- q rotated, pages <- quantised rotated k and v (q, k, v are not written; q_out may be q).  NeoX rotation in place position, angle

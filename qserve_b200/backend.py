@@ -342,7 +342,7 @@ def single_query_attention_quant(q, k, v, kv_pointers, length_per_sample, memory
 #
 # A flat batch of rows holds the last cu_seqlens[b + 1] - cu_seqlens[b] positions of sequence b (cu_seqlens int32 [B + 1]; None: one row per sequence);
 # lengths int32 [B] counts what the sequence's pages hold with them, kv_pointers int64 [B, 2, blocks] as for single_query_attention, pages 16-byte aligned.
-# Heads are 128 wide and contiguous, rows start on 16-byte boundaries.  Rows behind the last sequence (a padded batch) are neither read nor written:
+# Heads are 128 wide and contiguous, rows start on 16-byte boundaries.  Rows behind the last sequence (a padded batch) are not written:
 # those of a given `out` stay as they are, those of a new result are unset.
 # --------------------------------------------------------------------------------------------------
 

@@ -328,7 +328,8 @@ PyObject* read_kv_cache(const Args& a) {
   const int tokens = a.small(3);
   require(tokens >= 0, "num_tokens must not be negative");
   const at::TensorOptions options = t.options().dtype(at::kHalf).requires_grad(false);
-  at::Tensor k = at::empty({tokens, c.heads_kv, 128}, options), v = at::empty({tokens, c.heads_kv, 128}, options);
+  const at::Tensor kv = at::empty({2, tokens, c.heads_kv, 128}, options);  // (one allocation)
+  at::Tensor k = kv.select(0, 0), v = kv.select(0, 1);
   void *kp = k.data_ptr(), *vp = v.data_ptr();
   launch(t, [&](void* s) { return qs_read_kv_cache(kp, vp, c.kvp, c.cu, c.lens, c.batch, tokens, c.max_blocks, c.heads_kv, 128, c.tpb, c.size, c.int4, c.zeros, s); });
   PyObject* const ko = THPVariable_Wrap(std::move(k));

@@ -243,7 +243,7 @@ int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_
   if (rc) return rc;
   QS_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0, "%s: heads %d / kv heads %d", op, num_heads, num_kv_heads);
   QS_REQUIRE(max_seqlen >= 0 && max_length >= 0, "%s: negative size", op);
-  QS_REQUIRE(softmax_scale > 0.f && softmax_scale < 3.0e38f, "%s: softmax_scale must be positive and finite", op);
+  QS_REQUIRE(softmax_scale > 0.f && softmax_scale < 1.0e30f, "%s: softmax_scale must be positive and finite", op);
   if (batch == 0 || num_tokens == 0 || max_seqlen == 0) return qs::QS_OK;
   if ((rc = paged_rows(op, "q", q, q_stride, num_heads)) || (rc = paged_rows(op, "out", out, out_stride, num_heads))) return rc;
   QS_REQUIRE(aligned16(workspace), "%s: workspace must be 16-byte aligned", op);
@@ -269,7 +269,7 @@ int qs_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64
   QS_REQUIRE(num_heads > 0 && num_heads % num_kv_heads == 0, "%s: heads %d / kv heads %d", op, num_heads, num_kv_heads);
   QS_REQUIRE(shared_blocks >= 0 && shared_blocks <= max_blocks_per_seq, "%s: shared_blocks=%d of %d pages per sequence", op, shared_blocks, max_blocks_per_seq);
   QS_REQUIRE(max_length >= 0, "%s: negative size", op);
-  QS_REQUIRE(softmax_scale > 0.f && softmax_scale < 3.0e38f, "%s: softmax_scale must be positive and finite", op);
+  QS_REQUIRE(softmax_scale > 0.f && softmax_scale < 1.0e30f, "%s: softmax_scale must be positive and finite", op);
   QS_REQUIRE(batch <= 65535 && num_heads <= 65535, "%s: batch=%d / heads=%d exceed the grid limits", op, batch, num_heads);
   if (batch == 0) return qs::QS_OK;
   if ((rc = paged_rows(op, "q", q, q_stride, num_heads)) || (rc = paged_rows(op, "out", out, out_stride, num_heads))) return rc;

@@ -56,9 +56,6 @@ __device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem) {
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int PENDING>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t smem, const void* gmem, bool live) {  // 16 zeros where not live
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(live ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -156,7 +153,7 @@ struct TileParams {
   long long q_stride, out_stride;
   const long long* kv_pointers;
   const int *cu, *lengths;
-  int batch, num_tokens, max_blocks, num_heads, num_kv_heads;
+  int batch, num_tokens, max_seqlen, max_blocks, num_heads, num_kv_heads;
   int row_blocks, nsplit, shared_blocks;  // shared_blocks > 0: the rows of all sequences over the first sequence's first pages
   int cluster, parts;                     // blocks that join their splits through one another's shared memory; partial rows that are left: nsplit / cluster
   float scale_log2;
@@ -198,9 +195,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the shuffle: the same in all lanes, also to the compiler)
   constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4, kCopyWarp = kIssueWarp + TILES;
   if (threadIdx.x == 0) {
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(&bar_q[t], 4);
-    }
+    for (int t = 0; t < 2; ++t) mbar_init(&bar_q[t], 4);
     for (int i = 0; i < C::kKStages; ++i) {
       mbar_init(&bar_kfull[i], 4);
       mbar_init(&bar_kfree[i], TILES);
@@ -239,7 +234,8 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   // Only now: what is launched next may read what this kernel's predecessors wrote (the tail kernel does, ahead of its own wait)
   pdl_launch_dependents();
 
-  const Portion portion = p.shared_blocks > 0 ? Portion{0, p.num_tokens, 0} : portion_of(p.cu, p.lengths, b, p.num_tokens);
+  Portion portion = p.shared_blocks > 0 ? Portion{0, p.num_tokens, 0} : portion_of(p.cu, p.lengths, b, p.num_tokens);
+  portion.count = min(portion.count, p.max_seqlen);
   const int n_rows = portion.count * group;
   const int row_base = rb * (TILES * kRows);
   const bool any = row_base < n_rows;
@@ -289,10 +285,11 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       for (int i = 0; i < kWords; ++i) r.v[i] = __ldcg(reinterpret_cast<const uint4*>(v + codes) + (i ^ (part * (kWords / 2))));
     };
     // ... or out of their raw slot
+    constexpr int kSlots = C::kRing ? C::kSlots : 1;
     auto take = [&](Raw& r, int j) {
-      const int slot = j % C::kSlots;
+      const int slot = j % kSlots;
       const uint8_t* from = smem + C::kOffRaw + slot * C::kSlotBytes;
-      mbar_wait(&bar_raw[slot], static_cast<uint32_t>(j / C::kSlots) & 1u);
+      mbar_wait(&bar_raw[slot], static_cast<uint32_t>(j / kSlots) & 1u);
       const __half* meta = reinterpret_cast<const __half*>(from + C::kMeta) + key;
       r.ks = meta[0]; r.kz = meta[64]; r.vs = meta[128]; r.vz = meta[192];
       const uint4* k = reinterpret_cast<const uint4*>(from + t * (G::kRow / 2));
@@ -363,7 +360,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       for (int j = 0; j < n_mine; ++j) {
         take(raw, j);
         step(raw, j);
-        if (lane == 0) mbar_arrive(&bar_used[j % C::kSlots]);
+        if (lane == 0) mbar_arrive(&bar_used[j % kSlots]);
       }
     } else {
       fetch(raw, 0);
@@ -376,6 +373,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     if constexpr (C::kShares) set_max_regs<false, kIssueRegs>();
     if (C::kRing && warp == kCopyWarp) {
       // ===================================== copies: six of a page, a lane each =====================================
+      constexpr int kSlots = C::kRing ? C::kSlots : 1;
       const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + page0;
       const long long* vptrs = kptrs + p.max_blocks;
       long long kp = 0, vp = 0;  // lane i: page 32 n + i
@@ -383,14 +381,14 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       const int what = lane >> 1, of_v = lane & 1;
       const long long from = what == 0 ? G::codes_at(hk) : what == 1 ? G::scales_at(hk, p.num_kv_heads) : G::zeros_at(hk, p.num_kv_heads);
       const int to = what == 0 ? of_v * C::kCodes : C::kMeta + of_v * 256 + (what - 1) * 128, bytes = what == 0 ? C::kCodes : 128;
-      if constexpr (C::kRing) for (int j = 0; j < n_mine; ++j) {
+      for (int j = 0; j < n_mine; ++j) {
         if ((j & 31) == 0 && j + lane < n_mine) {
-          kp = __ldg(kptrs + j + lane);
-          vp = __ldg(vptrs + j + lane);
+          kp = __ldcg(kptrs + j + lane);
+          vp = __ldcg(vptrs + j + lane);
         }
         const long long k = __shfl_sync(0xffffffffu, kp, j & 31), v = __shfl_sync(0xffffffffu, vp, j & 31);
-        const int slot = j % C::kSlots;
-        mbar_wait(&bar_used[slot], (static_cast<uint32_t>(j / C::kSlots) & 1u) ^ 1u);
+        const int slot = j % kSlots;
+        mbar_wait(&bar_used[slot], (static_cast<uint32_t>(j / kSlots) & 1u) ^ 1u);
         if (lane == 0) mbar_expect_tx(&bar_raw[slot], C::kSlotBytes);
         __syncwarp();
         if (lane < 6) bulk_copy_g2s(smem + C::kOffRaw + slot * C::kSlotBytes + to, reinterpret_cast<const uint8_t*>(of_v ? v : k) + from, bytes, &bar_raw[slot]);
@@ -457,7 +455,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const uint4* row = reinterpret_cast<const uint4*>(__shfl_sync(0xffffffffu, mine, 2 * k + (lane >> 4)));
-        x[k] = row ? __ldg(row + c) : make_uint4(0u, 0u, 0u, 0u);
+        x[k] = row ? __ldcg(row + c) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -473,7 +471,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     if (lane == 0) mbar_arrive(&bar_q[tile]);
     // the last position that the row sees, and the lowest of the warp's rows (one that is no row: its numbers go nowhere)
     int limit = n_keys - 1;
-    if (row_is) limit = p.shared_blocks > 0 ? min(__ldg(p.lengths + tok), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
+    if (row_is) limit = p.shared_blocks > 0 ? min(__ldcg(p.lengths + tok), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
     int lowest = limit;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, m));
@@ -690,7 +688,8 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileP
   const bool in = row < static_cast<long long>(p.num_tokens) * p.num_heads;
   const int token = in ? static_cast<int>(row / p.num_heads) : 0, head = in ? static_cast<int>(row - static_cast<long long>(token) * p.num_heads) : 0;
   pdl_wait();
-  const bool mine = in && sequence_of(p.cu, p.batch, token) >= 0;
+  const int b = in ? sequence_of(p.cu, p.batch, token) : -1;
+  const bool mine = b >= 0 && token - (p.cu ? p.cu[b] : b) < p.max_seqlen;
   float M = -CUDART_INF_F, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   // this warp's run of the splits
@@ -724,13 +723,14 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileP
 constexpr int kTailWarps = 4, kMaxG = 8, kSlice = 32, kMaxCluster = 8;
 constexpr int kOPitch = kD + 4;
 
-template <int BITS>
+// DEEP: more slices of a warp on their way, for calls of two blocks per multiprocessor at most; otherwise as many blocks as registers allow
+template <int BITS, bool DEEP>
 struct SliceCfg {
   static constexpr int kRow = Geom<BITS>::kRow;
   static constexpr int kCodes = kSlice * kRow;
   static constexpr int kOffV = kCodes, kOffMeta = 2 * kCodes;  // K scales, K zeros, V scales, V zeros: 64 bytes each
   static constexpr int kBytes = 2 * kCodes + 256;
-  static constexpr int kSlots = 2;
+  static constexpr int kSlots = !DEEP ? 2 : BITS == 4 ? 4 : 3;
   static constexpr int kWarpBytes = kSlots * kBytes;
   static_assert(kWarpBytes >= kMaxG * kOPitch * 4, "a warp's ring holds its partial rows at the end");
   static constexpr int kSmem = kTailWarps * kWarpBytes;
@@ -784,9 +784,10 @@ struct TailParams {
 
 // SHARED: a block (and its cluster) per sequence and run of heads, the warps take turns over the slices; otherwise a warp for each of them, which saves the joining of
 // warps where there are enough to fill the device.
-template <int BITS, bool SHARED>
-__global__ void __launch_bounds__(32 * kTailWarps, BITS == 4 ? 4 : 3) tail_kernel(const __grid_constant__ TailParams p) {
-  using SC = SliceCfg<BITS>;
+template <int BITS, bool SHARED, bool DEEP>
+__global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3) tail_kernel(const __grid_constant__ TailParams p) {
+  static_assert(SHARED || !DEEP, "a warp for each run of heads goes with many of them");
+  using SC = SliceCfg<BITS, DEEP>;
   using G = Geom<BITS>;
   extern __shared__ __align__(1024) uint8_t smem[];
   __shared__ __align__(16) __half s_queries[(SHARED ? 1 : kTailWarps) * kMaxG * kD];
@@ -1134,21 +1135,23 @@ Plan plan_tiles(long long rows, long long items, long long outputs, long long pa
   pl.tiles = rows <= kRows ? 1 : 2;
   pl.row_blocks = static_cast<int>((rows + pl.tiles * kRows - 1) / (pl.tiles * kRows));
   const long long blocks = items * pl.row_blocks, sms = num_sms();
+  const unsigned most = static_cast<unsigned>(pages < 1 ? 1 : pages);
   float best = 3.0e38f;
   pl.nsplit = pl.cluster = 1;
   for (int per_sm = 1; per_sm <= (pl.tiles == 1 ? 2 : 1); ++per_sm) {
     const float page = pl.tiles == 2 ? 0.92f : per_sm == 1 ? (rows <= 64 ? 0.7f : 0.95f) : (rows <= 64 ? 1.f : 1.2f);
-    for (int n = 1; n <= 128 && n <= (pages > 1 ? pages : 1); ++n) {
-      if (per_sm == 2 && blocks * n <= sms) continue;
-      if (n > 1 && blocks * n > sms * per_sm) break;
+    const float part = prompt ? outputs * (2.f * (kD * 2 + 8)) / kPartBytesPerUs : kJoinTail;
+    const long long room = blocks > 0 ? sms * per_sm / blocks : 1;  // splits of one round
+    const unsigned last = static_cast<unsigned>(room < 1 ? 1 : room > 128 ? 128 : room);
+    for (unsigned n = per_sm == 1 ? 1 : static_cast<unsigned>(sms / (blocks > 0 ? blocks : 1)) + 1; n <= last && n <= most; ++n) {
       const bool cluster = prompt && pl.tiles == 1 && per_sm == 1 && n > 1 && n <= kMostCluster && (n & (n - 1)) == 0;
-      const long long rounds = (blocks * n + sms * per_sm - 1) / (sms * per_sm), each = (pages + n - 1) / n;
-      float t = rounds * (each * page + kFixed);
-      if (n > 1) t += !prompt ? kJoinTail * n : cluster ? kJoinCluster : kJoinKernel + outputs * n * (2.f * (kD * 2 + 8)) / kPartBytesPerUs;
+      float t = ((most + n - 1) / n) * page + kFixed;
+      if (n == 1) t *= static_cast<float>((blocks + sms * per_sm - 1) / (sms * per_sm));
+      else t += cluster ? kJoinCluster : (prompt ? kJoinKernel : 0.f) + part * n;
       if (t < best) {
         best = t;
-        pl.nsplit = n;
-        pl.cluster = cluster ? n : 1;
+        pl.nsplit = static_cast<int>(n);
+        pl.cluster = cluster ? static_cast<int>(n) : 1;
       }
     }
   }
@@ -1203,7 +1206,7 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
   TileParams p{};
   p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths;
-  p.batch = a.batch; p.num_tokens = a.num_tokens; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
+  p.batch = a.batch; p.num_tokens = a.num_tokens; p.max_seqlen = a.max_seqlen; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   const long long rows = static_cast<long long>(a.num_tokens) * a.num_heads;
   if (pl.parts > 1) {
@@ -1238,7 +1241,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
                part_bytes(rows, pl.parts));
     TileParams p{};
     p.q = t.q; p.q_stride = t.q_stride; p.kv_pointers = t.kv_pointers; p.lengths = t.lengths;
-    p.batch = 1; p.num_tokens = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
+    p.batch = 1; p.num_tokens = p.max_seqlen = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
     p.shared_blocks = shared_blocks; p.scale_log2 = t.scale_log2;
     p.part = static_cast<__half*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
@@ -1252,17 +1255,24 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   const long long tail_pages = (static_cast<long long>(a.max_length) + kPage - 1) / kPage - shared_blocks;
   t.cluster = 1;
   while (t.cluster < kMaxCluster && blocks * t.cluster * 2 <= slots && tail_pages >= 2 * kTailWarps * t.cluster) t.cluster *= 2;
+  QS_REQUIRE(blocks <= 0x7fffffffll, "shared_prefix_attention: %lld runs of heads", blocks);
   const bool shared = blocks < 12 * num_sms();  // (a wave of warps; 128 sequences x 32 heads, INT8, 400 positions each behind 16384: 157 us by blocks, 142 by warps)
   if (!shared) t.cluster = 1;
   const dim3 grid = shared ? dim3(t.cluster, heads_y, a.batch) : dim3(static_cast<unsigned>((blocks + kTailWarps - 1) / kTailWarps));
-  auto run = [&](auto bits, auto by_block) {
+  // us, two slots / four (INT4): one sequence of 16384 positions 17.6 / 16.2, one of 2000 with 32 heads a group of one 8.1 / 6.2, four of up to 8000 17.3 / 12.1.  Not
+  // behind the tile kernel, whose blocks leave no room for it: 32 sequences, 100 positions behind 4096, 11.6 / 14.2
+  const bool deep = shared && t.nsplit == 0 && blocks * t.cluster <= 2 * num_sms();
+  auto run = [&](auto bits, auto by_block, auto more) {
     constexpr int kBits = decltype(bits)::value;
-    constexpr bool kShared = decltype(by_block)::value;
-    const int rc = allow_smem<tail_kernel<kBits, kShared>>(SliceCfg<kBits>::kSmem, "shared_prefix_attention: shared memory", [](int) { return true; });
+    constexpr bool kShared = decltype(by_block)::value, kDeep = decltype(more)::value;
+    const int rc = allow_smem<tail_kernel<kBits, kShared, kDeep>>(SliceCfg<kBits, kDeep>::kSmem, "shared_prefix_attention: shared memory", [](int) { return true; });
     if (rc) return rc;
-    return launch(tail_kernel<kBits, kShared>, grid, 32 * kTailWarps, SliceCfg<kBits>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
+    return launch(tail_kernel<kBits, kShared, kDeep>, grid, 32 * kTailWarps, SliceCfg<kBits, kDeep>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
   };
-  auto with = [&](auto bits) { return shared ? run(bits, std::true_type{}) : run(bits, std::false_type{}); };
+  auto with = [&](auto bits) {
+    if (!shared) return run(bits, std::false_type{}, std::false_type{});
+    return deep ? run(bits, std::true_type{}, std::true_type{}) : run(bits, std::true_type{}, std::false_type{});
+  };
   return a.cache.int4 ? with(std::integral_constant<int, 4>{}) : with(std::integral_constant<int, 8>{});
 }
 

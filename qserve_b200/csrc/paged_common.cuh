@@ -56,7 +56,7 @@ __device__ __forceinline__ Portion portion_of(const int* cu, const int* lengths,
   const int lo = cu ? cu[b] : b, hi = cu ? cu[b + 1] : b + 1;
   p.start = min(max(lo, 0), num_tokens);
   p.count = max(min(hi, num_tokens) - p.start, 0);
-  p.first = lengths[b] - max(hi - lo, 0);
+  p.first = min(max(lengths[b], 0), 1 << 30) - min(max(hi - lo, 0), 1 << 30);  // (within 31 bits whatever the tables say)
   return p;
 }
 // all lanes of a warp: the sequence that row t belongs to, -1 behind the last one (cu ascending)

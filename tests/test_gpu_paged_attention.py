@@ -223,3 +223,97 @@ def test_empty_calls(dev):
     assert backend.paged_prompt_attention(q, c.table, starts([0, 0], dev), c.lengths, 0, 64, *c.args).shape == (0, 8, D)
     assert backend.shared_prefix_attention(q, none, zero, 0, 0, *c.args).shape == (0, 8, D)
     assert backend.paged_prompt_attention(q, none, torch.zeros(1, dtype=torch.int32, device=dev), zero, 0, 0, *c.args).shape == (0, 8, D)
+
+
+def test_estimates_decide_nothing_else(dev):
+    """max_length below and far above the truth; a portion longer than max_seqlen: its rows behind that stay as they are."""
+    new, lens = [20, 33], [900, 1200]
+    c = Cache(lens, 2, 4, dev, seed=12)
+    q = queries(53, 8, dev)
+    want = prompt64(c, q, new, lens)
+    for top in (0, 1, 70, 100000):
+        check_attention(backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, 33, top, *c.args), want, SCALE)
+    for top in (1, 1200, 100000):  # one block for all keys; a cluster or join_kernel
+        out = torch.full((53, 8, D), 7.0, dtype=HALF, device=dev)
+        backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, 25, top, *c.args, out=out)
+        assert bool((out[45:] == 7).all())
+        check_attention(out[:45], [x[:45] for x in want], SCALE)
+
+
+@pytest.mark.parametrize("shared", [0, 2])
+def test_lengths_at_the_ends_of_their_type(dev, shared):
+    c = Cache([128, 128, 128], 2, 4, dev, shared=2 if shared else 0, seed=2)
+    q = queries(3, 8, dev)
+    want = shared64(c, q, [128, 128, 128])
+    c.lengths.copy_(torch.tensor([2 ** 31 - 1, -2 ** 31, 128], dtype=torch.int32))
+    for out in (backend.shared_prefix_attention(q, c.table, c.lengths, shared, 128, *c.args), backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 128, *c.args)):
+        assert bool((out[1] == 0).all())
+        check_attention(out[::2], [x[::2] for x in want], SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("lens,shared", [([300, 700, 290], 4), ([5000, 4300], 64), ([640] * 200, 9)])
+def test_a_shared_key_that_is_no_number(dev, bits, lens, shared):
+    """Every sequence that reaches it has no number then, in the prefix and behind it; one that ends ahead of it is as it was."""
+    lens = lens + [shared * PAGE - 60]
+    for at in (shared * PAGE - 50, lens[0] - 1):
+        c = Cache(lens, 2, bits, dev, shared=shared, seed=8)
+        q = queries(len(lens), 8, dev)
+        want = shared_row(c, q, lens, len(lens) - 1)  # the last sequence ends ahead of both
+        c.meta(1)[c.pages[0, at // PAGE], 0, :, at % PAGE] = float("nan")
+        out = backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args)
+        hit = [b for b, n in enumerate(lens) if n > at and (at < shared * PAGE or b == 0)]
+        rest = [b for b in range(len(lens)) if b not in hit]
+        assert bool(torch.isnan(out[hit]).all()) and bool(torch.isfinite(out[rest]).all())
+        check_attention(out[-1:], want, SCALE)
+
+
+def shared_row(c, q, lens, b):
+    return attention64(q[b:b + 1], c.values(0, b, lens[b]), c.values(1, b, lens[b]), torch.tensor([lens[b] - 1], device=c.dev), SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_many_sequences(dev, bits):
+    """Enough runs of heads for a warp each, their number no multiple of a block's warps; ragged, some empty."""
+    g = torch.Generator().manual_seed(5)
+    lens = [int(x) for x in torch.randint(0, 400, (231,), generator=g)]
+    for hq, hkv in ((32, 8), (9, 9)):
+        c = Cache(lens, hkv, bits, dev, shared=2, seed=7)
+        q = queries(len(lens), hq, dev)
+        check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, 2, max(lens), *c.args), shared64(c, q, lens), SCALE)
+        check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, 0, max(lens), *c.args), shared64(c, q, lens), SCALE)
+
+
+def test_large_values_stay_finite(dev):
+    """Values up to 60000: weights times scales and partial results stay in fp16's range."""
+    lens = [700, 900]
+    for bits in (4, 8):
+        c = Cache(lens, 1, bits, dev, shared=3, seed=3)
+        c.meta(1)[:, 0] *= 8000.0 if bits == 4 else 1000.0
+        q = queries(2, 4, dev)
+        for shared in (0, 3):
+            check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, shared, 900, *c.args), shared64(c, q, lens), SCALE)
+        check_attention(backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 900, *c.args), shared64(c, q, lens), SCALE)
+
+
+def test_calls_on_two_streams_at_once(dev):
+    """Eager calls of both operators on two streams, inputs of their own: what each gives alone."""
+    cases = []
+    for seed, lens in ((1, [3000, 2900, 3100, 2950] * 4), (2, [2800, 3300, 5000] * 5)):
+        c = Cache(lens, 2, 4, dev, shared=30, seed=seed)
+        q = queries(len(lens), 8, dev, seed)
+        cases.append((c, q, lens, torch.cuda.Stream()))
+
+    def both(c, q, lens):
+        return (backend.shared_prefix_attention(q, c.table, c.lengths, 30, max(lens), *c.args),
+                backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, max(lens), *c.args))
+    want = [both(*x[:3]) for x in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, q, lens, stream) in enumerate(cases):
+            with torch.cuda.stream(stream):
+                got[i].append(both(c, q, lens))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        assert all(torch.equal(a, b) for x in g for a, b in zip(x, w))
