@@ -94,8 +94,13 @@ class _Linear:
 class DecodeRunner:
     def __init__(self, model: str = "llama-3-8b", precision: str = "w4a8kv4", batch: int = 64, ctx: int = 1024,
                  device: Optional[torch.device] = None, tp_rank: int = 0, tp_size: int = 1, seed: int = 0, layers: Optional[int] = None,
-                 process_group=None, fused: bool = True, ops: Optional[OpSet] = None, tp_exact: bool = False, tp_peer: bool = False, no_comm: bool = False):
+                 process_group=None, fused: bool = True, ops: Optional[OpSet] = None, tp_exact: bool = False, tp_peer: bool = False, no_comm: bool = False,
+                 shared_prefix: int = 0):
         assert precision in PRECISIONS, precision
+        # the first `shared_prefix` positions of all sequences lie in the same pages (one system prompt): their attention is computed once for the batch
+        assert 0 <= shared_prefix <= ctx and shared_prefix % 64 == 0, "a shared prefix is whole pages of the context"
+        assert shared_prefix == 0 or (ops is None and tp_size == 1), "a shared prefix goes with this library's operators on one GPU"
+        self.shared_blocks = shared_prefix // 64
         self.ops = ops = ops or DEFAULT_OPS
         self.tp_exact = tp_exact
         self.fuse_attn_quant = True  # measured: attention + a separate per-token quant kernel is 1.3 % slower per step
@@ -145,9 +150,10 @@ class DecodeRunner:
         self.size_per_token = self.Hkv * D * self.kv_bits // 8
         code_bytes = 64 * self.size_per_token
         self.page_bytes = code_bytes + self.Hkv * 64 * 4  # cache_engine.py:62-66
-        n_pages = batch * self.blocks_per_seq
+        n_pages = self.shared_blocks + batch * (self.blocks_per_seq - self.shared_blocks)
         self.kpools, self.vpools, tables = [], [], []
-        blk = torch.arange(n_pages, device=dev, dtype=torch.int64).view(batch, self.blocks_per_seq)
+        blk = torch.arange(n_pages, device=dev, dtype=torch.int64)
+        blk = torch.cat([blk[:self.shared_blocks].expand(batch, -1), blk[self.shared_blocks:].view(batch, -1)], dim=1)
         for _ in range(self.L):
             pools = []
             for _kv in range(2):
@@ -220,6 +226,11 @@ class DecodeRunner:
         q = q.reshape(q.size(0), self.Hq, D)
         k = k.reshape(k.size(0), self.Hkv, D)
         v = v.reshape(v.size(0), self.Hkv, D)
+        if self.shared_blocks:
+            cache = (64, self.size_per_token, self.kv_bits == 4, True)
+            q = _ext.append_kv_cache(q, k, v, self.block_tables[li], None, self.context_lens, *cache[:2], D, cfg.rope_theta, *cache[2:])
+            attn = _ext.shared_prefix_attention(q, self.block_tables[li], self.context_lens, self.shared_blocks, self.max_seq_len, *cache, out=q)
+            return attn.reshape(q.size(0), -1)
         attn = self.ops.fused_attention.single_query_attention(
             q, k, v, self.block_tables[li], self.context_lens, None, min(8192, cfg.max_pos), 64, self.size_per_token,
             self.max_seq_len, D, cfg.rope_theta, True, self.kv_bits == 4, True)  # :265-281
@@ -276,7 +287,7 @@ class DecodeRunner:
         for li, ly in enumerate(self.layers):
             exact = self.tp_size > 1 and self.tp_exact
             ly["qkv"](self.q_hidden, self.q_scale, self.q_sum, self.qkv_buf)
-            if exact or not self.fuse_attn_quant:
+            if exact or not self.fuse_attn_quant or self.shared_blocks:
                 self._quant(self.q_attn, self._attention(li))
             else:
                 self._attention_quant(li, qsum)
@@ -299,7 +310,7 @@ class DecodeRunner:
             else:
                 ly["down"](self.q_mlp, self.q_scale, self.q_sum, self.out_buf)
                 self._allreduce(self.out_buf)
-            n += 11 if exact else 7
+            n += 11 if exact else 10 if self.shared_blocks else 7  # (append, prefix, rest and quantisation for one)
             if self.tp_peer:
                 # the last layer has no following norm: the same kernel delivers hidden + sum(partials) (its quantised output is not used)
                 gam = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else ly["ln1"]
@@ -411,5 +422,7 @@ class DecodeRunner:
     def kv_bytes_per_step(self) -> int:
         """Algorithmic KV traffic: codes + scale/zero of K and V for ctx tokens, + q in / o out."""
         B, D = self.batch, self.cfg.head_dim
-        per_layer = B * self.Hkv * self.ctx * D * self.kv_bits // 8 * 2 + B * self.Hkv * self.ctx * 8 + 4 * B * self.Hq * D
+        shared = 64 * self.shared_blocks
+        positions = B * (self.ctx - shared) + shared
+        per_layer = self.Hkv * positions * D * self.kv_bits // 8 * 2 + self.Hkv * positions * 8 + 4 * B * self.Hq * D
         return per_layer * self.L
