@@ -78,7 +78,7 @@ def _build_bind() -> str:
     cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.isabs(_nvcc()) else "/usr/local/cuda"
     inc = [f"-isystem{p}" for p in include_paths() + [sysconfig.get_paths()["include"], os.path.join(cuda, "include")]]
     cmd = ["g++", path, "-o", BIND] + flags + inc + [f"-L{p}" for p in library_paths()] + [f"-L{HERE}", "-l:libqserve_b200.so", "-lc10", "-lc10_cuda",
-           "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         sys.stderr.write(res.stdout + res.stderr)

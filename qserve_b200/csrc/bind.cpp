@@ -8,6 +8,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -294,15 +295,17 @@ Heads heads_of(const at::Tensor& t, const at::Tensor& like, const char* name) {
   // (a single row has no stride to speak of)
   return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : t.size(1) * 128, static_cast<int>(t.size(0)), static_cast<int>(t.size(1))};
 }
+// New tensors on q's device without the dispatcher's way to the allocator (read_kv_cache, two of them: 5.2 us a call on the host, 4.1 so)
+at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& q) { return at::detail::empty_cuda(size, type, q.device(), std::nullopt); }
 // the result's tensor: argument i, or a new one of q's sizes where it is None
 at::Tensor result_of(const Args& a, int i, const at::Tensor& q) {
-  if (a.none(i)) return at::empty({q.size(0), q.size(1), q.size(2)}, q.options().requires_grad(false));
+  if (a.none(i)) return fresh(q.sizes(), at::kHalf, q);
   const at::Tensor& t = a.tensor(i);
   require(t.dim() == 3 && t.size(0) == q.size(0) && t.size(1) == q.size(1) && t.size(2) == q.size(2), "out must have the sizes of q");
   return t;
 }
 // A work space of the call's own: calls on several streams and captured graphs never share one
-at::Tensor scratch(const at::Tensor& q, size_t bytes) { return at::empty({static_cast<int64_t>(bytes)}, q.options().dtype(at::kByte).requires_grad(false)); }
+at::Tensor scratch(const at::Tensor& q, size_t bytes) { return fresh({static_cast<int64_t>(bytes)}, at::kByte, q); }
 float scale_of(const Args& a, int i) { return a.none(i) ? 0.08838834764831845f : a.real(i); }
 
 // q, k, v, kv_pointers, cu_seqlens or None, lengths, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4, zeros, out or None
@@ -327,9 +330,7 @@ PyObject* read_kv_cache(const Args& a) {
   const Cache c = cache_of(a, t, 0, 1, 2, 4, 6);
   const int tokens = a.small(3);
   require(tokens >= 0, "num_tokens must not be negative");
-  const at::TensorOptions options = t.options().dtype(at::kHalf).requires_grad(false);
-  const at::Tensor kv = at::empty({2, tokens, c.heads_kv, 128}, options);  // (one allocation)
-  at::Tensor k = kv.select(0, 0), v = kv.select(0, 1);
+  at::Tensor k = fresh({tokens, c.heads_kv, 128}, at::kHalf, t), v = fresh({tokens, c.heads_kv, 128}, at::kHalf, t);
   void *kp = k.data_ptr(), *vp = v.data_ptr();
   launch(t, [&](void* s) { return qs_read_kv_cache(kp, vp, c.kvp, c.cu, c.lens, c.batch, tokens, c.max_blocks, c.heads_kv, 128, c.tpb, c.size, c.int4, c.zeros, s); });
   PyObject* const ko = THPVariable_Wrap(std::move(k));
