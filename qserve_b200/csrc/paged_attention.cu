@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     const bool alive = first_row < n_rows;  // warp-uniform; a warp without rows lets its part of Q, S and P be what it is
     const int r = first_row + lane, tok = r / group, head = hk * group + r - tok * group;
     const bool row_is = r < n_rows;
-    if (alive) {
+    if (alive && n_mine > 0) {  // (no page: the results' zeros would meet another warp's late queries in the same shared memory, for no product stands between them)
       // half a warp a row, 16 bytes a lane, all rows on their way together; where a row begins is worked out by the lane whose row it is
       uint8_t* dst = smem + tile * kQBytes;
       const int c = lane & 15;

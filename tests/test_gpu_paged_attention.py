@@ -317,3 +317,18 @@ def test_calls_on_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(a, b) for x in g for a, b in zip(x, w))
+
+
+@pytest.mark.parametrize("new,top", [([1300], 1800), ([1300], 64), ([20], 4000)])
+def test_blocks_without_a_key_write_zeros(dev, new, top):
+    """A portion whose length leaves only its last four rows a position: blocks (and splits) that see no key.  The queries come late, out of DRAM."""
+    c = Cache([4], 8, 4, dev, seed=1, extra_blocks=1)
+    q, cu = queries(new[0], 32, dev), starts(new, dev)
+    flush = torch.empty(64 << 20, dtype=torch.int32, device=dev)
+    want = attention64(q[-4:], c.values(0, 0, 4), c.values(1, 0, 4), torch.arange(4, device=dev), SCALE)
+    for i in range(10):
+        out = torch.full((new[0], 32, D), 7.0, dtype=HALF, device=dev)
+        flush.fill_(i)
+        backend.paged_prompt_attention(q, c.table, cu, c.lengths, new[0], top, *c.args, out=out)
+        assert bool((out[:-4] == 0).all())
+        check_attention(out[-4:], want, SCALE)
