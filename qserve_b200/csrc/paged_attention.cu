@@ -156,8 +156,10 @@ struct TileParams {
   int batch, num_tokens, max_seqlen, max_blocks, num_heads, num_kv_heads;
   int row_blocks, nsplit, shared_blocks;  // shared_blocks > 0: the rows of all sequences over the first sequence's first pages
   int cluster, parts;                     // blocks that join their splits through one another's shared memory; partial rows that are left: nsplit / cluster
+  int block_rows, split_from, run;        // of the items (of so many rows each; last rows first, sequence, kv head) those from here on are split; so many neighbours a run
   float scale_log2;
-  __half* part;                           // parts > 1: O / sum [rows][parts][128], rows = token * num_heads + head
+  // parts > 1: O / sum [rows][parts][128]: rows = token * num_heads + head where all items are split, otherwise those of the split items, one behind the other
+  __half* part;
   float2* part_ml;                        // (maximum, sum) [rows][parts]
 };
 
@@ -166,8 +168,28 @@ __device__ __forceinline__ uint2 scaled_h4(const float4& a, float L) {
   return make_uint2(as_u32(__floats2half2_rn(a.x * inv, a.y * inv)), as_u32(__floats2half2_rn(a.z * inv, a.w * inv)));
 }
 
-// What a block does with its rows: the result; a partial result; or its cluster's, joined first.
+// What a block does with its rows: the result; a partial result where its item is split; or its cluster's, joined first.
 enum : int { kWhole = 0, kPartial = 1, kCluster = 2 };
+// Which of the splits of which item a block takes: runs of items in turn, all of a run's first splits ahead of its second ones.  (Neighbours are the kv heads of the
+// same pages, which lie side by side.)
+struct Share {
+  unsigned item, split, nsplit;
+};
+template <int MODE>
+__device__ __forceinline__ Share share_of(const TileParams& p, unsigned block) {
+  Share s{block, 0, 1};
+  if constexpr (MODE == kCluster) {
+    s.nsplit = p.cluster;  // a power of two
+    s.split = block & (s.nsplit - 1);
+    s.item = block / s.nsplit;
+  } else if (MODE == kPartial && block >= static_cast<unsigned>(p.split_from)) {
+    s.nsplit = p.nsplit;
+    const unsigned behind = block - p.split_from, in_turn = behind / static_cast<unsigned>(p.run), run = in_turn / s.nsplit;
+    s.split = in_turn - run * s.nsplit;
+    s.item = p.split_from + run * p.run + (behind - in_turn * p.run);
+  }
+  return s;
+}
 template <int BITS, int TILES, int MODE>
 __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, TILES>::kBlocksPerSm) tile_kernel(const __grid_constant__ TileParams p) {
   using C = TileCfg<BITS, TILES>;
@@ -219,16 +241,11 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   // ---- this block's share ----
-  unsigned idx = blockIdx.x, rank = 0;
-  if constexpr (MODE == kCluster) {
-    rank = idx & (p.cluster - 1);  // a power of two
-    idx /= static_cast<unsigned>(p.cluster);
-  }
-  const int hk = idx % static_cast<unsigned>(p.num_kv_heads);
-  idx /= static_cast<unsigned>(p.num_kv_heads);
-  const int part = idx % static_cast<unsigned>(p.parts), split = MODE == kCluster ? part * p.cluster + rank : part;
-  idx /= static_cast<unsigned>(p.parts);
-  const int b = idx % static_cast<unsigned>(p.batch), rb = p.row_blocks - 1 - static_cast<int>(idx / static_cast<unsigned>(p.batch));  // the last rows see most keys: first
+  const Share share = share_of<MODE>(p, blockIdx.x);
+  int hk = share.item % static_cast<unsigned>(p.num_kv_heads);
+  const unsigned of_rows = share.item / static_cast<unsigned>(p.num_kv_heads);
+  int b = of_rows % static_cast<unsigned>(p.batch), rb = p.row_blocks - 1 - static_cast<int>(of_rows / static_cast<unsigned>(p.batch));  // the last rows see most keys: first
+  asm volatile("" : "+r"(hk), "+r"(b), "+r"(rb));  // (as they are, not worked out again inside the loops: INT8 spilled, 1 to 2 % of a call)
   const int group = static_cast<unsigned>(p.num_heads) / static_cast<unsigned>(p.num_kv_heads);
   pdl_wait();
   // Only now: what is launched next may read what this kernel's predecessors wrote (the tail kernel does, ahead of its own wait)
@@ -248,8 +265,9 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   }
   const int n_pages = (n_keys + kPage - 1) / kPage;
   // (nsplit <= 128 splits of at most 2^24 pages: 32 bits hold the products)
-  const int page0 = static_cast<int>(static_cast<unsigned>(split) * n_pages / p.nsplit);
-  const int n_mine = any ? static_cast<int>(static_cast<unsigned>(split + 1) * n_pages / p.nsplit) - page0 : 0;
+  int page0 = static_cast<int>(share.split * n_pages / share.nsplit);
+  int n_mine = any ? static_cast<int>((share.split + 1) * n_pages / share.nsplit) - page0 : 0;
+  asm volatile("" : "+r"(page0), "+r"(n_mine));
 
   if (warp >= kUnpackWarp && warp < kIssueWarp) {
     // ===================================== unpacking =====================================
@@ -259,6 +277,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     const int key = t >> 1, part = t & 1;
     const uint32_t row_at = part * kKvHalf + key * 128, swizzle = key & 7;
     const long long* ptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + page0;
+    asm volatile("" : "+l"(ptrs));  // (not worked out again for every page either)
     constexpr int kWords = BITS / 2;  // 16-byte words of a thread's 64 codes
     struct Raw {
       uint4 k[kWords], v[kWords];
@@ -547,9 +566,20 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
       // Through shared memory (the tile's queries are done with), so that half a warp stores a whole row
       uint8_t* mine = smem + tile * kQBytes + quarter * (kQBytes / 4);
-      const long long token = portion.start + tok, at = (token * p.num_heads + head) * p.parts + part;
+      const long long token = portion.start + tok;
+      bool partial = false;
+      long long at = 0;
+      if constexpr (MODE == kPartial) {
+        unsigned block;  // (read again, so that the loop above holds nothing of it: it has no register to spare)
+        asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block));
+        const Share mine = share_of<MODE>(p, block);
+        partial = block >= static_cast<unsigned>(p.split_from);
+        const int row = p.split_from == 0 ? static_cast<int>(token) * p.num_heads + head
+                                          : static_cast<int>(mine.item - p.split_from) * (TILES * kRows) + (tile * kRows + quarter * 32 + lane);
+        at = static_cast<long long>(row) * p.parts + mine.split;
+      }
       unsigned long long to = 0ull;
-      if (row_is) to = MODE == kPartial ? reinterpret_cast<unsigned long long>(p.part + at * kD)
+      if (row_is) to = partial ? reinterpret_cast<unsigned long long>(p.part + at * kD)
                                         : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
 #pragma unroll 1
       for (int c = 0; c < 4; ++c) {
@@ -580,7 +610,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
           const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
           if (row) row[chunk] = v;
         }
-        if (MODE == kPartial && row_is) p.part_ml[at] = make_float2(m_used, l);
+        if (partial && row_is) p.part_ml[at] = make_float2(m_used, l);
       } else {
         s_ml[quarter * 32 + lane] = make_float2(m_used, l);
       }
@@ -590,7 +620,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       cluster_sync();
       const int rows = min(n_rows - row_base, kRows), chunk = lane & 15;
 #pragma unroll 1
-      for (int i = static_cast<int>(rank) + p.cluster * (2 * warp + (lane >> 4)); i < rows; i += p.cluster * 8) {
+      for (int i = static_cast<int>(share.split) + p.cluster * (2 * warp + (lane >> 4)); i < rows; i += p.cluster * 8) {
         const uint8_t* at = smem + i * 256 + ((chunk ^ (i & 7)) << 4);
         uint4 x[kMostCluster];
         float2 ml[kMostCluster];
@@ -677,24 +707,41 @@ __device__ __forceinline__ void join_rows(const __half* part, const float2* ml, 
   }
 }
 
-// Rows of the result, WARPS warps each (they take turns over the splits); rows behind the last sequence are left as they are.
+// The rows that were split (all of them, by token and head; or those of some items), WARPS warps each (they take turns over the splits).  Rows behind the last
+// sequence are left as they are.
 template <int WARPS>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileParams p) {
   __shared__ __align__(16) float s_acc[4][kD];
   __shared__ float2 s_ml[4];
   pdl_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long row = static_cast<long long>(blockIdx.x) * (4 / WARPS) + warp / WARPS;
-  const bool in = row < static_cast<long long>(p.num_tokens) * p.num_heads;
-  const int token = in ? static_cast<int>(row / p.num_heads) : 0, head = in ? static_cast<int>(row - static_cast<long long>(token) * p.num_heads) : 0;
-  pdl_wait();
-  const int b = in ? sequence_of(p.cu, p.batch, token) : -1;
-  const bool mine = b >= 0 && token - (p.cu ? p.cu[b] : b) < p.max_seqlen;
+  const unsigned row = blockIdx.x * (4 / WARPS) + warp / WARPS;
+  bool mine;
+  long long token;
+  int head;
+  if (p.split_from == 0) {
+    const unsigned t = row / static_cast<unsigned>(p.num_heads);
+    token = t;
+    head = static_cast<int>(row - t * p.num_heads);
+    pdl_wait();
+    const int b = t < static_cast<unsigned>(p.num_tokens) ? sequence_of(p.cu, p.batch, static_cast<int>(t)) : -1;
+    mine = b >= 0 && static_cast<int>(t) - (p.cu ? p.cu[b] : b) < p.max_seqlen;
+  } else {
+    const unsigned behind = row / static_cast<unsigned>(p.block_rows), item = p.split_from + behind, of_rows = item / static_cast<unsigned>(p.num_kv_heads);
+    const int hk = item - of_rows * p.num_kv_heads, b = of_rows % static_cast<unsigned>(p.batch), rb = p.row_blocks - 1 - static_cast<int>(of_rows / static_cast<unsigned>(p.batch));
+    const int r = rb * p.block_rows + static_cast<int>(row - behind * p.block_rows), group = p.num_heads / p.num_kv_heads, tok = r / group;
+    pdl_wait();
+    const Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
+    mine = tok < min(portion.count, p.max_seqlen);
+    token = portion.start + tok;
+    head = hk * group + r - tok * group;
+  }
   float M = -CUDART_INF_F, L = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   // this warp's run of the splits
   const int part = warp % WARPS, s0 = p.parts * part / WARPS, s1 = p.parts * (part + 1) / WARPS;
-  if (mine) join_rows(p.part + (row * p.parts + s0) * kD, p.part_ml + row * p.parts + s0, s1 - s0, M, L, acc);
+  const long long at = static_cast<long long>(row) * p.parts + s0;
+  if (mine) join_rows(p.part + at * kD, p.part_ml + at, s1 - s0, M, L, acc);
   if constexpr (WARPS > 1) {
     reinterpret_cast<float4*>(s_acc[warp])[lane] = acc;
     if (lane == 0) s_ml[warp] = make_float2(M, L);
@@ -1119,40 +1166,65 @@ int allow_smem(int bytes, const char* what, Enough enough) {
   return rc;
 }
 
-// How a call over `rows` rows per kv head and sequence (`outputs` result rows in all) and at most `pages` pages is cut: tiles per block, and splits of the pages.  The
+// How a call over `rows` rows per kv head and sequence (`num_rows` of a kv head in all) and at most `pages` pages is cut: tiles per block, and splits of the pages.  The
 // cut whose time is estimated lowest: rounds of blocks over the device, each its pages and what comes ahead of the first and behind the last, and the joining of
-// the splits: by a cluster of up to eight blocks (one tile of a prompt), by join_kernel, or in the tail kernel.  The figures, in us, are those of the kernels' own
-// timelines; one or two one-tile blocks share a multiprocessor.  Measured, us: 17 tokens behind 500 in a cluster 7.8, with join_kernel 8.5; 4 behind 4000 9.2 and
-// 12.3; 24 behind 60000 one block per multiprocessor 54, two 46; 8 sequences behind 4096 shared positions two 13.9, one 11.6.  Splits that make more than one round
-// did not pay (4096 tokens behind 12000, three and a half rounds of blocks: 830, in two splits 865; six portions of 250: 64.5 and 81.8), nor clusters of two blocks
-// per multiprocessor (four of 20 behind 8000, INT8: 37.4, join_kernel 34.5).
+// the splits: by a cluster of up to eight blocks (one tile of a prompt), by join_kernel, or in the tail kernel.  All items are split where they leave room in one
+// round; in a prompt of more rounds the items of the last round, or of the last two, where those would not fill the device.  The figures, in us, are those of the
+// kernels' own timelines; one or two one-tile blocks share a multiprocessor.  Measured, us: 17 tokens behind 500 in a cluster 7.8, with join_kernel 8.5; 4 behind 4000
+// 9.2 and 12.3; 24 behind 60000 one block per multiprocessor 54, two 46; 8 sequences behind 4096 shared positions two 13.9, one 11.6.  Rounds left whole and with the
+// rest split: 4096 tokens behind 12000 (3.5 rounds) 846 and 783, 1500 behind 6000 196 and 155, 1200 of 32 kv heads behind 30000 (160 blocks) 912 and 545.  Not for
+// small gains over sequences of unequal length, whose last round is short anyway (six portions of 250: 64.4 and 68.7); nor all items of several rounds (81.8), nor
+// clusters of two blocks per multiprocessor (four of 20 behind 8000, INT8: 37.4, join_kernel 34.5).
 struct Plan {
   int tiles, row_blocks, nsplit, cluster, parts;
+  long long items, split;  // (rows of a block, kv head) pairs; the last so many of them are split
+  long long split_rows(long long all) const { return split == items ? all : split * tiles * kRows; }
 };
-Plan plan_tiles(long long rows, long long items, long long outputs, long long pages, bool prompt) {
-  constexpr float kFixed = 3.5f, kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 5e6f;
-  Plan pl;
+Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, long long pages, bool prompt) {
+  constexpr float kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 5e6f;
+  Plan pl{};
   pl.tiles = rows <= kRows ? 1 : 2;
-  pl.row_blocks = static_cast<int>((rows + pl.tiles * kRows - 1) / (pl.tiles * kRows));
-  const long long blocks = items * pl.row_blocks, sms = num_sms();
+  const long long block_rows = pl.tiles * kRows, sms = num_sms();
+  pl.row_blocks = static_cast<int>((rows + block_rows - 1) / block_rows);
+  pl.items = static_cast<long long>(pl.row_blocks) * batch * kv_heads;
+  // blocks that have rows: of portions of unequal length the shorter ones leave some without
+  long long blocks = static_cast<long long>(kv_heads) * ((2 * num_rows + batch * block_rows + 2 * block_rows - 1) / (2 * block_rows));
+  blocks = blocks < 1 ? 1 : blocks > pl.items ? pl.items : blocks;
   const unsigned most = static_cast<unsigned>(pages < 1 ? 1 : pages);
+  const float fixed = pl.tiles == 2 ? 5.5f : 3.5f;
   float best = 3.0e38f;
-  pl.nsplit = pl.cluster = 1;
+  auto take = [&](float t, unsigned n, unsigned cluster, long long split) {
+    if (t >= best) return;
+    best = t;
+    pl.nsplit = static_cast<int>(n);
+    pl.cluster = static_cast<int>(cluster);
+    pl.split = split;
+  };
   for (int per_sm = 1; per_sm <= (pl.tiles == 1 ? 2 : 1); ++per_sm) {
     const float page = pl.tiles == 2 ? 0.92f : per_sm == 1 ? (rows <= 64 ? 0.7f : 0.95f) : (rows <= 64 ? 1.f : 1.2f);
-    const float part = prompt ? outputs * (2.f * (kD * 2 + 8)) / kPartBytesPerUs : kJoinTail;
-    const long long room = blocks > 0 ? sms * per_sm / blocks : 1;  // splits of one round
-    const unsigned last = static_cast<unsigned>(room < 1 ? 1 : room > 128 ? 128 : room);
-    for (unsigned n = per_sm == 1 ? 1 : static_cast<unsigned>(sms / (blocks > 0 ? blocks : 1)) + 1; n <= last && n <= most; ++n) {
-      const bool cluster = prompt && pl.tiles == 1 && per_sm == 1 && n > 1 && n <= kMostCluster && (n & (n - 1)) == 0;
-      float t = ((most + n - 1) / n) * page + kFixed;
-      if (n == 1) t *= static_cast<float>((blocks + sms * per_sm - 1) / (sms * per_sm));
-      else t += cluster ? kJoinCluster : (prompt ? kJoinKernel : 0.f) + part * n;
-      if (t < best) {
-        best = t;
-        pl.nsplit = static_cast<int>(n);
-        pl.cluster = cluster ? static_cast<int>(n) : 1;
-      }
+    const long long slots = sms * per_sm;
+    auto block = [&](unsigned n) { return ((most + n - 1) / n) * page + fixed; };
+    // sequences of a batch differ in length, and the blocks of the last round are short beside the longest: half of what it lacks to be full
+    auto rounds = [&](long long of) {
+      const float full = static_cast<float>((of + slots - 1) / slots);
+      return batch == 1 || of <= slots ? full : 0.5f * (full + of / static_cast<float>(slots));
+    };
+    auto join = [&](long long split, unsigned n) {
+      return prompt ? kJoinKernel + (split * (num_rows * kv_heads / static_cast<float>(blocks)) * n) * (2.f * (kD * 2 + 8)) / kPartBytesPerUs : kJoinTail * n;
+    };
+    take(rounds(blocks) * block(1), 1, 1, prompt ? 0 : pl.items);
+    // splits of one round
+    const long long room = slots / blocks;
+    const unsigned last = static_cast<unsigned>(room > 128 ? 128 : room);
+    for (unsigned n = per_sm == 1 || sms < blocks ? 2 : static_cast<unsigned>(sms / blocks) + 1; n <= last && n <= most; ++n) {
+      const bool cluster = prompt && pl.tiles == 1 && per_sm == 1 && n <= kMostCluster && (n & (n - 1)) == 0;
+      take(block(n) + (cluster ? kJoinCluster : join(pl.items, n)), n, cluster ? n : 1, pl.items);
+    }
+    // whole rounds, and splits of the rest
+    for (long long whole = blocks / slots; prompt && whole >= 1 && whole + 1 >= blocks / slots; --whole) {
+      const long long rest = blocks - whole * slots;
+      const float of_doubt = batch == 1 ? 1.f : 1.1f;
+      for (unsigned n = 2; rest > 0 && n <= 8 && n <= most; ++n) take((whole * block(1) + rounds(rest * n) * block(n) + join(rest, n)) * of_doubt, n, 1, rest);
     }
   }
   pl.parts = pl.nsplit / pl.cluster;
@@ -1161,27 +1233,29 @@ Plan plan_tiles(long long rows, long long items, long long outputs, long long pa
 size_t part_bytes(long long rows, int parts) { return static_cast<size_t>(rows) * parts * (kD * sizeof(__half) + sizeof(float2)); }
 
 template <int BITS, int TILES, int MODE>
-int run_tiles(const TileParams& p, int batch_items, void* stream) {
+int run_tiles(const TileParams& p, long long blocks, void* stream) {
   using C = TileCfg<BITS, TILES>;
   const int rc = allow_smem<tile_kernel<BITS, TILES, MODE>>(C::kSmem, "paged attention: shared memory", [](int regs) { return !C::kShares || shares_suffice(regs); });
   if (rc) return rc;
-  const long long blocks = static_cast<long long>(p.row_blocks) * batch_items * p.nsplit * p.num_kv_heads;
   QS_REQUIRE(blocks <= 0x7fffffffll, "paged attention: %lld blocks", blocks);
   return launch(tile_kernel<BITS, TILES, MODE>, dim3(static_cast<unsigned>(blocks)), C::kThreads, C::kSmem, stream, "paged attention", p.cluster, p);
 }
-int tiles(TileParams& p, const Plan& pl, bool int4, int items, void* stream) {
+int tiles(TileParams& p, const Plan& pl, bool int4, void* stream) {
   p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.cluster = pl.cluster; p.parts = pl.parts;
+  p.split_from = static_cast<int>(pl.items - pl.split); p.block_rows = pl.tiles * kRows; p.run = p.split_from ? static_cast<int>(pl.split) : p.num_kv_heads;
+  const long long blocks = pl.items + pl.split * (pl.nsplit - 1);
   auto sized = [&](auto bits) {
     constexpr int kBits = decltype(bits)::value;
-    if (pl.tiles == 2) return p.part ? run_tiles<kBits, 2, kPartial>(p, items, stream) : run_tiles<kBits, 2, kWhole>(p, items, stream);
-    if (pl.cluster > 1) return run_tiles<kBits, 1, kCluster>(p, items, stream);
-    return p.part ? run_tiles<kBits, 1, kPartial>(p, items, stream) : run_tiles<kBits, 1, kWhole>(p, items, stream);
+    if (pl.tiles == 2) return p.part ? run_tiles<kBits, 2, kPartial>(p, blocks, stream) : run_tiles<kBits, 2, kWhole>(p, blocks, stream);
+    if (pl.cluster > 1) return run_tiles<kBits, 1, kCluster>(p, blocks, stream);
+    return p.part ? run_tiles<kBits, 1, kPartial>(p, blocks, stream) : run_tiles<kBits, 1, kWhole>(p, blocks, stream);
   };
   return int4 ? sized(std::integral_constant<int, 4>{}) : sized(std::integral_constant<int, 8>{});
 }
 
 Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
-  return plan_tiles(static_cast<long long>(max_seqlen) * (heads / kv_heads), static_cast<long long>(batch) * kv_heads, static_cast<long long>(num_tokens) * heads,
+  const int group = heads / kv_heads;
+  return plan_tiles(static_cast<long long>(max_seqlen) * group, batch, static_cast<long long>(num_tokens) * group, kv_heads,
                     (static_cast<long long>(max_length) + kPage - 1) / kPage, true);
 }
 // Few sequences or few shared pages: the tail kernel reads every sequence's whole table, one launch instead of two.  us, both kernels / the tail alone (INT4, 32 heads
@@ -1189,7 +1263,8 @@ Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int 
 // 4.9, behind 512 6.6 / 8.7.
 bool tail_alone(int batch, int shared_blocks) { return batch == 1 || static_cast<long long>(batch) * shared_blocks <= 16; }
 Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
-  return plan_tiles(static_cast<long long>(batch) * (heads / kv_heads), kv_heads, static_cast<long long>(batch) * heads, shared_blocks, false);
+  const long long rows = static_cast<long long>(batch) * (heads / kv_heads);
+  return plan_tiles(rows, 1, rows, kv_heads, shared_blocks, false);
 }
 
 }  // namespace
@@ -1197,7 +1272,7 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
   if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
   const Plan pl = plan_prompt(batch, num_tokens, max_seqlen, max_length, heads, kv_heads);
-  return pl.parts > 1 ? part_bytes(static_cast<long long>(num_tokens) * heads, pl.parts) : 0;
+  return pl.parts > 1 ? part_bytes(pl.split_rows(static_cast<long long>(num_tokens) * heads), pl.parts) : 0;
 }
 
 int paged_prompt_attention(const PagedAttnArgs& a) {
@@ -1208,7 +1283,7 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths;
   p.batch = a.batch; p.num_tokens = a.num_tokens; p.max_seqlen = a.max_seqlen; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  const long long rows = static_cast<long long>(a.num_tokens) * a.num_heads;
+  const long long rows = pl.split_rows(static_cast<long long>(a.num_tokens) * a.num_heads);
   if (pl.parts > 1) {
     QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.parts), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
                part_bytes(rows, pl.parts));
@@ -1216,7 +1291,7 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
     p.part = static_cast<__half*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
   }
-  const int rc = tiles(p, pl, a.cache.int4, a.batch, a.stream);
+  const int rc = tiles(p, pl, a.cache.int4, a.stream);
   if (rc || pl.parts == 1) return rc;
   const bool wide = pl.parts >= 8;  // (24 tokens behind 60000, 37 parts: a warp a row 52.8 us, four 48.9; 17 behind 500, nine: 11.0 and 10.5)
   return launch(wide ? join_kernel<4> : join_kernel<1>, dim3(static_cast<unsigned>(wide ? rows : (rows + 3) / 4)), 128, 0, a.stream, "paged_prompt_attention: join", 1, p);
@@ -1246,7 +1321,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
     p.part = static_cast<__half*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
     t.nsplit = pl.parts; t.part = p.part; t.part_ml = p.part_ml;
-    const int rc = tiles(p, pl, a.cache.int4, 1, a.stream);
+    const int rc = tiles(p, pl, a.cache.int4, a.stream);
     if (rc) return rc;
   }
   const int group = a.num_heads / t.num_kv_heads, heads_y = t.num_kv_heads * ((group + kMaxG - 1) / kMaxG);

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from qserve_b200 import backend
+from qserve_b200._lib import lib
 from tests.paged_util import D, F64, HALF, PAGE, Cache, attention64, check_attention
 
 pytestmark = pytest.mark.gpu
@@ -317,6 +318,28 @@ def test_calls_on_two_streams_at_once(dev):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(a, b) for x in g for a, b in zip(x, w))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,new,ahead", [(152, 152, [130], [400]), (32, 8, [1300], [500]), (32, 8, [20] * 30 + [0, 3] + [20] * 6, [2500, 2400] * 19)])
+def test_the_last_round_is_split(dev, bits, hq, hkv, new, ahead):
+    """More blocks than the device holds, so few of them in the last round that they are split (152 and 168 blocks of two tiles, 304 of one; a work space shows it)."""
+    lens = [n + m for n, m in zip(new, ahead)]
+    T, most = sum(new), max(new)
+    c = Cache(lens, hkv, bits, dev, seed=hq + len(new))
+    size = lib.qs_paged_prompt_attention_workspace_bytes(len(new), T, most, max(lens), hq, hkv)
+    assert 0 < size < 2 * T * hq * (2 * D + 8)
+    q = queries(T + 3, hq, dev)
+    out = torch.full((T + 3, hq, D), 7.0, dtype=HALF, device=dev)
+    backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, most, max(lens), *c.args, out=out)
+    assert bool((out[T:] == 7).all())
+    check_attention(out[:T], prompt64(c, q[:T], new, lens), SCALE)
+    # the last portion shorter than it says: its first rows have no position
+    c.lengths[-1] = 4
+    backend.paged_prompt_attention(q, c.table, starts(new, dev), c.lengths, most, max(lens), *c.args, out=out)
+    n = new[-1]
+    assert bool((out[T:] == 7).all()) and bool((out[T - n:T - 4] == 0).all())
+    check_attention(out[T - 4:T], attention64(q[T - 4:T], c.values(0, len(new) - 1, 4), c.values(1, len(new) - 1, 4), torch.arange(4, device=dev), SCALE), SCALE)
 
 
 @pytest.mark.parametrize("new,top", [([1300], 1800), ([1300], 64), ([20], 4000)])
