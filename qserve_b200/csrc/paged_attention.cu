@@ -929,7 +929,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
       if constexpr (BITS == 4) {
         const int k0 = 4 * (s >> 1) + (s & 1);
         qb0[s] = __byte_perm(qw[k0], qw[k0 + 2], 0x5410);
-        qb1[s] = as_u32(__hmul2(as_h2(__byte_perm(qw[k0], qw[k0 + 2], 0x7632)), __float2half2_rn(0.0625f)));  // high nibbles are 16 u
+        qb1[s] = __byte_perm(qw[k0], qw[k0 + 2], 0x7632);
       } else {
         qb0[s] = qw[2 * s];
         qb1[s] = qw[2 * s + 1];
@@ -940,7 +940,8 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
   float o[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-  float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f, c0 = 0.f, c1 = 0.f;
+  float m0 = -CUDART_INF_F, m1 = -CUDART_INF_F, ref0 = -CUDART_INF_F, ref1 = -CUDART_INF_F, l0 = 0.f, l1 = 0.f, c0 = 0.f, c1 = 0.f;
+  float s_top = 5.9604645e-8f;  // 2^-24, the smallest scale
   const int tokA = (g & 1) * 4 + (g >> 1);
   const uint32_t k_at = SC::place(tokA, BITS == 4 ? q4 : 2 * q4);
   const uint32_t v_at = SC::place((lane & 1) * 4 + ((lane >> 1) & 3) + (lane & 8), lane >> 4) + SC::kOffV;
@@ -964,18 +965,22 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
     }
     __syncwarp();
     float sc[2][4] = {};
+    float vmax = 0.f;  // of the values' scales
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       const uint8_t* krow = st + c * 16 * SC::kRow + k_at;
       if constexpr (BITS == 4) {
         const uint4 ka = *reinterpret_cast<const uint4*>(krow), kb = *reinterpret_cast<const uint4*>(krow + 8 * SC::kRow);
         const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kb.x, kb.y, kb.z, kb.w};
+        float high[4] = {};  // of the high nibbles, which are 16 u: by themselves, for q / 16 may not be an fp16 number
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t xa = wa[w], xb = wb[w], ta = xa >> 8, tb = xb >> 8;
-          mma_16816(sc[c], xa & 0x000f000fu, xb & 0x000f000fu, xa & 0x00f000f0u, xb & 0x00f000f0u, qb0[2 * w], qb1[2 * w]);
-          mma_16816(sc[c], ta & 0x000f000fu, tb & 0x000f000fu, ta & 0x00f000f0u, tb & 0x00f000f0u, qb0[2 * w + 1], qb1[2 * w + 1]);
+          mma_16816(sc[c], xa & 0x000f000fu, xb & 0x000f000fu, ta & 0x000f000fu, tb & 0x000f000fu, qb0[2 * w], qb0[2 * w + 1]);
+          mma_16816(high, xa & 0x00f000f0u, xb & 0x00f000f0u, ta & 0x00f000f0u, tb & 0x00f000f0u, qb1[2 * w], qb1[2 * w + 1]);
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sc[c][e] = fmaf(high[e], 0.0625f, sc[c][e]);
       } else {
         const uint8_t* krow1 = st + c * 16 * SC::kRow + (k_at ^ 16u);
         const uint4 ka0 = *reinterpret_cast<const uint4*>(krow), ka1 = *reinterpret_cast<const uint4*>(krow1);
@@ -995,6 +1000,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
       const float2 kA = s_meta[warp][0][c * 16 + tokA], kB = s_meta[warp][0][c * 16 + 8 + tokA];
       const float2 vA = s_meta[warp][1][c * 16 + tokA], vB = s_meta[warp][1][c * 16 + 8 + tokA];
       vs[c][0] = vA.x; vs[c][1] = vB.x; vc[c][0] = vA.y; vc[c][1] = vB.y;
+      vmax = fmaxf(vmax, fmaxf(fabsf(vA.x), fabsf(vB.x)));
       tl[c][0] = fmaf(kA.x, sc[c][0], kA.y * sumq0);
       tl[c][1] = fmaf(kA.x, sc[c][1], kA.y * sumq1);
       tl[c][2] = fmaf(kB.x, sc[c][2], kB.y * sumq0);
@@ -1004,18 +1010,23 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
         if (t0 + c * 16 + 8 + tokA >= len) tl[c][2] = tl[c][3] = -CUDART_INF_F;
       }
     }
-    // A weight is at most 1 (a slice always has a key, so the maxima are numbers): p s stays in the range of fp16 whatever a value's scale is
+    // The weights are 2^up times those against the maximum, 2^up times the largest scale of a value so far 2^15: p s stays in the range of fp16 whatever the scales
+    // are, and is no subnormal number where they are small.  (A slice always has a key, so the maxima are numbers.)
     float mh0 = fmaxf(fmaxf(tl[0][0], tl[0][2]), fmaxf(tl[1][0], tl[1][2])), mh1 = fmaxf(fmaxf(tl[0][1], tl[0][3]), fmaxf(tl[1][1], tl[1][3]));
-    if (__any_sync(0xffffffffu, mh0 > m0 || mh1 > m1)) {
+    if (__any_sync(0xffffffffu, mh0 > m0 || mh1 > m1 || vmax > s_top)) {
 #pragma unroll
       for (int m = 4; m <= 16; m <<= 1) {
         mh0 = fmaxf(mh0, __shfl_xor_sync(0xffffffffu, mh0, m));
         mh1 = fmaxf(mh1, __shfl_xor_sync(0xffffffffu, mh1, m));
+        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, m));
       }
-      const bool n0 = mh0 > m0, n1 = mh1 > m1;
-      const float a0 = n0 ? ex2(m0 - mh0) : 1.f, a1 = n1 ? ex2(m1 - mh1) : 1.f;
-      if (n0) m0 = mh0;
-      if (n1) m1 = mh1;
+      if (vmax > s_top) s_top = __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u);  // the next power of two
+      const float up = static_cast<float>(142 - static_cast<int>(__float_as_uint(s_top) >> 23));
+      m0 = fmaxf(m0, mh0);
+      m1 = fmaxf(m1, mh1);
+      const float a0 = ex2(ref0 - (m0 - up)), a1 = ex2(ref1 - (m1 - up));  // (nothing so far: 2^-inf)
+      ref0 = m0 - up;
+      ref1 = m1 - up;
       l0 *= a0; c0 *= a0; l1 *= a1; c1 *= a1;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -1026,7 +1037,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
     uint32_t bp[2][2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const float pA0 = ex2(tl[c][0] - m0), pA1 = ex2(tl[c][1] - m1), pB0 = ex2(tl[c][2] - m0), pB1 = ex2(tl[c][3] - m1);
+      const float pA0 = ex2(tl[c][0] - ref0), pA1 = ex2(tl[c][1] - ref1), pB0 = ex2(tl[c][2] - ref0), pB1 = ex2(tl[c][3] - ref1);
       l0 += pA0 + pB0; l1 += pA1 + pB1;
       c0 = fmaf(pA0, vc[c][0], fmaf(pB0, vc[c][1], c0));
       c1 = fmaf(pA1, vc[c][0], fmaf(pB1, vc[c][1], c1));
@@ -1069,7 +1080,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
     c1 += __shfl_xor_sync(0xffffffffu, c1, m);
   }
   if (g == 0) {
-    s_m[warp][2 * q4] = m0; s_m[warp][2 * q4 + 1] = m1;
+    s_m[warp][2 * q4] = ref0; s_m[warp][2 * q4 + 1] = ref1;
     s_l[warp][2 * q4] = l0; s_l[warp][2 * q4 + 1] = l1;
   }
   {

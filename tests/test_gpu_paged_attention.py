@@ -355,3 +355,24 @@ def test_blocks_without_a_key_write_zeros(dev, new, top):
         backend.paged_prompt_attention(q, c.table, cu, c.lengths, new[0], top, *c.args, out=out)
         assert bool((out[:-4] == 0).all())
         check_attention(out[-4:], want, SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("shared,lens", [(0, [700]), (1, [65, 130, 333] * 5), (3, [200, 1500] * 9), (1, [150] * 300)])
+@pytest.mark.parametrize("how", ["small queries", "small values", "growing values", "falling values"])
+def test_small_numbers(dev, bits, shared, lens, how):
+    """Queries of 2^-13 (as products of nibbles 16 u they would be halved four times) and values' scales down to 2^-8 of the others' (subnormal numbers of INT8): as exact
+    as any others."""
+    c = Cache(lens, 2, bits, dev, shared=shared, seed=sum(lens))
+    q, scale = queries(len(lens), 8, dev), SCALE
+    if how == "small queries":
+        q, scale = q * 2.0 ** -13, SCALE * 2.0 ** 13
+    else:
+        at = torch.arange(c.blocks, device=dev) * 8.0 / max(c.blocks - 1, 1)  # by page
+        power = {"small values": at * 0 - 8, "growing values": at - 8, "falling values": -at}[how]
+        for b in range(len(lens)):
+            for j in range(c.blocks):
+                if b == 0 or j >= shared:
+                    c.meta(1)[c.pages[b, j], 0] *= float(2.0 ** power[j])
+    out = backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args, softmax_scale=scale)
+    check_attention(out, shared64(c, q, lens, scale), scale)
