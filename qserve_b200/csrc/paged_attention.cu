@@ -114,6 +114,7 @@ constexpr int kKvBytes = kPage * kD * 2;     // a page's K or V as fp16, two hal
 constexpr int kKvHalf = kKvBytes / 2;
 constexpr int kMostCluster = 8;
 constexpr float kRescale = 8.f;              // log2 units that a row's maximum may grow before O is rescaled
+constexpr float kLift = 6.f;                 // log2 of the largest weight after that: fp16 holds 2^14, and weights down to 2^-20 of the largest are no subnormal numbers
 // Of a tile's tensor memory columns: S and then P of even pages [0, 64), of odd pages [64, 128), O [128, 256).  A page's P takes the place of its own S, so the next
 // page's S is there before this one's softmax ends, and P waits for no product.
 constexpr uint32_t kTileCols = 256, kColO = 128;
@@ -520,13 +521,13 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
           for (int i = 0; i < 32; i += 2) top[(i >> 1) & 3] = max3(top[(i >> 1) & 3], __uint_as_float(x[c][i]), __uint_as_float(x[c][i + 1]));
         const float m_page = fmaxf(max3(top[0], top[1], top[2]), top[3]) * p.scale_log2;
         if (j == 0) {
-          m_used = m_page;
+          m_used = m_page - kLift;
         } else {
-          const bool grow = m_page - m_used > kRescale;  // also from -inf; a row that has seen nothing yet and sees nothing here: NaN, no
+          const bool grow = m_page - m_used > kLift + kRescale;  // also from -inf; a row that has seen nothing yet and sees nothing here: NaN, no
           if (__any_sync(0xffffffffu, grow)) {
             mbar_wait(&bar_o[tile * 2 + ((j - 1) & 1)], static_cast<uint32_t>((j - 1) >> 1) & 1u);  // the O += P V before
             tc_fence_after();
-            const float m_new = grow ? m_page : m_used;
+            const float m_new = grow ? m_page - kLift : m_used;
             const float alpha = grow ? ex2(m_used - m_new) : 1.f;
 #pragma unroll 1
             for (int c = 0; c < kD / 32; ++c) {
