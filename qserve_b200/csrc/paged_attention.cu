@@ -319,8 +319,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 #pragma unroll
       for (int i = 0; i < kWords; ++i) r.v[i] = v[i ^ (part * (kWords / 2))];
     };
-    auto unpack = [&](const uint4 (&raw)[kWords], __half s, __half c, uint8_t* dst) {
-      const __half2 s2 = __half2half2(s), c2 = __half2half2(c);
+    auto unpack = [&](const uint4 (&raw)[kWords], __half2 s2, __half2 c2, uint8_t* dst) {
       uint8_t* row = dst + row_at;
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
@@ -355,24 +354,42 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       __syncwarp();
     };
     auto step = [&](Raw& raw, int j) {
-      // A row of K or V whose scale or zero is no finite number stands for NaN: the key's score is NaN then (and goes where the key is masked), its value 0, so
-      // that a weight of 0 in a row that does not see it stays 0.
       const bool live = (page0 + j) * kPage + key < n_keys;
-      __half ks = raw.ks, kz = raw.kz, vs = raw.vs, vz = raw.vz;
-      auto endless = [](__half h) { return (__half_as_ushort(h) & 0x7c00u) == 0x7c00u; };
-      bool bad = endless(ks) || endless(kz) || endless(vs) || endless(vz);
-      __half kc = BITS == 4 ? __hmul(__hneg(ks), kz) : kz, vc = BITS == 4 ? __hmul(__hneg(vs), vz) : vz;
-      bad = bad || endless(kc) || endless(vc);
-      if (!live || bad) {
-        vs = vc = __ushort_as_half(0);
-        ks = kc = __ushort_as_half(live ? 0x7fffu : 0);
+      // (K, V)
+      __half2 s = __halves2half2(raw.ks, raw.vs), c = __halves2half2(raw.kz, raw.vz), most;  // what the row's codes stand for is no further from 0
+      if constexpr (BITS == 4) {
+        c = __hmul2(__hneg2(s), c);
+        most = __hmax2(__habs2(__hfma2(s, __float2half2_rn(15.f), c)), __habs2(c));
+      } else {
+        most = __hmul2(__habs2(s), __hmax2(__habs2(c), __habs2(__hsub2(__float2half2_rn(255.f), c))));
+      }
+      const uint32_t endless = as_u32(most) & 0x7c007c00u;
+      if (!live) {
+        s = c = __float2half2_rn(0.f);
+      } else if ((endless & 0xffffu) == 0x7c00u || endless >= 0x7c000000u) {
+        // A row of K or V whose scale or zero is no finite number stands for NaN: the key's score is NaN then (and goes where the key is masked), its value 0, so
+        // that a weight of 0 in a row that does not see it stays 0.  One whose numbers are finite, but past fp16's (the rounded scale of a row that reaches the ends of
+        // fp16 does that), is taken as far smaller as brings it inside: an infinity times a weight of 0 would be NaN as well.
+        auto none = [](__half h) { return (__half_as_ushort(h) & 0x7c00u) == 0x7c00u; };
+        if (none(__low2half(s)) || none(__high2half(s)) || none(__low2half(c)) || none(__high2half(c))) {
+          s = c = __halves2half2(__ushort_as_half(0x7fffu), __ushort_as_half(0));
+        } else {
+          const float2 sf = __half22float2(s), cf = __half22float2(c);
+          auto inside = [](float scale, float other) {
+            const float end = BITS == 4 ? fmaxf(fabsf(fmaf(scale, 15.f, other)), fabsf(other)) : fabsf(scale) * fmaxf(fabsf(other), fabsf(255.f - other));
+            return end > 65000.f ? 65000.f / end : 1.f;
+          };
+          const float k = inside(sf.x, cf.x), v = inside(sf.y, cf.y);
+          s = __floats2half2_rn(sf.x * k, sf.y * v);
+          if constexpr (BITS == 4) c = __floats2half2_rn(cf.x * k, cf.y * v);
+        }
       }
       const int ks_at = j % C::kKStages, vs_at = j % C::kVStages;
       mbar_wait(&bar_kfree[ks_at], (static_cast<uint32_t>(j / C::kKStages) & 1u) ^ 1u);
-      unpack(raw.k, ks, kc, smem + C::kOffK + ks_at * kKvBytes);
+      unpack(raw.k, __low2half2(s), __low2half2(c), smem + C::kOffK + ks_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_kfull[ks_at]);
       mbar_wait(&bar_vfree[vs_at], (static_cast<uint32_t>(j / C::kVStages) & 1u) ^ 1u);
-      unpack(raw.v, vs, vc, smem + C::kOffV + vs_at * kKvBytes);
+      unpack(raw.v, __high2half2(s), __high2half2(c), smem + C::kOffV + vs_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_vfull[vs_at]);
     };
     Raw raw;
@@ -1283,7 +1300,7 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 
 size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
   if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  const Plan pl = plan_prompt(batch, num_tokens, max_seqlen, max_length, heads, kv_heads);
+  const Plan pl = plan_prompt(batch, num_tokens, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads);
   return pl.parts > 1 ? part_bytes(pl.split_rows(static_cast<long long>(num_tokens) * heads), pl.parts) : 0;
 }
 

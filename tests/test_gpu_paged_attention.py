@@ -376,3 +376,37 @@ def test_small_numbers(dev, bits, shared, lens, how):
                     c.meta(1)[c.pages[b, j], 0] *= float(2.0 ** power[j])
     out = backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args, softmax_scale=scale)
     check_attention(out, shared64(c, q, lens, scale), scale)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,n", [(8, 2, 20), (32, 8, 150)])
+def test_values_at_the_ends_of_their_type(dev, bits, hq, hkv, n):
+    """A token in the middle of the portion whose key and value reach +- 65504: with the rounded scale some of their codes stand for more.  Rows ahead of it do not
+    see it and are as they were; rows behind it are numbers (or too large for one)."""
+    c = Cache([100 + n], hkv, bits, dev, seed=n)
+    q, at = queries(n, hq, dev), 100 + n // 2
+    want = prompt64(c, q, [n], c.lens)
+    top = 2 ** bits - 1
+    for which in (0, 1):
+        meta, page, slot = c.meta(which), c.pages[0, at // PAGE], at % PAGE
+        meta[page, 0, :, slot] = 131008.0 / top * 1.01  # a hundredth too much
+        meta[page, 1, :, slot] = top // 2
+    assert float(c.values(1, 0, at + 1)[at].abs().max()) > 65520
+    out = run_prompt(c, q, [n])
+    check_attention(out[:n // 2], [x[:n // 2] for x in want], SCALE)
+    assert not bool(torch.isnan(out).any())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("hq,hkv,new,ahead", [(8, 2, [20, 3], [100, 700]), (32, 8, [150], [60])])
+def test_values_near_one_end_of_their_type(dev, bits, sign, hq, hkv, new, ahead):
+    """Values from -57000 to 5000, or the other way round: a scale times the largest code is past fp16, what it stands for is not."""
+    lens = [n + m for n, m in zip(new, ahead)]
+    c = Cache(lens, hkv, bits, dev, seed=4)
+    top = 2 ** bits - 1
+    scale, zero = c.meta(1)[:, 0], c.meta(1)[:, 1]
+    scale.copy_(torch.where(scale.isnan(), scale, 62000.0 / top))
+    zero.copy_(torch.where(zero.isnan(), zero, top * (57 / 62 if sign > 0 else 5 / 62)))
+    q = queries(sum(new), hq, dev)
+    check_attention(run_prompt(c, q, new), prompt64(c, q, new, lens), SCALE)

@@ -82,6 +82,8 @@ def test_a_work_space_that_is_missing():
     assert need > 0
     assert prompt(tokens=24, seq=24, top=60000, blocks=940, heads=32, kv_heads=8, size=512, qs=4096, os=4096, ws=A, bytes=need - 1) == -1
     assert b"workspace" in lib.qs_last_error()
+    # portions are no longer than the rows, whatever max_seqlen says
+    assert lib.qs_paged_prompt_attention_workspace_bytes(1, 24, 24000, 60000, 32, 8) == need
     # nothing to join, or joined by a cluster; and sizes that are none
     for args in ((1, 17, 17, 517, 32, 8), (8, 4096, 512, 4000, 32, 8), (0, 1, 1, 1, 4, 1), (1, 1, 1, 1, 4, 3), (1, -1, 1, 1, 4, 1)):
         assert lib.qs_paged_prompt_attention_workspace_bytes(*args) == 0
