@@ -287,22 +287,26 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     // a page's codes, scales and zeros out of the pages ...
     const long long codes = G::codes_at(hk) + t * (G::kRow / 2), scale = G::scales_at(hk, p.num_kv_heads) + key * 2, zero = G::zeros_at(hk, p.num_kv_heads) + key * 2;
     long long kp = 0, vp = 0;  // lane i: page 32 n + i
-    auto fetch = [&](Raw& r, int j) {
+    // INT8: K's codes follow as soon as the page's own are unpacked, while its values are; INT4, half as many, all behind both (30 tokens behind 30000, us: INT8 34.8
+    // all behind both, 33.1 so; INT4 27.1 and 27.5)
+    constexpr bool kEarly = !C::kRing && BITS == 8;
+    const uint8_t *k_page = nullptr, *v_page = nullptr;
+    auto turn = [&](Raw& r, int j) {  // to page j: its scales and zeros
       if (j >= n_mine) return;
       if ((j & 31) == 0 && j + lane < n_mine) {
         kp = __ldcg(ptrs + j + lane);
         vp = __ldcg(ptrs + p.max_blocks + j + lane);
       }
-      const uint8_t* k = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp, j & 31));
-      const uint8_t* v = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp, j & 31));
-      r.ks = __ldcg(reinterpret_cast<const __half*>(k + scale));
-      r.kz = __ldcg(reinterpret_cast<const __half*>(k + zero));
-      r.vs = __ldcg(reinterpret_cast<const __half*>(v + scale));
-      r.vz = __ldcg(reinterpret_cast<const __half*>(v + zero));
+      k_page = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp, j & 31));
+      v_page = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp, j & 31));
+      r.ks = __ldcg(reinterpret_cast<const __half*>(k_page + scale));
+      r.kz = __ldcg(reinterpret_cast<const __half*>(k_page + zero));
+      r.vs = __ldcg(reinterpret_cast<const __half*>(v_page + scale));
+      r.vz = __ldcg(reinterpret_cast<const __half*>(v_page + zero));
+    };
+    auto fetch = [&](uint4 (&code)[kWords], const uint8_t* page) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) r.k[i] = __ldcg(reinterpret_cast<const uint4*>(k + codes) + (i ^ (part * (kWords / 2))));
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) r.v[i] = __ldcg(reinterpret_cast<const uint4*>(v + codes) + (i ^ (part * (kWords / 2))));
+      for (int i = 0; i < kWords; ++i) code[i] = __ldcg(reinterpret_cast<const uint4*>(page + codes) + (i ^ (part * (kWords / 2))));
     };
     // ... or out of their raw slot
     constexpr int kSlots = C::kRing ? C::kSlots : 1;
@@ -384,13 +388,20 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
           if constexpr (BITS == 4) c = __floats2half2_rn(cf.x * k, cf.y * v);
         }
       }
+      if constexpr (kEarly) turn(raw, j + 1);
       const int ks_at = j % C::kKStages, vs_at = j % C::kVStages;
       mbar_wait(&bar_kfree[ks_at], (static_cast<uint32_t>(j / C::kKStages) & 1u) ^ 1u);
       unpack(raw.k, __low2half2(s), __low2half2(c), smem + C::kOffK + ks_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_kfull[ks_at]);
+      if constexpr (kEarly) {
+        if (j + 1 < n_mine) fetch(raw.k, k_page);
+      }
       mbar_wait(&bar_vfree[vs_at], (static_cast<uint32_t>(j / C::kVStages) & 1u) ^ 1u);
       unpack(raw.v, __high2half2(s), __high2half2(c), smem + C::kOffV + vs_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_vfull[vs_at]);
+      if constexpr (kEarly) {
+        if (j + 1 < n_mine) fetch(raw.v, v_page);
+      }
     };
     Raw raw;
     if constexpr (C::kRing) {
@@ -400,10 +411,16 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         if (lane == 0) mbar_arrive(&bar_used[j % kSlots]);
       }
     } else {
-      fetch(raw, 0);
+      auto all = [&](int j) {
+        if (j >= n_mine) return;
+        turn(raw, j);
+        fetch(raw.k, k_page);
+        fetch(raw.v, v_page);
+      };
+      all(0);
       for (int j = 0; j < n_mine; ++j) {
         step(raw, j);
-        fetch(raw, j + 1);
+        if constexpr (!kEarly) all(j + 1);
       }
     }
   } else if (warp >= kIssueWarp) {
