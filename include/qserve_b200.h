@@ -147,6 +147,8 @@ QS_API int qs_read_kv_cache(void* k_out, void* v_out, const int64_t* kv_pointers
 /* out [T, num_heads, 128]: causal attention of every row over positions 0 .. its own of its sequence, all out of the pages (also the portion's own:
  * append first).  q rotated; softmax_scale > 0.  max_seqlen >= the longest portion (rows behind it are left as they are), max_length >= the
  * longest sequence (decides how the keys are split, nothing else).  A row without a position (lengths[b] smaller than the portion) gets zeros.
+ * Keys, values and weights are fp16 operands, sums fp32.  A cached row whose scale or zero is no finite number is NaN to the rows that see it and nothing to
+ * the others; one whose codes stand for more than fp16 holds is taken as large as fits.
  * workspace: qs_paged_prompt_attention_workspace_bytes(...) of the same numbers, any contents, not shared by calls that run at the same time. */
 QS_API size_t qs_paged_prompt_attention_workspace_bytes(int batch, int num_tokens, int max_seqlen, int max_length, int num_heads, int num_kv_heads);
 QS_API int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
