@@ -806,7 +806,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileP
 //
 // A warp takes half pages (32 keys) in turn.  Codes go into the products as they lie: a nibble or byte in the low bits of an fp16 word
 // is the subnormal number u 2^-24, exact as an operand, so there is no conversion and nothing to take off again; scales, zeros and 2^24 are applied to scores and
-// weights in fp32:  q.k = s 2^24 (q.u 2^-24) + c sum(q),  sum p v = 2^24 sum (p s) u 2^-24 + sum p c.
+// weights in fp32:  q.k = s 2^24 (q.u 2^-24) + c sum(q),  sum p v = 2^24 sum (p s) u 2^-24 + sum (p s) (c / s).
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int kTailWarps = 4, kMaxG = 8, kSlice = 32, kMaxCluster = 8;
 constexpr int kOPitch = kD + 4;
@@ -992,14 +992,23 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
     const uint32_t slot = (u % SC::kSlots) * SC::kBytes;
     const uint8_t* st = ring + slot;
     const int t0 = p.shared_blocks * kPage + (mine + u * stride) * kSlice;
-    // (scale, c) per key in fp32, the scores' with the softmax scale; keys past the end: zeros
+    // Per key in fp32: (scale, c) for the scores, with the softmax scale; (scale, c / scale) for the values, whose c goes with the rounded weight as their codes do, so
+    // that a weight's rounding is one of the value and not of its codes.  One that is no finite number makes both NaN.  Keys past the end: zeros
     {
       const __half* mp = reinterpret_cast<const __half*>(st + SC::kOffMeta) + lane;
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const __half s = mp[64 * w], z = mp[64 * w + 32];
-        float2 f = make_float2(__half2float(s), BITS == 4 ? __half2float(__hmul(__hneg(s), z)) : -__half2float(s) * __half2float(z));
-        if (w == 0) f = make_float2(f.x * (p.scale_log2 * kUp), f.y * p.scale_log2);
+        float2 f = make_float2(__half2float(s), -__half2float(z));
+        if constexpr (BITS == 4) {
+          f.y = __half2float(__hmul(__hneg(s), z));
+          if (w == 1) f.y = __fdividef(f.y, f.x == 0.f ? 1.f : f.x);
+        } else if (w == 0) {
+          f.y *= f.x;
+        }
+        const float none = fmaf(f.x, 0.f, f.y * 0.f);
+        if (w == 0) f = make_float2(fmaf(f.x, p.scale_log2 * kUp, none), f.y * p.scale_log2);
+        else f.y += none;
         if (t0 + lane >= len) f = make_float2(0.f, 0.f);
         s_meta[warp][w][lane] = f;
       }
@@ -1080,11 +1089,13 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
     for (int c = 0; c < 2; ++c) {
       const float pA0 = ex2(tl[c][0] - ref0), pA1 = ex2(tl[c][1] - ref1), pB0 = ex2(tl[c][2] - ref0), pB1 = ex2(tl[c][3] - ref1);
       l0 += pA0 + pB0; l1 += pA1 + pB1;
-      c0 = fmaf(pA0, vc[c][0], fmaf(pB0, vc[c][1], c0));
-      c1 = fmaf(pA1, vc[c][0], fmaf(pB1, vc[c][1], c1));
       // the products' operand: p s rounded to fp16
-      bp[c][0] = movmatrix_trans(as_u32(__floats2half2_rn(pA0 * vs[c][0], pA1 * vs[c][0])));
-      bp[c][1] = movmatrix_trans(as_u32(__floats2half2_rn(pB0 * vs[c][1], pB1 * vs[c][1])));
+      const __half2 a = __floats2half2_rn(pA0 * vs[c][0], pA1 * vs[c][0]), b = __floats2half2_rn(pB0 * vs[c][1], pB1 * vs[c][1]);
+      bp[c][0] = movmatrix_trans(as_u32(a));
+      bp[c][1] = movmatrix_trans(as_u32(b));
+      const float2 af = __half22float2(a), bf = __half22float2(b);
+      c0 = fmaf(af.x, vc[c][0], fmaf(bf.x, vc[c][1], c0));
+      c1 = fmaf(af.y, vc[c][0], fmaf(bf.y, vc[c][1], c1));
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {

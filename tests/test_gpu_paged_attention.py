@@ -410,3 +410,35 @@ def test_values_near_one_end_of_their_type(dev, bits, sign, hq, hkv, new, ahead)
     zero.copy_(torch.where(zero.isnan(), zero, top * (57 / 62 if sign > 0 else 5 / 62)))
     q = queries(sum(new), hq, dev)
     check_attention(run_prompt(c, q, new), prompt64(c, q, new, lens), SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("lens,shared", [([300, 700], 2), ([200] * 700, 1)])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), float("nan")])
+def test_scales_and_zeros_that_are_no_numbers(dev, bits, lens, shared, value):
+    """Scale or zero of a key or a value, in the shared page or behind it: NaN, never an infinity or a key that has gone."""
+    for which in (0, 1):
+        for field in (0, 1):
+            for at in (10, 190):
+                c = Cache(lens, 2, bits, dev, shared=shared, seed=8)
+                q = queries(len(lens), 8, dev)
+                c.meta(which)[c.pages[0, at // PAGE], field, :, at % PAGE] = value
+                out = backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args)
+                hit = slice(0, 1) if at >= shared * PAGE else slice(None)
+                assert bool(torch.isnan(out[hit]).all())
+                assert at < shared * PAGE or bool(torch.isfinite(out[1:]).all())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("lens,shared", [([1, 2, 2, 3] * 5, 0), ([2] * 700, 0)])
+def test_values_near_their_zero(dev, bits, lens, shared):
+    """Few positions, values that are differences of much larger products of codes and zeros: off by the roundings of the values, not by those of the products."""
+    c = Cache(lens, 2, bits, dev, shared=shared, seed=12)
+    top = 2 ** bits - 1
+    for b in range(len(lens)):
+        meta = c.meta(1)[c.pages[b, 0]]
+        meta[1, :, :lens[b]] = top / 2 + 0.0625
+        raw = c.pools[1][c.pages[b, 0], :c.cut]
+        raw.fill_(0x78 if bits == 4 else 0x80)  # half the top and the code behind it
+    q = queries(len(lens), 8, dev)
+    check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args), shared64(c, q, lens), SCALE)
