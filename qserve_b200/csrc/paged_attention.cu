@@ -1243,6 +1243,7 @@ struct Plan {
   long long items, split;  // (rows of a block, kv head) pairs; the last so many of them are split
   long long split_rows(long long all) const { return split == items ? all : split * tiles * kRows; }
 };
+constexpr float kTwoTilesPage = 0.92f, kTwoTilesFixed = 5.5f;  // us
 Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, long long pages, bool prompt) {
   constexpr float kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 5e6f;
   Plan pl{};
@@ -1254,7 +1255,7 @@ Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, lon
   long long blocks = static_cast<long long>(kv_heads) * ((2 * num_rows + batch * block_rows + 2 * block_rows - 1) / (2 * block_rows));
   blocks = blocks < 1 ? 1 : blocks > pl.items ? pl.items : blocks;
   const unsigned most = static_cast<unsigned>(pages < 1 ? 1 : pages);
-  const float fixed = pl.tiles == 2 ? 5.5f : 3.5f;
+  const float fixed = pl.tiles == 2 ? kTwoTilesFixed : 3.5f;
   float best = 3.0e38f;
   auto take = [&](float t, unsigned n, unsigned cluster, long long split) {
     if (t >= best) return;
@@ -1264,7 +1265,7 @@ Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, lon
     pl.split = split;
   };
   for (int per_sm = 1; per_sm <= (pl.tiles == 1 ? 2 : 1); ++per_sm) {
-    const float page = pl.tiles == 2 ? 0.92f : per_sm == 1 ? (rows <= 64 ? 0.7f : 0.95f) : (rows <= 64 ? 1.f : 1.2f);
+    const float page = pl.tiles == 2 ? kTwoTilesPage : per_sm == 1 ? (rows <= 64 ? 0.7f : 0.95f) : (rows <= 64 ? 1.f : 1.2f);
     const long long slots = sms * per_sm;
     auto block = [&](unsigned n) { return ((most + n - 1) / n) * page + fixed; };
     // sequences of a batch differ in length, and the blocks of the last round are short beside the longest: half of what it lacks to be full
@@ -1365,6 +1366,39 @@ size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_h
   return part_bytes(static_cast<long long>(batch) * heads, plan_shared(batch, shared_blocks, heads, kv_heads).parts);
 }
 
+// The tail kernel's blocks start while the prefix's run, on the multiprocessors that those leave, as many on each as it holds.  (Blocks of two tiles leave no room beside
+// them; one-tile blocks do.)  So where the tail's fit, fewer splits of the prefix and a bound on the tail's blocks per multiprocessor let both end at about the same time.
+// Chooses the splits, no more than planned, and returns that bound; one behind the other, the bound spreads the tail evenly.  The tail's estimate, us: start and join, that of
+// its blocks' issue slots, and its warps' half pages, each its own chain or its share of the issue slots.  Measured, one behind the other / side by side, 8 kv heads: 38
+// sequences, 500 positions behind 1024, 19.0 / 11.4 (INT8 17.1 / 11.4); 64, 1000 behind 2048, 29.5 / 24.0; bounded alone: 38, 1000 behind 16384, 40.3 / 37.1.  Not for small
+// estimated gains (INT8, 38, 200 behind 4096: 17.3 / 20.4).
+int side_by_side(Plan& pl, int shared_blocks, long long tail, long long tail_pages, int cluster, int most) {
+  const long long sms = num_sms(), even = (tail + sms - 1) / sms;
+  if (pl.tiles == 1 || even > most) return most;
+  const int steps = static_cast<int>(tail_pages > 0 ? (2 * tail_pages + kTailWarps * cluster - 1) / (kTailWarps * cluster) : 0);
+  auto prefix = [&](long long n) { return ((shared_blocks + n - 1) / n) * kTwoTilesPage + kTwoTilesFixed; };
+  auto own = [&](long long k) {
+    const float busy = (most == 4 ? 0.4f : 0.45f) * k;
+    return 3.f + 1.1f * k + steps * (busy > 0.9f ? busy : 0.9f);
+  };
+  int room = static_cast<int>(even);
+  float best = 0.85f * (prefix(pl.nsplit) + own(even));
+  long long splits = pl.nsplit;
+  for (int k = 1; k <= most; ++k) {
+    long long n = (sms - (tail + k - 1) / k) / pl.items;
+    n = n < pl.nsplit ? n : pl.nsplit;
+    if (n < 1) continue;
+    const float t = prefix(n) > own(k) ? prefix(n) : own(k);
+    if (t < best) {
+      best = t;
+      splits = n;
+      room = k;
+    }
+  }
+  pl.nsplit = pl.parts = static_cast<int>(splits);
+  return room;
+}
+
 int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   if (a.batch == 0) return QS_OK;
   if (tail_alone(a.batch, shared_blocks)) shared_blocks = 0;
@@ -1373,10 +1407,22 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   t.q = static_cast<const __half*>(a.q); t.out = static_cast<__half*>(a.out); t.q_stride = a.q_stride; t.out_stride = a.out_stride;
   t.batch = a.batch; t.kv_pointers = a.cache.kv_pointers; t.lengths = a.cache.lengths; t.max_blocks = a.cache.max_blocks; t.num_heads = a.num_heads;
   t.num_kv_heads = a.cache.num_kv_heads; t.shared_blocks = shared_blocks; t.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const int group = a.num_heads / t.num_kv_heads, heads_y = t.num_kv_heads * ((group + kMaxG - 1) / kMaxG);
+  // shares of a sequence's pages: as many blocks as the device holds at a time, a page for each warp pair at least
+  const int most = a.cache.int4 ? 4 : 3;  // blocks per multiprocessor
+  const long long sms = num_sms(), slots = sms * most, blocks = static_cast<long long>(heads_y) * a.batch;
+  const long long tail_pages = (static_cast<long long>(a.max_length) + kPage - 1) / kPage - shared_blocks;
+  t.cluster = 1;
+  while (t.cluster < kMaxCluster && blocks * t.cluster * 2 <= slots && tail_pages >= 2 * kTailWarps * t.cluster) t.cluster *= 2;
+  QS_REQUIRE(blocks <= 0x7fffffffll, "shared_prefix_attention: %lld runs of heads", blocks);
+  const bool shared = blocks < 12 * num_sms();  // (a wave of warps; 128 sequences x 32 heads, INT8, 400 positions each behind 16384: 157 us by blocks, 142 by warps)
+  if (!shared) t.cluster = 1;
+  int room = most;
   if (shared_blocks > 0) {
-    const Plan pl = plan_shared(a.batch, shared_blocks, a.num_heads, a.cache.num_kv_heads);
+    Plan pl = plan_shared(a.batch, shared_blocks, a.num_heads, a.cache.num_kv_heads);
     QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.parts), "shared_prefix_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
                part_bytes(rows, pl.parts));
+    if (shared) room = side_by_side(pl, shared_blocks, blocks * t.cluster, tail_pages, t.cluster, most);
     TileParams p{};
     p.q = t.q; p.q_stride = t.q_stride; p.kv_pointers = t.kv_pointers; p.lengths = t.lengths;
     p.batch = 1; p.num_tokens = p.max_seqlen = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
@@ -1387,15 +1433,6 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
     const int rc = tiles(p, pl, a.cache.int4, a.stream);
     if (rc) return rc;
   }
-  const int group = a.num_heads / t.num_kv_heads, heads_y = t.num_kv_heads * ((group + kMaxG - 1) / kMaxG);
-  // shares of a sequence's pages: as many blocks as the device holds at a time, a page for each warp pair at least
-  const long long slots = static_cast<long long>(num_sms()) * (a.cache.int4 ? 4 : 3), blocks = static_cast<long long>(heads_y) * a.batch;
-  const long long tail_pages = (static_cast<long long>(a.max_length) + kPage - 1) / kPage - shared_blocks;
-  t.cluster = 1;
-  while (t.cluster < kMaxCluster && blocks * t.cluster * 2 <= slots && tail_pages >= 2 * kTailWarps * t.cluster) t.cluster *= 2;
-  QS_REQUIRE(blocks <= 0x7fffffffll, "shared_prefix_attention: %lld runs of heads", blocks);
-  const bool shared = blocks < 12 * num_sms();  // (a wave of warps; 128 sequences x 32 heads, INT8, 400 positions each behind 16384: 157 us by blocks, 142 by warps)
-  if (!shared) t.cluster = 1;
   const dim3 grid = shared ? dim3(t.cluster, heads_y, a.batch) : dim3(static_cast<unsigned>((blocks + kTailWarps - 1) / kTailWarps));
   // us, two slots / four (INT4): one sequence of 16384 positions 17.6 / 16.2, one of 2000 with 32 heads a group of one 8.1 / 6.2, four of up to 8000 17.3 / 12.1.  Not
   // behind the tile kernel, whose blocks leave no room for it: 32 sequences, 100 positions behind 4096, 11.6 / 14.2
@@ -1403,9 +1440,11 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   auto run = [&](auto bits, auto by_block, auto more) {
     constexpr int kBits = decltype(bits)::value;
     constexpr bool kShared = decltype(by_block)::value, kDeep = decltype(more)::value;
-    const int rc = allow_smem<tail_kernel<kBits, kShared, kDeep>>(SliceCfg<kBits, kDeep>::kSmem, "shared_prefix_attention: shared memory", [](int) { return true; });
+    constexpr int kSm = 228 * 1024, kOwn = SliceCfg<kBits, kDeep>::kSmem;
+    const int rc = allow_smem<tail_kernel<kBits, kShared, kDeep>>(kOwn > kSm / 2 ? kOwn : kSm / 2, "shared_prefix_attention: shared memory", [](int) { return true; });
     if (rc) return rc;
-    return launch(tail_kernel<kBits, kShared, kDeep>, grid, 32 * kTailWarps, SliceCfg<kBits, kDeep>::kSmem, a.stream, "shared_prefix_attention", t.cluster, t);
+    const int smem = room < most && kOwn < kSm / (room + 1) ? kSm / (room + 1) : kOwn;  // so much that no more than `room` blocks share a multiprocessor
+    return launch(tail_kernel<kBits, kShared, kDeep>, grid, 32 * kTailWarps, smem, a.stream, "shared_prefix_attention", t.cluster, t);
   };
   auto with = [&](auto bits) {
     if (!shared) return run(bits, std::false_type{}, std::false_type{});

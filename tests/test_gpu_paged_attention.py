@@ -442,3 +442,17 @@ def test_values_near_their_zero(dev, bits, lens, shared):
         raw.fill_(0x78 if bits == 4 else 0x80)  # half the top and the code behind it
     q = queries(len(lens), 8, dev)
     check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args), shared64(c, q, lens), SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("batch,shared,own", [(38, 16, 500), (40, 32, 900), (64, 16, 400)])
+def test_prefix_and_own_pages_side_by_side(dev, bits, batch, shared, own):
+    """Batches whose own pages are read while the prefix is: fewer splits of it than the work space has room for, whatever max_length says."""
+    lens = [shared * PAGE + (own * (7 + 5 * b % 9)) // 16 for b in range(batch)]
+    lens[3] = shared * PAGE - 5
+    c = Cache(lens, 8, bits, dev, shared=shared, seed=batch)
+    q = queries(batch, 32, dev)
+    want = shared64(c, q, lens)
+    for top in (max(lens), 1, 100000):
+        for _ in range(3):
+            check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, shared, top, *c.args), want, SCALE)
