@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     if (lane == 0) mbar_arrive(&bar_q[tile]);
     // the last position that the row sees, and the lowest of the warp's rows (one that is no row: its numbers go nowhere)
     int limit = n_keys - 1;
-    if (row_is) limit = p.shared_blocks > 0 ? min(__ldcg(p.lengths + tok), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
+    if (row_is) limit = p.shared_blocks > 0 ? min(max(__ldcg(p.lengths + tok), 0), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
     int lowest = limit;
 #pragma unroll
     for (int m = 16; m >= 1; m >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, m));
@@ -896,7 +896,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
   // The tile kernel before this one started this one after its own wait: everything ahead of the tile kernel is there.  Without one, this kernel waits itself.
   if (p.nsplit == 0) pdl_wait();
 
-  const int len = live ? min(__ldcg(p.lengths + b), p.max_blocks * kPage) : 0;
+  const int len = live ? min(max(__ldcg(p.lengths + b), 0), p.max_blocks * kPage) : 0;  // (whatever the table says: no difference below wraps)
   const int slices = max((len - p.shared_blocks * kPage + kSlice - 1) / kSlice, 0);
   // the cluster's blocks and their warps take turns over the slices
   const int stride = SHARED ? p.cluster * kTailWarps : 1, mine = SHARED ? rank * kTailWarps + warp : 0;
