@@ -63,6 +63,7 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int PENDING>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();  // the barrier's aligned form is for whole warps, and whoever calls may come out of a branch or loop that lanes left one by one
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // eight bytes at this place of the shared memory of block `rank` of the cluster

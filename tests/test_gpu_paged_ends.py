@@ -40,3 +40,12 @@ def test_lengths_at_the_ends_of_their_type_behind_a_prefix(dev, bits, hq, hkv, b
     out = backend.shared_prefix_attention(q, c.table, c.lengths, 2, 4 * PAGE, *c.args)
     assert bool((out[said <= 0] == 0).all())
     check_attention(out[said > 0], [x[said > 0] for x in want], SCALE)
+
+
+# ---- rows that a cluster's half warps share out unevenly ----
+@pytest.mark.parametrize("bits", [4, 8])
+def test_any_number_of_rows_in_a_cluster(dev, bits):
+    for n in [*range(1, 20), 31, 33, 47, 64, 65, 100, 127, 128]:
+        c = Cache([n + 600], 1, bits, dev, seed=n)
+        q = queries(n, 1, dev)
+        check_attention(run_prompt(c, q, [n]), prompt64(c, q, [n], c.lens), SCALE)
