@@ -375,24 +375,53 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         most = __hmul2(__habs2(s), __hmax2(__habs2(c), __habs2(__hsub2(__float2half2_rn(255.f), c))));
       }
       const uint32_t endless = as_u32(most) & 0x7c007c00u;
-      if (!live) {
-        s = c = __float2half2_rn(0.f);
-      } else if ((endless & 0xffffu) == 0x7c00u || endless >= 0x7c000000u) {
+      const bool wide = live && ((endless & 0xffffu) == 0x7c00u || endless >= 0x7c000000u);
+      if (!live) s = c = __float2half2_rn(0.f);
+      if (__any_sync(0xffffffffu, wide)) {
         // A row of K or V whose scale or zero is no finite number stands for NaN: the key's score is NaN then (and goes where the key is masked), its value 0, so
-        // that a weight of 0 in a row that does not see it stays 0.  One whose numbers are finite, but past fp16's (the rounded scale of a row that reaches the ends of
-        // fp16 does that), is taken as far smaller as brings it inside: an infinity times a weight of 0 would be NaN as well.
+        // that a weight of 0 in a row that does not see it stays 0.  Otherwise what counts is the codes that the row has (a row of one value is held as 1 x that value, and 15 or
+        // 255 of it would be past fp16): one with a number past fp16's all the same (the rounded scale of a row that reaches the ends of fp16 does that) is taken as
+        // much smaller as brings it inside, for an infinity times a weight of 0 would be NaN as well.  65520 is the least that rounds to infinity; 65376 leaves room for the
+        // roundings of the smaller scale and zero (INT4: 15 x 4 + 16 at most; INT8: 2^-11 of each).
+        const float2 sf = __half22float2(s), cf = __half22float2(c);
+        auto inside = [&](const uint4 (&code)[kWords], float scale, float other) {
+          uint32_t lo = 0xffffffffu, hi = 0u;
+#pragma unroll
+          for (int i = 0; i < kWords; ++i) {
+            const uint32_t words[4] = {code[i].x, code[i].y, code[i].z, code[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (BITS == 4) {
+                const uint32_t even = words[k] & 0x0f0f0f0fu, odd = (words[k] >> 4) & 0x0f0f0f0fu;
+                lo = __vminu4(lo, __vminu4(even, odd));
+                hi = __vmaxu4(hi, __vmaxu4(even, odd));
+              } else {
+                lo = __vminu4(lo, words[k]);
+                hi = __vmaxu4(hi, words[k]);
+              }
+            }
+          }
+          lo = __vminu4(lo, __shfl_xor_sync(0xffffffffu, lo, 1));  // the row's other thread
+          hi = __vmaxu4(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+#pragma unroll
+          for (int m = 16; m >= 8; m >>= 1) {
+            lo = __vminu4(lo, lo >> m | lo << (32 - m));
+            hi = __vmaxu4(hi, hi >> m | hi << (32 - m));
+          }
+          const float least = static_cast<float>(lo & 255u), largest = static_cast<float>(hi & 255u);
+          const float end = BITS == 4 ? fmaxf(fabsf(fmaf(scale, least, other)), fabsf(fmaf(scale, largest, other)))
+                                      : fabsf(scale) * fmaxf(fabsf(least - other), fabsf(largest - other));
+          return end >= 65520.f ? 65376.f / end : 1.f;
+        };
+        const float k = inside(raw.k, sf.x, cf.x), v = inside(raw.v, sf.y, cf.y);
         auto none = [](__half h) { return (__half_as_ushort(h) & 0x7c00u) == 0x7c00u; };
-        if (none(__low2half(s)) || none(__high2half(s)) || none(__low2half(c)) || none(__high2half(c))) {
-          s = c = __halves2half2(__ushort_as_half(0x7fffu), __ushort_as_half(0));
-        } else {
-          const float2 sf = __half22float2(s), cf = __half22float2(c);
-          auto inside = [](float scale, float other) {
-            const float end = BITS == 4 ? fmaxf(fabsf(fmaf(scale, 15.f, other)), fabsf(other)) : fabsf(scale) * fmaxf(fabsf(other), fabsf(255.f - other));
-            return end > 65000.f ? 65000.f / end : 1.f;
-          };
-          const float k = inside(sf.x, cf.x), v = inside(sf.y, cf.y);
-          s = __floats2half2_rn(sf.x * k, sf.y * v);
-          if constexpr (BITS == 4) c = __floats2half2_rn(cf.x * k, cf.y * v);
+        if (wide) {
+          if (none(__low2half(s)) || none(__high2half(s)) || none(__low2half(c)) || none(__high2half(c))) {
+            s = c = __halves2half2(__ushort_as_half(0x7fffu), __ushort_as_half(0));
+          } else {
+            s = __floats2half2_rn(sf.x * k, sf.y * v);
+            if constexpr (BITS == 4) c = __floats2half2_rn(cf.x * k, cf.y * v);
+          }
         }
       }
       if constexpr (kEarly) turn(raw, j + 1);

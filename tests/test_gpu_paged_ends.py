@@ -49,3 +49,41 @@ def test_any_number_of_rows_in_a_cluster(dev, bits):
         c = Cache([n + 600], 1, bits, dev, seed=n)
         q = queries(n, 1, dev)
         check_attention(run_prompt(c, q, [n]), prompt64(c, q, [n], c.lens), SCALE)
+
+
+# ---- rows whose codes could stand for more than fp16 holds, and do not ----
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,new,ahead", [(8, 2, [20, 3], [100, 700]), (32, 8, [150], [60]), (8, 2, [6], [2600])])
+def test_rows_of_one_value(dev, bits, hq, hkv, new, ahead):
+    """Values that append holds as 1 x scale or 0 - 1 x scale, up to the end of fp16; and rows of few codes: the numbers that the pages stand for."""
+    lens = [n + m for n, m in zip(new, ahead)]
+    c = Cache(lens, hkv, bits, dev, seed=14)
+    for b, n in enumerate(lens):
+        g = torch.Generator().manual_seed(b)
+        size = torch.exp2(torch.rand(n, hkv, generator=g) * 16).clamp(max=64992)
+        some = torch.rand(n, hkv, generator=g) < 0.5
+        sign = (torch.rand(n, hkv, generator=g) < 0.5)
+        fill(c, 1, b, (~sign & some).long()[..., None].expand(-1, -1, D), torch.where(some, size, 0.01), torch.where(some, sign.half(), 5.0))
+        # codes 0 .. 3 around a zero of 1.5: +- 1.5 scales, where the largest code would stand for 13.5 of them, or 253.5
+        few = torch.rand(n, hkv, generator=g) < 0.2
+        u = torch.randint(0, 4, (n, hkv, D), generator=g)
+        page, slot = c.pages[b][torch.arange(n, device=dev) // PAGE], torch.arange(n, device=dev) % PAGE
+        old = c.codes(1)[page, :, slot].cpu()
+        s, z = (c.meta(1)[page, i, :, slot].cpu().float() for i in (0, 1))
+        fill(c, 1, b, torch.where(few[..., None], u, old.long()), torch.where(few, (size * 0.6).clamp(max=43000), s), torch.where(few, 1.5, z))
+    q = queries(sum(new), hq, dev)
+    check_attention(run_prompt(c, q, new), prompt64(c, q, new, lens), SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("value", [300.0, -4400.0, 64992.0, -64992.0])
+def test_appended_rows_of_one_value_are_attended_to(dev, bits, value):
+    """Appended values that are all equal come out of both kernels of attention as they went in (a weighted mean of equal numbers: the weights' rounding, 2 H)."""
+    n, hkv = 70, 2
+    c = Cache([n], hkv, bits, dev, seed=3)
+    k = torch.randn(n, hkv, D, generator=torch.Generator().manual_seed(4)).half().to(dev)
+    v = torch.full_like(k, value)
+    backend.append_kv_cache(k, k, v, c.table, starts([n], dev), c.lengths, PAGE, c.size, D, BASE, bits == 4, True)
+    q = queries(n, 8, dev)
+    for out in (backend.paged_prompt_attention(q, c.table, starts([n], dev), c.lengths, n, n, *c.args), backend.shared_prefix_attention(q[:1], c.table, c.lengths, 0, n, *c.args)):
+        assert bool(((out.float() - value).abs() <= 2 * H * abs(value)).all()), float((out.float() / value - 1).abs().max())
