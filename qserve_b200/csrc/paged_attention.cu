@@ -8,7 +8,7 @@
 //     S = Q K^T       8 x tcgen05.mma 128 x 64 x 16, accumulators in tensor memory
 //     softmax         4 warps, thread = row (tensor memory lane): running maximum and sum in 32 bits, P = exp2(..) rounded to fp16, into tensor memory
 //     O += P V        4 x tcgen05.mma 128 x 128 x 16, A from tensor memory
-// fp16 holds the operands (keys, values and weights, each off by 2^-11 of itself at most): a product of exact codes would want every score multiplied by its key's
+// fp16 holds the operands (keys, values and weights, each off by 2^-11 of itself at most, INT8 keys and values by another 2^-12 of their scale): a product of exact codes would want every score multiplied by its key's
 // scale and every weight by its value's, a third more instructions of softmax warps that are the bound already.
 // A long axis of keys is split over blocks where the rows alone do not fill the device, or not its last round.  A split leaves its rows' maximum and sum in fp32 and
 // O / sum in fp16, rounded as a result is (in fp32 they were most of what 64 sequences behind 8192 shared positions move: 32.2 us, now 30.8); the cluster that holds
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 #pragma unroll
       for (int i = 0; i < kWords; ++i) r.v[i] = v[i ^ (part * (kWords / 2))];
     };
-    auto unpack = [&](const uint4 (&raw)[kWords], __half2 s2, __half2 c2, uint8_t* dst) {
+    auto unpack = [&](const uint4 (&raw)[kWords], __half2 s2, __half2 c2, __half2 low2, uint8_t* dst) {
       uint8_t* row = dst + row_at;
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
@@ -352,11 +352,11 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             __half2 lo[2], hi[2];
-            codes_of_word8(words[2 * k], lo);
-            codes_of_word8(words[2 * k + 1], hi);
+            codes_of_word8(words[2 * k], low2, lo);
+            codes_of_word8(words[2 * k + 1], low2, hi);
             __half2 u[4] = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) u[e] = __hmul2(__hsub2(u[e], c2), s2);
+            for (int e = 0; e < 4; ++e) u[e] = __hfma2(u[e], s2, c2);
             put(2 * at + k, u);
           }
         }
@@ -424,16 +424,24 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
           }
         }
       }
+      __half2 low = c;
+      if constexpr (BITS == 8) {
+        // s (u - z) in one rounding: u less the nearest whole number to z, exact, times s, plus s times the rest of z (at most 1 / 2; a zero further than 1024 from 0, which is
+        // whole, leaves more there, and that product is rounded too).  u - z itself may have more bits than fp16: 255 less a zero of 54.6875 does
+        const __half2 end = __float2half2_rn(1024.f), whole = h2rint(__hmax2(__hmin2(c, end), __hneg2(end)));
+        low = __hneg2(__hadd2(whole, end));
+        c = __hmul2(s, __hsub2(whole, c));
+      }
       if constexpr (kEarly) turn(raw, j + 1);
       const int ks_at = j % C::kKStages, vs_at = j % C::kVStages;
       mbar_wait(&bar_kfree[ks_at], (static_cast<uint32_t>(j / C::kKStages) & 1u) ^ 1u);
-      unpack(raw.k, __low2half2(s), __low2half2(c), smem + C::kOffK + ks_at * kKvBytes);
+      unpack(raw.k, __low2half2(s), __low2half2(c), __low2half2(low), smem + C::kOffK + ks_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_kfull[ks_at]);
       if constexpr (kEarly) {
         if (j + 1 < n_mine) fetch(raw.k, k_page);
       }
       mbar_wait(&bar_vfree[vs_at], (static_cast<uint32_t>(j / C::kVStages) & 1u) ^ 1u);
-      unpack(raw.v, __high2half2(s), __high2half2(c), smem + C::kOffV + vs_at * kKvBytes);
+      unpack(raw.v, __high2half2(s), __high2half2(c), __high2half2(low), smem + C::kOffV + vs_at * kKvBytes);
       if (lane == 0) mbar_arrive(&bar_vfull[vs_at]);
       if constexpr (kEarly) {
         if (j + 1 < n_mine) fetch(raw.v, v_page);

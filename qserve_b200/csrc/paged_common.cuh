@@ -39,9 +39,8 @@ __device__ __forceinline__ void codes_of_word4(uint32_t w, __half2 (&u)[4]) {
   u[2] = __hadd2(as_h2(lop3_and_or(t, 0x000f000fu, 0x64006400u)), low);
   u[3] = __hfma2(as_h2(lop3_and_or(t, 0x00f000f0u, 0x64006400u)), sixteenth, high);
 }
-// INT8: the four codes of a word as (0, 1), (2, 3)
-__device__ __forceinline__ void codes_of_word8(uint32_t w, __half2 (&u)[2]) {
-  const __half2 low = __float2half2_rn(-1024.f);
+// INT8: the four codes of a word as (0, 1), (2, 3), each plus 1024 + low: exact for whole numbers low from -2048 to 0
+__device__ __forceinline__ void codes_of_word8(uint32_t w, __half2 low, __half2 (&u)[2]) {
   u[0] = __hadd2(as_h2(__byte_perm(w, 0x64006400u, 0x7150)), low);
   u[1] = __hadd2(as_h2(__byte_perm(w, 0x64006400u, 0x7352)), low);
 }

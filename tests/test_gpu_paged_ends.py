@@ -87,3 +87,28 @@ def test_appended_rows_of_one_value_are_attended_to(dev, bits, value):
     q = queries(n, 8, dev)
     for out in (backend.paged_prompt_attention(q, c.table, starts([n], dev), c.lengths, n, n, *c.args), backend.shared_prefix_attention(q[:1], c.table, c.lengths, 0, n, *c.args)):
         assert bool(((out.float() - value).abs() <= 2 * H * abs(value)).all()), float((out.float() / value - 1).abs().max())
+
+
+# ---- one rounding of a value ----
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("shared", [0, 1])
+def test_a_value_alone_is_rounded_once(dev, bits, shared):
+    """Sequences of a single position: its weight is 1, the result what its codes stand for, rounded once.  INT8 adds the rounding of scale times the zero's part behind the point, at
+    most half a scale.  Zeros of every size from fractions to 1000.  fp32 rounds scores (2^-18 of a weight) and products of scale with code and zero (2^-20)."""
+    batch, hq, hkv = 40, 4, 1
+    c = Cache([1] * batch, hkv, bits, dev, shared=0, seed=2)
+    g = torch.Generator().manual_seed(7)
+    for b in range(batch):
+        z = (torch.rand(1, hkv, generator=g) * 2 - 1) * (15.0 if bits == 4 else [4.0, 200.0, 1000.0][b % 3])
+        fill(c, 1, b, random_codes(1, hkv, bits, b), 0.01 + torch.rand(1, hkv, generator=g), z)
+    q = queries(batch, hq, dev)
+    if shared:
+        out = backend.shared_prefix_attention(q, c.table, c.lengths, 0, 1, *c.args)
+    else:
+        out = backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 1, *c.args)
+    for b in range(batch):
+        want = c.values(1, b, 1)[0].repeat_interleave(hq // hkv, 0)
+        s, z = (float(c.meta(1)[c.pages[b, 0], i, 0, 0]) for i in (0, 1))
+        room = H * want.abs() * (1 + 2.0 ** -7) + (0 if bits == 4 else H * s / 2 * (1 + H)) + s * (abs(z) + 2 ** bits) * 2.0 ** -20
+        off = (out[b].to(F64) - want).abs()
+        assert (off <= room).all(), (b, float((off / room).max()))
