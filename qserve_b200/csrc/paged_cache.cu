@@ -85,6 +85,33 @@ __device__ __forceinline__ Quantised<BITS> quantise_row(const f2 (&x)[8]) {
     r.zero = __float2half_rn(c < 0.f ? 1.f : 0.f);
     inv = 0.f;
     z = c > 0.f ? 1.f : 0.f;
+  } else if (fmaxf(hi, -lo) > 65000.f) {
+    // A row that reaches the ends of fp16, whose rounded scale and zero may take its first or its last code past them: the scale is rounded down then, and if that is not enough the
+    // zero goes to the next number towards the other end.  (All pairs of least and largest number with one above 65000 tried on the CPU: 145000 of 4 million are past the ends as
+    // rounded, 798 with the scale rounded down, none with the zero moved; and none of those that stay below.)
+    bool below, above;
+    auto ends = [&] {
+      if constexpr (BITS == 4) {
+        const __half c = __float2half_rn(-__fmul_rn(s, z));
+        below = __half_as_ushort(c) == 0xfc00u;
+        above = fmaf(s, kTop, __half2float(c)) >= 65520.f;  // (65520 is the least number that rounds to infinity)
+      } else {
+        below = __fmul_rn(s, z) >= 65520.f;
+        above = __fmul_rn(s, kTop - z) >= 65520.f;
+      }
+    };
+    ends();
+    if (below || above) {
+      r.scale = __float2half_rd(__fdiv_rn(span, kTop));
+      s = __half2float(r.scale);
+      ends();
+      if (below || above) {
+        const int bits = __half_as_ushort(r.zero), next = ((bits & 0x8000) ? -(bits & 0x7fff) : bits) + (below ? -1 : 1);
+        r.zero = __ushort_as_half(static_cast<unsigned short>(next < 0 ? 0x8000 - next : next));
+        z = __half2float(r.zero);
+      }
+      inv = __fdiv_rn(1.f, s);
+    }
   }
 #pragma unroll
   for (int k = 0; k < BITS / 2; ++k) r.word[k] = 0u;

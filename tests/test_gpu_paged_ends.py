@@ -112,3 +112,62 @@ def test_a_value_alone_is_rounded_once(dev, bits, shared):
         room = H * want.abs() * (1 + 2.0 ** -7) + (0 if bits == 4 else H * s / 2 * (1 + H)) + s * (abs(z) + 2 ** bits) * 2.0 ** -20
         off = (out[b].to(F64) - want).abs()
         assert (off <= room).all(), (b, float((off / room).max()))
+
+
+# ---- rows at the ends of fp16 ----
+@pytest.mark.parametrize("bits", [4, 8])
+def test_appended_rows_at_the_ends_of_fp16(dev, bits):
+    """Finite rows read back as finite numbers, off by half a code's step (a whole one at the ends), the rounding of scale and zero, and one of the result; attention takes them as they are.
+    The scale is rounded down where the rounded one reaches past fp16 (2 H of it for each code), the zero moved by one of its steps (2 H of it, each a scale)."""
+    top = 2 ** bits - 1
+    g = torch.Generator().manual_seed(1)
+    ends = [(-65504, 65504), (-65504, 65472), (-65472, 65504), (-65504, 0), (0, 65504), (-65504, 60000), (-60000, 65504), (64992, 65504), (-65504, -64992), (65472, 65504), (-65504, -65472),
+            (-65504, -32768), (32768, 65504), (-65440, 65440), (-65504, 4096), (-65408, 65376)]
+    n = len(ends)
+    x = torch.empty(n, 1, D)
+    for i, (lo, hi) in enumerate(ends):
+        x[i] = lo + (hi - lo) * torch.rand(D, generator=g)
+        x[i, 0, 3], x[i, 0, 90] = lo, hi
+    x = x.half().to(dev)
+    k = torch.randn(n, 1, D, generator=g).half().to(dev)
+    c = Cache([n], 1, bits, dev)
+    backend.append_kv_cache(k, k, x, c.table, starts([n], dev), c.lengths, PAGE, c.size, D, BASE, bits == 4, True)
+    got = backend.read_kv_cache(c.table, starts([n], dev), c.lengths, n, *c.args)[1]
+    assert bool(torch.isfinite(got).all())
+    span = (x.amax(-1) - x.amin(-1).float())[..., None]
+    room = span / top + (span + 3 * x.float().abs().amax(-1, keepdim=True)) * 2 * H + 32
+    assert bool(((got.float() - x.float()).abs() <= room).all())
+    assert bool(torch.isfinite(c.values(1, 0, n)).all()) and float(c.values(1, 0, n).abs().max()) < 65520
+    q = queries(n, 8, dev)
+    want = prompt64(c, q, [n], [n])
+    check_attention(run_prompt(c, q, [n]), want, SCALE)
+    check_attention(backend.shared_prefix_attention(q[-1:], c.table, c.lengths, 0, n, *c.args), [w[-1:] for w in want], SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+def test_appended_rows_of_any_ends_are_finite(dev, bits):
+    """Rows from one number to another, one of them above 65000 in size: whatever their codes, the pages stand for finite numbers, as near as a code's step, the scale rounded down
+    (2 H of its codes) and the zero's step (2 H of the zero) allow."""
+    top, n = 2 ** bits - 1, 6000
+    g = torch.Generator().manual_seed(9)
+    ends = torch.randint(0, 0x7c00, (n, 2), generator=g).to(torch.int16)
+    ends[:, 0] = torch.randint(0x7bf0, 0x7c00, (n,), generator=g).to(torch.int16)
+    ends[::2, 1] = torch.randint(0x7800, 0x7c00, (n // 2,), generator=g).to(torch.int16)
+    ends = ends.view(HALF).float() * (torch.randint(0, 2, (n, 2), generator=g) * 2 - 1)
+    lo, hi = ends.amin(1, keepdim=True), ends.amax(1, keepdim=True)
+    x = lo + (hi - lo) * torch.rand(n, D, generator=g)
+    x[:, :1], x[:, 70:71] = lo, hi
+    x = x.half().to(dev)[:, None]
+    k = torch.randn(n, 1, D, generator=g).half().to(dev)
+    c = Cache([n], 1, bits, dev)
+    backend.append_kv_cache(k, k, x, c.table, starts([n], dev), c.lengths, PAGE, c.size, D, BASE, bits == 4, True)
+    got = backend.read_kv_cache(c.table, starts([n], dev), c.lengths, n, *c.args)[1]
+    assert bool(torch.isfinite(got).all())
+    least, most = x.amin(-1).float(), x.amax(-1).float()
+    room = (most - least) / top + (most - least + 3 * torch.maximum(most, -least)) * 2 * H + 32
+    assert bool(((got.float() - x.float()).abs() <= room[..., None]).all())
+    scale, zero = (c.meta(1)[c.pages[0, torch.arange(n, device=dev) // PAGE], i, 0, torch.arange(n, device=dev) % PAGE].to(F64) for i in (0, 1))
+    u = c.codes(1)[c.pages[0, torch.arange(n, device=dev) // PAGE], 0, torch.arange(n, device=dev) % PAGE]
+    for u in (u.amin(-1), u.amax(-1)):  # (of a row of one value: 1 x scale, whose 15 or 255 fold is nothing that it stands for)
+        stands = u * scale + (-scale * zero).half().to(F64) if bits == 4 else scale * (u - zero)
+        assert float(stands.abs().max()) < 65520
