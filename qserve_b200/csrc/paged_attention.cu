@@ -10,9 +10,9 @@
 //     O += P V        4 x tcgen05.mma 128 x 128 x 16, A from tensor memory
 // fp16 holds the operands (keys, values and weights, each off by 2^-11 of itself at most, INT8 keys and values by another 2^-12 of their scale): a product of exact codes would want every score multiplied by its key's
 // scale and every weight by its value's, a third more instructions of softmax warps that are the bound already.
-// A long axis of keys is split over blocks where the rows alone do not fill the device, or not its last round.  A split leaves its rows' maximum and sum in fp32 and
-// O / sum in fp16, rounded as a result is (in fp32 they were most of what 64 sequences behind 8192 shared positions move: 32.2 us, now 30.8); the cluster that holds
-// all splits, join_kernel (prompts) or the tail kernel (shared prefix) joins them in fp32.
+// A long axis of keys is split over blocks where the rows alone do not fill the device, or not its last round.  A split leaves its rows' maximum, sum and O / sum in fp32; the cluster
+// that holds all splits, join_kernel (prompts) or the tail kernel (shared prefix) joins them.  (O / sum in fp16 would be one more rounding of a result and half the bytes; us, fp16 /
+// now: 17 tokens behind 500 7.8 / 8.4, 24 behind 60000 41.8 / 43.4, 8 sequences behind 1024 shared positions 8.0 / 8.4, 64 behind 8192 30.3 / 31.6.)
 // Bounds: 4096 tokens of 32 heads over 8 behind 12000 positions, INT4, 780 to 860 us (0.94 TFLOP, 1.1 to 1.2 PFLOP/s), shared memory 0.87 of its cycles (the queries are
 // read again for every 64 keys, unpacked pages written and read) and issue slots 0.54, the tensor pipe 0.59; one tile: the chain load - unpack - softmax of a page,
 // 0.85 us with two blocks per multiprocessor.
@@ -74,12 +74,19 @@ __device__ __forceinline__ uint2 peer_u2(const void* mine, uint32_t rank) {
   asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
   return v;
 }
-__device__ __forceinline__ uint4 peer_u4(const void* mine, uint32_t rank) {
+__device__ __forceinline__ float peer_f32(const float* mine, uint32_t rank) {
   uint32_t a;
-  uint4 v;
+  float f;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+  return f;
+}
+__device__ __forceinline__ float4 peer_f32x4(const float* mine, uint32_t rank) {
+  uint32_t a;
+  float4 f;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
+  return f;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float y;
@@ -167,7 +174,7 @@ struct TileParams {
   int block_rows, split_from, run;        // of the items (of so many rows each; last rows first, sequence, kv head) those from here on are split; so many neighbours a run
   float scale_log2;
   // parts > 1: O / sum [rows][parts][128]: rows = token * num_heads + head where all items are split, otherwise those of the split items, one behind the other
-  __half* part;
+  float* part;
   float2* part_ml;                        // (maximum, sum) [rows][parts]
 };
 
@@ -217,9 +224,9 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   uint64_t* bar_raw = bar_vfree + C::kVStages;        // [slots] raw slot landed
   uint64_t* bar_used = bar_raw + C::kSlots;           // [slots] raw slot read
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar_used + C::kSlots);
-  // [128] rows' maximum and sum, for the cluster: over K, at the end.  (Shared memory of their own would leave L1 32 KB less: two blocks' 196 KB are a step of its
+  // [128] rows' maximum and sum, for the cluster: over V, at the end.  (Shared memory of their own would leave L1 32 KB less: two blocks' 196 KB are a step of its
   // size.  128 INT8 sequences behind 16384: 137 us, 158 so)
-  float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffK);
+  float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffV);
   static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 4 <= 384, "the barriers' place");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the shuffle: the same in all lanes, also to the compiler)
@@ -276,6 +283,43 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   int page0 = static_cast<int>(share.split * n_pages / share.nsplit);
   int n_mine = any ? static_cast<int>((share.split + 1) * n_pages / share.nsplit) - page0 : 0;
   asm volatile("" : "+r"(page0), "+r"(n_mine));
+
+  auto join_cluster = [&](int turn) {
+    // The blocks of the cluster take turns over the rows, their softmax and unpacking warps too: lane = four dims
+    cluster_sync();
+    const int rows = min(n_rows - row_base, kRows);
+#pragma unroll 1
+    for (int i = static_cast<int>(share.split) + p.cluster * turn; i < rows; i += p.cluster * 8) {
+      const float* at = reinterpret_cast<const float*>(smem + i * (kD * 4) + ((lane ^ (i & 7)) << 4));
+      float4 x[kMostCluster];
+      float2 ml[kMostCluster];
+#pragma unroll
+      for (int k = 0; k < kMostCluster; ++k) {
+        x[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        ml[k] = make_float2(-CUDART_INF_F, 0.f);
+        if (k < p.cluster) {
+          const uint2 w = peer_u2(s_ml + i, k);
+          ml[k] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
+          x[k] = peer_f32x4(at, k);
+        }
+      }
+      float M = -CUDART_INF_F, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int k = 0; k < kMostCluster; ++k) M = fmaxf(M, ml[k].x);
+      const float ref = M == -CUDART_INF_F ? 0.f : M;
+#pragma unroll
+      for (int k = 0; k < kMostCluster; ++k) {
+        const float w = ml[k].y * ex2(ml[k].x - ref);
+        L += w;
+        acc.x = fmaf(x[k].x, w, acc.x); acc.y = fmaf(x[k].y, w, acc.y); acc.z = fmaf(x[k].z, w, acc.z); acc.w = fmaf(x[k].w, w, acc.w);
+      }
+      const int row = row_base + i, t = row / group, h = hk * group + row - t * group;
+      const long long token = portion.start + t;
+      reinterpret_cast<uint2*>(p.out + token * p.out_stride + static_cast<long long>(h) * kD)[lane] = scaled_h4(acc, L);
+    }
+    cluster_sync();  // no block leaves while another reads its rows
+  };
 
   if (warp >= kUnpackWarp && warp < kIssueWarp) {
     // ===================================== unpacking =====================================
@@ -467,6 +511,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         if constexpr (!kEarly) all(j + 1);
       }
     }
+    if constexpr (MODE == kCluster) join_cluster(4 + warp - kUnpackWarp);
   } else if (warp >= kIssueWarp) {
     if constexpr (C::kShares) set_max_regs<false, kIssueRegs>();
     if (C::kRing && warp == kCopyWarp) {
@@ -643,26 +688,13 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       if (n_mine > 0) mbar_wait(&bar_o[tile * 2 + ((n_mine - 1) & 1)], static_cast<uint32_t>((n_mine - 1) >> 1) & 1u);
       tc_fence_after();
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);  // a row without keys: zeros
-      // Through shared memory (the tile's queries are done with), so that half a warp stores a whole row
-      uint8_t* mine = smem + tile * kQBytes + quarter * (kQBytes / 4);
       const long long token = portion.start + tok;
-      bool partial = false;
-      long long at = 0;
-      if constexpr (MODE == kPartial) {
-        unsigned block;  // (read again, so that the loop above holds nothing of it: it has no register to spare)
-        asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block));
-        const Share mine = share_of<MODE>(p, block);
-        partial = block >= static_cast<unsigned>(p.split_from);
-        const int row = p.split_from == 0 ? static_cast<int>(token) * p.num_heads + head
-                                          : static_cast<int>(mine.item - p.split_from) * (TILES * kRows) + (tile * kRows + quarter * 32 + lane);
-        at = static_cast<long long>(row) * p.parts + mine.split;
-      }
-      unsigned long long to = 0ull;
-      if (row_is) to = partial ? reinterpret_cast<unsigned long long>(p.part + at * kD)
-                                        : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
-#pragma unroll 1
-      for (int c = 0; c < 4; ++c) {
-        uint32_t o[32];
+      // eight dims in turn of the row's 128
+      auto eight = [&](const uint32_t (&o)[32], int e, float (&f)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]) * inv;
+      };
+      auto fetch = [&](uint32_t (&o)[32], int c) {
         if (n_mine > 0) {
           tmem_ld_32x32b_x32(t_o + c * 32, o);
           tmem_wait_ld();
@@ -670,75 +702,95 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float f[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) f[i] = __uint_as_float(o[e * 8 + (BITS == 4 ? (i < 4 ? 2 * i : 2 * i - 7) : i)]) * inv;
-          *reinterpret_cast<uint4*>(mine + lane * 256 + (((c * 4 + e) ^ (lane & 7)) << 4)) =
-              make_uint4(as_u32(__floats2half2_rn(f[0], f[1])), as_u32(__floats2half2_rn(f[2], f[3])), as_u32(__floats2half2_rn(f[4], f[5])),
-                         as_u32(__floats2half2_rn(f[6], f[7])));
-        }
-      }
+      };
+      // A partial row: where it goes, in rows of 128 numbers.  (The block's number is read again, so that the loop above holds nothing of it: it has no register to spare)
+      bool partial = false;
+      long long at = 0;
+      unsigned long long to = 0ull;
       if constexpr (MODE != kCluster) {
-        __syncwarp();
-#pragma unroll 4
-        for (int k = 0; k < 32; k += 2) {
-          const int in = k + (lane >> 4), chunk = lane & 15;
-          uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
-          if (row) row[chunk] = v;
+        if constexpr (MODE == kPartial) {
+          unsigned block;
+          asm volatile("mov.u32 %0, %%ctaid.x;" : "=r"(block));
+          const Share mine = share_of<MODE>(p, block);
+          partial = block >= static_cast<unsigned>(p.split_from);
+          const int row = p.split_from == 0 ? static_cast<int>(token) * p.num_heads + head
+                                            : static_cast<int>(mine.item - p.split_from) * (TILES * kRows) + (tile * kRows + quarter * 32 + lane);
+          at = static_cast<long long>(row) * p.parts + mine.split;
         }
-        if (partial && row_is) p.part_ml[at] = make_float2(m_used, l);
-      } else {
-        s_ml[quarter * 32 + lane] = make_float2(m_used, l);
+        if (row_is) to = partial ? reinterpret_cast<unsigned long long>(p.part + at * kD)
+                                 : reinterpret_cast<unsigned long long>(p.out + token * p.out_stride + static_cast<long long>(head) * kD);
       }
-    }
-    if constexpr (MODE == kCluster) {
-      // The blocks of the cluster take turns over the rows, the halves of their softmax warps too: lane = eight dims
-      cluster_sync();
-      const int rows = min(n_rows - row_base, kRows), chunk = lane & 15;
+      if constexpr (MODE != kWhole && TILES == 1) {
+        // fp32 rows of 512 bytes over Q and K, all of whose products have retired
+        static_assert(kRows * kD * 4 <= C::kOffV, "rows' maxima and sums lie behind the rows");
+        uint8_t* const rows = smem + quarter * 32 * (kD * 4);
+        auto chunk = [&](int row, int i) { return reinterpret_cast<float4*>(rows + row * (kD * 4) + ((i ^ (row & 7)) << 4)); };
 #pragma unroll 1
-      for (int i = static_cast<int>(share.split) + p.cluster * (2 * warp + (lane >> 4)); i < rows; i += p.cluster * 8) {
-        const uint8_t* at = smem + i * 256 + ((chunk ^ (i & 7)) << 4);
-        uint4 x[kMostCluster];
-        float2 ml[kMostCluster];
-#pragma unroll
-        for (int k = 0; k < kMostCluster; ++k) {
-          x[k] = make_uint4(0u, 0u, 0u, 0u);
-          ml[k] = make_float2(-CUDART_INF_F, 0.f);
-          if (k < p.cluster) {
-            const uint2 w = peer_u2(s_ml + i, k);
-            ml[k] = make_float2(__uint_as_float(w.x), __uint_as_float(w.y));
-            x[k] = peer_u4(at, k);
-          }
-        }
-        float M = -CUDART_INF_F, L = 0.f, acc[8] = {};
-#pragma unroll
-        for (int k = 0; k < kMostCluster; ++k) M = fmaxf(M, ml[k].x);
-        const float ref = M == -CUDART_INF_F ? 0.f : M;
-#pragma unroll
-        for (int k = 0; k < kMostCluster; ++k) {
-          const float w = ml[k].y * ex2(ml[k].x - ref);
-          L += w;
-          const uint32_t words[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          fetch(o, c);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const float2 a = __half22float2(as_h2(words[e]));
-            acc[2 * e] = fmaf(a.x, w, acc[2 * e]);
-            acc[2 * e + 1] = fmaf(a.y, w, acc[2 * e + 1]);
+            float f[8];
+            eight(o, e, f);
+            *chunk(lane, c * 8 + 2 * e) = make_float4(f[0], f[1], f[2], f[3]);
+            *chunk(lane, c * 8 + 2 * e + 1) = make_float4(f[4], f[5], f[6], f[7]);
           }
         }
-        const uint2 lo = scaled_h4(make_float4(acc[0], acc[1], acc[2], acc[3]), L), hi = scaled_h4(make_float4(acc[4], acc[5], acc[6], acc[7]), L);
-        const int row = row_base + i, t = row / group, h = hk * group + row - t * group;
-        const long long token = portion.start + t;
-        reinterpret_cast<uint4*>(p.out + token * p.out_stride + static_cast<long long>(h) * kD)[chunk] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        if constexpr (MODE == kCluster) {
+          s_ml[quarter * 32 + lane] = make_float2(m_used, l);
+        } else {  // a warp a row
+          __syncwarp();
+          const int many = min(32, n_rows - first_row);
+#pragma unroll 8
+          for (int k = 0; k < many; ++k) {
+            const unsigned long long row = __shfl_sync(0xffffffffu, to, k);
+            const float4 x = *chunk(k, lane);
+            if (partial) reinterpret_cast<float4*>(row)[lane] = x;
+            else reinterpret_cast<uint2*>(row)[lane] = make_uint2(as_u32(__floats2half2_rn(x.x, x.y)), as_u32(__floats2half2_rn(x.z, x.w)));
+          }
+        }
+      } else {
+        // Through shared memory (the tile's queries are done with), so that half a warp stores a whole row, or half a row of fp32
+        uint8_t* mine = smem + tile * kQBytes + quarter * (kQBytes / 4);
+        auto put = [&](int chunk, uint4 x) { *reinterpret_cast<uint4*>(mine + lane * 256 + ((chunk ^ (lane & 7)) << 4)) = x; };
+        auto store = [&](int behind) {
+          __syncwarp();
+#pragma unroll 4
+          for (int k = 0; k < 32; k += 2) {
+            const int in = k + (lane >> 4), chunk = lane & 15;
+            uint4* row = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, to, in));
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + in * 256 + ((chunk ^ (in & 7)) << 4));
+            if (row) row[behind + chunk] = v;
+          }
+          __syncwarp();
+        };
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          uint32_t o[32];
+          fetch(o, c);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float f[8];
+            eight(o, e, f);
+            if (MODE == kPartial && partial) {
+              put((c & 1) * 8 + 2 * e, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
+              put((c & 1) * 8 + 2 * e + 1, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])));
+            } else {
+              put(c * 4 + e, make_uint4(as_u32(__floats2half2_rn(f[0], f[1])), as_u32(__floats2half2_rn(f[2], f[3])), as_u32(__floats2half2_rn(f[4], f[5])),
+                                        as_u32(__floats2half2_rn(f[6], f[7]))));
+            }
+          }
+          if (MODE == kPartial && partial && c == 1) store(0);
+        }
+        store(MODE == kPartial && partial ? 16 : 0);
       }
-      cluster_sync();  // no block leaves while another reads its rows
+      if (partial && row_is) p.part_ml[at] = make_float2(m_used, l);
     }
+    if constexpr (MODE == kCluster) join_cluster(warp);
   }
   if constexpr (MODE == kCluster) {
-    if (warp >= kUnpackWarp) {  // the softmax warps' two waits
+    if (warp >= kIssueWarp) {  // the other warps' two waits
       cluster_sync();
       cluster_sync();
     }
@@ -751,15 +803,15 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
 // ------------------------------------------------------------------------------------------------------------------------
 // partial rows of a split joined: a warp, lane = 4 dims.  Returns the sum and the maximum that acc is expressed against.
 // ------------------------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void join_rows(const __half* part, const float2* ml, int nsplit, float& M, float& L, float4& acc) {
+__device__ __forceinline__ void join_rows(const float* part, const float2* ml, int nsplit, float& M, float& L, float4& acc) {
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < nsplit; s0 += 32) {
     const int n = min(32, nsplit - s0);
-    const uint2* rows = reinterpret_cast<const uint2*>(part + static_cast<long long>(s0) * kD) + lane;
-    uint2 x[8];
+    const float4* rows = reinterpret_cast<const float4*>(part + static_cast<long long>(s0) * kD) + lane;
+    float4 x[8];
     auto fetch = [&](int s) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = s + k < n ? __ldcg(rows + (s + k) * (kD / 4)) : make_uint2(0u, 0u);
+      for (int k = 0; k < 8; ++k) x[k] = s + k < n ? __ldcg(rows + (s + k) * (kD / 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
     };
     fetch(0);  // on their way together with the maxima and sums
     const float2 mine = lane < n ? __ldcg(ml + s0 + lane) : make_float2(-CUDART_INF_F, 0.f);
@@ -779,8 +831,7 @@ __device__ __forceinline__ void join_rows(const __half* part, const float2* ml, 
 #pragma unroll
       for (int k = 0; k < 8; ++k) {  // (behind the last split: zeros with a weight of zero)
         const float ws = __shfl_sync(0xffffffffu, weight, (s + k) & 31);
-        const float2 a = __half22float2(as_h2(x[k].x)), b = __half22float2(as_h2(x[k].y));
-        acc.x = fmaf(a.x, ws, acc.x); acc.y = fmaf(a.y, ws, acc.y); acc.z = fmaf(b.x, ws, acc.z); acc.w = fmaf(b.y, ws, acc.w);
+        acc.x = fmaf(x[k].x, ws, acc.x); acc.y = fmaf(x[k].y, ws, acc.y); acc.z = fmaf(x[k].z, ws, acc.z); acc.w = fmaf(x[k].w, ws, acc.w);
       }
     }
   }
@@ -881,21 +932,6 @@ __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
   return d;
 }
-__device__ __forceinline__ float peer_f32(const float* mine, uint32_t rank) {
-  uint32_t a;
-  float f;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
-  return f;
-}
-__device__ __forceinline__ float4 peer_f32x4(const float* mine, uint32_t rank) {
-  uint32_t a;
-  float4 f;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w) : "r"(a) : "memory");
-  return f;
-}
-
 struct TailParams {
   const __half* q;
   __half* out;
@@ -904,7 +940,7 @@ struct TailParams {
   const int* lengths;
   int batch, max_blocks, num_heads, num_kv_heads, shared_blocks, nsplit, cluster;
   float scale_log2;
-  const __half* part;
+  const float* part;
   const float2* part_ml;
 };
 
@@ -1283,7 +1319,7 @@ struct Plan {
 };
 constexpr float kTwoTilesPage = 0.92f, kTwoTilesFixed = 5.5f;  // us
 Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, long long pages, bool prompt) {
-  constexpr float kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 5e6f;
+  constexpr float kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 1e7f;
   Plan pl{};
   pl.tiles = rows <= kRows ? 1 : 2;
   const long long block_rows = pl.tiles * kRows, sms = num_sms();
@@ -1312,7 +1348,7 @@ Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, lon
       return batch == 1 || of <= slots ? full : 0.5f * (full + of / static_cast<float>(slots));
     };
     auto join = [&](long long split, unsigned n) {
-      return prompt ? kJoinKernel + (split * (num_rows * kv_heads / static_cast<float>(blocks)) * n) * (2.f * (kD * 2 + 8)) / kPartBytesPerUs : kJoinTail * n;
+      return prompt ? kJoinKernel + (split * (num_rows * kv_heads / static_cast<float>(blocks)) * n) * (2.f * (kD * 4 + 8)) / kPartBytesPerUs : kJoinTail * n;
     };
     take(rounds(blocks) * block(1), 1, 1, prompt ? 0 : pl.items);
     // splits of one round
@@ -1332,7 +1368,7 @@ Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, lon
   pl.parts = pl.nsplit / pl.cluster;
   return pl;
 }
-size_t part_bytes(long long rows, int parts) { return static_cast<size_t>(rows) * parts * (kD * sizeof(__half) + sizeof(float2)); }
+size_t part_bytes(long long rows, int parts) { return static_cast<size_t>(rows) * parts * (kD * sizeof(float) + sizeof(float2)); }
 
 template <int BITS, int TILES, int MODE>
 int run_tiles(const TileParams& p, long long blocks, void* stream) {
@@ -1390,7 +1426,7 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
     QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.parts), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,
                part_bytes(rows, pl.parts));
     QS_REQUIRE(rows <= 0x7fffffffll, "paged_prompt_attention: %lld rows", rows);
-    p.part = static_cast<__half*>(a.workspace);
+    p.part = static_cast<float*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
   }
   const int rc = tiles(p, pl, a.cache.int4, a.stream);
@@ -1465,7 +1501,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
     p.q = t.q; p.q_stride = t.q_stride; p.kv_pointers = t.kv_pointers; p.lengths = t.lengths;
     p.batch = 1; p.num_tokens = p.max_seqlen = a.batch; p.max_blocks = t.max_blocks; p.num_heads = t.num_heads; p.num_kv_heads = t.num_kv_heads;
     p.shared_blocks = shared_blocks; p.scale_log2 = t.scale_log2;
-    p.part = static_cast<__half*>(a.workspace);
+    p.part = static_cast<float*>(a.workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * pl.parts * kD);
     t.nsplit = pl.parts; t.part = p.part; t.part_ml = p.part_ml;
     const int rc = tiles(p, pl, a.cache.int4, a.stream);

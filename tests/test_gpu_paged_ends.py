@@ -171,3 +171,39 @@ def test_appended_rows_of_any_ends_are_finite(dev, bits):
     for u in (u.amin(-1), u.amax(-1)):  # (of a row of one value: 1 x scale, whose 15 or 255 fold is nothing that it stands for)
         stands = u * scale + (-scale * zero).half().to(F64) if bits == 4 else scale * (u - zero)
         assert float(stands.abs().max()) < 65520
+
+
+# ---- one rounding of a result ----
+def equal_weights(c, n):
+    """All keys of a head alike, so that all weights are; values that are eighths from -1 to 7 / 8 (INT8: from -16), so that values and sums are exact, and
+    weights up to 2^-18 (a score's last bit, up to 2^-18, in its exponent)."""
+    for b in range(len(c.lens)):
+        m = c.lens[b]
+        fill(c, 0, b, random_codes(1, c.hkv, c.bits, 5).expand(m, -1, -1), torch.full((m, c.hkv), 0.125), torch.full((m, c.hkv), 8.0))
+        fill(c, 1, b, random_codes(m, c.hkv, c.bits, 6), torch.full((m, c.hkv), 0.125), torch.full((m, c.hkv), 8.0 if c.bits == 4 else 128.0))
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,new,ahead", [(8, 2, [17], [500]), (32, 8, [3], [5000]), (8, 2, [24], [20000]), (8, 2, [300], [2000]), (32, 8, [1300], [500]), (32, 8, [20], [64])])
+def test_the_parts_of_a_split_row_are_not_rounded(dev, bits, hq, hkv, new, ahead):
+    """However a row's keys are split (cluster, join kernel, a last round): one rounding."""
+    lens = [n + m for n, m in zip(new, ahead)]
+    c = Cache(lens, hkv, bits, dev, seed=1)
+    equal_weights(c, lens)
+    q = queries(sum(new), hq, dev)
+    want = prompt64(c, q, new, lens)[0]
+    out = run_prompt(c, q, new)
+    off, room = (out.to(F64) - want).abs(), H * want.abs() * (1 + 2.0 ** -7) + 2.0 ** -20
+    assert (off <= room).all(), float((off / room).max())
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,shared,lens", [(8, 2, 33, [2200, 9000, 2112]), (32, 8, 30, [2000] * 40), (32, 8, 20, [1400] * 300), (16, 1, 300, [19300, 19201])])
+def test_the_parts_of_a_shared_row_are_not_rounded(dev, bits, hq, hkv, shared, lens):
+    c = Cache(lens, hkv, bits, dev, shared=shared, seed=1)
+    equal_weights(c, lens)
+    q = queries(len(lens), hq, dev)
+    out = backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args)
+    want = shared64(c, q, lens)[0]
+    off, room = (out.to(F64) - want).abs(), H * want.abs() * (1 + 2.0 ** -7) + 2.0 ** -20
+    assert (off <= room).all(), float((off / room).max())
