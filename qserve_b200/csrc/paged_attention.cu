@@ -939,6 +939,7 @@ struct TailParams {
   const long long* kv_pointers;
   const int* lengths;
   int batch, max_blocks, num_heads, num_kv_heads, shared_blocks, nsplit, cluster;
+  int common;  // pages from the first on that the first sequence's row names for all (0 where the tile kernel has read them: shared_blocks > 0)
   float scale_log2;
   const float* part;
   const float2* part_ml;
@@ -976,7 +977,6 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
   const int stride = SHARED ? p.cluster * kTailWarps : 1, mine = SHARED ? rank * kTailWarps + warp : 0;
   const int n_my = slices > mine ? (slices - mine + stride - 1) / stride : 0;
   const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + p.shared_blocks;
-  const long long* vptrs = kptrs + p.max_blocks;
   uint8_t* ring = smem + warp * SC::kWarpBytes;
   const uint32_t ring_at = smem_u32(ring);
   const uint32_t lane_at = SC::place(lane * 16 / SC::kRow, lane * 16 % SC::kRow / 16);
@@ -984,8 +984,9 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
   auto issue = [&](int u) {
     if ((u & 31) == 0 && u + lane < n_my) {
       const int page = (mine + (u + lane) * stride) >> 1;
-      kp_l = __ldcg(kptrs + page);
-      vp_l = __ldcg(vptrs + page);
+      const long long* row = page < p.common ? p.kv_pointers : kptrs;
+      kp_l = __ldcg(row + page);
+      vp_l = __ldcg(row + p.max_blocks + page);
     }
     const int half = (mine + u * stride) & 1;
     const uint8_t* kp = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp_l, u & 31));
@@ -1396,7 +1397,7 @@ Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int 
   return plan_tiles(static_cast<long long>(max_seqlen) * group, batch, static_cast<long long>(num_tokens) * group, kv_heads,
                     (static_cast<long long>(max_length) + kPage - 1) / kPage, true);
 }
-// Few sequences or few shared pages: the tail kernel reads every sequence's whole table, one launch instead of two.  us, both kernels / the tail alone (INT4, 32 heads
+// Few sequences or few shared pages: the tail kernel reads the shared pages too, once per sequence (out of the first row of the table), one launch instead of two.  us, both kernels / the tail alone (INT4, 32 heads
 // over 8, 100 positions behind): one sequence behind 512 6.5 / 6.0, behind 4096 9.5 / 8.2; two behind 512 6.7 / 6.3, behind 2048 7.9 / 9.0; eight behind 128 6.4 /
 // 4.9, behind 512 6.6 / 8.7.
 bool tail_alone(int batch, int shared_blocks) { return batch == 1 || static_cast<long long>(batch) * shared_blocks <= 16; }
@@ -1475,9 +1476,12 @@ int side_by_side(Plan& pl, int shared_blocks, long long tail, long long tail_pag
 
 int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   if (a.batch == 0) return QS_OK;
-  if (tail_alone(a.batch, shared_blocks)) shared_blocks = 0;
-  const long long rows = static_cast<long long>(a.batch) * a.num_heads;
   TailParams t{};
+  if (tail_alone(a.batch, shared_blocks)) {
+    t.common = shared_blocks;
+    shared_blocks = 0;
+  }
+  const long long rows = static_cast<long long>(a.batch) * a.num_heads;
   t.q = static_cast<const __half*>(a.q); t.out = static_cast<__half*>(a.out); t.q_stride = a.q_stride; t.out_stride = a.out_stride;
   t.batch = a.batch; t.kv_pointers = a.cache.kv_pointers; t.lengths = a.cache.lengths; t.max_blocks = a.cache.max_blocks; t.num_heads = a.num_heads;
   t.num_kv_heads = a.cache.num_kv_heads; t.shared_blocks = shared_blocks; t.scale_log2 = a.softmax_scale * 1.4426950408889634f;

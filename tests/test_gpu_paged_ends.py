@@ -207,3 +207,15 @@ def test_the_parts_of_a_shared_row_are_not_rounded(dev, bits, hq, hkv, shared, l
     want = shared64(c, q, lens)[0]
     off, room = (out.to(F64) - want).abs(), H * want.abs() * (1 + 2.0 ** -7) + 2.0 ** -20
     assert (off <= room).all(), float((off / room).max())
+
+
+# ---- shared columns of the table ----
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,shared,lens", [(8, 2, 2, [200, 150, 100]), (8, 2, 16, [1300]), (8, 2, 6, [500, 384, 100, 7]), (32, 8, 3, [250] * 40)])
+def test_shared_pages_are_those_of_the_first_row(dev, bits, hq, hkv, shared, lens):
+    """The other rows hold other pages (the last sequence's own, NaN where it ends) in the shared columns: nothing reads them, however few sequences there are."""
+    c = Cache(lens, hkv, bits, dev, shared=shared, seed=sum(lens), extra_blocks=1)
+    q = queries(len(lens), hq, dev)
+    want = shared64(c, q, lens)
+    c.table[1:, :, :shared] = c.table[-1:, :, -1:]
+    check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args), want, SCALE)
