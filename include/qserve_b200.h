@@ -140,7 +140,8 @@ QS_API int qs_append_kv_cache(const void* q, const void* k, const void* v, int64
                               int64_t q_out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch,
                               int num_tokens, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block,
                               int size_per_token, int rotary_embedding_dim, float rotary_base, int int4_kv_cache, int kv_cache_with_zeros, void* stream);
-/* k_out, v_out fp16 [num_tokens, num_kv_heads, 128] <- what the pages stand for: half(s u + half(-s z)) (INT4), half(s (u - z)) (INT8) */
+/* k_out, v_out fp16 [num_tokens, num_kv_heads, 128] <- what the pages stand for: half(s u + half(-s z)) (INT4), half(s (u - z)) (INT8); zeros for a row that
+ * has no position in its sequence's pages */
 QS_API int qs_read_kv_cache(void* k_out, void* v_out, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch,
                             int num_tokens, int max_blocks_per_seq, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token,
                             int int4_kv_cache, int kv_cache_with_zeros, void* stream);

@@ -3,7 +3,7 @@
 // append: token i of sequence b's portion of n_b takes position p = lengths[b] - n_b + i.  Queries and keys are rotated (entry i with entry i + 64, angle
 // p base^(-2 i / 128)), keys and values quantised per (token, kv head): scale s = half((max - min) / L), zero z = half(-L min / (max - min)), code
 // clamp(round(x / s + z), 0, L), L = 15 or 255.
-// read: the same positions out of the pages again, as fp16.
+// read: the same positions out of the pages again, as fp16; zeros for a row that has none.
 #include <math_constants.h>
 
 #include <cmath>
@@ -288,16 +288,22 @@ __global__ void __launch_bounds__(32 * kWarps) read_kernel(const ReadParams p) {
   const Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
   const int pos = portion.first + t - portion.start;
   const int block = pos >> 6, slot = pos & (kPage - 1);
-  if (pos < 0 || block >= p.max_blocks) return;
-  const long long* table = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + block;
-  const uint8_t* const pages[2] = {reinterpret_cast<const uint8_t*>(table[0]), reinterpret_cast<const uint8_t*>(table[p.max_blocks])};
+  const bool held = pos >= 0 && block < p.max_blocks;  // a row without a position gets zeros, as attention gives it
+  const uint8_t* pages[2] = {nullptr, nullptr};
+  if (held) {
+    const long long* table = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks + block;
+    pages[0] = reinterpret_cast<const uint8_t*>(table[0]);
+    pages[1] = reinterpret_cast<const uint8_t*>(table[p.max_blocks]);
+  }
   Word lo[ROWS], hi[ROWS];
   __half s[ROWS], z[ROWS];
   const int r0 = blockIdx.y * 4 * ROWS + sub;
 #pragma unroll
   for (int e = 0; e < ROWS; ++e) {
     const int r = r0 + 4 * e, which = r >= p.num_kv_heads, head = r - which * p.num_kv_heads;
-    if (r < 2 * p.num_kv_heads) {
+    lo[e] = hi[e] = Word{};
+    s[e] = z[e] = __ushort_as_half(0);
+    if (r < 2 * p.num_kv_heads && held) {
       const uint8_t* page = which ? pages[1] : pages[0];
       const Word* row = reinterpret_cast<const Word*>(page + G::codes_at(head) + slot * G::kRow);
       lo[e] = row[l];

@@ -219,3 +219,22 @@ def test_shared_pages_are_those_of_the_first_row(dev, bits, hq, hkv, shared, len
     want = shared64(c, q, lens)
     c.table[1:, :, :shared] = c.table[-1:, :, -1:]
     check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, shared, max(lens), *c.args), want, SCALE)
+
+
+# ---- rows without a position ----
+@pytest.mark.parametrize("bits", [4, 8])
+def test_rows_without_a_position_read_as_zeros(dev, bits):
+    """A length smaller than the portion, none, one past the table: zeros where there is no position, whatever lay in the memory of the result."""
+    c = Cache([70, 64, 128, 40], 2, bits, dev, seed=6)
+    new, T = [20, 3, 10, 2], 35
+    c.lengths.copy_(torch.tensor([12, 0, 2 * PAGE + 4, 40], dtype=torch.int32))
+    for _ in range(3):
+        old = torch.full((2, T, 2, D), 7.0, dtype=HALF, device=dev)
+        del old
+        k, v = backend.read_kv_cache(c.table, starts(new, dev), c.lengths, T, *c.args)
+        for which, got in ((0, k), (1, v)):
+            none = torch.zeros(T, dtype=torch.bool)
+            none[:8] = none[20:23] = none[29:33] = True
+            assert bool((got[none] == 0).all())
+            want = torch.cat([c.values(which, 0, 12), c.values(which, 2, 128)[122:], c.values(which, 3, 40)[38:]])
+            assert ((got[~none].to(F64) - want).abs() <= H * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -23).all()
