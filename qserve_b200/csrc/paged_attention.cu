@@ -178,9 +178,16 @@ struct TileParams {
   float2* part_ml;                        // (maximum, sum) [rows][parts]
 };
 
+// Two results in fp16, no further from 0 than its largest number (NaN stays NaN): a mean of values is no larger than they are, but rounded weights over the sum of the unrounded ones may be
+// 2^-11 more than 1, and 65504 of that rounds to infinity
+__device__ __forceinline__ uint32_t results(float a, float b) {
+  uint32_t d;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
+  return d;
+}
 __device__ __forceinline__ uint2 scaled_h4(const float4& a, float L) {
   const float inv = L > 0.f ? 1.f / L : (L == 0.f ? 0.f : L);
-  return make_uint2(as_u32(__floats2half2_rn(a.x * inv, a.y * inv)), as_u32(__floats2half2_rn(a.z * inv, a.w * inv)));
+  return make_uint2(results(a.x * inv, a.y * inv), results(a.z * inv, a.w * inv));
 }
 
 // What a block does with its rows: the result; a partial result where its item is split; or its cluster's, joined first.
@@ -747,7 +754,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
             const unsigned long long row = __shfl_sync(0xffffffffu, to, k);
             const float4 x = *chunk(k, lane);
             if (partial) reinterpret_cast<float4*>(row)[lane] = x;
-            else reinterpret_cast<uint2*>(row)[lane] = make_uint2(as_u32(__floats2half2_rn(x.x, x.y)), as_u32(__floats2half2_rn(x.z, x.w)));
+            else reinterpret_cast<uint2*>(row)[lane] = make_uint2(results(x.x, x.y), results(x.z, x.w));
           }
         }
       } else {
@@ -777,8 +784,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
               put((c & 1) * 8 + 2 * e, make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])));
               put((c & 1) * 8 + 2 * e + 1, make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7])));
             } else {
-              put(c * 4 + e, make_uint4(as_u32(__floats2half2_rn(f[0], f[1])), as_u32(__floats2half2_rn(f[2], f[3])), as_u32(__floats2half2_rn(f[4], f[5])),
-                                        as_u32(__floats2half2_rn(f[6], f[7]))));
+              put(c * 4 + e, make_uint4(results(f[0], f[1]), results(f[2], f[3]), results(f[4], f[5]), results(f[6], f[7])));
             }
           }
           if (MODE == kPartial && partial && c == 1) store(0);

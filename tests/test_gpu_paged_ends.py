@@ -238,3 +238,23 @@ def test_rows_without_a_position_read_as_zeros(dev, bits):
             assert bool((got[none] == 0).all())
             want = torch.cat([c.values(which, 0, 12), c.values(which, 2, 128)[122:], c.values(which, 3, 40)[38:]])
             assert ((got[~none].to(F64) - want).abs() <= H * want.abs() * (1 + 2.0 ** -10) + 2.0 ** -23).all()
+
+
+# ---- results at the ends of fp16 ----
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("value", [65504.0, -65504.0])
+@pytest.mark.parametrize("n", [40, 700, 5000])
+def test_a_mean_of_the_largest_values_is_one(dev, bits, value, n):
+    """All values +- 65504: rounded weights over their unrounded sum may be more than 1 by H / 2 and more, the result is still no infinity.  One key a page scores higher than the others, which
+    all have the same weight, so that roundings add up."""
+    hkv, new = 2, min(n, 30)
+    c = Cache([n], hkv, bits, dev, seed=3)
+    u = random_codes(1, hkv, bits, 5).expand(n, -1, -1).clone()
+    u[::PAGE] = random_codes(1, hkv, bits, 6)
+    fill(c, 0, 0, u, torch.full((n, hkv), 0.2 / 2 ** (bits - 4)), torch.full((n, hkv), 2.0 ** (bits - 1)))
+    fill(c, 1, 0, torch.full((n, hkv, D), int(value > 0)), torch.full((n, hkv), abs(value)), torch.full((n, hkv), float(value < 0)))
+    q = queries(new, 32, dev)
+    one = c.table.expand(new, -1, -1).contiguous()
+    lens = torch.full((new,), n, dtype=torch.int32, device=dev)
+    for out in (run_prompt(c, q, [new]), backend.shared_prefix_attention(q, one, lens, 0, n, *c.args), backend.shared_prefix_attention(q, one, lens, n // PAGE, n, *c.args)):
+        assert bool(((out.float() - value).abs() <= 2 * H * abs(value)).all()), float((out.float() / value - 1).abs().max())
