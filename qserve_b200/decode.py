@@ -32,6 +32,7 @@ import qserve_backend.qgemm_w4a8_per_chn as qgemm_chn
 import qserve_backend.qgemm_w4a8_per_group as qgemm_grp
 import qserve_backend.qgemm_w8a8 as qgemm_w8
 from qserve_b200 import backend as _ext
+from qserve_b200._lib import lib
 
 
 @dataclass(frozen=True)
@@ -191,6 +192,9 @@ class DecodeRunner:
         self.tokens_out = torch.zeros(M, dtype=torch.int64, device=dev)
         self.graph: Optional[torch.cuda.CUDAGraph] = None
         self.launches_per_step = 0
+        self.attention_launches = 1
+        if self.shared_blocks:  # append, the shared pages where they are read by a kernel of their own (which needs a work space), the sequences' own
+            self.attention_launches = 3 if lib.qs_shared_prefix_attention_workspace_bytes(batch, self.shared_blocks, self.Hq, self.Hkv) else 2
 
     # ---------------------------------------------------------------------------------------------------------
     def _norm_quant(self, x, gamma):
@@ -267,7 +271,7 @@ class DecodeRunner:
             ly["down"](self.q_mlp, self.q_scale, self.q_sum, self.out_buf)
             self._allreduce(self.out_buf)
             hidden = residual + self.out_buf  # :360
-            n += 10
+            n += 9 + self.attention_launches
         out = torch.empty_like(hidden)
         self.ops.layernorm_ops.rms_norm(out, hidden, self.norm_w, cfg.eps, False)  # final norm (:408)
         logits = torch.nn.functional.linear(out, self.lm_head)           # fp16 lm_head (:474-476)
@@ -310,7 +314,7 @@ class DecodeRunner:
             else:
                 ly["down"](self.q_mlp, self.q_scale, self.q_sum, self.out_buf)
                 self._allreduce(self.out_buf)
-            n += 11 if exact else 10 if self.shared_blocks else 7  # (append, prefix, rest and quantisation for one)
+            n += 11 if exact else 7 + self.attention_launches if self.shared_blocks else 7  # (attention and quantisation for one)
             if self.tp_peer:
                 # the last layer has no following norm: the same kernel delivers hidden + sum(partials) (its quantised output is not used)
                 gam = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else ly["ln1"]

@@ -258,3 +258,31 @@ def test_a_mean_of_the_largest_values_is_one(dev, bits, value, n):
     lens = torch.full((new,), n, dtype=torch.int32, device=dev)
     for out in (run_prompt(c, q, [new]), backend.shared_prefix_attention(q, one, lens, 0, n, *c.args), backend.shared_prefix_attention(q, one, lens, n // PAGE, n, *c.args)):
         assert bool(((out.float() - value).abs() <= 2 * H * abs(value)).all()), float((out.float() / value - 1).abs().max())
+
+
+# ---- the decode runner ----
+def kernels_of(r):
+    """Kernel nodes of the runner's step, captured."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    r.forward(r.tokens_in)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    with torch.cuda.graph(graph):
+        r.tokens_out.copy_(r.forward(r.tokens_in))
+    raw = rt.cudaGraph_t(graph.raw_cuda_graph())
+    err, _, n = rt.cudaGraphGetNodes(raw)
+    assert int(err) == 0
+    err, nodes, n = rt.cudaGraphGetNodes(raw, n)
+    assert int(err) == 0
+    types = [rt.cudaGraphNodeGetType(x)[1] for x in nodes[:n]]
+    return sum(t == rt.cudaGraphNodeType.cudaGraphNodeTypeKernel for t in types)
+
+
+@pytest.mark.parametrize("fused", [True, False])
+@pytest.mark.parametrize("batch,shared", [(6, 256), (2, 128), (1, 256)])
+def test_the_runner_counts_its_launches(dev, fused, batch, shared):
+    """A shared prefix adds as many kernels to the captured step as the runner says, with the shared pages in a kernel of their own or not."""
+    from qserve_b200.decode import DecodeRunner
+    a, b = (DecodeRunner("tiny", "w4a8kv4", batch=batch, ctx=300, device=dev, fused=fused, shared_prefix=n) for n in (0, shared))
+    more = kernels_of(b) - kernels_of(a)
+    assert more > 0 and b.launches_per_step - a.launches_per_step == more
