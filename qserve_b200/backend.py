@@ -358,7 +358,7 @@ def append_kv_cache(q, k, v, kv_pointers, cu_seqlens: Optional[torch.Tensor], le
 
 def read_kv_cache(kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, num_tokens: int, tokens_per_block: int, size_per_token: int, int4_kv_cache: bool,
                   kv_cache_with_zeros: bool):
-    """What the pages stand for at the last positions of the sequences: two new tensors k, v fp16 [num_tokens,Hkv,128] in one allocation (num_tokens >= cu_seqlens[-1]).
+    """What the pages stand for at the last positions of the sequences: two new tensors k, v fp16 [num_tokens,Hkv,128] (num_tokens >= cu_seqlens[-1]).
     A whole sequence is read with cu_seqlens over its length.  Zeros for a row without a position in its sequence's pages."""
     return _bind.read_kv_cache(kv_pointers, cu_seqlens, lengths, num_tokens, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros)
 

@@ -295,7 +295,7 @@ Heads heads_of(const at::Tensor& t, const at::Tensor& like, const char* name) {
   // (a single row has no stride to speak of)
   return {t.data_ptr(), t.size(0) > 1 ? t.stride(0) : t.size(1) * 128, static_cast<int>(t.size(0)), static_cast<int>(t.size(1))};
 }
-// New tensors on q's device without the dispatcher's way to the allocator (read_kv_cache, then two of them: 5.2 us a call on the host, 4.1 so)
+// New tensors on q's device without the dispatcher's way to the allocator
 at::Tensor fresh(at::IntArrayRef size, at::ScalarType type, const at::Tensor& q) { return at::detail::empty_cuda(size, type, q.device(), std::nullopt); }
 // the result's tensor: argument i, or a new one of q's sizes where it is None
 at::Tensor result_of(const Args& a, int i, const at::Tensor& q) {
@@ -330,13 +330,7 @@ PyObject* read_kv_cache(const Args& a) {
   const Cache c = cache_of(a, t, 0, 1, 2, 4, 6);
   const int tokens = a.small(3);
   require(tokens >= 0, "num_tokens must not be negative");
-  // both in one allocation
-  at::Tensor k = fresh({2, tokens, c.heads_kv, 128}, at::kHalf, t);
-  at::Tensor v = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(k.storage()), k.key_set(), k.dtype());
-  const int64_t sizes[3] = {tokens, c.heads_kv, 128};
-  k.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-  v.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
-  v.unsafeGetTensorImpl()->set_storage_offset(k.numel());
+  at::Tensor k = fresh({tokens, c.heads_kv, 128}, at::kHalf, t), v = fresh({tokens, c.heads_kv, 128}, at::kHalf, t);
   void *kp = k.data_ptr(), *vp = v.data_ptr();
   launch(t, [&](void* s) { return qs_read_kv_cache(kp, vp, c.kvp, c.cu, c.lens, c.batch, tokens, c.max_blocks, c.heads_kv, 128, c.tpb, c.size, c.int4, c.zeros, s); });
   PyObject* const ko = THPVariable_Wrap(std::move(k));

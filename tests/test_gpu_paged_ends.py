@@ -286,3 +286,15 @@ def test_the_runner_counts_its_launches(dev, fused, batch, shared):
     a, b = (DecodeRunner("tiny", "w4a8kv4", batch=batch, ctx=300, device=dev, fused=fused, shared_prefix=n) for n in (0, shared))
     more = kernels_of(b) - kernels_of(a)
     assert more > 0 and b.launches_per_step - a.launches_per_step == more
+
+
+# ---- what read_kv_cache returns ----
+def test_read_keys_and_values_are_tensors_of_their_own(dev):
+    """Growing one in place leaves the other alone, and one that is kept does not keep the other."""
+    c = Cache([64], 2, 4, dev)
+    k, v = backend.read_kv_cache(c.table, starts([64], dev), c.lengths, 64, *c.args)
+    assert k.untyped_storage().data_ptr() != v.untyped_storage().data_ptr()
+    assert k.untyped_storage().nbytes() == v.untyped_storage().nbytes() == 64 * 2 * D * 2
+    keep = v.clone()
+    k.resize_(128, 2, D).fill_(7.0)
+    assert torch.equal(v, keep)
