@@ -70,12 +70,18 @@ void require_cuda(const at::Tensor& t, const char* name) {
   if (!t.is_cuda()) throw std::runtime_error(std::string(name) + " must be on CUDA");
 }
 
+// t's device is the current one as long as this lives
+struct OnDevice {
+  c10::cuda::OptionalCUDAGuard guard;
+  explicit OnDevice(const at::Tensor& t) {
+    if (c10::cuda::current_device() != t.get_device()) guard.set_index(static_cast<c10::DeviceIndex>(t.get_device()));
+  }
+};
 // fn(stream) with t's device current, on that device's current stream, without the interpreter lock
 template <typename F>
 void launch(const at::Tensor& t, F fn) {
   const int dev = t.get_device();
-  c10::cuda::OptionalCUDAGuard guard;
-  if (c10::cuda::current_device() != dev) guard.set_index(static_cast<c10::DeviceIndex>(dev));
+  const OnDevice on(t);
   void* stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream();
   int rc;
   Py_BEGIN_ALLOW_THREADS rc = fn(stream);
@@ -349,6 +355,7 @@ PyObject* paged_prompt_attention(const Args& a) {
   const Heads o = heads_of(out, qt, "out");
   const int max_seqlen = a.small(4), max_length = a.small(5);
   const float scale = scale_of(a, 10);
+  const OnDevice on(qt);  // how the keys are cut, and with it the work space, goes by the device
   const size_t need = qs_paged_prompt_attention_workspace_bytes(c.batch, q.rows, max_seqlen < q.rows ? max_seqlen : q.rows, max_length, q.heads, c.heads_kv);
   at::Tensor ws;
   if (need > 0) ws = scratch(qt, need);
@@ -369,6 +376,7 @@ PyObject* shared_prefix_attention(const Args& a) {
   const Heads o = heads_of(out, qt, "out");
   const int shared = a.small(3), max_length = a.small(4);
   const float scale = scale_of(a, 9);
+  const OnDevice on(qt);
   const size_t need = qs_shared_prefix_attention_workspace_bytes(c.batch, shared, q.heads, c.heads_kv);
   at::Tensor ws;
   if (need > 0) ws = scratch(qt, need);

@@ -298,3 +298,16 @@ def test_read_keys_and_values_are_tensors_of_their_own(dev):
     keep = v.clone()
     k.resize_(128, 2, D).fill_(7.0)
     assert torch.equal(v, keep)
+
+
+# ---- another device than the current one ----
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="one GPU")
+def test_tensors_on_another_device_than_the_current_one(dev):
+    """How the keys are cut goes by the tensors' device, work space and launch alike."""
+    for bits in (4, 8):
+        c = Cache([3000, 2900], 2, bits, torch.device("cuda:1"), shared=30, seed=1)
+        q = queries(2, 8, c.dev)
+        want = shared64(c, q, c.lens)
+        with torch.cuda.device(0):
+            check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, 30, 3000, *c.args), want, SCALE)
+            check_attention(backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 3000, *c.args), want, SCALE)
