@@ -135,7 +135,9 @@ QS_API int qs_prefill_attention(const void* q, const void* k, const void* v, int
 /* q_out <- q rotated, pages <- quantised rotated k and v (q, k, v are not written; q_out may be q).  NeoX rotation in place position, angle
  * position * rotary_base^(-2i/128), sine and cosine correct to fp32 at any position.  Codes, scale and zero per (token, kv head) as
  * qs_apply_bias_rope_update_kv_cache stores them, except that a code is never more than 15 (INT4), that a row whose values are equal, or too near
- * to one another for a zero in fp16, is held as its middle value, and that a row with an infinity or NaN reads as NaN. */
+ * to one another for a scale or a zero in fp16, is held as its middle value, that a row which reaches the ends of fp16 reads as finite numbers (its scale
+ * rounded down, its zero moved by one step, where its first or last code would stand for an infinity), and that a row with an infinity or NaN reads
+ * as NaN. */
 QS_API int qs_append_kv_cache(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out,
                               int64_t q_out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch,
                               int num_tokens, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block,
@@ -148,8 +150,9 @@ QS_API int qs_read_kv_cache(void* k_out, void* v_out, const int64_t* kv_pointers
 /* out [T, num_heads, 128]: causal attention of every row over positions 0 .. its own of its sequence, all out of the pages (also the portion's own:
  * append first).  q rotated; softmax_scale > 0.  max_seqlen >= the longest portion (rows behind it are left as they are), max_length >= the
  * longest sequence (decides how the keys are split, nothing else).  A row without a position (lengths[b] smaller than the portion) gets zeros.
- * Keys, values and weights are fp16 operands, sums fp32.  A cached row whose scale or zero is no finite number is NaN to the rows that see it and nothing to
- * the others; one whose codes stand for more than fp16 holds is taken as large as fits.
+ * Keys, values and weights are fp16 operands, sums and the parts of split rows fp32.  A cached row whose scale or zero (INT4: or their product) is no finite
+ * number is NaN to the rows that see it and nothing to the others; one whose own codes stand for more than fp16 holds is taken as much smaller as fits.
+ * Results are no further from 0 than 65504.
  * workspace: qs_paged_prompt_attention_workspace_bytes(...) of the same numbers, any contents, not shared by calls that run at the same time. */
 QS_API size_t qs_paged_prompt_attention_workspace_bytes(int batch, int num_tokens, int max_seqlen, int max_length, int num_heads, int num_kv_heads);
 QS_API int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
@@ -157,8 +160,9 @@ QS_API int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out,
                                      int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache,
                                      int kv_cache_with_zeros, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 /* out [batch, num_heads, 128]: attention of one row per sequence over its lengths[b] positions, all out of the pages, where the first shared_blocks
- * pages of all sequences are the same ones (they are taken from kv_pointers[0]): their keys are read and unpacked once for all rows.  A
- * sequence may be shorter than the shared pages; lengths[b] 0 gets zeros.  workspace: qs_shared_prefix_attention_workspace_bytes(...). */
+ * pages of all sequences are the same ones (they are taken from kv_pointers[0], whatever the other rows hold there): their keys are read and unpacked
+ * once for all rows.  A sequence may be shorter than the shared pages; lengths[b] 0 or less gets zeros.  Numbers as in qs_paged_prompt_attention, except that
+ * pages of a sequence's own (all pages, for few sequences) are taken exactly, those whose codes stand for more than fp16 holds among them.  workspace: qs_shared_prefix_attention_workspace_bytes(...). */
 QS_API size_t qs_shared_prefix_attention_workspace_bytes(int batch, int shared_blocks, int num_heads, int num_kv_heads);
 QS_API int qs_shared_prefix_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* lengths,
                                       int batch, int shared_blocks, int max_length, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim,

@@ -351,7 +351,8 @@ def append_kv_cache(q, k, v, kv_pointers, cu_seqlens: Optional[torch.Tensor], le
                     rotary_base: float, int4_kv_cache: bool, kv_cache_with_zeros: bool, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """RoPE of q [T,Hq,128] and k [T,Hkv,128] at the rows' positions, per-token-per-head quantisation of k and v into the pages: what
     apply_bias_rope_update_kv_cache does for whole prompts, for portions that continue sequences (single tokens among them).  Returns the rotated q (`out`
-    may be q itself); q, k and v are not changed.  A row of equal values is held as that value; one with an infinity or NaN reads as NaN."""
+    may be q itself); q, k and v are not changed.  A row of equal values is held as that value; one that reaches the ends of fp16 reads
+    as finite numbers, one with an infinity or NaN as NaN."""
     return _bind.append_kv_cache(q, k, v, kv_pointers, cu_seqlens, lengths, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4_kv_cache,
                                  kv_cache_with_zeros, out)
 
@@ -376,8 +377,8 @@ def paged_prompt_attention(q, kv_pointers, cu_seqlens: Optional[torch.Tensor], l
 def shared_prefix_attention(q, kv_pointers, lengths, shared_blocks: int, max_length: int, tokens_per_block: int, size_per_token: int, int4_kv_cache: bool,
                             kv_cache_with_zeros: bool, softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Attention of one rotated row per sequence, q [B,Hq,128], over its lengths[b] positions, all out of the pages (the new token's too: append_kv_cache first),
-    where the first `shared_blocks` pages of all sequences are the same pages (they are taken from kv_pointers[0]): those are read and unpacked once for the
-    whole batch.  A sequence may end within the shared pages; lengths[b] = 0 gets zeros.  max_length >= the longest sequence."""
+    where the first `shared_blocks` pages of all sequences are the same pages (they are taken from kv_pointers[0], whatever the other rows hold there): those are read
+    and unpacked once for the whole batch.  A sequence may end within the shared pages; lengths[b] = 0 gets zeros.  max_length >= the longest sequence."""
     return _bind.shared_prefix_attention(q, kv_pointers, lengths, shared_blocks, max_length, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros,
                                          softmax_scale, out)
 

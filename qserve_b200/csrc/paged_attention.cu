@@ -8,18 +8,21 @@
 //     S = Q K^T       8 x tcgen05.mma 128 x 64 x 16, accumulators in tensor memory
 //     softmax         4 warps, thread = row (tensor memory lane): running maximum and sum in 32 bits, P = exp2(..) rounded to fp16, into tensor memory
 //     O += P V        4 x tcgen05.mma 128 x 128 x 16, A from tensor memory
-// fp16 holds the operands (keys, values and weights, each off by 2^-11 of itself at most, INT8 keys and values by another 2^-12 of their scale): a product of exact codes would want every score multiplied by its key's
-// scale and every weight by its value's, a third more instructions of softmax warps that are the bound already.
-// A long axis of keys is split over blocks where the rows alone do not fill the device, or not its last round.  A split leaves its rows' maximum, sum and O / sum in fp32; the cluster
-// that holds all splits, join_kernel (prompts) or the tail kernel (shared prefix) joins them.  (O / sum in fp16 would be one more rounding of a result and half the bytes; us, fp16 /
-// now: 17 tokens behind 500 7.8 / 8.4, 24 behind 60000 41.8 / 43.4, 8 sequences behind 1024 shared positions 8.0 / 8.4, 64 behind 8192 30.3 / 31.6.)
-// Bounds: 4096 tokens of 32 heads over 8 behind 12000 positions, INT4, 780 to 860 us (0.94 TFLOP, 1.1 to 1.2 PFLOP/s), shared memory 0.87 of its cycles (the queries are
-// read again for every 64 keys, unpacked pages written and read) and issue slots 0.54, the tensor pipe 0.59; one tile: the chain load - unpack - softmax of a page,
+// fp16 holds the operands (keys, values and weights, each off by 2^-11 of itself at most, INT8 keys and values by another 2^-12 of their scale): a product of exact
+// codes would want every score multiplied by its key's scale and every weight by its value's, a third more instructions of softmax warps that are the bound already.
+// A result is off by 4.2e-4 to 4.7e-4 so, where its own rounding alone is 2.1e-4.
+// A long axis of keys is split over blocks where the rows alone do not fill the device, or not its last round.  A split leaves its rows' maximum, sum and O / sum in
+// fp32; the cluster that holds all splits, join_kernel (prompts) or the tail kernel (shared prefix) joins them.  (O / sum in fp16 would be one more rounding of a
+// result and half the bytes; us, fp16 / now: 17 tokens behind 500 7.8 / 8.4, 24 behind 60000 41.8 / 43.4, 8 sequences behind 1024 shared positions 8.0 / 8.4, 64
+// behind 8192 30.3 / 31.6.)
+// Bounds: 4096 tokens of 32 heads over 8 behind 12000 positions, INT4, 798 us at 1965 MHz (0.94 TFLOP, 1.18 PFLOP/s; 870 to 920 in runs
+// of seconds, where the power limit leaves 1.67 GHz), shared memory 0.88 of its cycles (the queries are read again for every 64 keys, unpacked pages written and read)
+// and issue slots 0.54, the tensor pipe 0.60; one tile: the chain load - unpack - softmax of a page,
 // 0.85 us with two blocks per multiprocessor.
 //
 // Tail kernel (shared prefix): the pages behind the shared ones (all pages, for few sequences) on mma.sync, eight query heads a product, codes taken as they lie.  A
 // cluster of blocks per (sequence, run of heads) that deals the pages out to its warps, or, for batches that fill the device that way, a warp each; joins its warps',
-// its cluster's and the prefix's partial rows and writes the result.  200 sequences of 2000 positions, 8 kv heads, INT4: 75 us for 328 MB.
+// its cluster's and the prefix's partial rows and writes the result.  200 sequences of 2000 positions, 8 kv heads, INT4: 78 us, prefix of a page and all, for 328 MB.
 #include <math_constants.h>
 
 #include <type_traits>
@@ -149,8 +152,8 @@ struct TileCfg {
   static constexpr int kBlocksPerSm = TILES == 1 ? 2 : 1;
   static constexpr int kKStages = 2, kVStages = 2;
   // One tile: the unpacking threads load codes, scales and zeros themselves, a page ahead in registers.  Two: a warp of its own has bulk copies bring them into a ring
-  // of raw slots.  us, ring / registers: 17 tokens behind 500 10.5 / 9.3, 8 sequences behind 1024 shared positions 9.8 / 8.3; 4096 tokens behind 12000 852 / 960 (two tiles
-  // leave the unpacking threads no time for loads).
+  // of raw slots.  us when it was chosen, ring / registers: 17 tokens behind 500 10.5 / 9.3, 8 sequences behind 1024 shared positions 9.8 / 8.3; 4096 tokens behind
+  // 12000 852 / 960 (two tiles leave the unpacking threads no time for loads).
   static constexpr bool kRing = TILES == 2;
   static constexpr int kSlots = kRing ? (BITS == 4 ? 8 : 5) : 0;
   static constexpr int kCodes = Geom<BITS>::kCodes;
@@ -178,8 +181,8 @@ struct TileParams {
   float2* part_ml;                        // (maximum, sum) [rows][parts]
 };
 
-// Two results in fp16, no further from 0 than its largest number (NaN stays NaN): a mean of values is no larger than they are, but rounded weights over the sum of the unrounded ones may be
-// 2^-11 more than 1, and 65504 of that rounds to infinity
+// Two results in fp16, no further from 0 than its largest number (NaN stays NaN): a mean of values is no larger than they are, but rounded weights over the sum of the
+// unrounded ones may be 2^-11 more than 1, and 65504 of that rounds to infinity
 __device__ __forceinline__ uint32_t results(float a, float b) {
   uint32_t d;
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(b), "f"(a));
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   uint64_t* bar_used = bar_raw + C::kSlots;           // [slots] raw slot read
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(bar_used + C::kSlots);
   // [128] rows' maximum and sum, for the cluster: over V, at the end.  (Shared memory of their own would leave L1 32 KB less: two blocks' 196 KB are a step of its
-  // size.  128 INT8 sequences behind 16384: 137 us, 158 so)
+  // size.  128 INT8 sequences behind 16384, when it was chosen: 137 us, 158 so)
   float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffV);
   static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 4 <= 384, "the barriers' place");
 
@@ -345,8 +348,8 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     // a page's codes, scales and zeros out of the pages ...
     const long long codes = G::codes_at(hk) + t * (G::kRow / 2), scale = G::scales_at(hk, p.num_kv_heads) + key * 2, zero = G::zeros_at(hk, p.num_kv_heads) + key * 2;
     long long kp = 0, vp = 0;  // lane i: page 32 n + i
-    // INT8: K's codes follow as soon as the page's own are unpacked, while its values are; INT4, half as many, all behind both (30 tokens behind 30000, us: INT8 34.8
-    // all behind both, 33.1 so; INT4 27.1 and 27.5)
+    // INT8: K's codes follow as soon as the page's own are unpacked, while its values are; INT4, half as many, all behind both (30 tokens behind 30000, us: INT8 32.9
+    // all behind both, 32.2 so; INT4 27.1 and 27.9)
     constexpr bool kEarly = !C::kRing && BITS == 8;
     const uint8_t *k_page = nullptr, *v_page = nullptr;
     auto turn = [&](Raw& r, int j) {  // to page j: its scales and zeros
@@ -430,10 +433,10 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       if (!live) s = c = __float2half2_rn(0.f);
       if (__any_sync(0xffffffffu, wide)) {
         // A row of K or V whose scale or zero is no finite number stands for NaN: the key's score is NaN then (and goes where the key is masked), its value 0, so
-        // that a weight of 0 in a row that does not see it stays 0.  Otherwise what counts is the codes that the row has (a row of one value is held as 1 x that value, and 15 or
-        // 255 of it would be past fp16): one with a number past fp16's all the same (the rounded scale of a row that reaches the ends of fp16 does that) is taken as
-        // much smaller as brings it inside, for an infinity times a weight of 0 would be NaN as well.  65520 is the least that rounds to infinity; 65376 leaves room for the
-        // roundings of the smaller scale and zero (INT4: 15 x 4 + 16 at most; INT8: 2^-11 of each).
+        // that a weight of 0 in a row that does not see it stays 0.  Otherwise what counts is the codes that the row has (a row of one value is held as 1 x that
+        // value, and 15 or 255 of it would be past fp16): one with a number past fp16's all the same (the rounded scale of a row that reaches the ends of fp16 does
+        // that) is taken as much smaller as brings it inside, for an infinity times a weight of 0 would be NaN as well.  65520 is the least that rounds to infinity;
+        // 65376 leaves room for the roundings of the smaller scale and zero (INT4: 15 x 4 + 16 at most; INT8: 2^-11 of each).
         const float2 sf = __half22float2(s), cf = __half22float2(c);
         auto inside = [&](const uint4 (&code)[kWords], float scale, float other) {
           uint32_t lo = 0xffffffffu, hi = 0u;
@@ -477,8 +480,8 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
       }
       __half2 low = c;
       if constexpr (BITS == 8) {
-        // s (u - z) in one rounding: u less the nearest whole number to z, exact, times s, plus s times the rest of z (at most 1 / 2; a zero further than 1024 from 0, which is
-        // whole, leaves more there, and that product is rounded too).  u - z itself may have more bits than fp16: 255 less a zero of 54.6875 does
+        // s (u - z) in one rounding: u less the nearest whole number to z, exact, times s, plus s times the rest of z (at most 1 / 2; a zero further than 1024 from 0,
+        // which is whole, leaves more there, and that product is rounded too).  u - z itself may have more bits than fp16: 255 less a zero of 54.6875 does
         const __half2 end = __float2half2_rn(1024.f), whole = h2rint(__hmax2(__hmin2(c, end), __hneg2(end)));
         low = __hneg2(__hadd2(whole, end));
         c = __hmul2(s, __hsub2(whole, c));
@@ -710,7 +713,8 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
       };
-      // A partial row: where it goes, in rows of 128 numbers.  (The block's number is read again, so that the loop above holds nothing of it: it has no register to spare)
+      // A partial row: where it goes, in rows of 128 numbers.  (The block's number is read again, so that the loop above holds nothing of it: it has no register to
+      // spare)
       bool partial = false;
       long long at = 0;
       unsigned long long to = 0ull;
@@ -1310,15 +1314,16 @@ int allow_smem(int bytes, const char* what, Enough enough) {
   return rc;
 }
 
-// How a call over `rows` rows per kv head and sequence (`num_rows` of a kv head in all) and at most `pages` pages is cut: tiles per block, and splits of the pages.  The
-// cut whose time is estimated lowest: rounds of blocks over the device, each its pages and what comes ahead of the first and behind the last, and the joining of
+// How a call over `rows` rows per kv head and sequence (`num_rows` of a kv head in all) and at most `pages` pages is cut: tiles per block, and splits of the pages.
+// The cut whose time is estimated lowest: rounds of blocks over the device, each its pages and what comes ahead of the first and behind the last, and the joining of
 // the splits: by a cluster of up to eight blocks (one tile of a prompt), by join_kernel, or in the tail kernel.  All items are split where they leave room in one
 // round; in a prompt of more rounds the items of the last round, or of the last two, where those would not fill the device.  The figures, in us, are those of the
-// kernels' own timelines; one or two one-tile blocks share a multiprocessor.  Measured, us: 17 tokens behind 500 in a cluster 7.8, with join_kernel 8.5; 4 behind 4000
-// 9.2 and 12.3; 24 behind 60000 one block per multiprocessor 54, two 46; 8 sequences behind 4096 shared positions two 13.9, one 11.6.  Rounds left whole and with the
-// rest split: 4096 tokens behind 12000 (3.5 rounds) 846 and 783, 1500 behind 6000 196 and 155, 1200 of 32 kv heads behind 30000 (160 blocks) 912 and 545.  Not for
-// small gains over sequences of unequal length, whose last round is short anyway (six portions of 250: 64.4 and 68.7); nor all items of several rounds (81.8), nor
-// clusters of two blocks per multiprocessor (four of 20 behind 8000, INT8: 37.4, join_kernel 34.5).
+// kernels' own timelines; one or two one-tile blocks share a multiprocessor.  Measured, us: 17 tokens behind 500 in a cluster 8.5, with join_kernel 9.0; 32 behind
+// 500, INT8, 9.6 and 11.8; 100 of 32 kv heads behind 400 9.8 and 12.1; 24 behind 60000 one block per multiprocessor 72, two 43.6; 8 sequences behind 1024 shared
+// positions two 19.2, one 8.4.  Rounds left whole and with the rest split: 4096 tokens behind 12000 (3.5 rounds) 923 and 888 (in a row, at the power limit), 1500
+// behind 6000 201 and 159, 1200 of 32 kv heads behind 30000 (160 blocks) 904 and 620.  Not, when this was chosen, for small gains over sequences of unequal length,
+// whose last round is short anyway (six portions of 250: 64.4 and 68.7); nor all items of several rounds (81.8), nor clusters of two blocks per multiprocessor (four
+// of 20 behind 8000, INT8: 37.4, join_kernel 34.5).
 struct Plan {
   int tiles, row_blocks, nsplit, cluster, parts;
   long long items, split;  // (rows of a block, kv head) pairs; the last so many of them are split
@@ -1403,9 +1408,10 @@ Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int 
   return plan_tiles(static_cast<long long>(max_seqlen) * group, batch, static_cast<long long>(num_tokens) * group, kv_heads,
                     (static_cast<long long>(max_length) + kPage - 1) / kPage, true);
 }
-// Few sequences or few shared pages: the tail kernel reads the shared pages too, once per sequence (out of the first row of the table), one launch instead of two.  us, both kernels / the tail alone (INT4, 32 heads
-// over 8, 100 positions behind): one sequence behind 512 6.5 / 6.0, behind 4096 9.5 / 8.2; two behind 512 6.7 / 6.3, behind 2048 7.9 / 9.0; eight behind 128 6.4 /
-// 4.9, behind 512 6.6 / 8.7.
+// Few sequences or few shared pages: the tail kernel reads the shared pages too, once per sequence (out of the first row of the table), one launch instead of two.
+// us, both kernels / the tail alone (INT4, 32 heads over 8, 100 positions behind): one sequence behind 512 6.7 / 6.0, behind 4096 9.6 / 8.2; two behind 512 6.8 / 6.1;
+// eight behind 128 7.5 / 4.9.  With 8 kv heads more would gain (two behind 2048 8.3 / 7.1, eight behind 512 7.7 / 7.1), with 32 no longer (eight behind 512 9.3 /
+// 10.5).
 bool tail_alone(int batch, int shared_blocks) { return batch == 1 || static_cast<long long>(batch) * shared_blocks <= 16; }
 Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
   const long long rows = static_cast<long long>(batch) * (heads / kv_heads);
@@ -1438,7 +1444,7 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
   }
   const int rc = tiles(p, pl, a.cache.int4, a.stream);
   if (rc || pl.parts == 1) return rc;
-  const bool wide = pl.parts >= 8;  // (24 tokens behind 60000, 37 parts: a warp a row 52.8 us, four 48.9; 17 behind 500, nine: 11.0 and 10.5)
+  const bool wide = pl.parts >= 8;  // (24 tokens behind 60000, 37 parts: a warp a row 44.3 us, four 43.6; 4 behind 4000 10.9 and 9.9; 1500 behind 6000, a few: 160 and 175)
   return launch(wide ? join_kernel<4> : join_kernel<1>, dim3(static_cast<unsigned>(wide ? rows : (rows + 3) / 4)), 128, 0, a.stream, "paged_prompt_attention: join", 1, p);
 }
 
@@ -1447,12 +1453,12 @@ size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_h
   return part_bytes(static_cast<long long>(batch) * heads, plan_shared(batch, shared_blocks, heads, kv_heads).parts);
 }
 
-// The tail kernel's blocks start while the prefix's run, on the multiprocessors that those leave, as many on each as it holds.  (Blocks of two tiles leave no room beside
-// them; one-tile blocks do.)  So where the tail's fit, fewer splits of the prefix and a bound on the tail's blocks per multiprocessor let both end at about the same time.
-// Chooses the splits, no more than planned, and returns that bound; one behind the other, the bound spreads the tail evenly.  The tail's estimate, us: start and join, that of
-// its blocks' issue slots, and its warps' half pages, each its own chain or its share of the issue slots.  Measured, one behind the other / side by side, 8 kv heads: 38
-// sequences, 500 positions behind 1024, 19.0 / 11.4 (INT8 17.1 / 11.4); 64, 1000 behind 2048, 29.5 / 24.0; bounded alone: 38, 1000 behind 16384, 40.3 / 37.1.  Not for small
-// estimated gains (INT8, 38, 200 behind 4096: 17.3 / 20.4).
+// The tail kernel's blocks start while the prefix's run, on the multiprocessors that those leave, as many on each as it holds.  (Blocks of two tiles leave no room
+// beside them; one-tile blocks do.)  So where the tail's fit, fewer splits of the prefix and a bound on the tail's blocks per multiprocessor let both end at about the
+// same time. Chooses the splits, no more than planned, and returns that bound; one behind the other, the bound spreads the tail evenly.  The tail's estimate, us:
+// start and join, that of its blocks' issue slots, and its warps' half pages, each its own chain or its share of the issue slots.  Measured, one behind the other /
+// side by side, 8 kv heads: 38 sequences, 500 positions behind 1024, 20.1 / 12.5 (INT8 18.3 / 12.9); 64, 1000 behind 2048, 29.0 / 24.8; bounded alone: 38, 1000 behind
+// 16384, 40.3 / 37.1.  Not for small estimated gains (INT8, 38, 200 behind 4096: 18.5 / 21.6).
 int side_by_side(Plan& pl, int shared_blocks, long long tail, long long tail_pages, int cluster, int most) {
   const long long sms = num_sms(), even = (tail + sms - 1) / sms;
   if (pl.tiles == 1 || even > most) return most;
@@ -1499,7 +1505,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   t.cluster = 1;
   while (t.cluster < kMaxCluster && blocks * t.cluster * 2 <= slots && tail_pages >= 2 * kTailWarps * t.cluster) t.cluster *= 2;
   QS_REQUIRE(blocks <= 0x7fffffffll, "shared_prefix_attention: %lld runs of heads", blocks);
-  const bool shared = blocks < 12 * num_sms();  // (a wave of warps; 128 sequences x 32 heads, INT8, 400 positions each behind 16384: 157 us by blocks, 142 by warps)
+  const bool shared = blocks < 12 * num_sms();  // (a wave of warps; 128 sequences x 32 heads, INT8, up to 511 positions each behind 16384: 155 us by blocks, 127 by warps)
   if (!shared) t.cluster = 1;
   int room = most;
   if (shared_blocks > 0) {
@@ -1519,7 +1525,7 @@ int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks) {
   }
   const dim3 grid = shared ? dim3(t.cluster, heads_y, a.batch) : dim3(static_cast<unsigned>((blocks + kTailWarps - 1) / kTailWarps));
   // us, two slots / four (INT4): one sequence of 16384 positions 17.6 / 16.2, one of 2000 with 32 heads a group of one 8.1 / 6.2, four of up to 8000 17.3 / 12.1.  Not
-  // behind the tile kernel, whose blocks leave no room for it: 32 sequences, 100 positions behind 4096, 11.6 / 14.2
+  // behind the tile kernel, whose blocks leave no room for it: 32 sequences, 100 positions behind 4096, 13.1 / 15.8
   const bool deep = shared && t.nsplit == 0 && blocks * t.cluster <= 2 * num_sms();
   auto run = [&](auto bits, auto by_block, auto more) {
     constexpr int kBits = decltype(bits)::value;

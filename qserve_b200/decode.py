@@ -98,7 +98,8 @@ class DecodeRunner:
                  process_group=None, fused: bool = True, ops: Optional[OpSet] = None, tp_exact: bool = False, tp_peer: bool = False, no_comm: bool = False,
                  shared_prefix: int = 0):
         assert precision in PRECISIONS, precision
-        # the first `shared_prefix` positions of all sequences lie in the same pages (one system prompt): their attention is computed once for the batch
+        # the first `shared_prefix` positions of all sequences lie in the same pages (one system prompt): their attention is computed once for the batch, with keys, values
+        # and weights rounded to fp16 where single_query_attention takes codes as they are, and quantised by a launch of its own
         assert 0 <= shared_prefix <= ctx and shared_prefix % 64 == 0, "a shared prefix is whole pages of the context"
         assert shared_prefix == 0 or (ops is None and tp_size == 1), "a shared prefix goes with this library's operators on one GPU"
         self.shared_blocks = shared_prefix // 64
