@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         c = __hmul2(__hneg2(s), c);
         most = __hmax2(__habs2(__hfma2(s, __float2half2_rn(15.f), c)), __habs2(c));
       } else {
-        most = __hmul2(__habs2(s), __hmax2(__habs2(c), __habs2(__hsub2(__float2half2_rn(255.f), c))));
+        // (taken 2^-8 more: its three roundings are others than those of the numbers below, 2^-11 each)
+        most = __hmul2(__hmul2(__habs2(s), __float2half2_rn(1.f + 1.f / 256.f)), __hmax2(__habs2(c), __habs2(__hsub2(__float2half2_rn(255.f), c))));
       }
       const uint32_t endless = as_u32(most) & 0x7c007c00u;
       const bool wide = live && ((endless & 0xffffu) == 0x7c00u || endless >= 0x7c000000u);
@@ -463,8 +464,13 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
             hi = __vmaxu4(hi, hi >> m | hi << (32 - m));
           }
           const float least = static_cast<float>(lo & 255u), largest = static_cast<float>(hi & 255u);
-          const float end = BITS == 4 ? fmaxf(fabsf(fmaf(scale, least, other)), fabsf(fmaf(scale, largest, other)))
-                                      : fabsf(scale) * fmaxf(fabsf(least - other), fabsf(largest - other));
+          float end;
+          if constexpr (BITS == 4) {
+            end = fmaxf(fabsf(fmaf(scale, least, other)), fabsf(fmaf(scale, largest, other)));
+          } else {  // with the rounding of what the zero leaves behind its whole part
+            const float rest = fabsf(other - rintf(fminf(fmaxf(other, -1024.f), 1024.f)));
+            end = fabsf(scale) * (fmaxf(fabsf(least - other), fabsf(largest - other)) + rest * 4.8828125e-4f);
+          }
           return end >= 65520.f ? 65376.f / end : 1.f;
         };
         const float k = inside(raw.k, sf.x, cf.x), v = inside(raw.v, sf.y, cf.y);

@@ -311,3 +311,42 @@ def test_tensors_on_another_device_than_the_current_one(dev):
         with torch.cuda.device(0):
             check_attention(backend.shared_prefix_attention(q, c.table, c.lengths, 30, 3000, *c.args), want, SCALE)
             check_attention(backend.paged_prompt_attention(q, c.table, None, c.lengths, 1, 3000, *c.args), want, SCALE)
+
+
+# ---- rows whose largest number lies about fp16's end ----
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("which", [0, 1])
+def test_rows_about_the_end_of_fp16_reach_no_row_that_does_not_see_them(dev, bits, which):
+    """Two positions a sequence, the second's largest number from 65400 to 65650 in size: an infinity in its operand would make the first row, whose weight for it is 0, no number.  What the
+    second row makes of values: half of the first value and the second's share, each as exact as two roundings (of value and result) and the 0.3 % that a row past the end may be taken smaller."""
+    batch, hkv, top = 3000, 1, 2 ** bits - 1
+    c = Cache([2] * batch, hkv, bits, dev, seed=5)
+    g = torch.Generator().manual_seed(11)
+    far = 65400 + 250 * torch.rand(batch, generator=g)  # of the last code, or of the first
+    kind = torch.arange(batch) % 3
+    last = torch.where(kind == 2, torch.randint(1, 4, (batch,), generator=g), top).float()  # the largest code that the row has
+    z = torch.where(kind == 0, (torch.rand(batch, generator=g) - 0.9) * 60, torch.rand(batch, generator=g) * top).half().float()
+    z = torch.where(kind == 2, torch.rand(batch, generator=g).half().float(), z)
+    s = (far / torch.maximum((last - z).abs(), z.abs())).half()
+    u = (torch.rand(batch, D, generator=g) * (last[:, None] + 1)).floor().clamp(max=255)
+    u[:, 0], u[:, 1] = 0, last
+    page = c.pages[:, 0]
+    if bits == 4:
+        packed = u[:, 0::2].to(torch.uint8) | (u[:, 1::2].to(torch.uint8) << 4)
+    else:
+        packed = u.to(torch.uint8)
+    c.pools[which][:, :c.cut].view(-1, hkv, PAGE, D * bits // 8)[page, 0, 1] = packed.to(dev)
+    c.meta(which)[page, 0, 0, 1] = s.to(dev)
+    c.meta(which)[page, 1, 0, 1] = z.half().to(dev)
+    q = queries(2 * batch, 4, dev) * (0 if which == 0 else 1)  # (no scores: keys of 65504 would outweigh everything)
+    out = run_prompt(c, q, [2] * batch).view(batch, 2, 4, D)
+    for b in range(0, batch, 7):
+        v = c.values(1, b, 2)
+        assert ((out[b, 0].to(F64) - v[0]).abs() <= H * 2 * v[0].abs() * (1 + H) + H * 2).all(), b
+    assert bool(torch.isfinite(out[:, 0]).all())
+    some = torch.isfinite((s.float() * z).half()) if bits == 4 else torch.isfinite(s)  # (a scale, or in INT4 its product with the zero, that is no finite number makes a row NaN)
+    assert bool(torch.isfinite(out[some, 1]).all())
+    if which == 0:
+        for b in some.nonzero()[::7, 0].tolist():  # equal weights
+            v = c.values(1, b, 2)
+            assert ((out[b, 1].to(F64) - v.mean(0)).abs() <= H * 2 * v.abs().mean(0) + H * 2).all(), b
