@@ -169,6 +169,52 @@ QS_API int qs_shared_prefix_attention(const void* q, int64_t q_stride, void* out
                                       int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros, float softmax_scale,
                                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* Steps of several drafted tokens, and tokens with places of their own (csrc/drafts.cu and the files above; extensions).  The tables, sizes and layouts are those of
+ * portions above.  Row 0 of a portion is the token that a step starts from, the others are drafted ones.
+ * qs_draft_tree: parents int32 [num_tokens], the parent's row within the portion, ahead of its child (that of row 0 is not looked at).  positions int32 [num_tokens] <-
+ * the portion's first position + the row's depth; visible int64 [num_tokens, (max_seqlen + 63) / 64] <- bit i: row i is the row itself or one of its ancestors.  A row
+ * whose parent does not lie ahead of it is padding: it sees nothing of its portion and counts as depth 0; what hangs below it sees its own ancestors up to there.
+ * max_seqlen <= 256; rows behind it are left as they are. */
+QS_API int qs_draft_tree(int32_t* positions, int64_t* visible, const int32_t* parents, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens,
+                         int max_seqlen, void* stream);
+/* qs_append_kv_cache, with pair i of a row turned by positions[axis(i)][row] * rotary_base^(-2i/128): positions int32 [axes, num_tokens] of any value, 1 to 4 axes;
+ * rotary_sections (axes numbers, in host memory, 64 together) says how many pairs go by each, one axis behind the other, or (interleaved) pair i by axis i mod axes as
+ * long as that one has pairs left and by the first axis then.  The places in the pages are those of qs_append_kv_cache. */
+QS_API int qs_append_kv_cache_at(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out,
+                                 int64_t q_out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* positions,
+                                 const int32_t* rotary_sections, int axes, int interleaved, int batch, int num_tokens, int max_blocks_per_seq, int num_heads,
+                                 int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int rotary_embedding_dim, float rotary_base,
+                                 int int4_kv_cache, int kv_cache_with_zeros, void* stream);
+/* qs_paged_prompt_attention, with what a row sees given: every position ahead of its portion, and of the portion those rows whose bits it has in
+ * visible [num_tokens, visible_words] (bit i % 64 of word i / 64; 64 * visible_words >= max_seqlen), its own place or later ones as well.  A row that sees nothing gets
+ * zeros.  Numbers and workspace as in qs_paged_prompt_attention. */
+QS_API int qs_paged_tree_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
+                                   const int32_t* lengths, const int64_t* visible, int visible_words, int batch, int num_tokens, int max_seqlen, int max_length,
+                                   int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token,
+                                   int int4_kv_cache, int kv_cache_with_zeros, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+/* Which drafted tokens the target takes, and the token behind them.  logits [num_tokens, vocab] (logits_type 0 fp16, 1 bf16, 2 fp32, rows of logits_stride numbers):
+ * row i's judge the children of row i.  tokens int64 [num_tokens] (row 0's is not looked at; one outside 0 .. vocab - 1 is never taken), parents as in qs_draft_tree,
+ * NULL: a chain.  coins fp32 [num_tokens] and draws fp32 [batch]: random numbers in [0, 1); temperatures fp32 [batch] or NULL (1).  With p = softmax(logits / t) of the
+ * current row, from row 0 on:
+ *   draft_probs q fp32 [num_tokens, vocab] (chains; row i's is what row i + 1's token x was drawn from): x is taken where coin q(x) < p(x), otherwise the sequence ends
+ *   with a token drawn from max(p - q, 0);
+ *   no draft_probs: the first child x_j with coin < p(x_1) + ... + p(x_j) is taken (children in the order of their rows, each token once), otherwise the sequence ends
+ *   with a token drawn from p without the children's tokens;
+ *   no child: it ends with one drawn from p.  (Where rounding leaves nothing to draw from: from p.)
+ * The token drawn is the first whose running sum of weights exceeds draw * their whole sum.  A temperature that is not above 0: the child with the row's largest logit,
+ * the lowest index of equal ones.  Logits of -inf or NaN are no tokens; of a row with nothing else the token is -1; where some are +inf, those share the weight alone.
+ * out_rows int32, out_tokens int64 [batch, max_seqlen]: rows 0, r1, r2, .. that were taken, and the token behind each; -1 beyond; out_counts int32 [batch]: how many,
+ * 0 for an empty portion.  max_seqlen <= 256; rows behind it are not looked at.  Sums are of 64 bits where a decision or a draw hangs on them. */
+QS_API int qs_verify_drafts(int64_t* out_tokens, int32_t* out_rows, int32_t* out_counts, const void* logits, int logits_type, int64_t logits_stride, const int64_t* tokens,
+                            const int32_t* parents, const float* draft_probs, int64_t probs_stride, const int32_t* cu_seqlens, const float* coins, const float* draws,
+                            const float* temperatures, int batch, int num_tokens, int vocab, int max_seqlen, void* stream);
+/* Position first + j of each portion (first: of its row 0) gets what position first + rows[b][j] holds, j < counts[b] (rows int32 [batch, max_rows], counts int32
+ * [batch]); new_lengths int32 [batch] <- first + counts[b].  All rows of a sequence are read before the first is written.  A row outside its portion, or outside the
+ * sequence's pages, leaves the place as it is; counts go up to the portion's rows and max_rows (<= 256).  new_lengths must not be lengths. */
+QS_API int qs_keep_kv_cache(int32_t* new_lengths, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* rows,
+                            const int32_t* counts, int max_rows, int batch, int num_tokens, int max_blocks_per_seq, int num_kv_heads, int head_dim,
+                            int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros, void* stream);
+
 /* qserve_backend.fused_attention.compute_padding_offsets         kernels/csrc/fused_attention/input_metadata_helper.cu:33-45 */
 QS_API int qs_compute_padding_offsets(int32_t* padding_offsets, const int32_t* cu_seqlens, int batch, int max_seqlen, void* stream);
 

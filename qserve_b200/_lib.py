@@ -39,6 +39,12 @@ SIGNATURES = {
     "qs_paged_prompt_attention": (c_int, [_P, _L, _P, _L, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
     "qs_shared_prefix_attention_workspace_bytes": (c_size_t, [_I, _I, _I, _I]),
     "qs_shared_prefix_attention": (c_int, [_P, _L, _P, _L, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
+    # drafted tokens, tokens with places of their own (csrc/drafts.cu and those above)
+    "qs_draft_tree": (c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
+    "qs_append_kv_cache_at": (c_int, [_P, _P, _P, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
+    "qs_paged_tree_attention": (c_int, [_P, _L, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
+    "qs_verify_drafts": (c_int, [_P, _P, _P, _P, _I, _L, _P, _P, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
+    "qs_keep_kv_cache": (c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "qs_rms_norm": (c_int, [_P, _P, _P, _F, _I, _I, _I, _P]),
     "qs_rms_norm_general": (c_int, [_P, _P, _P, _P, _F, _I, _I, _I, _P]),
     "qs_rms_norm_general_fuse_sum": (c_int, [_P, _P, _P, _P, _P, _F, _I, _I, _I, _P]),

@@ -383,6 +383,61 @@ def shared_prefix_attention(q, kv_pointers, lengths, shared_blocks: int, max_len
                                          softmax_scale, out)
 
 
+# --------------------------------------------------------------------------------------------------
+# steps of several drafted tokens, and tokens with places of their own (extensions)
+#
+# The rows of a portion as above: row 0 is the token that the step starts from, the others are drafted tokens, each with a parent among the rows ahead of it.  A step:
+# draft_tree, then append_kv_cache_at and paged_tree_attention in every layer, verify_drafts, keep_kv_cache in every layer.  (A chain needs no tree:
+# append_kv_cache, paged_prompt_attention, verify_drafts; what was not accepted lies behind the new lengths, lengths - portion + counts, and is written over.)
+# --------------------------------------------------------------------------------------------------
+
+
+def draft_tree(parents, cu_seqlens: Optional[torch.Tensor], lengths, max_seqlen: int):
+    """What the rows of drafted trees see of their portions, and where they are rotated: parents int32 [T] are rows within the portion, ahead of their children (row
+    0's is not looked at).  Returns positions int32 [T] (the portion's first position + depth) and visible int64 [T, ceil(max_seqlen / 64)], bit i of a row: row i is the
+    row itself or an ancestor.  A row whose parent does not lie ahead of it (-1) is padding and sees nothing of its portion.  max_seqlen <= 256."""
+    return _bind.draft_tree(parents, cu_seqlens, lengths, max_seqlen)
+
+
+def append_kv_cache_at(q, k, v, kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, positions, rotary_sections, tokens_per_block: int, size_per_token: int,
+                       rotary_embedding_dim: int, rotary_base: float, int4_kv_cache: bool, kv_cache_with_zeros: bool, interleaved: bool = False,
+                       out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """append_kv_cache with the angles given: positions int32 [T] (depths of a tree, with rotary_sections None or (64,)) or [axes, T] (time, height, width of images),
+    where rotary_sections says how many of a head's 64 pairs go by each of one to four axes, one axis behind the other; interleaved: pair i goes by axis i mod axes as long
+    as that one has pairs left, then by the first.  Where rows lie in the pages goes by lengths and cu_seqlens alone."""
+    return _bind.append_kv_cache_at(q, k, v, kv_pointers, cu_seqlens, lengths, positions, rotary_sections, tokens_per_block, size_per_token, rotary_embedding_dim,
+                                    rotary_base, int4_kv_cache, kv_cache_with_zeros, interleaved, out)
+
+
+def paged_tree_attention(q, kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, visible, max_seqlen: int, max_length: int, tokens_per_block: int,
+                         size_per_token: int, int4_kv_cache: bool, kv_cache_with_zeros: bool, softmax_scale: Optional[float] = None,
+                         out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """paged_prompt_attention with what a row sees given: all positions ahead of its portion, and of the portion the rows whose bits it has in visible int64 [T, words]
+    (bit i % 64 of word i / 64, 64 * words >= max_seqlen): a drafted tree's ancestors, an image that sees itself as a whole, several documents in one portion.  Its
+    own place counts only by its bit, and later rows may be seen.  A row that sees nothing gets zeros."""
+    return _bind.paged_tree_attention(q, kv_pointers, cu_seqlens, lengths, visible, max_seqlen, max_length, tokens_per_block, size_per_token, int4_kv_cache,
+                                      kv_cache_with_zeros, softmax_scale, out)
+
+
+def verify_drafts(logits, draft_tokens, cu_seqlens: Optional[torch.Tensor], max_seqlen: int, coins, draws, parents: Optional[torch.Tensor] = None,
+                  draft_probs: Optional[torch.Tensor] = None, temperatures: Optional[torch.Tensor] = None):
+    """Which drafted tokens the target takes, and the token behind them, so that all are distributed as if drawn from the target one by one.  logits [T, vocab] fp16,
+    bf16 or fp32, row i's behind row i; draft_tokens int64 [T] (row 0's is not looked at); coins fp32 [T] and draws fp32 [B] random in [0, 1); temperatures fp32 [B],
+    0 or less: greedy, None: 1.  Drafts as they come, a chain or (with parents, as in draft_tree) a tree: of a row's children the first one at which the sum of their
+    probabilities p exceeds the row's coin is taken, otherwise the sequence ends with a token drawn from the others.  Chains drawn at random from draft_probs fp32
+    [T, vocab] (row i: what row i + 1's token was drawn from): a token x is taken where coin q(x) < p(x), otherwise the sequence ends with one drawn from max(p - q, 0).
+    Returns tokens int64 [B, max_seqlen], rows int32 [B, max_seqlen] and counts int32 [B]: the rows taken, from row 0 on, the token behind each, and how many; -1 beyond.
+    Logits of -inf or NaN are no tokens; a row with nothing else gives -1.  max_seqlen <= 256."""
+    return _bind.verify_drafts(logits, draft_tokens, cu_seqlens, max_seqlen, coins, draws, parents, draft_probs, temperatures)
+
+
+def keep_kv_cache(kv_pointers, cu_seqlens: Optional[torch.Tensor], lengths, rows, counts, tokens_per_block: int, size_per_token: int, int4_kv_cache: bool,
+                  kv_cache_with_zeros: bool) -> torch.Tensor:
+    """The rows that verify_drafts took, side by side at the front of their portions: position first + j gets what first + rows[b, j] holds, j < counts[b] (rows int32
+    [B, <= 256], counts int32 [B]).  Returns the new lengths int32 [B], first + counts.  A row outside its portion (-1) leaves its place as it is."""
+    return _bind.keep_kv_cache(kv_pointers, cu_seqlens, lengths, rows, counts, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros)
+
+
 class PeerContext:
     """Peer-mapped buffers of a tensor-parallel group for the fused all-reduce (qs_add_rms_norm_general_peer): built once from
     torch.distributed._symmetric_memory (device memory + NVLink peer mappings are torch's plumbing; the kernel is ours).

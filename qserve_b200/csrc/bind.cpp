@@ -388,6 +388,171 @@ PyObject* shared_prefix_attention(const Args& a) {
   return THPVariable_Wrap(std::move(out));
 }
 
+// ---- drafted tokens ----
+// an optional vector or matrix of one type, rows contiguous behind one another
+const void* plain(const Args& a, int i, at::ScalarType type, at::IntArrayRef sizes, const at::Tensor& like, const char* name) {
+  if (a.none(i)) return nullptr;
+  const at::Tensor& t = a.tensor(i);
+  same_device(t, like, name);
+  if (t.scalar_type() != type || t.sizes() != sizes || !t.is_contiguous()) {
+    std::string want;
+    for (const int64_t n : sizes) want += (want.empty() ? "" : ", ") + std::to_string(n);
+    throw std::runtime_error(std::string(name) + " must be contiguous " + c10::toString(type) + " [" + want + "]");
+  }
+  return t.data_ptr();
+}
+int rows_within(int64_t n, const char* name) {
+  if (n > 0x7fffffff) throw std::runtime_error(std::string(name) + ": too many rows");
+  return static_cast<int>(n);
+}
+// parents, cu_seqlens or None, lengths, max_seqlen
+PyObject* draft_tree(const Args& a) {
+  const at::Tensor &up = a.tensor(0), &lens = a.tensor(2);
+  require(up.dim() == 1 && lens.dim() == 1, "parents and lengths must have one dimension");
+  const int tokens = rows_within(up.size(0), "parents"), batch = rows_within(lens.size(0), "lengths");
+  const int32_t* const parents = int32_vector(up, tokens, up, "parents");
+  const int32_t* const cu = a.none(1) ? nullptr : int32_vector(a.tensor(1), static_cast<int64_t>(batch) + 1, up, "cu_seqlens");
+  const int32_t* const lengths = int32_vector(lens, batch, up, "lengths");
+  const int max_seqlen = a.small(3);
+  require(max_seqlen >= 0, "max_seqlen must not be negative");
+  at::Tensor positions = fresh({tokens}, at::kInt, up), visible = fresh({tokens, (static_cast<int64_t>(max_seqlen) + 63) / 64}, at::kLong, up);
+  void *pp = positions.data_ptr(), *vp = visible.data_ptr();
+  launch(up, [&](void* s) { return qs_draft_tree(static_cast<int32_t*>(pp), static_cast<int64_t*>(vp), parents, cu, lengths, batch, tokens, max_seqlen, s); });
+  PyObject* const po = THPVariable_Wrap(std::move(positions));
+  PyObject* const vo = THPVariable_Wrap(std::move(visible));
+  PyObject* const both = po && vo ? PyTuple_Pack(2, po, vo) : nullptr;
+  Py_XDECREF(po);
+  Py_XDECREF(vo);
+  return both;
+}
+// q, k, v, kv_pointers, cu_seqlens or None, lengths, positions, rotary_sections or None, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4, zeros,
+// interleaved, out or None
+PyObject* append_kv_cache_at(const Args& a) {
+  const at::Tensor &qt = a.tensor(0), &kt = a.tensor(1), &vt = a.tensor(2), &at_ = a.tensor(6);
+  const Heads q = heads_of(qt, qt, "q"), k = heads_of(kt, qt, "k"), v = heads_of(vt, qt, "v");
+  require(q.rows == k.rows && q.rows == v.rows && k.heads == v.heads, "q, k, v must cover the same tokens; k and v the same heads");
+  const Cache c = cache_of(a, qt, 3, 4, 5, 8, 12);
+  same_device(at_, qt, "positions");
+  require(at_.scalar_type() == at::kInt && at_.is_contiguous() && (at_.dim() == 1 || at_.dim() == 2) && at_.size(-1) == q.rows,
+          "positions must be contiguous int32 [axes, tokens], or [tokens]");
+  const int axes = at_.dim() == 1 ? 1 : rows_within(at_.size(0), "positions");
+  int32_t sections[4] = {64, 0, 0, 0};
+  if (!a.none(7)) {
+    PyObject* const list = PySequence_Fast(a.a[7], "rotary_sections must be a sequence of whole numbers");
+    if (list == nullptr) throw python_error();
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+    bool ok = n == axes && n <= 4;
+    for (Py_ssize_t i = 0; ok && i < n; ++i) {
+      const long x = PyLong_AsLong(PySequence_Fast_GET_ITEM(list, i));
+      if (x == -1 && PyErr_Occurred()) {
+        Py_DECREF(list);
+        throw python_error();
+      }
+      ok = x >= 0 && x <= 64;
+      sections[i] = static_cast<int32_t>(x);
+    }
+    Py_DECREF(list);
+    require(ok, "rotary_sections must have a number of pairs for each of one to four axes of positions");
+  } else {
+    require(axes == 1, "positions of several axes need rotary_sections");
+  }
+  at::Tensor out = result_of(a, 15, qt);
+  const Heads o = heads_of(out, qt, "out");
+  const int rot = a.small(10), interleaved = a.truth(14);
+  const float base = a.real(11);
+  const int32_t* const positions = static_cast<const int32_t*>(at_.data_ptr());
+  launch(qt, [&](void* s) {
+    return qs_append_kv_cache_at(q.p, k.p, v.p, q.stride, k.stride, v.stride, o.p, o.stride, c.kvp, c.cu, c.lens, positions, sections, axes, interleaved, c.batch, q.rows,
+                                 c.max_blocks, q.heads, k.heads, 128, c.tpb, c.size, rot, base, c.int4, c.zeros, s);
+  });
+  return THPVariable_Wrap(std::move(out));
+}
+// q, kv_pointers, cu_seqlens or None, lengths, visible, max_seqlen, max_length, tokens_per_block, size_per_token, int4, zeros, softmax_scale or None, out or None
+PyObject* paged_tree_attention(const Args& a) {
+  const at::Tensor &qt = a.tensor(0), &seen = a.tensor(4);
+  const Heads q = heads_of(qt, qt, "q");
+  const Cache c = cache_of(a, qt, 1, 2, 3, 7, 9);
+  same_device(seen, qt, "visible");
+  require(seen.scalar_type() == at::kLong && seen.is_contiguous() && seen.dim() == 2 && seen.size(0) == q.rows && seen.size(1) <= 1 << 24,
+          "visible must be contiguous int64 [tokens, words]");
+  at::Tensor out = result_of(a, 12, qt);
+  const Heads o = heads_of(out, qt, "out");
+  const int max_seqlen = a.small(5), max_length = a.small(6), words = static_cast<int>(seen.size(1));
+  const float scale = scale_of(a, 11);
+  const int64_t* const visible = static_cast<const int64_t*>(seen.data_ptr());
+  const OnDevice on(qt);
+  const size_t need = qs_paged_prompt_attention_workspace_bytes(c.batch, q.rows, max_seqlen < q.rows ? max_seqlen : q.rows, max_length, q.heads, c.heads_kv);
+  at::Tensor ws;
+  if (need > 0) ws = scratch(qt, need);
+  void* const wp = need > 0 ? ws.data_ptr() : nullptr;
+  launch(qt, [&](void* s) {
+    return qs_paged_tree_attention(q.p, q.stride, o.p, o.stride, c.kvp, c.cu, c.lens, visible, words, c.batch, q.rows, max_seqlen, max_length, c.max_blocks, q.heads, c.heads_kv,
+                                   128, c.tpb, c.size, c.int4, c.zeros, scale, wp, need, s);
+  });
+  return THPVariable_Wrap(std::move(out));
+}
+// logits, draft_tokens, cu_seqlens or None, max_seqlen, coins, draws, parents or None, draft_probs or None, temperatures or None
+PyObject* verify_drafts(const Args& a) {
+  const at::Tensor &lt = a.tensor(0), &draws = a.tensor(5);
+  require_cuda(lt, "logits");
+  require(lt.dim() == 2 && (lt.size(0) == 0 || lt.size(1) == 1 || lt.stride(1) == 1), "logits must be [tokens, vocab] with contiguous rows");
+  const int type = lt.scalar_type() == at::kHalf ? 0 : lt.scalar_type() == at::kBFloat16 ? 1 : lt.scalar_type() == at::kFloat ? 2 : -1;
+  require(type >= 0, "logits must be float16, bfloat16 or float32");
+  const int tokens = rows_within(lt.size(0), "logits"), vocab = rows_within(lt.size(1), "logits"), max_seqlen = a.small(3);
+  require(draws.dim() == 1 && max_seqlen >= 0, "draws must have one dimension, max_seqlen must not be negative");
+  const int batch = rows_within(draws.size(0), "draws");
+  const int32_t* const cu = a.none(2) ? nullptr : int32_vector(a.tensor(2), static_cast<int64_t>(batch) + 1, lt, "cu_seqlens");
+  a.tensor(1);  // (neither may be None)
+  a.tensor(4);
+  const void* const ids = plain(a, 1, at::kLong, {tokens}, lt, "draft_tokens");
+  const void* const coins = plain(a, 4, at::kFloat, {tokens}, lt, "coins");
+  const void* const drawn = plain(a, 5, at::kFloat, {batch}, lt, "draws");
+  const void* const parents = plain(a, 6, at::kInt, {tokens}, lt, "parents");
+  const void* const heat = plain(a, 8, at::kFloat, {batch}, lt, "temperatures");
+  const void* probs = nullptr;
+  int64_t probs_stride = 0;
+  if (!a.none(7)) {
+    const at::Tensor& q = a.tensor(7);
+    same_device(q, lt, "draft_probs");
+    require(q.scalar_type() == at::kFloat && q.sizes() == lt.sizes() && (tokens == 0 || vocab == 1 || q.stride(1) == 1),
+            "draft_probs must be float32 of the sizes of logits with contiguous rows");
+    probs = q.data_ptr();
+    probs_stride = q.stride(0);
+  }
+  at::Tensor out = fresh({batch, max_seqlen}, at::kLong, lt), rows = fresh({batch, max_seqlen}, at::kInt, lt), counts = fresh({batch}, at::kInt, lt);
+  void *op = out.data_ptr(), *rp = rows.data_ptr(), *cp = counts.data_ptr(), *lp = lt.data_ptr();
+  const int64_t stride = lt.stride(0);
+  launch(lt, [&](void* s) {
+    return qs_verify_drafts(static_cast<int64_t*>(op), static_cast<int32_t*>(rp), static_cast<int32_t*>(cp), lp, type, stride, static_cast<const int64_t*>(ids),
+                            static_cast<const int32_t*>(parents), static_cast<const float*>(probs), probs_stride, cu, static_cast<const float*>(coins),
+                            static_cast<const float*>(drawn), static_cast<const float*>(heat), batch, tokens, vocab, max_seqlen, s);
+  });
+  PyObject* const oo = THPVariable_Wrap(std::move(out));
+  PyObject* const ro = THPVariable_Wrap(std::move(rows));
+  PyObject* const co = THPVariable_Wrap(std::move(counts));
+  PyObject* const all = oo && ro && co ? PyTuple_Pack(3, oo, ro, co) : nullptr;
+  Py_XDECREF(oo);
+  Py_XDECREF(ro);
+  Py_XDECREF(co);
+  return all;
+}
+// kv_pointers, cu_seqlens or None, lengths, rows, counts, tokens_per_block, size_per_token, int4, zeros
+PyObject* keep_kv_cache(const Args& a) {
+  const at::Tensor &t = a.tensor(0), &rt = a.tensor(3);
+  const Cache c = cache_of(a, t, 0, 1, 2, 5, 7);
+  same_device(rt, t, "rows");
+  require(rt.scalar_type() == at::kInt && rt.dim() == 2 && rt.size(0) == c.batch && rt.is_contiguous(), "rows must be contiguous int32 [batch, rows]");
+  const int most = rows_within(rt.size(1), "rows");
+  const int32_t* const counts = int32_vector(a.tensor(4), c.batch, t, "counts");
+  const int32_t* const rows = static_cast<const int32_t*>(rt.data_ptr());
+  at::Tensor lengths = fresh({c.batch}, at::kInt, t);
+  void* const lp = lengths.data_ptr();
+  launch(t, [&](void* s) {
+    return qs_keep_kv_cache(static_cast<int32_t*>(lp), c.kvp, c.cu, c.lens, rows, counts, most, c.batch, 0x7fffffff, c.max_blocks, c.heads_kv, 128, c.tpb, c.size, c.int4, c.zeros, s);
+  });
+  return THPVariable_Wrap(std::move(lengths));
+}
+
 // ---- row operators ----
 struct Rows {
   int tokens, width;
@@ -555,6 +720,11 @@ PyMethodDef methods[] = {QS_ENTRY(w4a8_per_chn, 8),
                          QS_ENTRY(read_kv_cache, 8),
                          QS_ENTRY(paged_prompt_attention, 12),
                          QS_ENTRY(shared_prefix_attention, 11),
+                         QS_ENTRY(draft_tree, 4),
+                         QS_ENTRY(append_kv_cache_at, 16),
+                         QS_ENTRY(paged_tree_attention, 13),
+                         QS_ENTRY(verify_drafts, 9),
+                         QS_ENTRY(keep_kv_cache, 9),
                          QS_ENTRY(rms_norm_general, 6),
                          QS_ENTRY(rms_norm_general_fuse_sum, 7),
                          QS_ENTRY(invoke_quant, 3),

@@ -195,12 +195,10 @@ static int paged_rows(const char* op, const char* name, const void* t, int64_t s
   return qs::QS_OK;
 }
 
-int qs_append_kv_cache(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out, int64_t q_out_stride,
-                       const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens, int max_blocks_per_seq,
-                       int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int rotary_embedding_dim, float rotary_base,
-                       int int4_kv_cache, int kv_cache_with_zeros, void* stream) {
-  const char* op = "append_kv_cache";
-  AppendArgs a;
+static int append(AppendArgs& a, const char* op, const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out,
+                  int64_t q_out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens, int max_blocks_per_seq,
+                  int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int rotary_embedding_dim, float rotary_base,
+                  int int4_kv_cache, int kv_cache_with_zeros, void* stream) {
   int rc = paged_cache(a.cache, op, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
                        int4_kv_cache, kv_cache_with_zeros);
   if (rc) return rc;
@@ -214,6 +212,63 @@ int qs_append_kv_cache(const void* q, const void* k, const void* v, int64_t q_st
   a.q = q; a.k = k; a.v = v; a.q_out = q_out; a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride; a.q_out_stride = q_out_stride;
   a.batch = batch; a.num_tokens = num_tokens; a.num_heads = num_heads; a.rotary_base = rotary_base; a.stream = stream;
   return append_kv_cache(a);
+}
+
+int qs_append_kv_cache(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out, int64_t q_out_stride,
+                       const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens, int max_blocks_per_seq,
+                       int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int rotary_embedding_dim, float rotary_base,
+                       int int4_kv_cache, int kv_cache_with_zeros, void* stream) {
+  AppendArgs a;
+  return append(a, "append_kv_cache", q, k, v, q_stride, k_stride, v_stride, q_out, q_out_stride, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq,
+                num_heads, num_kv_heads, head_dim, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4_kv_cache, kv_cache_with_zeros, stream);
+}
+
+int qs_append_kv_cache_at(const void* q, const void* k, const void* v, int64_t q_stride, int64_t k_stride, int64_t v_stride, void* q_out, int64_t q_out_stride,
+                          const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* positions, const int32_t* rotary_sections,
+                          int axes, int interleaved, int batch, int num_tokens, int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block,
+                          int size_per_token, int rotary_embedding_dim, float rotary_base, int int4_kv_cache, int kv_cache_with_zeros, void* stream) {
+  const char* op = "append_kv_cache_at";
+  QS_REQUIRE(axes >= 1 && axes <= 4, "%s: %d axes, 1 to 4 are supported", op, axes);
+  QS_REQUIRE(rotary_sections != nullptr, "%s: rotary_sections is null", op);
+  int sum = 0;
+  for (int i = 0; i < axes; ++i) {
+    QS_REQUIRE(rotary_sections[i] >= 0 && rotary_sections[i] <= 64, "%s: a rotary section of %d pairs", op, rotary_sections[i]);
+    sum += rotary_sections[i];
+  }
+  QS_REQUIRE(sum == 64, "%s: rotary sections of %d pairs in all, a head has 64", op, sum);
+  AppendArgs a;
+  if (interleaved) {  // pair i is of axis i mod axes as long as that has pairs left, then of the first
+    for (int i = 0; i < 64; ++i) a.axis_of[i] = static_cast<unsigned char>(i % axes > 0 && i / axes < rotary_sections[i % axes] ? i % axes : 0);
+    for (int i = 1; i < axes; ++i)
+      QS_REQUIRE(rotary_sections[i] <= (64 - i + axes - 1) / axes, "%s: %d interleaved pairs of axis %d of %d", op, rotary_sections[i], i, axes);
+  } else {
+    int axis = 0, end = rotary_sections[0];
+    for (int i = 0; i < 64; ++i) {
+      while (i >= end) end += rotary_sections[++axis];
+      a.axis_of[i] = static_cast<unsigned char>(axis);
+    }
+  }
+  if (batch > 0 && num_tokens > 0) QS_REQUIRE(positions != nullptr, "%s: positions is null", op);
+  a.positions = positions;
+  return append(a, op, q, k, v, q_stride, k_stride, v_stride, q_out, q_out_stride, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_heads,
+                num_kv_heads, head_dim, tokens_per_block, size_per_token, rotary_embedding_dim, rotary_base, int4_kv_cache, kv_cache_with_zeros, stream);
+}
+
+int qs_keep_kv_cache(int32_t* new_lengths, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, const int32_t* rows, const int32_t* counts,
+                     int max_rows, int batch, int num_tokens, int max_blocks_per_seq, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token,
+                     int int4_kv_cache, int kv_cache_with_zeros, void* stream) {
+  const char* op = "keep_kv_cache";
+  PagedCache c;
+  const int rc = paged_cache(c, op, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
+                             int4_kv_cache, kv_cache_with_zeros);
+  if (rc) return rc;
+  QS_REQUIRE(max_rows >= 0 && max_rows <= kMostDrafted, "%s: %d rows of a portion, at most %d are supported", op, max_rows, kMostDrafted);
+  QS_REQUIRE(batch <= 65535, "%s: batch=%d exceeds the grid limits", op, batch);
+  if (batch == 0) return qs::QS_OK;
+  QS_REQUIRE(new_lengths && lengths && counts && (rows || max_rows == 0), "%s: null tensor", op);
+  QS_REQUIRE(new_lengths != lengths, "%s: the new lengths must have a place of their own", op);
+  QS_REQUIRE(kv_pointers || max_blocks_per_seq == 0, "%s: null tensor", op);
+  return keep_kv_cache(new_lengths, c, rows, counts, max_rows, batch, num_tokens, stream);
 }
 
 int qs_read_kv_cache(void* k_out, void* v_out, const int64_t* kv_pointers, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens,
@@ -232,12 +287,10 @@ size_t qs_paged_prompt_attention_workspace_bytes(int batch, int num_tokens, int 
   return paged_prompt_workspace(batch, num_tokens, max_seqlen, max_length, num_heads, num_kv_heads);
 }
 
-int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
-                              const int32_t* lengths, int batch, int num_tokens, int max_seqlen, int max_length, int max_blocks_per_seq, int num_heads,
-                              int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros,
-                              float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
-  const char* op = "paged_prompt_attention";
-  PagedAttnArgs a;
+static int prompt_attention(PagedAttnArgs& a, const char* op, const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers,
+                            const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens, int max_seqlen, int max_length, int max_blocks_per_seq, int num_heads,
+                            int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros, float softmax_scale,
+                            void* workspace, size_t workspace_bytes, void* stream) {
   int rc = paged_cache(a.cache, op, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_blocks_per_seq, num_kv_heads, head_dim, tokens_per_block, size_per_token,
                        int4_kv_cache, kv_cache_with_zeros);
   if (rc) return rc;
@@ -251,6 +304,69 @@ int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_
   a.max_seqlen = max_seqlen < num_tokens ? max_seqlen : num_tokens; a.max_length = max_length; a.softmax_scale = softmax_scale;
   a.workspace = workspace; a.workspace_bytes = workspace_bytes; a.stream = stream;
   return paged_prompt_attention(a);
+}
+
+int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
+                              const int32_t* lengths, int batch, int num_tokens, int max_seqlen, int max_length, int max_blocks_per_seq, int num_heads,
+                              int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache, int kv_cache_with_zeros,
+                              float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  PagedAttnArgs a;
+  return prompt_attention(a, "paged_prompt_attention", q, q_stride, out, out_stride, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_seqlen, max_length,
+                          max_blocks_per_seq, num_heads, num_kv_heads, head_dim, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros, softmax_scale, workspace,
+                          workspace_bytes, stream);
+}
+
+int qs_paged_tree_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
+                            const int32_t* lengths, const int64_t* visible, int visible_words, int batch, int num_tokens, int max_seqlen, int max_length,
+                            int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache,
+                            int kv_cache_with_zeros, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "paged_tree_attention";
+  PagedAttnArgs a;
+  if (batch > 0 && num_tokens > 0 && max_seqlen > 0) {
+    QS_REQUIRE(visible != nullptr && (reinterpret_cast<uintptr_t>(visible) & 7) == 0, "%s: visible must be there, on an 8-byte boundary", op);
+    QS_REQUIRE(visible_words > 0 && visible_words <= (1 << 24) && static_cast<long long>(visible_words) * 64 >= (max_seqlen < num_tokens ? max_seqlen : num_tokens),
+               "%s: %d words of 64 rows for portions of %d", op, visible_words, max_seqlen);
+  }
+  a.visible = reinterpret_cast<const unsigned long long*>(visible);
+  a.visible_words = visible_words;
+  return prompt_attention(a, op, q, q_stride, out, out_stride, kv_pointers, cu_seqlens, lengths, batch, num_tokens, max_seqlen, max_length,
+                          max_blocks_per_seq, num_heads, num_kv_heads, head_dim, tokens_per_block, size_per_token, int4_kv_cache, kv_cache_with_zeros, softmax_scale, workspace,
+                          workspace_bytes, stream);
+}
+
+int qs_draft_tree(int32_t* positions, int64_t* visible, const int32_t* parents, const int32_t* cu_seqlens, const int32_t* lengths, int batch, int num_tokens, int max_seqlen,
+                  void* stream) {
+  QS_REQUIRE(batch >= 0 && num_tokens >= 0, "draft_tree: negative size");
+  QS_REQUIRE(max_seqlen >= 0 && max_seqlen <= kMostDrafted, "draft_tree: max_seqlen=%d, at most %d rows of a portion are supported", max_seqlen, kMostDrafted);
+  if (batch == 0 || num_tokens == 0 || max_seqlen == 0) return qs::QS_OK;
+  QS_REQUIRE(positions && visible && parents && lengths, "draft_tree: null tensor");
+  return draft_tree(positions, reinterpret_cast<long long*>(visible), parents, cu_seqlens, lengths, batch, num_tokens, max_seqlen, stream);
+}
+
+int qs_verify_drafts(int64_t* out_tokens, int32_t* out_rows, int32_t* out_counts, const void* logits, int logits_type, int64_t logits_stride, const int64_t* tokens,
+                     const int32_t* parents, const float* draft_probs, int64_t probs_stride, const int32_t* cu_seqlens, const float* coins, const float* draws,
+                     const float* temperatures, int batch, int num_tokens, int vocab, int max_seqlen, void* stream) {
+  const char* op = "verify_drafts";
+  QS_REQUIRE(batch >= 0 && num_tokens >= 0, "%s: negative size", op);
+  QS_REQUIRE(max_seqlen >= 0 && max_seqlen <= kMostDrafted, "%s: max_seqlen=%d, at most %d rows of a portion are supported", op, max_seqlen, kMostDrafted);
+  QS_REQUIRE(logits_type >= 0 && logits_type <= 2, "%s: logits of type %d", op, logits_type);
+  QS_REQUIRE(vocab > 0 && vocab <= (1 << 28), "%s: vocab=%d", op, vocab);
+  QS_REQUIRE(batch <= (1 << 24), "%s: %d sequences", op, batch);
+  QS_REQUIRE(!(parents && draft_probs), "%s: draft probabilities go with chains, not with parents", op);
+  if (batch == 0) return qs::QS_OK;
+  QS_REQUIRE(out_counts && ((out_tokens && out_rows) || max_seqlen == 0), "%s: null tensor", op);
+  if (num_tokens > 0) {
+    QS_REQUIRE(logits && tokens && coins && draws, "%s: null tensor", op);
+    QS_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (logits_type == 2 ? 3 : 1)) == 0, "%s: logits must start on a boundary of their type", op);
+    QS_REQUIRE(num_tokens == 1 || logits_stride >= vocab, "%s: row stride of logits smaller than the row", op);
+    QS_REQUIRE(!draft_probs || num_tokens == 1 || probs_stride >= vocab, "%s: row stride of draft_probs smaller than the row", op);
+  }
+  VerifyArgs a;
+  a.logits = logits; a.type = logits_type; a.logits_stride = logits_stride; a.probs_stride = probs_stride; a.tokens = reinterpret_cast<const long long*>(tokens);
+  a.parents = parents; a.probs = draft_probs; a.cu_seqlens = cu_seqlens; a.coins = coins; a.draws = draws; a.temperatures = temperatures;
+  a.out_tokens = reinterpret_cast<long long*>(out_tokens); a.out_rows = out_rows; a.out_counts = out_counts; a.batch = batch; a.num_tokens = num_tokens; a.vocab = vocab;
+  a.max_seqlen = max_seqlen; a.stream = stream;
+  return verify_drafts(a);
 }
 
 size_t qs_shared_prefix_attention_workspace_bytes(int batch, int shared_blocks, int num_heads, int num_kv_heads) {

@@ -140,10 +140,14 @@ struct AppendArgs {
   PagedCache cache;
   int batch = 0, num_tokens = 0, num_heads = 0;
   float rotary_base = 10000.f;
+  const int* positions = nullptr;  // [axes, num_tokens]; null: the rows' places
+  unsigned char axis_of[64] = {};  // of each pair
   void* stream = nullptr;
 };
 int append_kv_cache(const AppendArgs& a);
 int read_kv_cache(void* k_out, void* v_out, const PagedCache& c, int batch, int num_tokens, void* stream);
+constexpr int kMostDrafted = 256;  // rows of a portion that draft_tree, verify_drafts and keep_kv_cache take
+int keep_kv_cache(int* new_lengths, const PagedCache& c, const int* rows, const int* counts, int row_stride, int batch, int num_tokens, void* stream);
 struct PagedAttnArgs {
   const void* q = nullptr;  // fp16 [T, Hq, 128], rotated
   void* out = nullptr;
@@ -151,6 +155,8 @@ struct PagedAttnArgs {
   PagedCache cache;
   int batch = 0, num_tokens = 0, num_heads = 0, max_seqlen = 0, max_length = 0;
   float softmax_scale = 0.f;
+  const unsigned long long* visible = nullptr;  // [num_tokens, visible_words]: which rows of its portion a row sees; null: those up to itself
+  int visible_words = 0;
   void* workspace = nullptr;
   size_t workspace_bytes = 0;
   void* stream = nullptr;
@@ -159,5 +165,23 @@ size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max
 int paged_prompt_attention(const PagedAttnArgs& a);
 size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_heads);
 int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks);
+
+// drafts.cu: drafted tokens of a step, a chain or a tree per sequence
+int draft_tree(int* positions, long long* visible, const int* parents, const int* cu_seqlens, const int* lengths, int batch, int num_tokens, int max_seqlen, void* stream);
+struct VerifyArgs {
+  const void* logits = nullptr;  // [num_tokens, vocab], rows of logits_stride numbers
+  int type = 0;                  // 0 fp16, 1 bf16, 2 fp32
+  long long logits_stride = 0, probs_stride = 0;
+  const long long* tokens = nullptr;     // [num_tokens]
+  const int* parents = nullptr;          // [num_tokens]; null: every row's is the one before it
+  const float* probs = nullptr;          // [num_tokens, vocab]; null: drafts are not drawn at random
+  const int* cu_seqlens = nullptr;
+  const float *coins = nullptr, *draws = nullptr, *temperatures = nullptr;
+  long long* out_tokens = nullptr;       // [batch, max_seqlen]
+  int *out_rows = nullptr, *out_counts = nullptr;
+  int batch = 0, num_tokens = 0, vocab = 0, max_seqlen = 0;
+  void* stream = nullptr;
+};
+int verify_drafts(const VerifyArgs& a);
 
 }  // namespace qs

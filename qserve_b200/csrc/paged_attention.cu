@@ -179,6 +179,8 @@ struct TileParams {
   // parts > 1: O / sum [rows][parts][128]: rows = token * num_heads + head where all items are split, otherwise those of the split items, one behind the other
   float* part;
   float2* part_ml;                        // (maximum, sum) [rows][parts]
+  const unsigned long long* visible;      // masked: [num_tokens][words], bit i: the row sees row i of its portion
+  int words;
 };
 
 // Two results in fp16, no further from 0 than its largest number (NaN stays NaN): a mean of values is no larger than they are, but rounded weights over the sum of the
@@ -215,7 +217,23 @@ __device__ __forceinline__ Share share_of(const TileParams& p, unsigned block) {
   }
   return s;
 }
-template <int BITS, int TILES, int MODE>
+// Which of the 64 keys from `at` of its portion on (below zero: ahead of it) a row sees: all that lie ahead of the portion, and the new rows that its bits name.
+// `left`: keys from the first of them to the portion's end.
+__device__ __forceinline__ unsigned long long seen_of(const unsigned long long* row, int words, int at, int left) {
+  unsigned long long m = ~0ull;
+  if (at >= 0) {
+    const int w = at >> 6, s = at & 63;
+    m = w < words ? __ldcg(row + w) >> s : 0ull;
+    if (s > 0 && w + 1 < words) m |= __ldcg(row + w + 1) << (64 - s);
+  } else if (at > -64) {
+    m = (~0ull >> (64 + at)) | (__ldcg(row) << -at);
+  }
+  return left >= 64 ? m : left <= 0 ? 0ull : m & (~0ull >> (64 - left));
+}
+
+// MASKED: a row sees all keys ahead of its portion and those of the portion that its bits name, wherever it lies itself.  The bits are looked at in the pages that hold
+// new rows, at most one of them more than the portion fills; in all others, as without a mask, nothing is compared.
+template <int BITS, int TILES, int MODE, bool MASKED>
 __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, TILES>::kBlocksPerSm) tile_kernel(const __grid_constant__ TileParams p) {
   using C = TileCfg<BITS, TILES>;
   using G = Geom<BITS>;
@@ -286,7 +304,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     n_keys = p.shared_blocks * kPage;
   } else {
     const int last = min(n_rows, row_base + TILES * kRows) - 1;
-    n_keys = any ? min(max(portion.first + last / group + 1, 0), p.max_blocks * kPage) : 0;
+    n_keys = any ? min(max(portion.first + (MASKED ? portion.count : last / group + 1), 0), p.max_blocks * kPage) : 0;
   }
   const int n_pages = (n_keys + kPage - 1) / kPage;
   // (nsplit <= 128 splits of at most 2^24 pages: 32 bits hold the products)
@@ -632,8 +650,12 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
     int limit = n_keys - 1;
     if (row_is) limit = p.shared_blocks > 0 ? min(max(__ldcg(p.lengths + tok), 0), n_keys) - 1 : min(portion.first + tok, n_keys - 1);
     int lowest = limit;
+    if constexpr (MASKED) {
+      lowest = min(portion.first, n_keys) - 1;
+    } else {
 #pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, m));
+      for (int m = 16; m >= 1; m >>= 1) lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, m));
+    }
     const uint32_t t_s = tmem + tile * kTileCols + (static_cast<uint32_t>(quarter * 32) << 16), t_o = t_s + kColO;
     float m_used = -CUDART_INF_F, l = 0.f;  // what O and the sum are expressed against (log2 units)
     for (int j = 0; j < n_mine; ++j) {
@@ -647,6 +669,16 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         tmem_wait_ld();
         const int key0 = (page0 + j) * kPage;
         if (key0 + kPage - 1 > lowest) {  // warp-uniform
+          if constexpr (MASKED) {
+            const unsigned long long seen =
+                row_is ? seen_of(p.visible + static_cast<long long>(portion.start + tok) * p.words, p.words, key0 - portion.first, n_keys - key0) : 0ull;
+            const uint32_t half[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (!(half[c] & (1u << i))) x[c][i] = 0xff800000u;  // -inf
+          } else
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -1388,13 +1420,17 @@ Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, lon
 }
 size_t part_bytes(long long rows, int parts) { return static_cast<size_t>(rows) * parts * (kD * sizeof(float) + sizeof(float2)); }
 
-template <int BITS, int TILES, int MODE>
-int run_tiles(const TileParams& p, long long blocks, void* stream) {
+template <int BITS, int TILES, int MODE, bool MASKED>
+int run_tiles_as(const TileParams& p, long long blocks, void* stream) {
   using C = TileCfg<BITS, TILES>;
-  const int rc = allow_smem<tile_kernel<BITS, TILES, MODE>>(C::kSmem, "paged attention: shared memory", [](int regs) { return !C::kShares || shares_suffice(regs); });
+  const int rc = allow_smem<tile_kernel<BITS, TILES, MODE, MASKED>>(C::kSmem, "paged attention: shared memory", [](int regs) { return !C::kShares || shares_suffice(regs); });
   if (rc) return rc;
   QS_REQUIRE(blocks <= 0x7fffffffll, "paged attention: %lld blocks", blocks);
-  return launch(tile_kernel<BITS, TILES, MODE>, dim3(static_cast<unsigned>(blocks)), C::kThreads, C::kSmem, stream, "paged attention", p.cluster, p);
+  return launch(tile_kernel<BITS, TILES, MODE, MASKED>, dim3(static_cast<unsigned>(blocks)), C::kThreads, C::kSmem, stream, "paged attention", p.cluster, p);
+}
+template <int BITS, int TILES, int MODE>
+int run_tiles(const TileParams& p, long long blocks, void* stream) {
+  return p.visible ? run_tiles_as<BITS, TILES, MODE, true>(p, blocks, stream) : run_tiles_as<BITS, TILES, MODE, false>(p, blocks, stream);
 }
 int tiles(TileParams& p, const Plan& pl, bool int4, void* stream) {
   p.row_blocks = pl.row_blocks; p.nsplit = pl.nsplit; p.cluster = pl.cluster; p.parts = pl.parts;
@@ -1440,6 +1476,7 @@ int paged_prompt_attention(const PagedAttnArgs& a) {
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths;
   p.batch = a.batch; p.num_tokens = a.num_tokens; p.max_seqlen = a.max_seqlen; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.visible = a.visible; p.words = a.visible_words;
   const long long rows = pl.split_rows(static_cast<long long>(a.num_tokens) * a.num_heads);
   if (pl.parts > 1) {
     QS_REQUIRE(a.workspace && a.workspace_bytes >= part_bytes(rows, pl.parts), "paged_prompt_attention: workspace of %zu bytes, %zu needed", a.workspace_bytes,

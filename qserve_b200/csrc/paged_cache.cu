@@ -3,7 +3,10 @@
 // append: token i of sequence b's portion of n_b takes position p = lengths[b] - n_b + i.  Queries and keys are rotated (entry i with entry i + 64, angle
 // p base^(-2 i / 128)), keys and values quantised per (token, kv head): scale s = half((max - min) / L), zero z = half(-L min / (max - min)), code
 // clamp(round(x / s + z), 0, L), L = 15 or 255.
+// append at positions: the place in the pages as above, but pair i of a row is turned by positions[axis(i)][row] base^(-2 i / 128): depths of drafted trees, or time,
+// height and width of images, each with pairs of its own.
 // read: the same positions out of the pages again, as fp16; zeros for a row that has none.
+// keep: position first + j of a portion gets what first + rows[j] holds: the accepted rows of a drafted tree, side by side.
 #include <math_constants.h>
 
 #include <cmath>
@@ -139,10 +142,13 @@ struct AppendParams {
   const int *cu, *lengths;
   int batch, num_tokens, max_blocks, num_heads, num_kv_heads, rows_per_warp;
   Turns turns;
+  const int* positions;                // at positions: [axes][num_tokens]
+  unsigned char axis_of[kD / 2];       //   which of them turns pair i
 };
 
 // A warp per token and run of its head rows, four rows at a time with eight lanes each.  ROWS: groups of four rows whose loads are on their way together.
-template <int BITS, int ROWS>
+// AT: the angles go by given positions.  (A variant of its own: the branch alone would cost the other nothing that could be measured, its registers would.)
+template <int BITS, int ROWS, bool AT>
 __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_constant__ AppendParams p) {
   using G = Geom<BITS>;
   __shared__ __align__(16) float s_cos[kWarps][kD / 2], s_sin[kWarps][kD / 2];
@@ -187,7 +193,9 @@ __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_consta
   if (begin < rotated) {
 #pragma unroll
     for (int i = lane; i < kD / 2; i += 32) {
-      const double turns = p.turns.per_position[i] * pos;
+      int at = pos;
+      if constexpr (AT) at = p.positions[static_cast<long long>(p.axis_of[i]) * p.num_tokens + t];
+      const double turns = p.turns.per_position[i] * at;
       double sn, cs;
       sincospi(2.0 * (turns - rint(turns)), &sn, &cs);
       s_sin[warp][i] = static_cast<float>(sn);
@@ -345,6 +353,59 @@ __global__ void __launch_bounds__(32 * kWarps) read_kernel(const ReadParams p) {
   }
 }
 
+// A block per sequence, kv head and tensor.  All kept rows are in shared memory before the first is written, so a place may be another row's source.
+struct KeepParams {
+  const long long* kv_pointers;
+  const int *cu, *lengths, *rows, *counts;
+  int* new_lengths;
+  int num_tokens, max_blocks, num_kv_heads, row_stride;
+};
+constexpr int kKeepThreads = 128;
+
+template <int BITS>
+__global__ void __launch_bounds__(kKeepThreads) keep_kernel(const KeepParams p) {
+  using G = Geom<BITS>;
+  constexpr int kWords = G::kRow / 16;
+  __shared__ __align__(16) uint4 s_codes[kMostDrafted * kWords];
+  __shared__ __half s_scale[kMostDrafted], s_zero[kMostDrafted];
+  __shared__ int s_from[kMostDrafted];  // position; -1: the row stays what it is
+  pdl_launch_dependents();
+  pdl_wait();
+  const int b = blockIdx.y, head = blockIdx.x >> 1, which = blockIdx.x & 1, tid = threadIdx.x;
+  const Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
+  const int count = min(min(max(p.counts[b], 0), portion.count), p.row_stride);
+  if (blockIdx.x == 0 && tid == 0) p.new_lengths[b] = max(portion.first + count, 0);
+  const long long* table = p.kv_pointers + (static_cast<long long>(b) * 2 + which) * p.max_blocks;
+  auto held = [&](int pos) { return pos >= 0 && (pos >> 6) < p.max_blocks; };
+  for (int j = tid; j < count; j += kKeepThreads) {
+    const int row = p.rows[static_cast<long long>(b) * p.row_stride + j], from = portion.first + row;
+    const bool moves = row >= 0 && row < portion.count && row != j && held(from) && held(portion.first + j);
+    s_from[j] = moves ? from : -1;
+    if (!moves) continue;
+    const uint8_t* page = reinterpret_cast<const uint8_t*>(table[from >> 6]);
+    s_scale[j] = *reinterpret_cast<const __half*>(page + G::scales_at(head, p.num_kv_heads) + (from & (kPage - 1)) * 2);
+    s_zero[j] = *reinterpret_cast<const __half*>(page + G::zeros_at(head, p.num_kv_heads) + (from & (kPage - 1)) * 2);
+  }
+  __syncthreads();
+  for (int i = tid; i < count * kWords; i += kKeepThreads) {
+    const int from = s_from[i / kWords];
+    if (from < 0) continue;
+    const uint8_t* page = reinterpret_cast<const uint8_t*>(table[from >> 6]);
+    s_codes[i] = reinterpret_cast<const uint4*>(page + G::codes_at(head) + (from & (kPage - 1)) * G::kRow)[i % kWords];
+  }
+  __syncthreads();
+  for (int i = tid; i < count * kWords; i += kKeepThreads) {
+    const int j = i / kWords, to = portion.first + j;
+    if (s_from[j] < 0) continue;
+    uint8_t* page = reinterpret_cast<uint8_t*>(table[to >> 6]);
+    reinterpret_cast<uint4*>(page + G::codes_at(head) + (to & (kPage - 1)) * G::kRow)[i % kWords] = s_codes[i];
+    if (i % kWords == 0) {
+      *reinterpret_cast<__half*>(page + G::scales_at(head, p.num_kv_heads) + (to & (kPage - 1)) * 2) = s_scale[j];
+      *reinterpret_cast<__half*>(page + G::zeros_at(head, p.num_kv_heads) + (to & (kPage - 1)) * 2) = s_zero[j];
+    }
+  }
+}
+
 }  // namespace
 
 int append_kv_cache(const AppendArgs& a) {
@@ -364,7 +425,10 @@ int append_kv_cache(const AppendArgs& a) {
   p.rows_per_warp = static_cast<int>(fair >= rows ? rows : 8 * (fair / 8 + 1));
   const dim3 grid(blocks, (rows + p.rows_per_warp - 1) / p.rows_per_warp);
   auto run = [&](auto kern) { return launch(kern, grid, 32 * kWarps, 0, a.stream, "append_kv_cache", 1, p); };
-  return a.cache.int4 ? run(append_kernel<4, 2>) : run(append_kernel<8, 2>);
+  if (a.positions == nullptr) return a.cache.int4 ? run(append_kernel<4, 2, false>) : run(append_kernel<8, 2, false>);
+  p.positions = a.positions;
+  for (int i = 0; i < kD / 2; ++i) p.axis_of[i] = a.axis_of[i];
+  return a.cache.int4 ? run(append_kernel<4, 2, true>) : run(append_kernel<8, 2, true>);
 }
 
 int read_kv_cache(void* k_out, void* v_out, const PagedCache& c, int batch, int num_tokens, void* stream) {
@@ -376,6 +440,16 @@ int read_kv_cache(void* k_out, void* v_out, const PagedCache& c, int batch, int 
   const dim3 grid((num_tokens + kWarps - 1) / kWarps, (2 * c.num_kv_heads + 4 * kRows - 1) / (4 * kRows));
   auto run = [&](auto kern) { return launch(kern, grid, 32 * kWarps, 0, stream, "read_kv_cache", 1, p); };
   return c.int4 ? run(read_kernel<4, kRows>) : run(read_kernel<8, kRows>);
+}
+
+int keep_kv_cache(int* new_lengths, const PagedCache& c, const int* rows, const int* counts, int row_stride, int batch, int num_tokens, void* stream) {
+  if (batch == 0) return QS_OK;
+  KeepParams p{};
+  p.kv_pointers = c.kv_pointers; p.cu = c.cu_seqlens; p.lengths = c.lengths; p.rows = rows; p.counts = counts; p.new_lengths = new_lengths;
+  p.num_tokens = num_tokens; p.max_blocks = c.max_blocks; p.num_kv_heads = c.num_kv_heads; p.row_stride = row_stride;
+  const dim3 grid(2 * c.num_kv_heads, batch);
+  auto run = [&](auto kern) { return launch(kern, grid, kKeepThreads, 0, stream, "keep_kv_cache", 1, p); };
+  return c.int4 ? run(keep_kernel<4>) : run(keep_kernel<8>);
 }
 
 }  // namespace qs
