@@ -186,13 +186,14 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 // 1 + g + g^2 / 2 + g^3 / 6 + g^4 / 24 of the rest |g| <= ln(2) / 64: off by g^5 / 120 = 1.2e-12 of itself at most.  Nine operations of 64 bits, where exp() has about
 // 25; a table of 32 entries meets every bank of shared memory twice at most.  (A larger table and one product less took longer.)
 struct Weigh {
-  double top, per_unit;  // 32 log2(e) / t
+  double per_unit, span;  // 32 log2(e) / t; 2^14 of those
+  double top;
   uint32_t power;        // 2^(i / 32), in shared memory
   float least;           // what is above it weighs 2^-512 at least
   bool odd;              // the largest has no end, and those without one share the weight; or there is no number to take for all that weigh nothing
   __device__ __forceinline__ void against(float largest) {
     top = largest;
-    least = __double2float_rd(top - fmax(16384.0 / per_unit, fabs(top) * 1e-12));  // y below 2^14; a number below top in any case
+    least = __double2float_rd(top - fmax(span, fabs(top) * 1e-12));  // y below 2^14; a number below top in any case
     odd = !((top - static_cast<double>(least)) * per_unit < 30000.0);  // (2^-1022 is 2^(-32704 / 32))
   }
   __device__ __forceinline__ double finite(float x) const {
@@ -389,7 +390,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   const double inverse = greedy ? 1.0 : 1.0 / static_cast<double>(heat);
   const float per_unit = fminf(static_cast<float>(inverse * 1.4426950408889634), 3.0e38f);  // in octaves
   int turn = 0, turn_sum = 0;  // of the cluster's exchanges: their places alternate, so that none is written while a block still reads the one before
-  Weigh weigh{0.0, inverse * (kSteps * 1.4426950408889634), smem_u32(s_power), 0.f, false};
+  Weigh weigh{inverse * (kSteps * 1.4426950408889634), 16384.0 / (inverse * (kSteps * 1.4426950408889634)), 0.0, smem_u32(s_power), 0.f, false};
 
   int node = 0, accepted = 0;
   float top = 0.f;     // of the current row
@@ -429,34 +430,39 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     for (int r = 0; r < p.cluster; ++r) sum += s_shares[turn_sum ^ 1][i][r];
     return sum;
   };
-  // A warp's decision on a row: the child that is taken, 0 for none, -1 where the sum of 32 bits could err by `doubt` of itself.  (weigh is of this row.)
-  auto decide = [&](int r, double sum, int largest, double doubt) {
-    if (!greedy && doubt > 0.0 && !(sum >= 0.5 && sum < 1e30)) return -1;
-    const double u = static_cast<double>(s_coin[r]);
-    double mass = 0.0;
+  // A warp's decision on row r with largest number m (or, greedy, largest token) and sum of weights: the child that is taken, 0 for none, -1 where this could err.  In
+  // Real's bits; those of 32 are off by no more than `doubt`.
+  auto decide = [&](int r, float m, auto sum, int largest, auto doubt) {
+    using Real = decltype(sum);
+    constexpr bool kFast = sizeof(Real) == 4;
+    if (kFast && !greedy && !(sum >= Real(0.5) && sum < Real(1e30))) return -1;
+    const Real u = static_cast<Real>(s_coin[r]);
+    Real mass = 0;
     for (int i0 = (r + 1) & ~31; i0 < n; i0 += 32) {
       const int i = i0 + lane;
       const bool child = i < n && i > r && s_parent[i] == r && s_token[i] >= 0;
       if (!__any_sync(0xffffffffu, child)) continue;
       bool take = child && s_token[i] == largest, close = false;
       if (!greedy) {
-        const double w = child && !s_again[i] ? weigh(s_x[i]) : 0.0;
-        double left = u * sum, right;
+        Real w = 0;
+        if (child && !s_again[i]) {
+          if constexpr (kFast) w = ex2((s_x[i] - m) * per_unit);
+          else w = weigh(s_x[i]);
+        }
+        Real left = u * sum, right = w;
         if (probs) {
-          left *= static_cast<double>(child ? s_q[i] : 0.f);
-          right = w;
+          left *= static_cast<Real>(child ? s_q[i] : 0.f);
         } else {
-          double run = w;
 #pragma unroll
           for (int d = 1; d < 32; d <<= 1) {
-            const double below = __shfl_up_sync(0xffffffffu, run, d);
-            if (lane >= d) run += below;
+            const Real below = __shfl_up_sync(0xffffffffu, right, d);
+            if (lane >= d) right += below;
           }
-          right = mass + run;
-          mass += __shfl_sync(0xffffffffu, run, 31);
+          right += mass;
+          mass = __shfl_sync(0xffffffffu, right, 31);
         }
-        take = child && w > 0.0 && left < right;
-        close = doubt > 0.0 && child && fabs(left - right) <= doubt * (left + right);
+        take = child && w > Real(0) && left < right;
+        close = kFast && child && !(fabs(left - right) > doubt * (left + right));
       }
       const unsigned first = __ballot_sync(0xffffffffu, take), border = __ballot_sync(0xffffffffu, close);
       if (border && (!first || __ffs(border) <= __ffs(first))) return -1;  // (one behind the first that is taken decides nothing)
@@ -659,9 +665,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
         for (int i = kN - 1; i >= 0; --i)
           if (number(x[i]) == m) largest = word * kN - row.skip + i;
       }
-      weigh.against(m);
       // A weight of 32 bits is off by 2^-24 of the numbers that its exponent comes from, top / t and their difference of 40 octaves at most, and by ex2's 2^-22
-      const int taken = decide(r, s, largest, 1e-5 + fabs(static_cast<double>(m) * per_unit) * 2.4e-7);
+      const int taken = decide(r, m, s, largest, 1e-5f + fabsf(m * per_unit) * 2.4e-7f);
       if (lane == 0) {
         s_next[warp] = taken;
         s_largest[warp] = largest;
@@ -679,7 +684,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
         share_out(shares_of_row(node, nullptr, 0));
         total = sum_of(0);
         if (warp == 0) {
-          const int t = decide(node, total, -1, 0.0);
+          const int t = decide(node, top, total, -1, 0.0);
           if (lane == 0) s_next[k] = t;
         }
         __syncthreads();
@@ -762,10 +767,15 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       double w[kN], mine = 0.0;
       auto weights_of = [&](int c) {
         const int first = c * kN - row.skip;
-        const uint4 its = row.word(c);
-        const T* x = reinterpret_cast<const T*>(&its);
+        float x[kN];
+        numbers_of<T>(row.word(c), x);
+        if (weigh.odd) {
 #pragma unroll
-        for (int k = 0; k < kN; ++k) w[k] = weigh(number(x[k]));
+          for (int k = 0; k < kN; ++k) w[k] = weigh(x[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < kN; ++k) w[k] = x[k] > weigh.least ? weigh.finite(fmaxf(x[k], weigh.least)) : 0.0;
+        }
         for (int j = 0; j < kids; ++j) {
           const int at = s_kids[j] - first;
 #pragma unroll
