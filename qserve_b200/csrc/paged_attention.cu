@@ -1336,6 +1336,419 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
 }
 
 // ------------------------------------------------------------------------------------------------------------------------
+// row kernel: portions of few rows with a mask among them (a step's drafted tokens)
+//
+// Up to 16 rows (token, head of the group) of a kv head.  Codes go into the products as they lie, as in the tail kernel, but as their second operand: the rows are the
+// first one's 16, and a product's scores are the next one's operand as they are.  A block's warps take turns over half pages, a cluster of blocks over their runs.
+// A warp takes 1.0 us for a half page, 1.45 where two blocks share a multiprocessor (registers hold no third: with 168 a thread the code takes 1.4 times as long), of
+// which products are a quarter: one chain of copies - scales - scores - weights - values.  Against the tile kernel, whose products are for 128 rows and whose pages are
+// unpacked first, us: 18 sequences of 4 rows of 32 heads over 8 behind 3000, INT4, 25.5 and 50; 37 43 and 72; 32 of 8 rows, 32 heads over 32, behind 1000 to 2000, INT8,
+// 92 and 166; error 2.9e-4 and 4.5e-4.  With 16 rows more a warp, or warps that share half pages, for up to 64 rows: 131 where the tile kernel takes 64.
+// ------------------------------------------------------------------------------------------------------------------------
+constexpr int kMostRows = 16, kMostRowBlocks = 16;
+
+template <int BITS>
+struct RowsCfg {
+  using SC = SliceCfg<BITS, true>;
+  static constexpr int kSlots = BITS == 4 ? 4 : 3;
+  static constexpr int kWarpBytes = kSlots * SC::kBytes;
+  static constexpr int kOffOut = kTailWarps * kWarpBytes;  // the block's rows
+  static constexpr int kSmem = kOffOut + kMostRows * kD * 4;
+  static_assert(kWarpBytes >= kMostRows * kOPitch * 4, "a warp's ring holds its partial rows at the end");
+};
+struct RowsParams {
+  const __half* q;
+  __half* out;
+  long long q_stride, out_stride;
+  const long long* kv_pointers;
+  const int *cu, *lengths;
+  const unsigned long long* visible;
+  int words, num_tokens, max_seqlen, max_blocks, num_heads, num_kv_heads, cluster;
+  float scale_log2;
+};
+
+// a product that the compiler may place where it likes: the order of the chains below is then its own
+__device__ __forceinline__ void mma_any(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_constant__ RowsParams p) {
+  using C = RowsCfg<BITS>;
+  using SC = typename C::SC;
+  using G = Geom<BITS>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  __shared__ float s_m[kTailWarps][kMostRows], s_l[kTailWarps][kMostRows];
+  __shared__ float2 s_meta[kTailWarps][2][kSlice];
+  __shared__ float s_bm[kMostRows], s_bl[kMostRows];
+  float* const s_o = reinterpret_cast<float*>(smem + C::kOffOut);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const unsigned item = blockIdx.x / static_cast<unsigned>(p.cluster);
+  const int rank = static_cast<int>(blockIdx.x - item * p.cluster);
+  const int b = item / static_cast<unsigned>(p.num_kv_heads), hk = item - b * p.num_kv_heads;
+  const int group = static_cast<unsigned>(p.num_heads) / static_cast<unsigned>(p.num_kv_heads);
+  pdl_launch_dependents();
+  pdl_wait();
+  Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
+  portion.count = min(portion.count, p.max_seqlen);
+  const int n_rows = portion.count * group;
+  if (n_rows == 0) return;  // the whole cluster
+  const int n_keys = min(max(portion.first + portion.count, 0), p.max_blocks * kPage);
+  const int slices = (n_keys + kSlice - 1) / kSlice;
+  // the block's run of them (16 blocks of at most 2^25: 32 bits hold the products), and the warp's turns
+  const int s0 = static_cast<int>(static_cast<unsigned>(rank) * static_cast<unsigned>(slices) / p.cluster);
+  const int s1 = static_cast<int>((static_cast<unsigned>(rank) + 1u) * static_cast<unsigned>(slices) / p.cluster);
+  const int mine = s0 + warp, n_my = s1 > mine ? (s1 - mine + kTailWarps - 1) / kTailWarps : 0;
+  const long long* kptrs = p.kv_pointers + static_cast<long long>(b) * 2 * p.max_blocks;
+  uint8_t* const ring = smem + warp * C::kWarpBytes;
+  const uint32_t ring_at = smem_u32(ring);
+  const uint32_t lane_at = SC::place(lane * 16 / SC::kRow, lane * 16 % SC::kRow / 16);
+  long long kp_l = 0, vp_l = 0;  // lane i: the pages of slices 32 n + i
+  auto issue = [&](int u) {
+    if ((u & 31) == 0 && u + lane < n_my) {
+      const int page = (mine + (u + lane) * kTailWarps) >> 1;
+      kp_l = __ldcg(kptrs + page);
+      vp_l = __ldcg(kptrs + p.max_blocks + page);
+    }
+    const int half = (mine + u * kTailWarps) & 1;
+    const uint8_t* kp = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, kp_l, u & 31));
+    const uint8_t* vp = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp_l, u & 31));
+    const uint32_t dst = ring_at + (u % C::kSlots) * SC::kBytes;
+    const long long codes = G::codes_at(hk) + half * SC::kCodes + lane * 16;
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int i = 0; i < SC::kCodes / 512; ++i)
+        cp_async16(dst + w * SC::kOffV + i * 512 + (BITS == 8 && (i & 1) ? lane_at ^ 16u : lane_at), (w ? vp : kp) + codes + i * 512);
+    if (lane < 16) {
+      const uint8_t* page_at = lane < 8 ? kp : vp;
+      const long long meta = (lane & 4) ? G::zeros_at(hk, p.num_kv_heads) : G::scales_at(hk, p.num_kv_heads);
+      cp_async16(dst + SC::kOffMeta + lane * 16, page_at + meta + half * 64 + (lane & 3) * 16);
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < C::kSlots - 1; ++u) {
+    if (u < n_my) issue(u);
+    cp_async_commit();
+  }
+  // ---- the queries, rows g and g + 8 of the warp's, in the order of the codes: this lane's 32 dims, as in the tail kernel ----
+  uint32_t qa[2][8], qh[2][8];  // INT4: of the low nibbles, of the high ones; INT8: of a word's first two codes, its others
+  float sumq[2];
+  unsigned long long bits[2];   // of the rows: no more than 64, so one word
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int r = 8 * e + g, tok = r / group;
+    uint32_t qw[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) qw[k] = 0u;
+    bits[e] = 0ull;
+    if (r < n_rows) {
+      const uint4* qv = reinterpret_cast<const uint4*>(p.q + (portion.start + tok) * p.q_stride + static_cast<long long>(hk * group + r - tok * group) * kD + 32 * q4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 x = __ldcg(qv + k);
+        qw[4 * k] = x.x; qw[4 * k + 1] = x.y; qw[4 * k + 2] = x.z; qw[4 * k + 3] = x.w;
+      }
+      bits[e] = __ldcg(p.visible + static_cast<long long>(portion.start + tok) * p.words);
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float2 f = __half22float2(as_h2(qw[k]));
+      sum += f.x + f.y;
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sumq[e] = sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      if constexpr (BITS == 4) {
+        const int k0 = 4 * (s >> 1) + (s & 1);
+        qa[e][s] = __byte_perm(qw[k0], qw[k0 + 2], 0x5410);
+        qh[e][s] = __byte_perm(qw[k0], qw[k0 + 2], 0x7632);
+      } else {
+        qa[e][s] = qw[2 * s];
+        qh[e][s] = qw[2 * s + 1];
+      }
+    }
+  }
+  constexpr float kUp = 16777216.f;  // 2^24
+  // O: tile i, rows g (0, 1) and g + 8 (2, 3).  INT4: dims 32 (i / 4) + 4 n + i % 4 of column n, the odd ones 16 times as large; INT8: 16 (i / 2) + 2 n + i % 2
+  float o[16][4];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, ref[2] = {}, l[2] = {}, cv[2] = {};
+  float s_top = 5.9604645e-8f;  // 2^-24, the smallest scale
+  // Column n of a product over eight keys is key (n & 1) * 4 + (n >> 1) of them: this lane's columns 2 q4 and 2 q4 + 1 are keys q4 and q4 + 4, and its K row key
+  const uint32_t k_at = SC::place((g & 1) * 4 + (g >> 1), BITS == 4 ? q4 : 2 * q4);
+  const uint32_t v_at = SC::place((lane & 1) * 4 + ((lane >> 1) & 3) + (lane & 8), lane >> 4) + SC::kOffV;
+  for (int u = 0; u < n_my; ++u) {
+    cp_async_wait<C::kSlots - 2>();
+    __syncwarp();
+    if (u + C::kSlots - 1 < n_my) issue(u + C::kSlots - 1);
+    cp_async_commit();
+    const uint32_t slot = (u % C::kSlots) * SC::kBytes;
+    const uint8_t* st = ring + slot;
+    const int t0 = (mine + u * kTailWarps) * kSlice;
+    {  // per key, as in the tail kernel; keys q4 and q4 + 4 of eight side by side
+      const __half* mp = reinterpret_cast<const __half*>(st + SC::kOffMeta) + lane;
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const __half s = mp[64 * w], z = mp[64 * w + 32];
+        float2 f = make_float2(__half2float(s), -__half2float(z));
+        if constexpr (BITS == 4) {
+          f.y = __half2float(__hmul(__hneg(s), z));
+          if (w == 1) f.y = __fdividef(f.y, f.x == 0.f ? 1.f : f.x);
+        } else if (w == 0) {
+          f.y *= f.x;
+        }
+        const float none = fmaf(f.x, 0.f, f.y * 0.f);
+        if (w == 0) f = make_float2(fmaf(f.x, p.scale_log2 * kUp, none), f.y * p.scale_log2);
+        else f = make_float2(f.x + none, f.y + none);
+        if (t0 + lane >= n_keys) f = make_float2(0.f, 0.f);
+        s_meta[warp][w][(lane & 24) + 2 * (lane & 3) + ((lane >> 2) & 1)] = f;
+      }
+    }
+    __syncwarp();
+    float sc[4][4], hi[4][4];  // the high nibbles, which are 16 u, by themselves, for q / 16 may not be an fp16 number; INT8: two sums for shorter chains
+    constexpr int kWords = BITS;  // of a lane's 32 codes of a key
+    uint32_t words[4][kWords];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // rows 8 apart of the half page lie 8 rows' bytes apart, in the same order of words
+#pragma unroll
+      for (int h = 0; h < BITS / 4; ++h) {
+        const uint4 k = *reinterpret_cast<const uint4*>(st + j * 8 * SC::kRow + (k_at ^ (16u * h)));
+        words[j][4 * h] = k.x; words[j][4 * h + 1] = k.y; words[j][4 * h + 2] = k.z; words[j][4 * h + 3] = k.w;
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[j][e] = hi[j][e] = 0.f;
+    }
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (BITS == 4) {
+          const uint32_t x = words[j][w], y = x >> 8;
+          mma_any(sc[j], qa[0][2 * w], qa[1][2 * w], qa[0][2 * w + 1], qa[1][2 * w + 1], x & 0x000f000fu, y & 0x000f000fu);
+          mma_any(hi[j], qh[0][2 * w], qh[1][2 * w], qh[0][2 * w + 1], qh[1][2 * w + 1], x & 0x00f000f0u, y & 0x00f000f0u);
+        } else {
+          const uint32_t x = words[j][2 * w], y = words[j][2 * w + 1];
+          mma_any(sc[j], qa[0][2 * w], qa[1][2 * w], qh[0][2 * w], qh[1][2 * w], __byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342));
+          mma_any(hi[j], qa[0][2 * w + 1], qa[1][2 * w + 1], qh[0][2 * w + 1], qh[1][2 * w + 1], __byte_perm(y, 0u, 0x4140), __byte_perm(y, 0u, 0x4342));
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sc[j][e] = BITS == 4 ? fmaf(hi[j][e], 0.0625f, sc[j][e]) : sc[j][e] + hi[j][e];
+    float4 vm[4];  // of keys q4 and q4 + 4: (scale, c / scale) twice
+    float vmax = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float4 km = *reinterpret_cast<const float4*>(&s_meta[warp][0][8 * j + 2 * q4]);
+      vm[j] = *reinterpret_cast<const float4*>(&s_meta[warp][1][8 * j + 2 * q4]);
+      vmax = fmaxf(vmax, fmaxf(fabsf(vm[j].x), fabsf(vm[j].z)));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        sc[j][2 * e] = fmaf(km.x, sc[j][2 * e], km.y * sumq[e]);
+        sc[j][2 * e + 1] = fmaf(km.z, sc[j][2 * e + 1], km.w * sumq[e]);
+      }
+    }
+    const bool masked = t0 + kSlice > min(portion.first, n_keys);  // the same in all lanes
+    if (masked) {
+      const int at = t0 - portion.first, left = n_keys - t0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        unsigned long long w = ~0ull;
+        if (at >= 0) w = at < 64 ? bits[e] >> at : 0ull;
+        else if (at > -64) w = (~0ull >> (64 + at)) | (bits[e] << -at);
+        if (left < 32) w &= left <= 0 ? 0ull : (1ull << left) - 1;
+        const uint32_t seen = static_cast<uint32_t>(w) >> q4;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (!(seen >> (8 * j) & 1u)) sc[j][2 * e] = -CUDART_INF_F;
+          if (!(seen >> (8 * j + 4) & 1u)) sc[j][2 * e + 1] = -CUDART_INF_F;
+        }
+      }
+    }
+    // The weights are 2^up times those against the maximum, as in the tail kernel; a row that has seen no key so far: against 0
+    float mh[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      mh[e] = fmaxf(fmaxf(fmaxf(sc[0][2 * e], sc[0][2 * e + 1]), fmaxf(sc[1][2 * e], sc[1][2 * e + 1])),
+                    fmaxf(fmaxf(sc[2][2 * e], sc[2][2 * e + 1]), fmaxf(sc[3][2 * e], sc[3][2 * e + 1])));
+    if (__any_sync(0xffffffffu, mh[0] > m[0] || mh[1] > m[1] || vmax > s_top)) {
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1) {
+        mh[0] = fmaxf(mh[0], __shfl_xor_sync(0xffffffffu, mh[0], d));
+        mh[1] = fmaxf(mh[1], __shfl_xor_sync(0xffffffffu, mh[1], d));
+        vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
+      }
+      if (vmax > s_top) s_top = __uint_as_float((__float_as_uint(vmax) + 0x7fffffu) & 0x7f800000u);  // the next power of two
+      const float up = static_cast<float>(142 - static_cast<int>(__float_as_uint(s_top) >> 23));
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float m_new = fmaxf(m[e], mh[e]), ref_new = (m_new == -CUDART_INF_F ? 0.f : m_new) - up;
+        const float a = m[e] == -CUDART_INF_F ? 0.f : ex2(ref[e] - ref_new);
+        m[e] = m_new;
+        ref[e] = ref_new;
+        l[e] *= a;
+        cv[e] *= a;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          o[i][2 * e] *= a;
+          o[i][2 * e + 1] *= a;
+        }
+      }
+    }
+    uint32_t pa[4][2];  // weights times scales, rounded to fp16: the next products' operand
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float p0 = ex2(sc[j][2 * e] - ref[e]), p1 = ex2(sc[j][2 * e + 1] - ref[e]);
+        l[e] += p0 + p1;
+        float w0 = p0 * vm[j].x, w1 = p1 * vm[j].z;
+        if (masked) {  // a value that is no number is nothing to a row that does not see it
+          w0 = p0 == 0.f ? 0.f : w0;
+          w1 = p1 == 0.f ? 0.f : w1;
+        }
+        const __half2 w = __floats2half2_rn(w0, w1);
+        pa[j][e] = as_u32(w);
+        const float2 f = __half22float2(w);
+        if (masked) {
+          if (p0 != 0.f) cv[e] = fmaf(f.x, vm[j].y, cv[e]);
+          if (p1 != 0.f) cv[e] = fmaf(f.y, vm[j].w, cv[e]);
+        } else {
+          cv[e] = fmaf(f.x, vm[j].y, fmaf(f.y, vm[j].w, cv[e]));
+        }
+      }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int h = 0; h < kD / (256 / BITS); ++h) {
+        uint32_t w[4];  // keys 0 to 7 and 8 to 15 of these sixteen, 16 bytes of each; then the next 16 bytes
+        ldmatrix_x4_trans(w, ring_at + slot + c * 16 * SC::kRow + (v_at ^ (h * 32u)));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t x = w[2 * e], y = w[2 * e + 1];
+          if constexpr (BITS == 4) {
+            const int i = 8 * h + 4 * e;
+            const uint32_t x8 = x >> 8, y8 = y >> 8;
+            mma_any(o[i], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x & 0x000f000fu, y & 0x000f000fu);
+            mma_any(o[i + 1], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x & 0x00f000f0u, y & 0x00f000f0u);
+            mma_any(o[i + 2], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x8 & 0x000f000fu, y8 & 0x000f000fu);
+            mma_any(o[i + 3], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x8 & 0x00f000f0u, y8 & 0x00f000f0u);
+          } else {
+            const int i = 4 * h + 2 * e;
+            mma_any(o[i], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], __byte_perm(x, 0u, 0x4240), __byte_perm(y, 0u, 0x4240));
+            mma_any(o[i + 1], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], __byte_perm(x, 0u, 0x4341), __byte_perm(y, 0u, 0x4341));
+          }
+        }
+      }
+    }
+    __syncwarp();
+  }
+  // ---- a warp's partial rows into its ring ----
+  cp_async_wait<0>();
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {
+      l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
+      cv[e] += __shfl_xor_sync(0xffffffffu, cv[e], d);
+    }
+    if (q4 == 0) {
+      s_m[warp][8 * e + g] = l[e] == 0.f ? -CUDART_INF_F : ref[e];
+      s_l[warp][8 * e + g] = l[e];
+    }
+  }
+  __syncwarp();
+  {
+    float* const rows = reinterpret_cast<float*>(ring);
+    constexpr float kOdd = BITS == 4 ? kUp * 0.0625f : kUp;  // INT4: odd dims are the high nibbles, 16 u
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float* const row = rows + (8 * e + g) * kOPitch;
+#pragma unroll
+      for (int i = 0; i < 16; i += BITS == 4 ? 4 : 2)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {  // column 2 q4 + k
+          if constexpr (BITS == 4) {
+            *reinterpret_cast<float4*>(row + 8 * i + 8 * q4 + 4 * k) = make_float4(fmaf(o[i][2 * e + k], kUp, cv[e]), fmaf(o[i + 1][2 * e + k], kOdd, cv[e]),
+                                                                                   fmaf(o[i + 2][2 * e + k], kUp, cv[e]), fmaf(o[i + 3][2 * e + k], kOdd, cv[e]));
+          } else {
+            *reinterpret_cast<float2*>(row + 8 * i + 4 * q4 + 2 * k) = make_float2(fmaf(o[i][2 * e + k], kUp, cv[e]), fmaf(o[i + 1][2 * e + k], kUp, cv[e]));
+          }
+        }
+    }
+  }
+  __syncthreads();
+  // ---- the block's rows: the warps' joined, a warp a row.  Results, or for the cluster ----
+  // where rows go, in halfs: lane i has row i
+  const long long to = (portion.start + lane / group) * p.out_stride + static_cast<long long>(hk * group + lane % group) * kD;
+  auto write = [&](int r, const float4& acc, float L) {
+    const long long at = __shfl_sync(0xffffffffu, to, r);
+    reinterpret_cast<uint2*>(p.out + at)[lane] = scaled_h4(acc, L);
+  };
+#pragma unroll 2
+  for (int r = warp; r < n_rows; r += kTailWarps) {
+    float M = -CUDART_INF_F;
+#pragma unroll
+    for (int k = 0; k < kTailWarps; ++k) M = fmaxf(M, s_m[k][r]);
+    const float base = M == -CUDART_INF_F ? 0.f : M;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float L = 0.f;
+#pragma unroll
+    for (int k = 0; k < kTailWarps; ++k) {
+      const float e = ex2(s_m[k][r] - base);
+      const float4 x = reinterpret_cast<const float4*>(smem + k * C::kWarpBytes + r * kOPitch * 4)[lane];
+      acc.x = fmaf(x.x, e, acc.x); acc.y = fmaf(x.y, e, acc.y); acc.z = fmaf(x.z, e, acc.z); acc.w = fmaf(x.w, e, acc.w);
+      L = fmaf(s_l[k][r], e, L);
+    }
+    if (p.cluster == 1) {
+      write(r, acc, L);
+      continue;
+    }
+    reinterpret_cast<float4*>(s_o + r * kD)[lane] = acc;
+    if (lane == 0) {
+      s_bm[r] = M;
+      s_bl[r] = L;
+    }
+  }
+  if (p.cluster == 1) return;
+  cluster_sync();
+  // ---- the cluster's blocks take turns over the rows, their warps too: all of a row's parts on their way together ----
+  for (int r = rank + p.cluster * warp; r < n_rows; r += p.cluster * kTailWarps) {
+    float mine = -CUDART_INF_F, sum = 0.f;  // lane k: of block k
+    if (lane < p.cluster) {
+      mine = peer_f32(s_bm + r, lane);
+      sum = peer_f32(s_bl + r, lane);
+    }
+    float4 x[kMostRowBlocks];
+#pragma unroll
+    for (int k = 0; k < kMostRowBlocks; ++k) x[k] = k < p.cluster ? peer_f32x4(s_o + r * kD + 4 * lane, k) : make_float4(0.f, 0.f, 0.f, 0.f);
+    float M = mine;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+    const float w = ex2(mine - (M == -CUDART_INF_F ? 0.f : M));
+    float L = sum * w;
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kMostRowBlocks; ++k) {
+      const float wk = __shfl_sync(0xffffffffu, w, k);
+      acc.x = fmaf(x[k].x, wk, acc.x); acc.y = fmaf(x[k].y, wk, acc.y); acc.z = fmaf(x[k].z, wk, acc.z); acc.w = fmaf(x[k].w, wk, acc.w);
+    }
+    write(r, acc, L);
+  }
+  cluster_sync();  // no block leaves while another reads its rows
+}
+
+// ------------------------------------------------------------------------------------------------------------------------
 // host side
 // ------------------------------------------------------------------------------------------------------------------------
 template <auto Kern, typename Enough>
@@ -1460,6 +1873,50 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
   return plan_tiles(rows, 1, rows, kv_heads, shared_blocks, false);
 }
 
+
+// Blocks of a cluster that share out the keys of a sequence and kv head, for portions of few rows; 0: the tile kernel's case.  By the times above: rounds of blocks
+// over the device, one or two on a multiprocessor, each 5 us ahead of and behind its warps' half pages, two more where a cluster joins.
+int plan_rows(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
+  if (static_cast<long long>(max_seqlen) * (heads / kv_heads) > kMostRows) return 0;
+  const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
+  int cluster = 1;
+  float best = 3.0e38f;
+  for (int n = 1; n <= kMostRowBlocks; n *= 2) {
+    for (int per_sm = 1; per_sm <= 2; ++per_sm) {
+      const float rounds = items * n / static_cast<float>(num_sms() * per_sm), full = static_cast<float>((items * n + num_sms() * per_sm - 1) / (num_sms() * per_sm));
+      const float time = (full > 1.f ? 0.5f * (full + rounds) : 1.f) * (5.f + (n > 1 ? 2.f : 0.f) + (pages / (2.f * n)) * (per_sm == 1 ? 1.05f : 1.45f));
+      if (time >= best) continue;
+      best = time;
+      cluster = n;
+    }
+  }
+  return cluster;
+}
+template <int BITS>
+int run_rows(const RowsParams& p, long long items, void* stream) {
+  using C = RowsCfg<BITS>;
+  static bool done[kMaxDevices] = {};  // of this kernel
+  bool& d = done[device_ordinal()];
+  if (!d) {
+    const int rc = check_cuda(cudaFuncSetAttribute(rows_kernel<BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "paged_tree_attention: clusters of sixteen");
+    if (rc) return rc;
+    d = true;
+  }
+  const int rc = allow_smem<rows_kernel<BITS>>(C::kSmem, "paged_tree_attention: shared memory", [](int) { return true; });
+  if (rc) return rc;
+  QS_REQUIRE(items * p.cluster <= 0x7fffffffll, "paged_tree_attention: %lld blocks", items * p.cluster);
+  return launch(rows_kernel<BITS>, dim3(static_cast<unsigned>(items * p.cluster)), 32 * kTailWarps, C::kSmem, stream, "paged_tree_attention", p.cluster, p);
+}
+int few_rows(const PagedAttnArgs& a, int cluster) {
+  RowsParams p{};
+  p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
+  p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths; p.visible = a.visible; p.words = a.visible_words;
+  p.num_tokens = a.num_tokens; p.max_seqlen = a.max_seqlen; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
+  p.cluster = cluster; p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  const long long items = static_cast<long long>(a.batch) * a.cache.num_kv_heads;
+  return a.cache.int4 ? run_rows<4>(p, items, a.stream) : run_rows<8>(p, items, a.stream);
+}
+
 }  // namespace
 
 size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
@@ -1470,6 +1927,10 @@ size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max
 
 int paged_prompt_attention(const PagedAttnArgs& a) {
   if (a.batch == 0 || a.num_tokens == 0 || a.max_seqlen == 0) return QS_OK;
+  if (a.visible) {
+    const int cluster = plan_rows(a.batch, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
+    if (cluster) return few_rows(a, cluster);
+  }
   const Plan pl = plan_prompt(a.batch, a.num_tokens, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
   TileParams p{};
   p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
