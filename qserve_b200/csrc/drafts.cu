@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kMostDrafted) tree_kernel(int* positions, unsi
 // bits could get wrong is taken again with a sum of 64 bits.  The token that the sequence ends with is drawn with weights and sums of 64 bits: among 10^5 tokens one
 // border or another lies within 32 bits' error of one draw in a hundred.  For that the last row is read once more, out of L2.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 8;
+constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16;
 constexpr int kMostWindow = 8;
 constexpr int kSteps = 32;  // of an octave, in the table of powers of two
 // Words of 16 bytes of a lane: so many are copied to shared memory and taken out of it together, and so many such groups are on their way, 128 KB a multiprocessor.
@@ -833,6 +833,8 @@ int launch_verify(const VerifyParams& p, int batch, void* stream) {
   if (!d) {
     const int rc = check_cuda(cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes), "verify_drafts: shared memory");
     if (rc) return rc;
+    const int rn = check_cuda(cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "verify_drafts: clusters of sixteen");
+    if (rn) return rn;
     d = true;
   }
   return paged::launch(verify_kernel<T>, dim3(static_cast<unsigned>(batch) * p.cluster), kVerifyThreads, kRingBytes, stream, "verify_drafts", p.cluster, p);
@@ -862,7 +864,7 @@ int verify_drafts(const VerifyArgs& a) {
   }
   // Rows of a window: of a chain all, for the slowest sequence of a batch is likely to walk it to the end (64 chains of 6, 128256 tokens: a row at a time 59 us); of a
   // tree, where the first child is one of several, few
-  p.window = a.parents ? 3 : kMostWindow;
+  p.window = a.parents ? 2 : kMostWindow;
   return a.type == 0 ? launch_verify<__half>(p, a.batch, a.stream) : a.type == 1 ? launch_verify<__nv_bfloat16>(p, a.batch, a.stream) : launch_verify<float>(p, a.batch, a.stream);
 }
 
