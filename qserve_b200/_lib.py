@@ -42,6 +42,7 @@ SIGNATURES = {
     # drafted tokens, tokens with places of their own (csrc/drafts.cu and those above)
     "qs_draft_tree": (c_int, [_P, _P, _P, _P, _P, _I, _I, _I, _P]),
     "qs_append_kv_cache_at": (c_int, [_P, _P, _P, _L, _L, _L, _P, _L, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _I, _I, _P]),
+    "qs_paged_tree_attention_workspace_bytes": (c_size_t, [_I, _I, _I, _I, _I, _I]),
     "qs_paged_tree_attention": (c_int, [_P, _L, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _F, _P, _Z, _P]),
     "qs_verify_drafts": (c_int, [_P, _P, _P, _P, _I, _L, _P, _P, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "qs_keep_kv_cache": (c_int, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),

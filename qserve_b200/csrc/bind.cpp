@@ -481,7 +481,7 @@ PyObject* paged_tree_attention(const Args& a) {
   const float scale = scale_of(a, 11);
   const int64_t* const visible = static_cast<const int64_t*>(seen.data_ptr());
   const OnDevice on(qt);
-  const size_t need = qs_paged_prompt_attention_workspace_bytes(c.batch, q.rows, max_seqlen < q.rows ? max_seqlen : q.rows, max_length, q.heads, c.heads_kv);
+  const size_t need = qs_paged_tree_attention_workspace_bytes(c.batch, q.rows, max_seqlen < q.rows ? max_seqlen : q.rows, max_length, q.heads, c.heads_kv);
   at::Tensor ws;
   if (need > 0) ws = scratch(qt, need);
   void* const wp = need > 0 ? ws.data_ptr() : nullptr;

@@ -316,6 +316,10 @@ int qs_paged_prompt_attention(const void* q, int64_t q_stride, void* out, int64_
                           workspace_bytes, stream);
 }
 
+size_t qs_paged_tree_attention_workspace_bytes(int batch, int num_tokens, int max_seqlen, int max_length, int num_heads, int num_kv_heads) {
+  return paged_tree_workspace(batch, num_tokens, max_seqlen, max_length, num_heads, num_kv_heads);
+}
+
 int qs_paged_tree_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
                             const int32_t* lengths, const int64_t* visible, int visible_words, int batch, int num_tokens, int max_seqlen, int max_length,
                             int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token, int int4_kv_cache,
@@ -359,6 +363,7 @@ int qs_verify_drafts(int64_t* out_tokens, int32_t* out_rows, int32_t* out_counts
     QS_REQUIRE(logits && tokens && coins && draws, "%s: null tensor", op);
     QS_REQUIRE((reinterpret_cast<uintptr_t>(logits) & (logits_type == 2 ? 3 : 1)) == 0, "%s: logits must start on a boundary of their type", op);
     QS_REQUIRE(num_tokens == 1 || logits_stride >= vocab, "%s: row stride of logits smaller than the row", op);
+    QS_REQUIRE((reinterpret_cast<uintptr_t>(draft_probs) & 3) == 0, "%s: draft_probs must start on a boundary of its type", op);
     QS_REQUIRE(!draft_probs || num_tokens == 1 || probs_stride >= vocab, "%s: row stride of draft_probs smaller than the row", op);
   }
   VerifyArgs a;

@@ -162,6 +162,7 @@ struct PagedAttnArgs {
   void* stream = nullptr;
 };
 size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads);
+size_t paged_tree_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads);
 int paged_prompt_attention(const PagedAttnArgs& a);
 size_t shared_prefix_workspace(int batch, int shared_blocks, int heads, int kv_heads);
 int shared_prefix_attention(const PagedAttnArgs& a, int shared_blocks);

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   // [128] rows' maximum and sum, for the cluster: over V, at the end.  (Shared memory of their own would leave L1 32 KB less: two blocks' 196 KB are a step of its
   // size.  128 INT8 sequences behind 16384, when it was chosen: 137 us, 158 so)
   float2* s_ml = reinterpret_cast<float2*>(smem + C::kOffV);
-  static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 4 <= 384, "the barriers' place");
+  static_assert((14 + 2 * C::kKStages + 2 * C::kVStages + 2 * C::kSlots) * 8 + 8 <= 384, "the barriers' place");
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // (the shuffle: the same in all lanes, also to the compiler)
   constexpr int kUnpackWarp = C::kSoftmaxWarps, kIssueWarp = kUnpackWarp + 4, kCopyWarp = kIssueWarp + TILES;
@@ -305,6 +305,28 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
   } else {
     const int last = min(n_rows, row_base + TILES * kRows) - 1;
     n_keys = any ? min(max(portion.first + (MASKED ? portion.count : last / group + 1), 0), p.max_blocks * kPage) : 0;
+  }
+  if constexpr (MASKED) {
+    // No further than the last new row that any of the block's rows sees, where that may save a page: half of a long portion's pages, if rows see mostly what lies ahead
+    // (2 x 1500 rows with an image, without context 115 -> 68 us, behind 12001 636 -> 580)
+    if (any && portion.count > kPage) {  // (the same in all threads)
+      int* const s_last = reinterpret_cast<int*>(s_tmem) + 1;
+      if (threadIdx.x == 0) *s_last = -1;
+      __syncthreads();
+      const int tok0 = row_base / group, tok1 = (min(n_rows, row_base + TILES * kRows) - 1) / group + 1;
+      const unsigned long long* const words = p.visible + static_cast<long long>(portion.start + tok0) * p.words;
+      const int many = (portion.count + 63) >> 6;  // words that matter of a row
+      int last = -1;
+      for (int i = threadIdx.x; i < (tok1 - tok0) * many; i += C::kThreads) {
+        const int tok = i / many, w = i - tok * many;
+        const unsigned long long x = __ldcg(words + static_cast<long long>(tok) * p.words + w);
+        if (x) last = max(last, 64 * w + 63 - __clzll(static_cast<long long>(x)));
+      }
+      last = __reduce_max_sync(0xffffffffu, last);
+      if (lane == 0) atomicMax(s_last, last);
+      __syncthreads();
+      n_keys = min(n_keys, max(portion.first + min(*s_last + 1, portion.count), 0));
+    }
   }
   const int n_pages = (n_keys + kPage - 1) / kPage;
   // (nsplit <= 128 splits of at most 2^24 pages: 32 bits hold the products)
@@ -671,13 +693,15 @@ __global__ void __launch_bounds__(TileCfg<BITS, TILES>::kThreads, TileCfg<BITS, 
         if (key0 + kPage - 1 > lowest) {  // warp-uniform
           if constexpr (MASKED) {
             const unsigned long long seen =
-                row_is ? seen_of(p.visible + static_cast<long long>(portion.start + tok) * p.words, p.words, key0 - portion.first, n_keys - key0) : 0ull;
-            const uint32_t half[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
+                row_is ? seen_of(p.visible + static_cast<long long>(portion.start + tok) * p.words, p.words, key0 - portion.first, n_keys - key0) : ~0ull;
+            if (!__all_sync(0xffffffffu, seen == ~0ull)) {
+              const uint32_t half[2] = {static_cast<uint32_t>(seen), static_cast<uint32_t>(seen >> 32)};
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+              for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(half[c] & (1u << i))) x[c][i] = 0xff800000u;  // -inf
+                for (int i = 0; i < 32; ++i)
+                  if (!(half[c] & (1u << i))) x[c][i] = 0xff800000u;  // -inf
+            }
           } else
 #pragma unroll
           for (int c = 0; c < 2; ++c)
@@ -1923,6 +1947,12 @@ size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max
   if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
   const Plan pl = plan_prompt(batch, num_tokens, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads);
   return pl.parts > 1 ? part_bytes(pl.split_rows(static_cast<long long>(num_tokens) * heads), pl.parts) : 0;
+}
+
+size_t paged_tree_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
+  if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
+  if (plan_rows(batch, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads)) return 0;
+  return paged_prompt_workspace(batch, num_tokens, max_seqlen, max_length, heads, kv_heads);
 }
 
 int paged_prompt_attention(const PagedAttnArgs& a) {

@@ -65,7 +65,7 @@ def test_tree_refuses(change):
 
 
 @pytest.mark.parametrize("change", [dict(out=None), dict(rows=None), dict(counts=None), dict(logits=None), dict(logits=A + 1), dict(logits=A + 2, type=2), dict(type=3), dict(type=-1),
-                                    dict(stride=63), dict(tokens=None), dict(probs=A, ps=63), dict(probs=A, ps=64, parents=A), dict(coins=None), dict(draws=None), dict(batch=-1), dict(T=-1),
+                                    dict(stride=63), dict(tokens=None), dict(probs=A, ps=63), dict(probs=A + 2, ps=64), dict(probs=A, ps=64, parents=A), dict(coins=None), dict(draws=None), dict(batch=-1), dict(T=-1),
                                     dict(vocab=0), dict(vocab=-1), dict(vocab=1 << 29), dict(seq=-1), dict(seq=257), dict(batch=1 << 25)], ids=str)
 def test_verify_refuses(change):
     assert verify(**change) == -1
