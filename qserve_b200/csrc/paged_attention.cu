@@ -1391,11 +1391,25 @@ struct RowsParams {
   float scale_log2;
 };
 
-// a product that the compiler may place where it likes: the order of the chains below is then its own
+// products that the compiler may place where it likes: the order of the chains below is then its own
+__device__ __forceinline__ void mma_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void mma_any(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// N runs of 512 bytes, 16 of each by this lane: the even ones to `even`, the odd ones to `odd`
+template <int N, int I = 0>
+__device__ __forceinline__ void copy_runs(uint32_t even, uint32_t odd, const uint8_t* from) {
+  if constexpr (I < N) {
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %2], 16;" ::"r"(I & 1 ? odd : even), "l"(from), "n"(I * 512) : "memory");
+    copy_runs<N, I + 1>(even, odd, from);
+  }
 }
 
 template <int BITS>
@@ -1441,11 +1455,10 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
     const uint8_t* vp = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, vp_l, u & 31));
     const uint32_t dst = ring_at + (u % C::kSlots) * SC::kBytes;
     const long long codes = G::codes_at(hk) + half * SC::kCodes + lane * 16;
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int i = 0; i < SC::kCodes / 512; ++i)
-        cp_async16(dst + w * SC::kOffV + i * 512 + (BITS == 8 && (i & 1) ? lane_at ^ 16u : lane_at), (w ? vp : kp) + codes + i * 512);
+    const uint8_t *k_from = kp + codes, *v_from = vp + codes;
+    const uint32_t even = dst + lane_at, odd = BITS == 8 ? dst + (lane_at ^ 16u) : even;
+    copy_runs<SC::kCodes / 512>(even, odd, k_from);
+    copy_runs<SC::kCodes / 512>(even + SC::kOffV, odd + SC::kOffV, v_from);
     if (lane < 16) {
       const uint8_t* page_at = lane < 8 ? kp : vp;
       const long long meta = (lane & 4) ? G::zeros_at(hk, p.num_kv_heads) : G::scales_at(hk, p.num_kv_heads);
@@ -1546,21 +1559,23 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
         const uint4 k = *reinterpret_cast<const uint4*>(st + j * 8 * SC::kRow + (k_at ^ (16u * h)));
         words[j][4 * h] = k.x; words[j][4 * h + 1] = k.y; words[j][4 * h + 2] = k.z; words[j][4 * h + 3] = k.w;
       }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sc[j][e] = hi[j][e] = 0.f;
     }
+    auto product = [](bool first, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+      if (first) mma_new(d, a0, a1, a2, a3, b0, b1);
+      else mma_any(d, a0, a1, a2, a3, b0, b1);
+    };
 #pragma unroll
     for (int w = 0; w < 4; ++w)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (BITS == 4) {
           const uint32_t x = words[j][w], y = x >> 8;
-          mma_any(sc[j], qa[0][2 * w], qa[1][2 * w], qa[0][2 * w + 1], qa[1][2 * w + 1], x & 0x000f000fu, y & 0x000f000fu);
-          mma_any(hi[j], qh[0][2 * w], qh[1][2 * w], qh[0][2 * w + 1], qh[1][2 * w + 1], x & 0x00f000f0u, y & 0x00f000f0u);
+          product(w == 0, sc[j], qa[0][2 * w], qa[1][2 * w], qa[0][2 * w + 1], qa[1][2 * w + 1], x & 0x000f000fu, y & 0x000f000fu);
+          product(w == 0, hi[j], qh[0][2 * w], qh[1][2 * w], qh[0][2 * w + 1], qh[1][2 * w + 1], x & 0x00f000f0u, y & 0x00f000f0u);
         } else {
           const uint32_t x = words[j][2 * w], y = words[j][2 * w + 1];
-          mma_any(sc[j], qa[0][2 * w], qa[1][2 * w], qh[0][2 * w], qh[1][2 * w], __byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342));
-          mma_any(hi[j], qa[0][2 * w + 1], qa[1][2 * w + 1], qh[0][2 * w + 1], qh[1][2 * w + 1], __byte_perm(y, 0u, 0x4140), __byte_perm(y, 0u, 0x4342));
+          product(w == 0, sc[j], qa[0][2 * w], qa[1][2 * w], qh[0][2 * w], qh[1][2 * w], __byte_perm(x, 0u, 0x4140), __byte_perm(x, 0u, 0x4342));
+          product(w == 0, hi[j], qa[0][2 * w + 1], qa[1][2 * w + 1], qh[0][2 * w + 1], qh[1][2 * w + 1], __byte_perm(y, 0u, 0x4140), __byte_perm(y, 0u, 0x4342));
         }
       }
 #pragma unroll
@@ -1580,8 +1595,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
         sc[j][2 * e + 1] = fmaf(km.z, sc[j][2 * e + 1], km.w * sumq[e]);
       }
     }
-    const bool masked = t0 + kSlice > min(portion.first, n_keys);  // the same in all lanes
-    if (masked) {
+    if (t0 + kSlice > min(portion.first, n_keys)) {  // new rows, or the end: the same in all lanes
       const int at = t0 - portion.first, left = n_keys - t0;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -1592,9 +1606,17 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
         const uint32_t seen = static_cast<uint32_t>(w) >> q4;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
+          // a value that is no number makes the rows none that see it, and is nothing to the others
           if (!(seen >> (8 * j) & 1u)) sc[j][2 * e] = -CUDART_INF_F;
+          else l[e] = fmaf(vm[j].x, 0.f, l[e]);
           if (!(seen >> (8 * j + 4) & 1u)) sc[j][2 * e + 1] = -CUDART_INF_F;
+          else l[e] = fmaf(vm[j].z, 0.f, l[e]);
         }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!(vm[j].x == vm[j].x)) vm[j].x = vm[j].y = 0.f;
+        if (!(vm[j].z == vm[j].z)) vm[j].z = vm[j].w = 0.f;
       }
     }
     // The weights are 2^up times those against the maximum, as in the tail kernel; a row that has seen no key so far: against 0
@@ -1627,27 +1649,19 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
         }
       }
     }
-    uint32_t pa[4][2];  // weights times scales, rounded to fp16: the next products' operand
+    uint32_t pa[4][2], pr[4][2];  // weights times scales as two fp16 numbers, the second what the first's rounding left: the next products' operands
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const float p0 = ex2(sc[j][2 * e] - ref[e]), p1 = ex2(sc[j][2 * e + 1] - ref[e]);
         l[e] += p0 + p1;
-        float w0 = p0 * vm[j].x, w1 = p1 * vm[j].z;
-        if (masked) {  // a value that is no number is nothing to a row that does not see it
-          w0 = p0 == 0.f ? 0.f : w0;
-          w1 = p1 == 0.f ? 0.f : w1;
-        }
+        const float w0 = p0 * vm[j].x, w1 = p1 * vm[j].z;
         const __half2 w = __floats2half2_rn(w0, w1);
         pa[j][e] = as_u32(w);
         const float2 f = __half22float2(w);
-        if (masked) {
-          if (p0 != 0.f) cv[e] = fmaf(f.x, vm[j].y, cv[e]);
-          if (p1 != 0.f) cv[e] = fmaf(f.y, vm[j].w, cv[e]);
-        } else {
-          cv[e] = fmaf(f.x, vm[j].y, fmaf(f.y, vm[j].w, cv[e]));
-        }
+        pr[j][e] = as_u32(__floats2half2_rn(w0 - f.x, w1 - f.y));
+        cv[e] = fmaf(w0, vm[j].y, fmaf(w1, vm[j].w, cv[e]));
       }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -1661,14 +1675,19 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
           if constexpr (BITS == 4) {
             const int i = 8 * h + 4 * e;
             const uint32_t x8 = x >> 8, y8 = y >> 8;
-            mma_any(o[i], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x & 0x000f000fu, y & 0x000f000fu);
-            mma_any(o[i + 1], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x & 0x00f000f0u, y & 0x00f000f0u);
-            mma_any(o[i + 2], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x8 & 0x000f000fu, y8 & 0x000f000fu);
-            mma_any(o[i + 3], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], x8 & 0x00f000f0u, y8 & 0x00f000f0u);
+            const uint32_t first[4] = {x & 0x000f000fu, x & 0x00f000f0u, x8 & 0x000f000fu, x8 & 0x00f000f0u};
+            const uint32_t second[4] = {y & 0x000f000fu, y & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_any(o[i + k], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], first[k], second[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) mma_any(o[i + k], pr[2 * c][0], pr[2 * c][1], pr[2 * c + 1][0], pr[2 * c + 1][1], first[k], second[k]);
           } else {
             const int i = 4 * h + 2 * e;
-            mma_any(o[i], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], __byte_perm(x, 0u, 0x4240), __byte_perm(y, 0u, 0x4240));
-            mma_any(o[i + 1], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], __byte_perm(x, 0u, 0x4341), __byte_perm(y, 0u, 0x4341));
+            const uint32_t first[2] = {__byte_perm(x, 0u, 0x4240), __byte_perm(x, 0u, 0x4341)}, second[2] = {__byte_perm(y, 0u, 0x4240), __byte_perm(y, 0u, 0x4341)};
+#pragma unroll
+            for (int k = 0; k < 2; ++k) mma_any(o[i + k], pa[2 * c][0], pa[2 * c][1], pa[2 * c + 1][0], pa[2 * c + 1][1], first[k], second[k]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) mma_any(o[i + k], pr[2 * c][0], pr[2 * c][1], pr[2 * c + 1][0], pr[2 * c + 1][1], first[k], second[k]);
           }
         }
       }
