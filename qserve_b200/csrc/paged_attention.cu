@@ -1365,9 +1365,10 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
 // Up to 16 rows (token, head of the group) of a kv head.  Codes go into the products as they lie, as in the tail kernel, but as their second operand: the rows are the
 // first one's 16, and a product's scores are the next one's operand as they are.  A block's warps take turns over half pages, a cluster of blocks over their runs.
 // A warp takes 1.0 us for a half page, 1.45 where two blocks share a multiprocessor (registers hold no third: with 168 a thread the code takes 1.4 times as long), of
-// which products are a quarter: one chain of copies - scales - scores - weights - values.  Against the tile kernel, whose products are for 128 rows and whose pages are
-// unpacked first, us: 18 sequences of 4 rows of 32 heads over 8 behind 3000, INT4, 25.5 and 50; 37 43 and 72; 32 of 8 rows, 32 heads over 32, behind 1000 to 2000, INT8,
-// 92 and 166; error 2.9e-4 and 4.5e-4.  With 16 rows more a warp, or warps that share half pages, for up to 64 rows: 131 where the tile kernel takes 64.
+// which products are a third: one chain of copies - scales - scores - weights - values.  Weights go into the products as two fp16 numbers, so that results are off by their
+// own rounding alone (2.1e-4; with one number 2.9e-4, for 5 % of the time; tile kernel 4.5e-4).  Against the tile kernel, whose products are for 128 rows and whose
+// pages are unpacked first, us: 18 sequences of 4 rows of 32 heads over 8 behind 3000, INT4, 29 and 49; 37 47 and 70; 32 of 8 rows, 32 heads over 32, behind 1000 to
+// 2000, INT8, 96 and 165.  Warps that share half pages, for up to 64 rows: 131 where the tile kernel takes 64.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int kMostRows = 16, kMostRowBlocks = 16;
 
@@ -1918,10 +1919,12 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 
 
 // Blocks of a cluster that share out the keys of a sequence and kv head, for portions of few rows; 0: the tile kernel's case.  By the times above: rounds of blocks
-// over the device, one or two on a multiprocessor, each 5 us ahead of and behind its warps' half pages, two more where a cluster joins.
+// over the device, one or two on a multiprocessor, each 5 us ahead of and behind its warps' half pages, two more where a cluster joins.  (INT4, 32 heads over 8, us, of
+// one, two, four, eight, sixteen blocks: 16000 positions 135, 73, 40, 25, 19; 8 sequences of 8000 74, 53, 32, 30, 49; 64 of 3000 75, 83, 99, 148, 290.)  Few long
+// sequences are the tile kernel's, which cuts their keys into more than sixteen: 100000 positions 68 and 85 us, 2 x 60000 78 and 84; 4 x 30000 88 and 56.
 int plan_rows(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
-  if (static_cast<long long>(max_seqlen) * (heads / kv_heads) > kMostRows) return 0;
   const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
+  if (static_cast<long long>(max_seqlen) * (heads / kv_heads) > kMostRows || (items <= 16 && pages > 512)) return 0;
   int cluster = 1;
   float best = 3.0e38f;
   for (int n = 1; n <= kMostRowBlocks; n *= 2) {

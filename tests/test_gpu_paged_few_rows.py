@@ -159,5 +159,7 @@ def test_graphs_and_streams(dev):
 def test_no_work_space_is_needed(dev):
     from qserve_b200._lib import lib
     need = lib.qs_paged_tree_attention_workspace_bytes
-    assert need(1, 4, 4, 60000, 32, 8) == 0 and need(1, 16, 16, 60000, 8, 8) == 0 and need(0, 4, 4, 100, 32, 8) == 0 and need(2, 4, 0, 100, 32, 8) == 0
-    assert need(1, 24, 24, 60000, 32, 8) == lib.qs_paged_prompt_attention_workspace_bytes(1, 24, 24, 60000, 32, 8) > 0
+    assert need(1, 4, 4, 30000, 32, 8) == 0 and need(8, 32, 4, 60000, 32, 8) == 0 and need(0, 4, 4, 100, 32, 8) == 0 and need(2, 4, 0, 100, 32, 8) == 0
+    # more rows, and few rows of few long sequences: the prompt operator's
+    for a in ((1, 24, 24, 60000, 32, 8), (1, 4, 4, 60000, 32, 8)):
+        assert need(*a) == lib.qs_paged_prompt_attention_workspace_bytes(*a) > 0
