@@ -1924,10 +1924,11 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 // sequences are the tile kernel's, which cuts their keys into more than sixteen: 100000 positions 68 and 85 us, 2 x 60000 78 and 84; 4 x 30000 88 and 56.
 int plan_rows(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
   const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
-  if (static_cast<long long>(max_seqlen) * (heads / kv_heads) > kMostRows || (items <= 16 && pages > 512)) return 0;
+  const int most = items <= 8 ? kMostRowBlocks : kMostRowBlocks / 2;  // (of sixteen, eight find a place: 2 x 2000 positions 16.3 us, of eight 10.5)
+  if (static_cast<long long>(max_seqlen) * (heads / kv_heads) > kMostRows || (items <= 16 && pages > 32 * most)) return 0;
   int cluster = 1;
   float best = 3.0e38f;
-  for (int n = 1; n <= (items <= 8 ? kMostRowBlocks : kMostRowBlocks / 2); n *= 2) {  // (of sixteen, eight find a place: 2 x 2000 positions 16.3 us, of eight 10.5)
+  for (int n = 1; n <= most; n *= 2) {
     for (int per_sm = 1; per_sm <= 2; ++per_sm) {
       const float rounds = items * n / static_cast<float>(num_sms() * per_sm), full = static_cast<float>((items * n + num_sms() * per_sm - 1) / (num_sms() * per_sm));
       const float time = (full > 1.f ? 0.5f * (full + rounds) : 1.f) * (5.f + (n > 1 ? 2.f : 0.f) + (pages / (2.f * n)) * (per_sm == 1 ? 1.05f : 1.45f));
