@@ -278,7 +278,7 @@ __device__ __noinline__ Shares shares_of(const T* p, int vocab, int w0, int w1, 
         }
       } else {
 #pragma unroll
-        for (int k = 0; k < kN; ++k) of_q[k] = __ldg(from + k);
+        for (int k = 0; k < kN; ++k) of_q[k] = __ldcg(from + k);
       }
     }
   };
@@ -339,6 +339,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     }
     return;
   }
+  // (none writes to another block's shared memory before that has started: the wait for this comes ahead of the first exchange)
+  if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   const T* const logits = static_cast<const T*>(p.logits) + static_cast<long long>(start) * p.logits_stride;
   const float* const probs = p.probs ? p.probs + static_cast<long long>(start) * p.probs_stride : nullptr;
   const bool chain = p.parents == nullptr;
@@ -393,6 +395,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   Weigh weigh{inverse * (kSteps * 1.4426950408889634), 16384.0 / (inverse * (kSteps * 1.4426950408889634)), 0.0, smem_u32(s_power), 0.f, false};
 
   int node = 0, accepted = 0;
+  bool met = p.cluster == 1;
   float top = 0.f;     // of the current row
   double total = 0.0;  //   its sum, of 32 bits or of 64
   // sums over the cluster's warps: their shares stay in s_share, the blocks' in s_shares of the turn before
@@ -635,6 +638,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       s_again[tid] = again;
     }
     __syncthreads();
+    if (!met) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    met = true;
     auto parts_of = [&](const uint2* parts, int many, float& m, float& s, int& word) {
       const uint2 mine = lane < many ? parts[lane] : make_uint2(0xff800000u, 0u);
       m = __uint_as_float(mine.x);
@@ -850,7 +855,7 @@ int draft_tree(int* positions, long long* visible, const int* parents, const int
 }
 
 int verify_drafts(const VerifyArgs& a) {
-  if (a.batch == 0 || a.max_seqlen == 0) return QS_OK;
+  if (a.batch == 0) return QS_OK;
   VerifyParams p{};
   p.logits = a.logits; p.logits_stride = a.logits_stride; p.probs_stride = a.probs_stride; p.tokens = a.tokens; p.parents = a.parents; p.probs = a.probs; p.cu = a.cu_seqlens;
   p.coins = a.coins; p.draws = a.draws; p.temperatures = a.temperatures; p.out_tokens = a.out_tokens; p.out_rows = a.out_rows; p.out_counts = a.out_counts;

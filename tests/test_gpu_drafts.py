@@ -254,6 +254,9 @@ def test_empty_calls(dev):
         tokens, rows, counts = backend.verify_drafts(torch.zeros(T, 64, device=dev), torch.zeros(T, dtype=torch.int64, device=dev), torch.zeros(B + 1, dtype=torch.int32, device=dev), 2, none,
                                                      torch.zeros(B, device=dev))
         assert tokens.tolist() == [[-1, -1]] * B and rows.tolist() == [[-1, -1]] * B and counts.tolist() == [0] * B
+    x = inputs(dev, torch.float16, 64, [3, 2], "none", seed=1)
+    tokens, rows, counts = call(x, top=0)  # no row is looked at
+    assert tokens.shape == (2, 0) and rows.shape == (2, 0) and counts.tolist() == [0, 0]
     positions, visible = backend.draft_tree(torch.zeros(0, dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev), torch.zeros(0, dtype=torch.int32, device=dev), 0)
     assert positions.shape == (0,) and visible.shape == (0, 0)
 
