@@ -772,7 +772,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       double w[kN], mine = 0.0;
       auto weights_of = [&](int c) {
         const int first = c * kN - row.skip;
-        float x[kN];
+        float x[kN], qs[kN];  // (all of q's on their way with the word)
+#pragma unroll
+        for (int k = 0; k < kN; ++k) qs[k] = q && first + k >= 0 && first + k < p.vocab ? __ldcg(q + first + k) : 0.f;
         numbers_of<T>(row.word(c), x);
         if (weigh.odd) {
 #pragma unroll
@@ -789,7 +791,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
         }
         if (q && !from_p) {
 #pragma unroll
-          for (int k = 0; k < kN; ++k) w[k] = w[k] > 0.0 ? fmax(fma(-sum, static_cast<double>(q[first + k]), w[k]), 0.0) : 0.0;
+          for (int k = 0; k < kN; ++k) w[k] = w[k] > 0.0 ? fmax(fma(-sum, static_cast<double>(qs[k]), w[k]), 0.0) : 0.0;
         }
       };
       for (int c = c0; c < c1; ++c) {
