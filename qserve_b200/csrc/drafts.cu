@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kMostDrafted) tree_kernel(int* positions, unsi
 // bits could get wrong is taken again with a sum of 64 bits.  The token that the sequence ends with is drawn with weights and sums of 64 bits: among 10^5 tokens one
 // border or another lies within 32 bits' error of one draw in a hundred.  For that the last row is read once more, out of L2.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16;
+constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16, kLog2Warps = 4, kLog2Blocks = 4;
 constexpr int kMostWindow = 8;
 constexpr int kSteps = 32;  // of an octave, in the table of powers of two
 // Words of 16 bytes of a lane: so many are copied to shared memory and taken out of it together, and so many such groups are on their way, 128 KB a multiprocessor.
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   const bool chain = p.parents == nullptr;
   const int my_warp = rank * kVerifyWarps + warp;
   auto row_at = [&](int r) { return Row<T>(logits + r * p.logits_stride, p.vocab); };
-  const int log2_blocks = p.log2_warps - 4;
-  static_assert(kVerifyWarps == 16, "");
+  const int log2_blocks = p.log2_warps - kLog2Warps;
+  static_assert(kVerifyWarps == 1 << kLog2Warps && kMostBlocks == 1 << kLog2Blocks, "");
   auto begin_of_block = [&](const Row<T>& row, int r) { return static_cast<int>((static_cast<long long>(row.words) * r) >> log2_blocks); };
   // a warp's words of a row, where each row is shared out over the warps
   auto begin_of = [&](const Row<T>& row, int w) { return static_cast<int>((static_cast<long long>(row.words) * w) >> p.log2_warps); };
@@ -834,16 +834,25 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
 }
 
 template <typename T>
-int launch_verify(const VerifyParams& p, int batch, void* stream) {
-  static bool done[kMaxDevices] = {};  // of this type
-  bool& d = done[device_ordinal()];
-  if (!d) {
+int launch_verify(VerifyParams p, int batch, void* stream) {
+  static std::atomic<bool> done[kMaxDevices] = {};  // of this type
+  std::atomic<bool>& d = done[device_ordinal()];
+  if (!d.load(std::memory_order_relaxed)) {
     const int rc = check_cuda(cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes), "verify_drafts: shared memory");
     if (rc) return rc;
     const int rn = check_cuda(cudaFuncSetAttribute(verify_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "verify_drafts: clusters of sixteen");
     if (rn) return rn;
-    d = true;
+    d.store(true, std::memory_order_relaxed);
   }
+  // Blocks of a sequence: as many as find places for all sequences at once.  (Of sixteen, eight and four blocks 7, 15 and 32 clusters do, where 148 / 16 is 9.  Sequences
+  // that wait for the first ones' places, and fewer blocks: 8 chains of 5, 128256 tokens, 31.0 us and 21.4; 16 of them 36.5 and 28.9; 36 47.4 and 41.2.)
+  static std::atomic<int> held[kMaxDevices][kLog2Blocks + 1] = {};
+  int log2_blocks = kLog2Blocks;
+  while (log2_blocks > 0 &&
+         paged::clusters_at_once(held[device_ordinal()][log2_blocks], verify_kernel<T>, kVerifyThreads, kRingBytes, 1 << log2_blocks) < batch)
+    --log2_blocks;
+  p.cluster = 1 << log2_blocks;
+  p.log2_warps = kLog2Warps + log2_blocks;
   return paged::launch(verify_kernel<T>, dim3(static_cast<unsigned>(batch) * p.cluster), kVerifyThreads, kRingBytes, stream, "verify_drafts", p.cluster, p);
 }
 
@@ -862,13 +871,6 @@ int verify_drafts(const VerifyArgs& a) {
   p.logits = a.logits; p.logits_stride = a.logits_stride; p.probs_stride = a.probs_stride; p.tokens = a.tokens; p.parents = a.parents; p.probs = a.probs; p.cu = a.cu_seqlens;
   p.coins = a.coins; p.draws = a.draws; p.temperatures = a.temperatures; p.out_tokens = a.out_tokens; p.out_rows = a.out_rows; p.out_counts = a.out_counts;
   p.num_tokens = a.num_tokens; p.vocab = a.vocab; p.max_seqlen = a.max_seqlen;
-  // Blocks of a sequence: as many as fill the device in one round
-  p.cluster = 1;
-  p.log2_warps = 4;
-  while (p.cluster < kMostBlocks && static_cast<long long>(a.batch) * p.cluster * 2 <= num_sms()) {
-    p.cluster *= 2;
-    ++p.log2_warps;
-  }
   // Rows of a window: of a chain all, for the slowest sequence of a batch is likely to walk it to the end (64 chains of 6, 128256 tokens: a row at a time 59 us); of a
   // tree, where the first child is one of several, few
   p.window = a.parents ? 2 : kMostWindow;

@@ -3,6 +3,8 @@
 // A page holds 64 positions of all kv heads: codes [Hkv][64][128 * BITS / 8] | scales fp16 [Hkv][64] | zeros fp16 [Hkv][64].  INT4: the even element of a byte
 // in its low nibble.  Code u of a row with scale s and zero z stands for s u + half(-s z) (INT4), s (u - z) (INT8).
 #pragma once
+#include <atomic>
+
 #include "common.cuh"
 #include "launch.h"
 
@@ -84,6 +86,30 @@ int launch(Kern kern, dim3 grid, int threads, size_t smem, void* stream, const c
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
+}
+
+// Clusters of that many blocks that the current device runs at once: fewer than its multiprocessors would hold, for a cluster lies within one group of them.
+// `held` is the caller's, of this kernel, size and device; 0: not asked yet.
+template <typename Kern>
+int clusters_at_once(std::atomic<int>& held, Kern kern, int threads, size_t smem, int cluster) {
+  int n = held.load(std::memory_order_relaxed);
+  if (n > 0) return n;
+  cudaLaunchAttribute size;
+  size.id = cudaLaunchAttributeClusterDimension;
+  size.val.clusterDim.x = cluster;
+  size.val.clusterDim.y = size.val.clusterDim.z = 1;
+  cudaLaunchConfig_t ask{};
+  ask.gridDim = dim3(cluster);
+  ask.blockDim = dim3(threads);
+  ask.dynamicSmemBytes = smem;
+  ask.attrs = &size;
+  ask.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &ask) != cudaSuccess || n <= 0) {
+    cudaGetLastError();
+    n = num_sms() / cluster > 0 ? num_sms() / cluster : 1;
+  }
+  held.store(n, std::memory_order_relaxed);
+  return n;
 }
 
 }  // namespace paged
