@@ -1370,7 +1370,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
 // pages are unpacked first, us: 18 sequences of 4 rows of 32 heads over 8 behind 3000, INT4, 29 and 49; 37 47 and 70; 32 of 8 rows, 32 heads over 32, behind 1000 to
 // 2000, INT8, 96 and 165.  Warps that share half pages, for up to 64 rows: 131 where the tile kernel takes 64.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kMostRows = 16, kMostRowBlocks = 16;
+constexpr int kMostRows = 16, kLog2RowBlocks = 4, kMostRowBlocks = 1 << kLog2RowBlocks;
 
 template <int BITS>
 struct RowsCfg {
@@ -1918,50 +1918,59 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 }
 
 
-// Blocks of a cluster that share out the keys of a sequence and kv head, for portions of few rows; 0: the tile kernel's case.  By the times above: rounds of blocks
-// over the device, one or two on a multiprocessor, each 5 us ahead of and behind its warps' half pages, two more where a cluster joins.  (INT4, 32 heads over 8, us, of
-// one, two, four, eight, sixteen blocks: 16000 positions 135, 73, 40, 25, 19; 8 sequences of 8000 74, 53, 32, 30, 49; 64 of 3000 75, 83, 99, 148, 290.)  Few long
-// sequences are the tile kernel's, which cuts their keys into more than sixteen: 100000 positions 68 and 85 us, 2 x 60000 78 and 84; 4 x 30000 88 and 56.
-int plan_rows(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
+// Portions of few rows are the rows kernel's.  Few long sequences are the tile kernel's even so, which cuts their keys into more parts than a cluster has blocks:
+// 100000 positions 68 and 85 us, 2 x 60000 78 and 84; 4 x 30000 88 and 56.
+bool rows_few(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
   const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
-  const int most = items <= 8 ? kMostRowBlocks : kMostRowBlocks / 2;  // (of sixteen, eight find a place: 2 x 2000 positions 16.3 us, of eight 10.5)
-  if (static_cast<long long>(max_seqlen) * (heads / kv_heads) > kMostRows || (items <= 16 && pages > 32 * most)) return 0;
-  int cluster = 1;
+  return static_cast<long long>(max_seqlen) * (heads / kv_heads) <= kMostRows && !(items <= 16 && pages > 16 * (items <= 8 ? 32 : 16));
+}
+// Blocks of a cluster that share out the keys of a sequence and kv head, of one to sixteen: rounds of as many clusters as run at once (places[log2 blocks], two blocks
+// on a multiprocessor), a warp's half pages one after the other, 5 us ahead of and behind them, a cluster's join.  (INT4, 32 heads over 8, us, of one, two, four, eight,
+// sixteen blocks: one sequence of 500 positions 8.3, 8.2, 6.9, 6.9, 7.7; 9 of them 10.1, 9.5, 13.0, 20.6 (72 clusters of four find no place at once); one of 8000 71,
+// 41, 23, 16, 13; 8 of 8000 89, 56, 33, 39; 64 of 2000 63, 74, 93, 146.)
+int rows_log2_blocks(const int (&places)[kLog2RowBlocks + 1], long long items, int max_length) {
+  const long long halves = 2 * ((static_cast<long long>(max_length) + kPage - 1) / kPage);
+  int chosen = 0;
   float best = 3.0e38f;
-  for (int n = 1; n <= most; n *= 2) {
+  for (int l = 0; l <= kLog2RowBlocks; ++l) {
+    const int n = 1 << l, warps = kTailWarps * n;
     for (int per_sm = 1; per_sm <= 2; ++per_sm) {
-      const float rounds = items * n / static_cast<float>(num_sms() * per_sm), full = static_cast<float>((items * n + num_sms() * per_sm - 1) / (num_sms() * per_sm));
-      const float time = (full > 1.f ? 0.5f * (full + rounds) : 1.f) * (5.f + (n > 1 ? 2.f : 0.f) + (pages / (2.f * n)) * (per_sm == 1 ? 1.05f : 1.45f));
+      const float room = fmaxf(1.f, 0.5f * per_sm * places[l]), rounds = items / room, full = ceilf(rounds);
+      const float time = (0.75f * full + 0.25f * fmaxf(rounds, 1.f)) * (5.f + (n > 1 ? 1.f + 0.2f * n : 0.f) + (halves + warps - 1) / warps * (per_sm == 1 ? 1.05f : 1.45f));
       if (time >= best) continue;
       best = time;
-      cluster = n;
+      chosen = l;
     }
   }
-  return cluster;
+  return chosen;
 }
 template <int BITS>
-int run_rows(const RowsParams& p, long long items, void* stream) {
+int run_rows(RowsParams& p, long long items, int max_length, void* stream) {
   using C = RowsCfg<BITS>;
-  static bool done[kMaxDevices] = {};  // of this kernel
-  bool& d = done[device_ordinal()];
-  if (!d) {
+  static std::atomic<bool> done[kMaxDevices] = {};  // of this kernel
+  static std::atomic<int> held[kMaxDevices][kLog2RowBlocks + 1] = {};
+  const int dev = device_ordinal();
+  if (!done[dev].load(std::memory_order_relaxed)) {
     const int rc = check_cuda(cudaFuncSetAttribute(rows_kernel<BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "paged_tree_attention: clusters of sixteen");
     if (rc) return rc;
-    d = true;
+    done[dev].store(true, std::memory_order_relaxed);
   }
   const int rc = allow_smem<rows_kernel<BITS>>(C::kSmem, "paged_tree_attention: shared memory", [](int) { return true; });
   if (rc) return rc;
+  int places[kLog2RowBlocks + 1];
+  for (int l = 0; l <= kLog2RowBlocks; ++l) places[l] = clusters_at_once(held[dev][l], rows_kernel<BITS>, 32 * kTailWarps, C::kSmem, 1 << l);
+  p.cluster = 1 << rows_log2_blocks(places, items, max_length);
   QS_REQUIRE(items * p.cluster <= 0x7fffffffll, "paged_tree_attention: %lld blocks", items * p.cluster);
   return launch(rows_kernel<BITS>, dim3(static_cast<unsigned>(items * p.cluster)), 32 * kTailWarps, C::kSmem, stream, "paged_tree_attention", p.cluster, p);
 }
-int few_rows(const PagedAttnArgs& a, int cluster) {
+int few_rows(const PagedAttnArgs& a) {
   RowsParams p{};
   p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths; p.visible = a.visible; p.words = a.visible_words;
   p.num_tokens = a.num_tokens; p.max_seqlen = a.max_seqlen; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
-  p.cluster = cluster; p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
+  p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
   const long long items = static_cast<long long>(a.batch) * a.cache.num_kv_heads;
-  return a.cache.int4 ? run_rows<4>(p, items, a.stream) : run_rows<8>(p, items, a.stream);
+  return a.cache.int4 ? run_rows<4>(p, items, a.max_length, a.stream) : run_rows<8>(p, items, a.max_length, a.stream);
 }
 
 }  // namespace
@@ -1974,16 +1983,13 @@ size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max
 
 size_t paged_tree_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
   if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  if (plan_rows(batch, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads)) return 0;
+  if (rows_few(batch, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads)) return 0;
   return paged_prompt_workspace(batch, num_tokens, max_seqlen, max_length, heads, kv_heads);
 }
 
 int paged_prompt_attention(const PagedAttnArgs& a) {
   if (a.batch == 0 || a.num_tokens == 0 || a.max_seqlen == 0) return QS_OK;
-  if (a.visible) {
-    const int cluster = plan_rows(a.batch, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
-    if (cluster) return few_rows(a, cluster);
-  }
+  if (a.visible && rows_few(a.batch, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads)) return few_rows(a);
   const Plan pl = plan_prompt(a.batch, a.num_tokens, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
   TileParams p{};
   p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
