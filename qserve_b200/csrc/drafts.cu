@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kMostDrafted) tree_kernel(int* positions, unsi
 // bits could get wrong is taken again with a sum of 64 bits.  The token that the sequence ends with is drawn with weights and sums of 64 bits: among 10^5 tokens one
 // border or another lies within 32 bits' error of one draw in a hundred.  For that the last row is read once more, out of L2.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16, kLog2Warps = 4, kLog2Blocks = 4;
+constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16;
 constexpr int kMostWindow = 8;
 constexpr int kSteps = 32;  // of an octave, in the table of powers of two
 // Words of 16 bytes of a lane: so many are copied to shared memory and taken out of it together, and so many such groups are on their way, 128 KB a multiprocessor.
@@ -154,7 +154,7 @@ struct VerifyParams {
   const float *coins, *draws, *temperatures;
   long long* out_tokens;
   int *out_rows, *out_counts;
-  int num_tokens, vocab, max_seqlen, cluster, log2_warps, window;  // log2_warps: of the cluster
+  int num_tokens, vocab, max_seqlen, cluster, per_block, per_warp, window;  // per_block: a row's words of each block of the cluster, of each of its warps; the last ones' are fewer
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -321,7 +321,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   __shared__ int s_next[kMostWindow], s_largest[kMostWindow], s_num_kids, s_last;
   __shared__ float2 s_top[kMostWindow];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tid = threadIdx.x;
-  const int rank = static_cast<int>(blockIdx.x) & (p.cluster - 1), b = static_cast<int>(blockIdx.x) / p.cluster;
+  const int b = static_cast<int>(blockIdx.x) / p.cluster, rank = static_cast<int>(blockIdx.x) - b * p.cluster;
   pdl_launch_dependents();
   pdl_wait();
   const int lo = p.cu ? p.cu[b] : b, hi = p.cu ? p.cu[b + 1] : b + 1;
@@ -346,11 +346,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   const bool chain = p.parents == nullptr;
   const int my_warp = rank * kVerifyWarps + warp;
   auto row_at = [&](int r) { return Row<T>(logits + r * p.logits_stride, p.vocab); };
-  const int log2_blocks = p.log2_warps - kLog2Warps;
-  static_assert(kVerifyWarps == 1 << kLog2Warps && kMostBlocks == 1 << kLog2Blocks, "");
-  auto begin_of_block = [&](const Row<T>& row, int r) { return static_cast<int>((static_cast<long long>(row.words) * r) >> log2_blocks); };
+  auto begin_of_block = [&](const Row<T>& row, int r) { return min(row.words, p.per_block * r); };
   // a warp's words of a row, where each row is shared out over the warps
-  auto begin_of = [&](const Row<T>& row, int w) { return static_cast<int>((static_cast<long long>(row.words) * w) >> p.log2_warps); };
+  auto begin_of = [&](const Row<T>& row, int w) { return min(row.words, p.per_warp * w); };
   auto first_child = [&](int r) { return chain ? r + 1 : s_first[r]; };  // n or more: none
   auto meet = [&] {  // of the cluster
     if (p.cluster > 1) {
@@ -499,7 +497,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     if (warp < count && lane == 0) s_part[warp][kVerifyWarps] = make_uint2(0xff800000u, greedy ? 0x7fffffffu : 0u);
     __syncwarp();
     // (of a row where words begin at another of its numbers than in the next, a group may be empty)
-    const int per_row = (((p.vocab + 2 * kN) / kN >> log2_blocks) + 1 + 32 * kGroup) / (32 * kGroup), groups = count * per_row;
+    const int per_row = (p.per_block + 32 * kGroup - 1) / (32 * kGroup), groups = count * per_row;
     const int group0 = groups * warp / kVerifyWarps, group1 = groups * (warp + 1) / kVerifyWarps;
     struct Place {
       int k, in_row, word, end;  // row of the window, group of the row; this lane's first word of the group and the end of the block's
@@ -846,13 +844,13 @@ int launch_verify(VerifyParams p, int batch, void* stream) {
   }
   // Blocks of a sequence: as many as find places for all sequences at once.  (Of sixteen, eight and four blocks 7, 15 and 32 clusters do, where 148 / 16 is 9.  Sequences
   // that wait for the first ones' places, and fewer blocks: 8 chains of 5, 128256 tokens, 31.0 us and 21.4; 16 of them 36.5 and 28.9; 36 47.4 and 41.2.)
-  static std::atomic<int> held[kMaxDevices][kLog2Blocks + 1] = {};
-  int log2_blocks = kLog2Blocks;
-  while (log2_blocks > 0 &&
-         paged::clusters_at_once(held[device_ordinal()][log2_blocks], verify_kernel<T>, kVerifyThreads, kRingBytes, 1 << log2_blocks) < batch)
-    --log2_blocks;
-  p.cluster = 1 << log2_blocks;
-  p.log2_warps = kLog2Warps + log2_blocks;
+  static std::atomic<int> held[kMaxDevices][kMostBlocks + 1] = {};
+  p.cluster = kMostBlocks;
+  while (p.cluster > 1 && paged::clusters_at_once(held[device_ordinal()][p.cluster], verify_kernel<T>, kVerifyThreads, kRingBytes, p.cluster) < batch) --p.cluster;
+  const long long words = (static_cast<long long>(p.vocab) + 2 * Row<T>::kN - 2) / Row<T>::kN;  // of a row that begins at a word's last number
+  auto share = [&](int of) { return static_cast<int>((words + 32ll * of - 1) / (32ll * of) * 32); };  // (a warp takes 32 at a time in any case)
+  p.per_block = share(p.cluster);
+  p.per_warp = share(p.cluster * kVerifyWarps);
   return paged::launch(verify_kernel<T>, dim3(static_cast<unsigned>(batch) * p.cluster), kVerifyThreads, kRingBytes, stream, "verify_drafts", p.cluster, p);
 }
 
