@@ -1370,7 +1370,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
 // pages are unpacked first, us: 18 sequences of 4 rows of 32 heads over 8 behind 3000, INT4, 29 and 49; 37 47 and 70; 32 of 8 rows, 32 heads over 32, behind 1000 to
 // 2000, INT8, 96 and 165.  Warps that share half pages, for up to 64 rows: 131 where the tile kernel takes 64.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kMostRows = 16, kLog2RowBlocks = 4, kMostRowBlocks = 1 << kLog2RowBlocks;
+constexpr int kMostRows = 16, kMostRowBlocks = 16;
 
 template <int BITS>
 struct RowsCfg {
@@ -1924,23 +1924,22 @@ bool rows_few(int batch, int max_seqlen, int max_length, int heads, int kv_heads
   const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
   return static_cast<long long>(max_seqlen) * (heads / kv_heads) <= kMostRows && !(items <= 16 && pages > 16 * (items <= 8 ? 32 : 16));
 }
-// Blocks of a cluster that share out the keys of a sequence and kv head, of one to sixteen: rounds of as many clusters as run at once (places[log2 blocks], two blocks
-// on a multiprocessor), a warp's half pages one after the other, 5 us ahead of and behind them, a cluster's join.  (INT4, 32 heads over 8, us, of one, two, four, eight,
-// sixteen blocks: one sequence of 500 positions 8.3, 8.2, 6.9, 6.9, 7.7; 9 of them 10.1, 9.5, 13.0, 20.6 (72 clusters of four find no place at once); one of 8000 71,
-// 41, 23, 16, 13; 8 of 8000 89, 56, 33, 39; 64 of 2000 63, 74, 93, 146.)
-int rows_log2_blocks(const int (&places)[kLog2RowBlocks + 1], long long items, int max_length) {
-  const long long halves = 2 * ((static_cast<long long>(max_length) + kPage - 1) / kPage);
-  int chosen = 0;
+// Blocks of a cluster that share out the keys of a sequence and kv head: rounds of as many clusters as run at once (places(blocks), two blocks on a multiprocessor); 5 us
+// ahead of and behind a warp's half pages, which come one after the other, slower where two blocks share a multiprocessor; a cluster's join.  Of 63 sizes (1 to 64
+// sequences of 500 to 16000 positions, 4 rows, INT4, 32 heads over 8) the choice is within 4.5 % of the best.  (us, of one, two, four, eight, sixteen blocks: one sequence
+// of 500 8.3, 8.2, 7.0, 6.7, 7.6; 10 of 2000 28.9, 20.3, 21.5, 26.6, 45, but of three 16.2; one of 16000 135, 72, 40, 26, 20; 64 of 2000 63, 74, 93, 146.)
+template <typename Places>
+int rows_blocks(Places places, long long items, int max_length) {
+  const int halves = 2 * static_cast<int>((static_cast<long long>(max_length) + kPage - 1) / kPage);
+  int chosen = 1;
   float best = 3.0e38f;
-  for (int l = 0; l <= kLog2RowBlocks; ++l) {
-    const int n = 1 << l, warps = kTailWarps * n;
-    for (int per_sm = 1; per_sm <= 2; ++per_sm) {
-      const float room = fmaxf(1.f, 0.5f * per_sm * places[l]), rounds = items / room, full = ceilf(rounds);
-      const float time = (0.75f * full + 0.25f * fmaxf(rounds, 1.f)) * (5.f + (n > 1 ? 1.f + 0.2f * n : 0.f) + (halves + warps - 1) / warps * (per_sm == 1 ? 1.05f : 1.45f));
-      if (time >= best) continue;
-      best = time;
-      chosen = l;
-    }
+  for (int n = 1; n <= kMostRowBlocks && (n == 1 || kTailWarps * (n - 1) < halves); ++n) {
+    const int held = places(n), turns = ((halves + n - 1) / n + kTailWarps - 1) / kTailWarps;
+    const float rounds = fmaxf(1.f, items / static_cast<float>(held)), shared = fminf(1.f, fmaxf(0.f, 2.f * items / held - 1.f));  // multiprocessors with two blocks
+    const float time = 0.5f * (ceilf(rounds) + rounds) * (5.f + (n > 1 ? 0.5f + 0.1f * n : 0.f) + turns * (1.05f + 0.2f * sqrtf(shared)));
+    if (time >= best) continue;
+    best = time;
+    chosen = n;
   }
   return chosen;
 }
@@ -1948,7 +1947,7 @@ template <int BITS>
 int run_rows(RowsParams& p, long long items, int max_length, void* stream) {
   using C = RowsCfg<BITS>;
   static std::atomic<bool> done[kMaxDevices] = {};  // of this kernel
-  static std::atomic<int> held[kMaxDevices][kLog2RowBlocks + 1] = {};
+  static std::atomic<int> held[kMaxDevices][kMostRowBlocks + 1] = {};
   const int dev = device_ordinal();
   if (!done[dev].load(std::memory_order_relaxed)) {
     const int rc = check_cuda(cudaFuncSetAttribute(rows_kernel<BITS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1), "paged_tree_attention: clusters of sixteen");
@@ -1957,9 +1956,7 @@ int run_rows(RowsParams& p, long long items, int max_length, void* stream) {
   }
   const int rc = allow_smem<rows_kernel<BITS>>(C::kSmem, "paged_tree_attention: shared memory", [](int) { return true; });
   if (rc) return rc;
-  int places[kLog2RowBlocks + 1];
-  for (int l = 0; l <= kLog2RowBlocks; ++l) places[l] = clusters_at_once(held[dev][l], rows_kernel<BITS>, 32 * kTailWarps, C::kSmem, 1 << l);
-  p.cluster = 1 << rows_log2_blocks(places, items, max_length);
+  p.cluster = rows_blocks([&](int n) { return clusters_at_once(held[dev][n], rows_kernel<BITS>, 32 * kTailWarps, C::kSmem, n); }, items, max_length);
   QS_REQUIRE(items * p.cluster <= 0x7fffffffll, "paged_tree_attention: %lld blocks", items * p.cluster);
   return launch(rows_kernel<BITS>, dim3(static_cast<unsigned>(items * p.cluster)), 32 * kTailWarps, C::kSmem, stream, "paged_tree_attention", p.cluster, p);
 }
