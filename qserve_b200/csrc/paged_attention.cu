@@ -1825,16 +1825,17 @@ struct Plan {
   long long split_rows(long long all) const { return split == items ? all : split * tiles * kRows; }
 };
 constexpr float kTwoTilesPage = 0.92f, kTwoTilesFixed = 5.5f;  // us
-Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, long long pages, bool prompt) {
+Plan plan_tiles(long long rows, int batch, long long num_rows, int kv_heads, long long pages, bool prompt, bool step = false) {
   constexpr float kJoinCluster = 1.f, kJoinKernel = 4.f, kJoinTail = 0.1f, kPartBytesPerUs = 1e7f;
   Plan pl{};
   pl.tiles = rows <= kRows ? 1 : 2;
   const long long block_rows = pl.tiles * kRows, sms = num_sms();
   pl.row_blocks = static_cast<int>((rows + block_rows - 1) / block_rows);
   pl.items = static_cast<long long>(pl.row_blocks) * batch * kv_heads;
-  // blocks that have rows: of portions of unequal length the shorter ones leave some without
+  // blocks that have rows: of portions of unequal length the shorter ones leave some without; in a step of drafted rows no sequence is left out (4 rows each of 3
+  // sequences behind 100000, 4 kv heads: 119 us where they are taken for two, so 94)
   long long blocks = static_cast<long long>(kv_heads) * ((2 * num_rows + batch * block_rows + 2 * block_rows - 1) / (2 * block_rows));
-  blocks = blocks < 1 ? 1 : blocks > pl.items ? pl.items : blocks;
+  blocks = blocks < 1 ? 1 : blocks > pl.items || (step && pl.row_blocks == 1) ? pl.items : blocks;
   const unsigned most = static_cast<unsigned>(pages < 1 ? 1 : pages);
   const float fixed = pl.tiles == 2 ? kTwoTilesFixed : 3.5f;
   float best = 3.0e38f;
@@ -1902,10 +1903,10 @@ int tiles(TileParams& p, const Plan& pl, bool int4, void* stream) {
   return int4 ? sized(std::integral_constant<int, 4>{}) : sized(std::integral_constant<int, 8>{});
 }
 
-Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
+Plan plan_prompt(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads, bool step) {
   const int group = heads / kv_heads;
   return plan_tiles(static_cast<long long>(max_seqlen) * group, batch, static_cast<long long>(num_tokens) * group, kv_heads,
-                    (static_cast<long long>(max_length) + kPage - 1) / kPage, true);
+                    (static_cast<long long>(max_length) + kPage - 1) / kPage, true, step);
 }
 // Few sequences or few shared pages: the tail kernel reads the shared pages too, once per sequence (out of the first row of the table), one launch instead of two.
 // us, both kernels / the tail alone (INT4, 32 heads over 8, 100 positions behind): one sequence behind 512 6.7 / 6.0, behind 4096 9.6 / 8.2; two behind 512 6.8 / 6.1;
@@ -1918,11 +1919,12 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 }
 
 
-// Portions of few rows are the rows kernel's.  Few long sequences are the tile kernel's even so, which cuts their keys into more parts than a cluster has blocks:
-// 100000 positions 68 and 85 us, 2 x 60000 78 and 84; 4 x 30000 88 and 56.
+// Portions of few rows are the rows kernel's, but for few long sequences, which the tile kernel cuts into more parts than a cluster has blocks.  (INT4, 4 rows of 4
+// heads, us, tile and rows kernel, of one sequence and kv head behind 8000 positions 10.0 and 9.2, behind 60000 16 and 38; of eight in all 12.8 and 12.4, 40 and 52; of
+// twelve 15.4 and 12.4, 60 and 54; of 32 25 and 19, 146 and 99.)
 bool rows_few(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
   const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
-  return static_cast<long long>(max_seqlen) * (heads / kv_heads) <= kMostRows && !(items <= 16 && pages > 16 * (items <= 8 ? 32 : 16));
+  return static_cast<long long>(max_seqlen) * (heads / kv_heads) <= kMostRows && !(items <= 10 && pages > 192);
 }
 // Blocks of a cluster that share out the keys of a sequence and kv head: rounds of as many clusters as run at once (places(blocks), two blocks on a multiprocessor); 5 us
 // ahead of and behind a warp's half pages, which come one after the other, slower where two blocks share a multiprocessor; a cluster's join.  Of 63 sizes (1 to 64
@@ -1972,22 +1974,26 @@ int few_rows(const PagedAttnArgs& a) {
 
 }  // namespace
 
-size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
+namespace {
+size_t prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads, bool step) {
   if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  const Plan pl = plan_prompt(batch, num_tokens, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads);
+  max_seqlen = max_seqlen < num_tokens ? max_seqlen : num_tokens;
+  if (step && rows_few(batch, max_seqlen, max_length, heads, kv_heads)) return 0;
+  const Plan pl = plan_prompt(batch, num_tokens, max_seqlen, max_length, heads, kv_heads, step);
   return pl.parts > 1 ? part_bytes(pl.split_rows(static_cast<long long>(num_tokens) * heads), pl.parts) : 0;
 }
-
+}  // namespace
+size_t paged_prompt_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
+  return prompt_workspace(batch, num_tokens, max_seqlen, max_length, heads, kv_heads, false);
+}
 size_t paged_tree_workspace(int batch, int num_tokens, int max_seqlen, int max_length, int heads, int kv_heads) {
-  if (batch <= 0 || num_tokens <= 0 || max_seqlen <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads) return 0;
-  if (rows_few(batch, max_seqlen < num_tokens ? max_seqlen : num_tokens, max_length, heads, kv_heads)) return 0;
-  return paged_prompt_workspace(batch, num_tokens, max_seqlen, max_length, heads, kv_heads);
+  return prompt_workspace(batch, num_tokens, max_seqlen, max_length, heads, kv_heads, true);
 }
 
 int paged_prompt_attention(const PagedAttnArgs& a) {
   if (a.batch == 0 || a.num_tokens == 0 || a.max_seqlen == 0) return QS_OK;
   if (a.visible && rows_few(a.batch, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads)) return few_rows(a);
-  const Plan pl = plan_prompt(a.batch, a.num_tokens, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads);
+  const Plan pl = plan_prompt(a.batch, a.num_tokens, a.max_seqlen, a.max_length, a.num_heads, a.cache.num_kv_heads, a.visible != nullptr);
   TileParams p{};
   p.q = static_cast<const __half*>(a.q); p.out = static_cast<__half*>(a.out); p.q_stride = a.q_stride; p.out_stride = a.out_stride;
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths;

@@ -115,6 +115,14 @@ def test_verify(dev, dtype, kind, V, new):
 
 
 @pytest.mark.parametrize("kind", ["probs", "tree", "none"])
+@pytest.mark.parametrize("V", [17, 2051, 20011])
+@pytest.mark.parametrize("batch", [1, 7, 8, 9, 11, 14, 16, 19, 22, 25, 31, 38, 50, 75, 150])
+def test_batches(dev, kind, V, batch):
+    """Sequences share the device: each batch has blocks of its own number a sequence, and warps at the end of a row have few words or none."""
+    check(inputs(dev, TYPES[batch % 3], V, [2 + (i + batch) % 3 for i in range(batch)], kind, seed=V + batch))
+
+
+@pytest.mark.parametrize("kind", ["probs", "tree", "none"])
 @pytest.mark.parametrize("V", [9, 5003, 65536])
 def test_temperatures(dev, kind, V):
     new = [6, 7, 1, 12, 5, 6, 6, 3]

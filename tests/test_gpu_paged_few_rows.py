@@ -156,10 +156,31 @@ def test_graphs_and_streams(dev):
             check_attention(out, attend64(c, q, masks(kind, new, step), new, [m - 5 * step for m in lens]), SCALE)
 
 
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("batch", [1, 2, 3, 5, 6, 7, 9, 10, 11, 13, 15, 17])
+def test_batches(dev, bits, batch):
+    """Sequences share the device: each batch has blocks of its own number a sequence, some of which have a half page more than others or none."""
+    new, ahead = [1 + (i + batch) % 4 for i in range(batch)], [(1000 + 397 * i) % 2500 for i in range(batch)]
+    lens = [n + m for n, m in zip(new, ahead)]
+    c = Cache(lens, 4, bits, dev, seed=batch)
+    q, seen = queries(sum(new), 16, dev), masks("tree", new, batch)
+    check_attention(attend(c, q, seen, new), attend64(c, q, seen, new, lens), SCALE)
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("hq,hkv,new,ahead", [(8, 2, [2, 4, 1], [13000, 12, 14001]), (4, 1, [3, 1, 4, 2, 4, 1, 4, 2, 3, 1], [13000] + [700 * i for i in range(9)])], ids=lambda x: str(x)[:20])
+def test_few_long_sequences(dev, bits, hq, hkv, new, ahead):
+    """Those are cut into more parts than a cluster has blocks, every sequence's alike."""
+    lens = [n + m for n, m in zip(new, ahead)]
+    c = Cache(lens, hkv, bits, dev, seed=3)
+    q, seen = queries(sum(new), hq, dev), masks("tree", new, 7)
+    check_attention(attend(c, q, seen, new), attend64(c, q, seen, new, lens), SCALE)
+
+
 def test_no_work_space_is_needed(dev):
     from qserve_b200._lib import lib
     need = lib.qs_paged_tree_attention_workspace_bytes
-    assert need(1, 4, 4, 30000, 32, 8) == 0 and need(8, 32, 4, 60000, 32, 8) == 0 and need(0, 4, 4, 100, 32, 8) == 0 and need(2, 4, 0, 100, 32, 8) == 0
+    assert need(1, 4, 4, 10000, 32, 8) == 0 and need(2, 8, 4, 60000, 32, 8) == 0 and need(8, 32, 4, 60000, 32, 8) == 0 and need(0, 4, 4, 100, 32, 8) == 0 and need(2, 4, 0, 100, 32, 8) == 0
     # more rows, and few rows of few long sequences: the prompt operator's
     for a in ((1, 24, 24, 60000, 32, 8), (1, 4, 4, 60000, 32, 8)):
         assert need(*a) == lib.qs_paged_prompt_attention_workspace_bytes(*a) > 0
