@@ -147,7 +147,8 @@ struct AppendParams {
 };
 
 // A warp per token and run of its head rows, four rows at a time with eight lanes each.  ROWS: groups of four rows whose loads are on their way together.
-// AT: the angles go by given positions.  (A variant of its own: the branch alone would cost the other nothing that could be measured, its registers would.)
+// AT: the angles go by given positions: a load more ahead of each.  (8190 rows of 32 heads and 32 kv heads, three axes, INT8: 73.9 us, 71.9 without; 43 rows 6.3 and 4.4,
+// a load's latency.  A variant of its own: the branch alone would cost the other nothing that could be measured, its registers would.)
 template <int BITS, int ROWS, bool AT>
 __global__ void __launch_bounds__(32 * kWarps) append_kernel(const __grid_constant__ AppendParams p) {
   using G = Geom<BITS>;
