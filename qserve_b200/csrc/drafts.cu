@@ -750,26 +750,41 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     if (from_p) whole = sum;
     // Which of up to 16 shares the threshold falls into, given what lies ahead of them (then: of the one chosen); the last with any where it falls behind them all
     const double threshold = static_cast<double>(p.draws[b]) * whole;
-    auto choose = [&](double mine, double& ahead) {
-      double run = mine;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const double below = __shfl_up_sync(0xffffffffu, run, d);
-        if (lane >= d) run += below;
-      }
+    auto choose = [&](double mine, double run, double& ahead) {  // run: of the shares up to this one
       const unsigned any = __ballot_sync(0xffffffffu, mine > kNothing), past = __ballot_sync(0xffffffffu, mine > kNothing && ahead + run > threshold);
       const int chosen = past ? __ffs(past) - 1 : 31 - __clz(any);
       ahead += __shfl_sync(0xffffffffu, run - mine, chosen & 31);
       return chosen;
+    };
+    auto run_of = [&](double x) {
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double below = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += below;
+      }
+      return x;
+    };
+    auto runs_of = [&](double& x, double& y) {  // (both at once: a step is a shuffle's and a sum's latency)
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const double below_x = __shfl_up_sync(0xffffffffu, x, d), below_y = __shfl_up_sync(0xffffffffu, y, d);
+        if (lane >= d) {
+          x += below_x;
+          y += below_y;
+        }
+      }
     };
     auto share_of = [&](const double* of_all, const double* of_drawn, const double* of_draft, int many) {
       if (lane >= many) return 0.0;
       return from_p ? of_all[lane] : fmax(q ? of_drawn[lane] + correction * of_draft[lane] : of_drawn[lane], 0.0);
     };
     double ahead = 0.0;
-    if (choose(share_of(shares[0], shares[1], shares[2], p.cluster), ahead) == rank) {
+    const double of_block = share_of(shares[0], shares[1], shares[2], p.cluster), of_mine = share_of(s_share[0], s_share[1], s_share[2], kVerifyWarps);
+    double run_block = of_block, run_mine = of_mine;
+    runs_of(run_block, run_mine);
+    if (choose(of_block, run_block, ahead) == rank) {
       // the warp, then its run shared out over all of the block's lanes, then the number
-      const int of = rank * kVerifyWarps + choose(share_of(s_share[0], s_share[1], s_share[2], kVerifyWarps), ahead);
+      const int of = rank * kVerifyWarps + choose(of_mine, run_mine, ahead);
       const int w0 = begin_of(row, of), len = begin_of(row, of + 1) - w0;
       const int c0 = w0 + static_cast<int>(static_cast<long long>(len) * tid / kVerifyThreads), c1 = w0 + static_cast<int>(static_cast<long long>(len) * (tid + 1) / kVerifyThreads);
       const int kids = !q && !from_p ? kids_in(w0, w0 + len) : 0;
@@ -798,28 +813,33 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
           for (int k = 0; k < kN; ++k) w[k] = w[k] > 0.0 ? fmax(fma(-sum, static_cast<double>(qs[k]), w[k]), 0.0) : 0.0;
         }
       };
-      for (int c = c0; c < c1; ++c) {
+      unsigned some = 0;  // of a word's numbers those with a weight; w: the sums up to them from the lane's first on
+      auto sums_of = [&](int c, double& sum) {
         weights_of(c);
+        some = 0;
 #pragma unroll
-        for (int k = 0; k < kN; ++k) mine += w[k];
-      }
-      double of_warp = mine;
-#pragma unroll
-      for (int d = 16; d >= 1; d >>= 1) of_warp += __shfl_xor_sync(0xffffffffu, of_warp, d);
+        for (int k = 0; k < kN; ++k) {
+          some |= w[k] > 0.0 ? 1u << k : 0u;
+          w[k] = sum += w[k];
+        }
+      };
+      for (int c = c0; c < c1; ++c) sums_of(c, mine);
+      const double run = run_of(mine);
       __syncthreads();  // s_share has been read
-      if (lane == 0) s_share[0][warp] = of_warp;
+      if (lane == 31) s_share[0][warp] = run;
       __syncthreads();
-      if (choose(lane < kVerifyWarps ? s_share[0][lane] : 0.0, ahead) == warp && choose(mine, ahead) == lane) {
+      const double of_warp = lane < kVerifyWarps ? s_share[0][lane] : 0.0;
+      if (choose(of_warp, run_of(of_warp), ahead) == warp && choose(mine, run, ahead) == lane) {
         int found = -1, last = -1;  // the first past the threshold; the last with any weight
+        double sum = 0.0;
         for (int c = c0; c < c1 && found < 0; ++c) {
-          if (c1 - c0 > 1) weights_of(c);
+          if (c1 - c0 > 1) sums_of(c, sum);
 #pragma unroll
-          for (int k = 0; k < kN; ++k) {
-            ahead += w[k];
-            if (w[k] > 0.0) {
-              last = c * kN - row.skip + k;
-              if (found < 0 && ahead > threshold) found = last;
-            }
+          for (int k = kN - 1; k >= 0; --k) {
+            if (!(some >> k & 1u)) continue;
+            const int token = c * kN - row.skip + k;
+            if (ahead + w[k] > threshold) found = token;
+            last = max(last, token);
           }
         }
         out_tokens[accepted] = found >= 0 ? found : last;
