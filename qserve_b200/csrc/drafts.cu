@@ -64,10 +64,10 @@ __global__ void __launch_bounds__(kMostDrafted) tree_kernel(int* positions, unsi
 // bits could get wrong is taken again with a sum of 64 bits.  The token that the sequence ends with is drawn with weights and sums of 64 bits: among 10^5 tokens one
 // border or another lies within 32 bits' error of one draw in a hundred.  For that the last row is read once more, out of L2.
 //
-// 64 chains of up to 6 rows with the draft's probabilities, 128256 tokens, fp16, two blocks a chain: 47.4 us, of which maxima and sums take 19 (77 MB, 4.1 TB/s of 128
+// 64 chains of up to 6 rows with the draft's probabilities, 128256 tokens, fp16, two blocks a chain: 46.5 us, of which maxima and sums take 19 (77 MB, 4.1 TB/s of 128
 // multiprocessors' copies), the second reading of a row and its probabilities 15 (48 MB; issue slots and the 64-bit pipe: 46 cycles of it for a warp's 32 numbers), the
-// exchanges, decisions and the search for the drawn token 9, start and end 4.  Few sequences wait for one another's blocks instead: one chain of 5, 32000 tokens, 14.6.
-// Blocks of 8 warps, two on a multiprocessor, 51.7.
+// exchanges, decisions and the search for the drawn token 9, start and end 4.  Few sequences wait for one another's blocks instead: one chain of 5, 32000 tokens, 14.6,
+// a quarter of it for instructions.  Blocks of 8 warps, two on a multiprocessor, 51.7.
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16;
 constexpr int kMostWindow = 8;
@@ -742,12 +742,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     // With e the weights, S their sum and s that sum as 32 bits have it: what is drawn from is max(e - S q, 0).  S is not known before the row's end; but
     // sum (e - S q) over a run is sum (e - s q) + (s - S) sum q, and which numbers are above zero differs for those alone that are next to nothing.  One pass.
     share_out(shares_of_row(node, q, kids_in(begin_of(row, my_warp), begin_of(row, my_warp + 1))));
-    const double sum = sum_of(0), correction = total - sum;
+    const double all = sum_of(0), correction = total - all;
     const double (&shares)[3][kMostBlocks] = s_shares[turn_sum ^ 1];
     double whole = 0.0;
     for (int r = 0; r < p.cluster; ++r) whole += fmax(q ? shares[1][r] + correction * shares[2][r] : shares[1][r], 0.0);
     const bool from_p = !(whole > kNothing);  // nothing is left of what was asked for
-    if (from_p) whole = sum;
+    if (from_p) whole = all;
     // Which of up to 16 shares the threshold falls into, given what lies ahead of them (then: of the one chosen); the last with any where it falls behind them all
     const double threshold = static_cast<double>(p.draws[b]) * whole;
     auto choose = [&](double mine, double run, double& ahead) {  // run: of the shares up to this one
@@ -788,61 +788,65 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       const int w0 = begin_of(row, of), len = begin_of(row, of + 1) - w0;
       const int c0 = w0 + static_cast<int>(static_cast<long long>(len) * tid / kVerifyThreads), c1 = w0 + static_cast<int>(static_cast<long long>(len) * (tid + 1) / kVerifyThreads);
       const int kids = !q && !from_p ? kids_in(w0, w0 + len) : 0;
-      double w[kN], mine = 0.0;
-      auto weights_of = [&](int c) {
+      const float floor = top == CUDART_INF_F ? 3.4028235e38f : weigh.least;
+      double w[kN], sum = 0.0;  // of a word's numbers the sums up to them, from the lane's first on
+      unsigned some = 0;        // those with a weight
+      auto sums_of = [&](int c) {
         const int first = c * kN - row.skip;
         float x[kN], qs[kN];  // (all of q's on their way with the word)
 #pragma unroll
-        for (int k = 0; k < kN; ++k) qs[k] = q && first + k >= 0 && first + k < p.vocab ? __ldcg(q + first + k) : 0.f;
+        for (int k = 0; k < kN; ++k) qs[k] = q && static_cast<unsigned>(first + k) < static_cast<unsigned>(p.vocab) ? __ldcg(q + first + k) : 0.f;
         numbers_of<T>(row.word(c), x);
-        if (weigh.odd) {
 #pragma unroll
-          for (int k = 0; k < kN; ++k) w[k] = weigh(x[k]);
-        } else {
-#pragma unroll
-          for (int k = 0; k < kN; ++k) w[k] = x[k] > weigh.least ? weigh.finite(fmaxf(x[k], weigh.least)) : 0.0;
-        }
+        for (int k = 0; k < kN; ++k) w[k] = x[k] > floor ? (top == CUDART_INF_F ? 1.0 : weigh.finite(x[k])) : 0.0;
         for (int j = 0; j < kids; ++j) {
           const int at = s_kids[j] - first;
 #pragma unroll
           for (int k = 0; k < kN; ++k)
             if (k == at) w[k] = 0.0;
         }
-        if (q && !from_p) {
-#pragma unroll
-          for (int k = 0; k < kN; ++k) w[k] = w[k] > 0.0 ? fmax(fma(-sum, static_cast<double>(qs[k]), w[k]), 0.0) : 0.0;
-        }
-      };
-      unsigned some = 0;  // of a word's numbers those with a weight; w: the sums up to them from the lane's first on
-      auto sums_of = [&](int c, double& sum) {
-        weights_of(c);
         some = 0;
 #pragma unroll
         for (int k = 0; k < kN; ++k) {
+          if (q && !from_p) w[k] = w[k] > 0.0 ? fmax(fma(-all, static_cast<double>(qs[k]), w[k]), 0.0) : 0.0;
           some |= w[k] > 0.0 ? 1u << k : 0u;
           w[k] = sum += w[k];
         }
       };
-      for (int c = c0; c < c1; ++c) sums_of(c, mine);
-      const double run = run_of(mine);
-      __syncthreads();  // s_share has been read
-      if (lane == 31) s_share[0][warp] = run;
-      __syncthreads();
-      const double of_warp = lane < kVerifyWarps ? s_share[0][lane] : 0.0;
-      if (choose(of_warp, run_of(of_warp), ahead) == warp && choose(mine, run, ahead) == lane) {
-        int found = -1, last = -1;  // the first past the threshold; the last with any weight
-        double sum = 0.0;
-        for (int c = c0; c < c1 && found < 0; ++c) {
-          if (c1 - c0 > 1) sums_of(c, sum);
-#pragma unroll
-          for (int k = kN - 1; k >= 0; --k) {
-            if (!(some >> k & 1u)) continue;
-            const int token = c * kN - row.skip + k;
-            if (ahead + w[k] > threshold) found = token;
-            last = max(last, token);
+      // (The code of this is run through for the first time here and waits for its instructions, so it is there once: for the sums, and, for the chosen lane's numbers
+      // if it has several words, again.)
+      const int words = (len + kVerifyThreads - 1) / kVerifyThreads;  // of a lane at most
+      int i = 0, found = -1, last = -1;                               // the first past the threshold; the last with any weight
+      bool chosen = false;
+#pragma unroll 1
+      while (true) {
+        if (c0 + i < c1) sums_of(c0 + i);
+        if (!chosen) {
+          if (++i < words) continue;
+          const double run = run_of(sum);
+          __syncthreads();  // s_share has been read
+          if (lane == 31) s_share[0][warp] = run;
+          __syncthreads();
+          const double of_warp = lane < kVerifyWarps ? s_share[0][lane] : 0.0;
+          if (choose(of_warp, run_of(of_warp), ahead) != warp || choose(sum, run, ahead) != lane) break;
+          chosen = true;
+          i = 0;
+          if (words > 1) {
+            sum = 0.0;
+            continue;
           }
         }
-        out_tokens[accepted] = found >= 0 ? found : last;
+#pragma unroll
+        for (int k = kN - 1; k >= 0; --k) {
+          if (!(some >> k & 1u)) continue;
+          const int token = (c0 + i) * kN - row.skip + k;
+          if (ahead + w[k] > threshold) found = token;
+          last = max(last, token);
+        }
+        if (found >= 0 || c0 + ++i >= c1) {
+          out_tokens[accepted] = found >= 0 ? found : last;
+          break;
+        }
       }
     }
   }
