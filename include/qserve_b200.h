@@ -195,7 +195,7 @@ QS_API int qs_paged_tree_attention(const void* q, int64_t q_stride, void* out, i
                                    int max_blocks_per_seq, int num_heads, int num_kv_heads, int head_dim, int tokens_per_block, int size_per_token,
                                    int int4_kv_cache, int kv_cache_with_zeros, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 /* Which drafted tokens the target takes, and the token behind them.  logits [num_tokens, vocab] (logits_type 0 fp16, 1 bf16, 2 fp32, rows of logits_stride numbers):
- * row i's judge the children of row i.  tokens int64 [num_tokens] (row 0's is not looked at; one outside 0 .. vocab - 1 is never taken), parents as in qs_draft_tree,
+ * row i's decide on the children of row i.  tokens int64 [num_tokens] (row 0's is not looked at; one outside 0 .. vocab - 1 is never taken), parents as in qs_draft_tree,
  * NULL: a chain.  coins fp32 [num_tokens] and draws fp32 [batch]: random numbers in [0, 1); temperatures fp32 [batch] or NULL (1).  With p = softmax(logits / t) of the
  * current row, from row 0 on:
  *   draft_probs q fp32 [num_tokens, vocab] (chains; row i's is what row i + 1's token x was drawn from): x is taken where coin q(x) < p(x), otherwise the sequence ends

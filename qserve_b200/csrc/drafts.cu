@@ -1,7 +1,7 @@
 // qserve_b200 -- drafted tokens of a step: what the rows of a tree see of one another, and their verification against the target's probabilities.
 //
 // The rows of sequence b are a portion (as in paged_cache.cu): row 0 the token that the step starts from, every other one a drafted token with a parent
-// among the rows ahead of it.  Row i's logits are the target's behind row i, so they judge i's children.
+// among the rows ahead of it.  Row i's logits are the target's behind row i, so they decide on i's children.
 //
 // verify, of a sequence with temperature t > 0 (p = softmax(logits / t) of the current row, from row 0 on):
 //   drafts drawn from q, a chain:  the child x is taken where u q(x) < p(x); else the sequence ends with a token drawn from max(p - q, 0) / sum;
