@@ -187,8 +187,8 @@ QS_API int qs_append_kv_cache_at(const void* q, const void* k, const void* v, in
                                  int int4_kv_cache, int kv_cache_with_zeros, void* stream);
 /* qs_paged_prompt_attention, with what a row sees given: every position ahead of its portion, and of the portion those rows whose bits it has in
  * visible [num_tokens, visible_words] (bit i % 64 of word i / 64; 64 * visible_words >= max_seqlen), its own place or later ones as well.  A row that sees nothing gets
- * zeros.  Numbers as in qs_paged_prompt_attention; for up to 16 rows (max_seqlen * num_heads / num_kv_heads; not for few long sequences) the pages and the weights
- * are taken exactly, those whose codes stand for more than fp16 holds among them.  workspace: qs_paged_tree_attention_workspace_bytes(...) of the same numbers, any contents, not shared by calls at the same time. */
+ * zeros.  Numbers as in qs_paged_prompt_attention; for up to 16 rows (max_seqlen * num_heads / num_kv_heads; not for few long sequences), and for more in small calls, the pages and
+ * the weights are taken exactly, those whose codes stand for more than fp16 holds among them.  workspace: qs_paged_tree_attention_workspace_bytes(...) of the same numbers, any contents, not shared by calls at the same time. */
 QS_API size_t qs_paged_tree_attention_workspace_bytes(int batch, int num_tokens, int max_seqlen, int max_length, int num_heads, int num_kv_heads);
 QS_API int qs_paged_tree_attention(const void* q, int64_t q_stride, void* out, int64_t out_stride, const int64_t* kv_pointers, const int32_t* cu_seqlens,
                                    const int32_t* lengths, const int64_t* visible, int visible_words, int batch, int num_tokens, int max_seqlen, int max_length,

@@ -1364,7 +1364,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
 // ------------------------------------------------------------------------------------------------------------------------
 // row kernel: portions of few rows with a mask among them (a step's drafted tokens)
 //
-// Up to 16 rows (token, head of the group) of a kv head.  Codes go into the products as they lie, as in the tail kernel, but as their second operand: the rows are the
+// 16 rows (token, head of the group) of a kv head, of tokens whose masks are a word.  Codes go into the products as they lie, as in the tail kernel, but as their second operand: the rows are the
 // first one's 16, and a product's scores are the next one's operand as they are.  A block's warps take turns over half pages, a cluster of blocks over their runs.
 // A warp takes 1.0 us for a half page, 1.45 where two blocks share a multiprocessor (registers hold no third: with 168 a thread the code takes 1.4 times as long), of
 // which products are a third: one chain of copies - scales - scores - weights - values.  Weights go into the products as two fp16 numbers, so that results are off by their
@@ -1372,7 +1372,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, DEEP ? 2 : BITS == 4 ? 4 : 3)
 // pages are unpacked first, us: 18 sequences of 4 rows of 32 heads over 8 behind 3000, INT4, 29 and 49; 37 47 and 70; 32 of 8 rows, 32 heads over 32, behind 1000 to
 // 2000, INT8, 96 and 165.  Warps that share half pages, for up to 64 rows: 131 where the tile kernel takes 64.
 // ------------------------------------------------------------------------------------------------------------------------
-constexpr int kMostRows = 16, kMostRowBlocks = 16;
+constexpr int kMostRows = 16, kMostRowBlocks = 16, kMostRowTokens = 64;
 
 template <int BITS>
 struct RowsCfg {
@@ -1390,7 +1390,7 @@ struct RowsParams {
   const long long* kv_pointers;
   const int *cu, *lengths;
   const unsigned long long* visible;
-  int words, num_tokens, max_seqlen, max_blocks, num_heads, num_kv_heads, cluster;
+  int words, num_tokens, max_seqlen, max_blocks, num_heads, num_kv_heads, cluster, row_blocks;
   float scale_log2;
 };
 
@@ -1428,14 +1428,16 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   const unsigned item = blockIdx.x / static_cast<unsigned>(p.cluster);
   const int rank = static_cast<int>(blockIdx.x - item * p.cluster);
-  const int b = item / static_cast<unsigned>(p.num_kv_heads), hk = item - b * p.num_kv_heads;
+  const unsigned of_pages = item / static_cast<unsigned>(p.row_blocks);  // (a run of items reads the same pages)
+  const int row0 = static_cast<int>(item - of_pages * p.row_blocks) * kMostRows;
+  const int b = of_pages / static_cast<unsigned>(p.num_kv_heads), hk = of_pages - b * p.num_kv_heads;
   const int group = static_cast<unsigned>(p.num_heads) / static_cast<unsigned>(p.num_kv_heads);
   pdl_launch_dependents();
   pdl_wait();
   Portion portion = portion_of(p.cu, p.lengths, b, p.num_tokens);
   portion.count = min(portion.count, p.max_seqlen);
-  const int n_rows = portion.count * group;
-  if (n_rows == 0) return;  // the whole cluster
+  const int n_rows = min(portion.count * group - row0, kMostRows);
+  if (n_rows <= 0) return;  // the whole cluster
   const int n_keys = min(max(portion.first + portion.count, 0), p.max_blocks * kPage);
   const int slices = (n_keys + kSlice - 1) / kSlice;
   // the block's run of them (16 blocks of at most 2^25: 32 bits hold the products), and the warp's turns
@@ -1476,16 +1478,16 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
   // ---- the queries, rows g and g + 8 of the warp's, in the order of the codes: this lane's 32 dims, as in the tail kernel ----
   uint32_t qa[2][8], qh[2][8];  // INT4: of the low nibbles, of the high ones; INT8: of a word's first two codes, its others
   float sumq[2];
-  unsigned long long bits[2];   // of the rows: no more than 64, so one word
+  unsigned long long bits[2];   // of the rows: of no more than 64 tokens, so one word
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
-    const int r = 8 * e + g, tok = r / group;
+    const int r = 8 * e + g, tok = (row0 + r) / group;
     uint32_t qw[16];
 #pragma unroll
     for (int k = 0; k < 16; ++k) qw[k] = 0u;
     bits[e] = 0ull;
     if (r < n_rows) {
-      const uint4* qv = reinterpret_cast<const uint4*>(p.q + (portion.start + tok) * p.q_stride + static_cast<long long>(hk * group + r - tok * group) * kD + 32 * q4);
+      const uint4* qv = reinterpret_cast<const uint4*>(p.q + (portion.start + tok) * p.q_stride + static_cast<long long>(hk * group + row0 + r - tok * group) * kD + 32 * q4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint4 x = __ldcg(qv + k);
@@ -1734,7 +1736,7 @@ __global__ void __launch_bounds__(32 * kTailWarps, 2) rows_kernel(const __grid_c
   __syncthreads();
   // ---- the block's rows: the warps' joined, a warp a row.  Results, or for the cluster ----
   // where rows go, in halfs: lane i has row i
-  const long long to = (portion.start + lane / group) * p.out_stride + static_cast<long long>(hk * group + lane % group) * kD;
+  const long long to = (portion.start + (row0 + lane) / group) * p.out_stride + static_cast<long long>(hk * group + (row0 + lane) % group) * kD;
   auto write = [&](int r, const float4& acc, float L) {
     const long long at = __shfl_sync(0xffffffffu, to, r);
     reinterpret_cast<uint2*>(p.out + at)[lane] = scaled_h4(acc, L);
@@ -1921,12 +1923,17 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
 }
 
 
-// Portions of few rows are the rows kernel's, but for few long sequences, which the tile kernel cuts into more parts than a cluster has blocks.  (INT4, 4 rows of 4
-// heads, us, tile and rows kernel, of one sequence and kv head behind 8000 positions 10.0 and 9.2, behind 60000 16 and 38; of eight in all 12.8 and 12.4, 40 and 52; of
+// Portions of up to 16 rows are the row kernel's, but for few long sequences, which the tile kernel cuts into more parts than a cluster has blocks.  (INT4, 4 rows of 4
+// heads, us, tile and row kernel, of one sequence and kv head behind 8000 positions 10.0 and 9.2, behind 60000 16 and 38; of eight in all 12.8 and 12.4, 40 and 52; of
 // twelve 15.4 and 12.4, 60 and 54; of 32 25 and 19, 146 and 99.)
+// Those of more, whose pages it reads once for every 16, in small calls: by their half pages in all.  (32 heads over 8, INT4: 13 rows of one sequence behind 100 6.3 and
+// 4.9, behind 500 8.5 and 7.4, of four 10.2 and 10.7, of eight 12.1 and 12.3, of 16 13.3 and 23; 5 rows, which is twice 16, of eight behind 500 9.8 and 9.6, behind 2000
+// 20.1 and 19.7, behind 4000 28 and 32; 26 of 16 behind 100, more blocks than places, 7.2 and 18.)
 bool rows_few(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
-  const long long items = static_cast<long long>(batch) * kv_heads, pages = (static_cast<long long>(max_length) + kPage - 1) / kPage;
-  return static_cast<long long>(max_seqlen) * (heads / kv_heads) <= kMostRows && !(items <= 10 && pages > 192);
+  const long long pages = (static_cast<long long>(max_length) + kPage - 1) / kPage, rows = static_cast<long long>(max_seqlen) * (heads / kv_heads);
+  const long long times = (rows + kMostRows - 1) / kMostRows, items = static_cast<long long>(batch) * kv_heads * times;
+  if (times == 1) return !(items <= 10 && pages > 192);
+  return max_seqlen <= kMostRowTokens && items <= 2 * num_sms() && items * pages <= (times == 2 ? 2100 : 1200);
 }
 // Blocks of a cluster that share out the keys of a sequence and kv head: rounds of as many clusters as run at once (places(blocks), two blocks on a multiprocessor); 5 us
 // ahead of and behind a warp's half pages, which come one after the other, slower where two blocks share a multiprocessor; a cluster's join.  Of 63 sizes (1 to 64
@@ -1970,7 +1977,8 @@ int few_rows(const PagedAttnArgs& a) {
   p.kv_pointers = a.cache.kv_pointers; p.cu = a.cache.cu_seqlens; p.lengths = a.cache.lengths; p.visible = a.visible; p.words = a.visible_words;
   p.num_tokens = a.num_tokens; p.max_seqlen = a.max_seqlen; p.max_blocks = a.cache.max_blocks; p.num_heads = a.num_heads; p.num_kv_heads = a.cache.num_kv_heads;
   p.scale_log2 = a.softmax_scale * 1.4426950408889634f;
-  const long long items = static_cast<long long>(a.batch) * a.cache.num_kv_heads;
+  p.row_blocks = (a.max_seqlen * (a.num_heads / a.cache.num_kv_heads) + kMostRows - 1) / kMostRows;
+  const long long items = static_cast<long long>(a.batch) * a.cache.num_kv_heads * p.row_blocks;
   return a.cache.int4 ? run_rows<4>(p, items, a.max_length, a.stream) : run_rows<8>(p, items, a.max_length, a.stream);
 }
 

@@ -167,6 +167,25 @@ def test_batches(dev, bits, batch):
     check_attention(attend(c, q, seen, new), attend64(c, q, seen, new, lens), SCALE)
 
 
+MORE = [  # in small calls up to 64 tokens, 16 rows a block
+    (32, 8, [13], [500]),
+    (8, 2, [5, 0, 64, 33], [0, 12, 31, 200]),
+    (14, 2, [9, 3], [63, 64]),                   # seven heads: tokens across blocks' borders
+    (16, 1, [26, 1, 2], [700, 0, 65]),
+    (40, 8, [5, 5, 4], [130, 1, 700]),
+    (4, 4, [17], [2000]),
+    (32, 8, [8] * 4, [900, 500, 100, 1]),
+    (64, 64, [17], [1]),
+]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("kind", ["tree", "any", "all"])
+@pytest.mark.parametrize("hq,hkv,new,ahead", MORE, ids=lambda x: str(x)[:20])
+def test_more_rows_in_small_calls(dev, bits, kind, hq, hkv, new, ahead):
+    test_few_rows(dev, bits, kind, hq, hkv, new, ahead)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 @pytest.mark.parametrize("hq,hkv,new,ahead", [(8, 2, [2, 4, 1], [13000, 12, 14001]), (4, 1, [3, 1, 4, 2, 4, 1, 4, 2, 3, 1], [13000] + [700 * i for i in range(9)])], ids=lambda x: str(x)[:20])
 def test_few_long_sequences(dev, bits, hq, hkv, new, ahead):

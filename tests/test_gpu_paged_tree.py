@@ -176,6 +176,22 @@ def test_attend(dev, bits, kind, hq, hkv, new, ahead):
             assert (out[t] == 0).all()
 
 
+LARGE = [  # tiles in any case, of one for up to 128 rows a key/value head, of two
+    (32, 8, [13, 16, 1, 9, 0, 12, 16, 7], [3000, 2500, 3100, 0, 5, 63, 900, 2900]),
+    (8, 2, [31] * 24, [100 * i for i in range(24)]),
+    (16, 4, [65, 70], [300, 1]),
+    (32, 32, [20] * 12, [100 * i for i in range(12)]),
+    (14, 2, [16, 40], [7000, 6500]),
+]
+
+
+@pytest.mark.parametrize("bits", [4, 8])
+@pytest.mark.parametrize("kind", ["tree", "any", "all"])
+@pytest.mark.parametrize("hq,hkv,new,ahead", LARGE, ids=lambda x: str(x)[:20])
+def test_attend_large(dev, bits, kind, hq, hkv, new, ahead):
+    test_attend(dev, bits, kind, hq, hkv, new, ahead)
+
+
 @pytest.mark.parametrize("bits", [4, 8])
 def test_a_causal_mask_is_the_prompt_operator(dev, bits):
     """The same numbers to the last bit where both cut the keys alike: what the masked rows weigh is nothing either way."""
