@@ -740,12 +740,21 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       return any ? s_num_kids : 0;
     };
     // With e the weights, S their sum and s that sum as 32 bits have it: what is drawn from is max(e - S q, 0).  S is not known before the row's end; but
-    // sum (e - S q) over a run is sum (e - s q) + (s - S) sum q, and which numbers are above zero differs for those alone that are next to nothing.  One pass.
-    share_out(shares_of_row(node, q, kids_in(begin_of(row, my_warp), begin_of(row, my_warp + 1))));
-    const double all = sum_of(0), correction = total - all;
-    const double (&shares)[3][kMostBlocks] = s_shares[turn_sum ^ 1];
-    double whole = 0.0;
-    for (int r = 0; r < p.cluster; ++r) whole += fmax(q ? shares[1][r] + correction * shares[2][r] : shares[1][r], 0.0);
+    // sum (e - S q) over a run is sum (e - s q) + (s - S) sum q, over the numbers above zero: one pass.  Those for which e / q lies between s and S are counted
+    // on the wrong side by it, so what is drawn from is off by |s - S| times their share of q.  Where that may be more than 1e-4 of all of it -- a draft next to the
+    // target, down to one that is the target's best token, of which S q takes all that s q leaves -- the pass is gone through again with S for s.
+    double (*shares)[kMostBlocks];
+    double all, correction, whole;
+    for (int pass = 0;; ++pass) {
+      share_out(shares_of_row(node, q, kids_in(begin_of(row, my_warp), begin_of(row, my_warp + 1))));
+      shares = s_shares[turn_sum ^ 1];
+      all = sum_of(0);
+      correction = total - all;
+      whole = 0.0;
+      for (int r = 0; r < p.cluster; ++r) whole += fmax(q ? shares[1][r] + correction * shares[2][r] : shares[1][r], 0.0);
+      if (!q || pass == 1 || correction == 0.0 || whole >= 1e4 * fabs(correction)) break;  // (the cluster's threads all have the same numbers)
+      total = all;
+    }
     const bool from_p = !(whole > kNothing);  // nothing is left of what was asked for
     if (from_p) whole = all;
     // Which of up to 16 shares the threshold falls into, given what lies ahead of them (then: of the one chosen); the last with any where it falls behind them all
