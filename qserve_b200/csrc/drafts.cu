@@ -312,6 +312,93 @@ __device__ __noinline__ Shares shares_of(const T* p, int vocab, int w0, int w1, 
   return sum;
 }
 
+// all threads of a cluster
+__device__ __forceinline__ void meet_of(int cluster) {
+  if (cluster > 1) {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  } else {
+    __syncthreads();
+  }
+}
+
+// A token drawn from max(e - S q, 0), number by number, S = `all` the row's sum of 64 bits; where that leaves nothing, from the weights e.  The row's words are shared
+// out over the cluster's threads, a run each, gone through for its sum and, the one that the threshold falls into, again.  `of_warps`, `of_blocks`: places for sums, the
+// blocks' twice.  (A function of its own, with nothing to come back to but the end: the pass above once more, in a loop or called again, held registers that made 64 chains
+// of 6, 128256 tokens, 1 to 3 us longer where none needs it.)
+template <typename T>
+__device__ __noinline__ void draw_exactly(const T* p, int vocab, const float* q, double all, Weigh weigh, float draw, double* of_warps, double* of_blocks0, double* of_blocks1, int cluster, int rank,
+                                          long long* out) {
+  constexpr int kN = Row<T>::kN;
+  const Row<T> row(p, vocab);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = rank * kVerifyThreads + threadIdx.x, threads = cluster * kVerifyThreads;
+  const int c0 = static_cast<int>(static_cast<long long>(row.words) * me / threads), c1 = static_cast<int>(static_cast<long long>(row.words) * (me + 1) / threads);
+  // the run's sum; or its first number with which the sum from `ahead` on is past the threshold, the last with any weight if none is
+  auto go_through = [&](bool search, double ahead, double threshold, int& found) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int c = c0; c < c1; ++c) {
+      float x[kN];
+      numbers_of<T>(row.word(c), x);
+#pragma unroll
+      for (int k = 0; k < kN; ++k) {
+        const int token = row.first(c) + k;
+        double w = weigh(x[k]);
+        if (!(w > 0.0)) continue;  // (what lies outside the row among them)
+        if (q) w = fma(-all, static_cast<double>(__ldcg(q + token)), w);
+        if (!(w > 0.0)) continue;
+        sum += w;
+        if (!search) continue;
+        found = token;
+        if (ahead + sum > threshold) return sum;
+      }
+    }
+    return sum;
+  };
+  auto run_of = [&](double x) {
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double below = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += below;
+    }
+    return x;
+  };
+  int found = -1;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const double of_mine = go_through(false, 0.0, 0.0, found), run = run_of(of_mine);
+    double* const of_blocks = pass == 0 ? of_blocks0 : of_blocks1;
+    __syncthreads();  // what lay in the places has been read
+    if (lane == 31) of_warps[warp] = run;
+    __syncthreads();
+    const double of_warp = lane < kVerifyWarps ? of_warps[lane] : 0.0, run_warps = run_of(of_warp);
+    if (warp == 0) {
+      const double of_block = __shfl_sync(0xffffffffu, run_warps, 31);
+      if (cluster == 1) of_blocks[0] = of_block;
+      else if (lane < cluster) put_peer(&of_blocks[rank], lane, of_block);
+    }
+    meet_of(cluster);
+    const double of_block = lane < cluster ? of_blocks[lane] : 0.0, run_blocks = run_of(of_block), whole = __shfl_sync(0xffffffffu, run_blocks, 31);
+    if (q && !(whole > 0.0)) {  // all blocks alike
+      q = nullptr;
+      continue;
+    }
+    const double threshold = static_cast<double>(draw) * whole;
+    double ahead = 0.0;
+    auto choose = [&](double mine, double run_to) {
+      const unsigned any = __ballot_sync(0xffffffffu, mine > 0.0), past = __ballot_sync(0xffffffffu, mine > 0.0 && ahead + run_to > threshold);
+      const int chosen = past ? __ffs(past) - 1 : 31 - __clz(any);
+      ahead += __shfl_sync(0xffffffffu, run_to - mine, chosen & 31);
+      return chosen;
+    };
+    if (choose(of_block, run_blocks) == rank && choose(of_warp, run_warps) == warp && choose(of_mine, run) == lane) {
+      go_through(true, ahead, threshold, found);
+      *out = found;
+    }
+    return;
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_constant__ VerifyParams p) {
   constexpr int kN = Row<T>::kN;
@@ -356,14 +443,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
   // a warp's words of a row, where each row is shared out over the warps
   auto begin_of = [&](const Row<T>& row, int w) { return min(row.words, p.per_warp * w); };
   auto first_child = [&](int r) { return chain ? r + 1 : s_first[r]; };  // n or more: none
-  auto meet = [&] {  // of the cluster
-    if (p.cluster > 1) {
-      __syncwarp();
-      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    } else {
-      __syncthreads();
-    }
-  };
+  auto meet = [&] { meet_of(p.cluster); };
 
   const uint32_t ring = smem_u32(s_ring) + (warp * (kDepth * 32) + lane) * 16;  // a lane's words lie 512 bytes apart
 
@@ -742,19 +822,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     // With e the weights, S their sum and s that sum as 32 bits have it: what is drawn from is max(e - S q, 0).  S is not known before the row's end; but
     // sum (e - S q) over a run is sum (e - s q) + (s - S) sum q, over the numbers above zero: one pass.  Those for which e / q lies between s and S are counted
     // on the wrong side by it, so what is drawn from is off by |s - S| times their share of q.  Where that may be more than 1e-4 of all of it -- a draft next to the
-    // target, down to one that is the target's best token, of which S q takes all that s q leaves -- the pass is gone through again with S for s.
-    double (*shares)[kMostBlocks];
-    double all, correction, whole;
-    for (int pass = 0;; ++pass) {
-      share_out(shares_of_row(node, q, kids_in(begin_of(row, my_warp), begin_of(row, my_warp + 1))));
-      shares = s_shares[turn_sum ^ 1];
-      all = sum_of(0);
-      correction = total - all;
-      whole = 0.0;
-      for (int r = 0; r < p.cluster; ++r) whole += fmax(q ? shares[1][r] + correction * shares[2][r] : shares[1][r], 0.0);
-      if (!q || pass == 1 || correction == 0.0 || whole >= 1e4 * fabs(correction)) break;  // (the cluster's threads all have the same numbers)
-      total = all;
-    }
+    // target, down to one that is the target's best token, of which S q takes all that s q leaves -- the token is drawn number by number.
+    share_out(shares_of_row(node, q, kids_in(begin_of(row, my_warp), begin_of(row, my_warp + 1))));
+    const double all = sum_of(0), correction = total - all;
+    const double (&shares)[3][kMostBlocks] = s_shares[turn_sum ^ 1];
+    double whole = 0.0;
+    for (int r = 0; r < p.cluster; ++r) whole += fmax(q ? shares[1][r] + correction * shares[2][r] : shares[1][r], 0.0);
+    const bool exactly = q && correction != 0.0 && !(whole >= 1e4 * fabs(correction));  // the cluster's threads all alike
+    if (exactly) draw_exactly<T>(row.p, p.vocab, q, all, weigh, p.draws[b], s_share[0], s_shares[turn_sum][0], s_shares[turn_sum][1], p.cluster, rank, out_tokens + accepted);
     const bool from_p = !(whole > kNothing);  // nothing is left of what was asked for
     if (from_p) whole = all;
     // Which of up to 16 shares the threshold falls into, given what lies ahead of them (then: of the one chosen); the last with any where it falls behind them all
@@ -791,7 +866,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     const double of_block = share_of(shares[0], shares[1], shares[2], p.cluster), of_mine = share_of(s_share[0], s_share[1], s_share[2], kVerifyWarps);
     double run_block = of_block, run_mine = of_mine;
     runs_of(run_block, run_mine);
-    if (choose(of_block, run_block, ahead) == rank) {
+    if (!exactly && choose(of_block, run_block, ahead) == rank) {
       // the warp, then its run shared out over all of the block's lanes, then the number
       const int of = rank * kVerifyWarps + choose(of_mine, run_mine, ahead);
       const int w0 = begin_of(row, of), len = begin_of(row, of + 1) - w0;
