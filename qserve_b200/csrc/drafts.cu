@@ -754,8 +754,11 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
         for (int i = kN - 1; i >= 0; --i)
           if (number(x[i]) == m) largest = word * kN - row.skip + i;
       }
-      // A weight of 32 bits is off by 2^-24 of the numbers that its exponent comes from, top / t and their difference of 40 octaves at most, and by ex2's 2^-22
-      const int taken = decide(r, m, s, largest, 1e-5f + fabsf(m * per_unit) * 2.4e-7f);
+      // A weight of 32 bits is off by 2^-24 of the numbers that its exponent comes from, top / t and their difference of 40 octaves (what is less says nothing in the
+      // sum), and by ex2's 2^-22; the sum by 2^-24 for each number that a lane adds to what it has: in every group a fourth of its numbers, those of its own two halves,
+      // and five for the scaling where the maximum moves.  (Equal weights are all rounded one way: 2^20 of them beside a larger one, in a block, 4.8e-5.)
+      const int serial = (min(per_row, (groups + kVerifyWarps - 1) / kVerifyWarps) + 2) * (kGroup * kN / 4 + 8);
+      const int taken = decide(r, m, s, largest, 1e-5f + fabsf(m * per_unit) * 2.4e-7f + static_cast<float>(serial) * 2.9802322e-8f);
       if (lane == 0) {
         s_next[warp] = taken;
         s_largest[warp] = largest;

@@ -110,3 +110,20 @@ def test_coins_next_to_one_and_a_draft_that_is_the_target(dev, batch):
         start += 4
     tokens, counts, _ = check_ends(x)
     assert (counts < 4).any() and (counts == 4).any()
+
+
+def test_sums_of_long_rows(dev):
+    """2^20 equal weights beside a larger one, whose 32-bit sums are off one way, by up to 4.8e-5: decisions 1e-5 from their border are those of the sum itself."""
+    V, B, n = 1 << 20, 150, 8
+    down = (12 + torch.arange(B // 2, dtype=torch.float64) / 128).repeat(2)  # (fp16 numbers)
+    p = 1 / (1 + (V - 1) * torch.exp(-down))
+    side = torch.tensor([-1.0, 1.0]).repeat_interleave(B // 2)
+    logits = torch.empty(B * n, V, dtype=torch.float16, device=dev)
+    logits.view(B, n, V).copy_(-down.half().to(dev)[:, None, None].expand(B, n, V))
+    logits[:, 5] = 0.0
+    coins = (p * (1 + 1e-5 * side)).float().repeat_interleave(n)
+    x = {"logits": logits, "tokens": torch.full((B * n,), 5, dtype=torch.int64, device=dev), "parents": None, "probs": None, "coins": coins.to(dev),
+         "draws": torch.full((B,), 0.5, device=dev), "new": [n] * B, "heats": None}
+    tokens, rows, counts = call(x)
+    assert counts.tolist() == [n if s < 0 else 1 for s in side.tolist()]
+    assert (tokens[B // 2:, 0] != 5).all()
