@@ -518,7 +518,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
     return sum;
   };
   // A warp's decision on row r with largest number m (or, greedy, largest token) and sum of weights: the child that is taken, 0 for none, -1 where this could err.  In
-  // Real's bits; those of 32 are off by no more than `doubt`.
+  // Real's bits.  With those of 32 the two sides are off by no more than 2 (doubt + 1e-7 times the child's octaves below m) of themselves: a weight's exponent is off by
+  // 3 2^-24 of itself, ln(2) of which it makes of the weight, 1.24e-7 an octave; and by 1e-37 where numbers are next to 32 bits' smallest.
   auto decide = [&](int r, float m, auto sum, int largest, auto doubt) {
     using Real = decltype(sum);
     constexpr bool kFast = sizeof(Real) == 4;
@@ -531,10 +532,14 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
       if (!__any_sync(0xffffffffu, child)) continue;
       bool take = child && s_token[i] == largest, close = false;
       if (!greedy) {
-        Real w = 0;
+        Real w = 0, down = 0;
         if (child && !s_again[i]) {
-          if constexpr (kFast) w = ex2((s_x[i] - m) * per_unit);
-          else w = weigh(s_x[i]);
+          if constexpr (kFast) {
+            down = (s_x[i] - m) * per_unit;
+            w = ex2(down);
+          } else {
+            w = weigh(s_x[i]);
+          }
         }
         Real left = u * sum, right = w;
         if (probs) {
@@ -549,7 +554,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
           mass = __shfl_sync(0xffffffffu, right, 31);
         }
         take = child && w > Real(0) && left < right;
-        close = kFast && child && !(fabs(left - right) > doubt * (left + right));
+        if constexpr (kFast) close = child && !(fabsf(left - right) > (doubt - 1e-7f * fmaxf(down, -150.f)) * (left + right) + 1e-37f);  // (150 octaves: nothing)
       }
       const unsigned first = __ballot_sync(0xffffffffu, take), border = __ballot_sync(0xffffffffu, close);
       if (border && (!first || __ffs(border) <= __ffs(first))) return -1;  // (one behind the first that is taken decides nothing)

@@ -127,3 +127,22 @@ def test_sums_of_long_rows(dev):
     tokens, rows, counts = call(x)
     assert counts.tolist() == [n if s < 0 else 1 for s in side.tolist()]
     assert (tokens[B // 2:, 0] != 5).all()
+
+
+@pytest.mark.parametrize("batch", [2, 200])
+def test_weights_at_the_end_of_32_bits(dev, batch):
+    """Children whose weights and q lie about 2^-126, or below what 32 bits hold: decided by their numbers."""
+    for down in (60.0, 87.0, 87.25, 87.5, 88.0, 90.0, 95.0, 101.0, 103.5, 120.0):
+        for ratio in (0.25, 0.999, 1.001, 4.0):
+            q = torch.tensor(math.exp(-down) * ratio * 2, dtype=torch.float64).float()
+            V, new = 33, [2] * batch
+            logits = torch.full((2 * batch, V), -math.inf, device=dev)
+            logits[:, 3], logits[:, 9] = 0.0, -down
+            probs = torch.zeros(2 * batch, V, device=dev)
+            probs[:, 9], probs[:, 3] = q.to(dev), 1.0
+            x = {"logits": logits, "tokens": torch.full((2 * batch,), 9, dtype=torch.int64, device=dev), "parents": None, "probs": probs, "coins": torch.full((2 * batch,), 0.5, device=dev),
+                 "draws": torch.full((batch,), 0.5, device=dev), "new": new, "heats": None}
+            p, left = math.exp(-down) / (1 + math.exp(-down)), 0.5 * float(q)
+            if abs(left - p) <= 1e-9 * p:  # (q has few bits here: it may have been rounded to the border itself)
+                continue
+            assert call(x)[2].tolist() == [2 if left < p else 1] * batch, (down, ratio)
