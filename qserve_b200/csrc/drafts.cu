@@ -967,8 +967,8 @@ int launch_verify(VerifyParams p, int batch, void* stream) {
   // Blocks of a sequence: as many as find places for all sequences at once.  (Of sixteen, eight and four blocks 7, 15 and 32 clusters do, where 148 / 16 is 9.  Sequences
   // that wait for the first ones' places, and fewer blocks: 8 chains of 5, 128256 tokens, 31.0 us and 21.4; 16 of them 36.5 and 28.9; 36 47.4 and 41.2.)
   static std::atomic<int> held[kMaxDevices][kMostBlocks + 1] = {};
-  p.cluster = kMostBlocks;
-  while (p.cluster > 1 && paged::clusters_at_once(held[device_ordinal()][p.cluster], verify_kernel<T>, kVerifyThreads, kRingBytes, p.cluster) < batch) --p.cluster;
+  auto places = [&](int n) { return paged::clusters_at_once(held[device_ordinal()][n], verify_kernel<T>, kVerifyThreads, kRingBytes, n); };
+  p.cluster = paged::most_blocks_at_once(places, kMostBlocks, batch);
   const long long words = (static_cast<long long>(p.vocab) + 2 * Row<T>::kN - 2) / Row<T>::kN;  // of a row that begins at a word's last number
   auto share = [&](int of) { return static_cast<int>((words + 32ll * of - 1) / (32ll * of) * 32); };  // (a warp takes 32 at a time in any case)
   p.per_block = share(p.cluster);

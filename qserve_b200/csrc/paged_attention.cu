@@ -1935,25 +1935,6 @@ bool rows_few(int batch, int max_seqlen, int max_length, int heads, int kv_heads
   if (times == 1) return !(items <= 10 && pages > 192);
   return max_seqlen <= kMostRowTokens && items <= 2 * num_sms() && items * pages <= (times == 2 ? 2100 : 1200);
 }
-// Blocks of a cluster that share out the keys of a sequence and kv head: rounds of as many clusters as run at once (places(blocks), two blocks on a multiprocessor); 5 us
-// ahead of and behind a warp's half pages, which come one after the other, slower where two blocks share a multiprocessor; a cluster's join.  Of 63 sizes (1 to 64
-// sequences of 500 to 16000 positions, 4 rows, INT4, 32 heads over 8) the choice is within 4.5 % of the best.  (us, of one, two, four, eight, sixteen blocks: one sequence
-// of 500 8.3, 8.2, 7.0, 6.7, 7.6; 10 of 2000 28.9, 20.3, 21.5, 26.6, 45, but of three 16.2; one of 16000 135, 72, 40, 26, 20; 64 of 2000 63, 74, 93, 146.)
-template <typename Places>
-int rows_blocks(Places places, long long items, int max_length) {
-  const int halves = 2 * static_cast<int>((static_cast<long long>(max_length) + kPage - 1) / kPage);
-  int chosen = 1;
-  float best = 3.0e38f;
-  for (int n = 1; n <= kMostRowBlocks && (n == 1 || kTailWarps * (n - 1) < halves); ++n) {
-    const int held = places(n), turns = ((halves + n - 1) / n + kTailWarps - 1) / kTailWarps;
-    const float rounds = fmaxf(1.f, items / static_cast<float>(held)), shared = fminf(1.f, fmaxf(0.f, 2.f * items / held - 1.f));  // multiprocessors with two blocks
-    const float time = 0.5f * (ceilf(rounds) + rounds) * (5.f + (n > 1 ? 0.5f + 0.1f * n : 0.f) + turns * (1.05f + 0.2f * sqrtf(shared)));
-    if (time >= best) continue;
-    best = time;
-    chosen = n;
-  }
-  return chosen;
-}
 template <int BITS>
 int run_rows(RowsParams& p, long long items, int max_length, void* stream) {
   using C = RowsCfg<BITS>;
@@ -1967,7 +1948,9 @@ int run_rows(RowsParams& p, long long items, int max_length, void* stream) {
   }
   const int rc = allow_smem<rows_kernel<BITS>>(C::kSmem, "paged_tree_attention: shared memory", [](int) { return true; });
   if (rc) return rc;
-  p.cluster = rows_blocks([&](int n) { return clusters_at_once(held[dev][n], rows_kernel<BITS>, 32 * kTailWarps, C::kSmem, n); }, items, max_length);
+  auto places = [&](int n) { return clusters_at_once(held[dev][n], rows_kernel<BITS>, 32 * kTailWarps, C::kSmem, n); };
+  const int halves = 2 * static_cast<int>((static_cast<long long>(max_length) + kPage - 1) / kPage);
+  p.cluster = fastest_blocks(places, kMostRowBlocks, kTailWarps, items, halves);
   QS_REQUIRE(items * p.cluster <= 0x7fffffffll, "paged_tree_attention: %lld blocks", items * p.cluster);
   return launch(rows_kernel<BITS>, dim3(static_cast<unsigned>(items * p.cluster)), 32 * kTailWarps, C::kSmem, stream, "paged_tree_attention", p.cluster, p);
 }

@@ -5,6 +5,7 @@
 #pragma once
 #include <atomic>
 
+#include "clusters.h"
 #include "common.cuh"
 #include "launch.h"
 
@@ -88,12 +89,12 @@ int launch(Kern kern, dim3 grid, int threads, size_t smem, void* stream, const c
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
 }
 
-// Clusters of that many blocks that the current device runs at once: fewer than its multiprocessors would hold, for a cluster lies within one group of them.
-// `held` is the caller's, of this kernel, size and device; 0: not asked yet.
+// Clusters of that many blocks that the current device runs at once: fewer than its multiprocessors would hold, for a cluster lies within one group of them; 0: it has no
+// place for any.  `held` is the caller's, of this kernel, size and device: one more than that, 0: not asked yet.
 template <typename Kern>
 int clusters_at_once(std::atomic<int>& held, Kern kern, int threads, size_t smem, int cluster) {
   int n = held.load(std::memory_order_relaxed);
-  if (n > 0) return n;
+  if (n > 0) return n - 1;
   cudaLaunchAttribute size;
   size.id = cudaLaunchAttributeClusterDimension;
   size.val.clusterDim.x = cluster;
@@ -104,11 +105,10 @@ int clusters_at_once(std::atomic<int>& held, Kern kern, int threads, size_t smem
   ask.dynamicSmemBytes = smem;
   ask.attrs = &size;
   ask.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, kern, &ask) != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    n = num_sms() / cluster > 0 ? num_sms() / cluster : 1;
-  }
-  held.store(n, std::memory_order_relaxed);
+  const bool said = cudaOccupancyMaxActiveClusters(&n, kern, &ask) == cudaSuccess;
+  if (!said) cudaGetLastError();
+  n = places_of(said, n, num_sms(), cluster);
+  held.store(n + 1, std::memory_order_relaxed);
   return n;
 }
 
