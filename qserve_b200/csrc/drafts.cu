@@ -920,7 +920,12 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_kernel(const __grid_con
           if (lane == 31) s_share[0][warp] = run;
           __syncthreads();
           const double of_warp = lane < kVerifyWarps ? s_share[0][lane] : 0.0;
-          if (choose(of_warp, run_of(of_warp), ahead) != warp || choose(sum, run, ahead) != lane) break;
+          const int in = choose(of_warp, run_of(of_warp), ahead);
+          if (in < 0) {  // the share was rounding of sum q's 32 bits, none of its numbers is above zero: this block draws by itself
+            draw_exactly<T>(row.p, p.vocab, from_p ? nullptr : q, all, weigh, p.draws[b], s_share[0], s_shares[turn_sum][0], s_shares[turn_sum][1], 1, 0, out_tokens + accepted);
+            break;
+          }
+          if (in != warp || choose(sum, run, ahead) != lane) break;
           chosen = true;
           i = 0;
           if (words > 1) {
