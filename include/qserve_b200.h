@@ -206,7 +206,8 @@ QS_API int qs_paged_tree_attention(const void* q, int64_t q_stride, void* out, i
  * The token drawn is the first whose running sum of weights exceeds draw * their whole sum.  A temperature that is not above 0: the child with the row's largest logit,
  * the lowest index of equal ones.  Logits of -inf or NaN are no tokens; of a row with nothing else the token is -1; where some are +inf, those share the weight alone.
  * out_rows int32, out_tokens int64 [batch, max_seqlen]: rows 0, r1, r2, .. that were taken, and the token behind each; -1 beyond; out_counts int32 [batch]: how many,
- * 0 for an empty portion.  max_seqlen <= 256; rows behind it are not looked at.  Sums are of 64 bits where a decision or a draw hangs on them. */
+ * 0 for an empty portion.  max_seqlen <= 256; rows behind it are not looked at.  Sums are of 64 bits where a decision or a draw hangs on them; in max(p - q, 0) tokens
+ * whose p and q differ by less than a 32-bit sum's error may count with up to that error, no more than 1e-4 of what is drawn from in all. */
 QS_API int qs_verify_drafts(int64_t* out_tokens, int32_t* out_rows, int32_t* out_counts, const void* logits, int logits_type, int64_t logits_stride, const int64_t* tokens,
                             const int32_t* parents, const float* draft_probs, int64_t probs_stride, const int32_t* cu_seqlens, const float* coins, const float* draws,
                             const float* temperatures, int batch, int num_tokens, int vocab, int max_seqlen, void* stream);

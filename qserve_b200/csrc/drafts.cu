@@ -64,10 +64,10 @@ __global__ void __launch_bounds__(kMostDrafted) tree_kernel(int* positions, unsi
 // bits could get wrong is taken again with a sum of 64 bits.  The token that the sequence ends with is drawn with weights and sums of 64 bits: among 10^5 tokens one
 // border or another lies within 32 bits' error of one draw in a hundred.  For that the last row is read once more, out of L2.
 //
-// 64 chains of up to 6 rows with the draft's probabilities, 128256 tokens, fp16, two blocks a chain: 46.5 us, of which maxima and sums take 19 (77 MB, 4.1 TB/s of 128
-// multiprocessors' copies), the second reading of a row and its probabilities 15 (48 MB; issue slots and the 64-bit pipe: 46 cycles of it for a warp's 32 numbers), the
-// exchanges, decisions and the search for the drawn token 9, start and end 4.  Few sequences wait for one another's blocks instead: one chain of 5, 32000 tokens, 14.6,
-// a quarter of it for instructions.  Blocks of 8 warps, two on a multiprocessor, 51.7.
+// 64 chains of up to 6 rows with the draft's probabilities, 128256 tokens, fp16, two blocks a chain: 45.2 us, of which maxima and sums take 19 (77 MB, 4.1 TB/s of 128
+// multiprocessors' copies), the second reading of a row and its probabilities 14 (48 MB; 46 cycles of the 64-bit pipe for a warp's 32 numbers), exchanges and decisions 4,
+// the search for the drawn token 3.5, start and end 4; over all of it issue slots are at 0.47, the 64-bit pipe at 0.14.  Few sequences wait for one another's blocks
+// instead: one chain of 5, 32000 tokens, 13.3, a quarter of it for instructions.  Blocks of 8 warps, two on a multiprocessor, 51.7 (of 46.5 then).
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16;
 constexpr int kMostWindow = 8;
@@ -970,7 +970,8 @@ int launch_verify(VerifyParams p, int batch, void* stream) {
     d.store(true, std::memory_order_relaxed);
   }
   // Blocks of a sequence: as many as find places for all sequences at once.  (Of sixteen, eight and four blocks 7, 15 and 32 clusters do, where 148 / 16 is 9.  Sequences
-  // that wait for the first ones' places, and fewer blocks: 8 chains of 5, 128256 tokens, 31.0 us and 21.4; 16 of them 36.5 and 28.9; 36 47.4 and 41.2.)
+  // that wait for the first ones' places, and fewer blocks, of powers of two: 8 chains of 5, 128256 tokens, 31.0 us and 21.4; 16 of them 36.5 and 28.9; 36 47.4 and 41.2.
+  // Of any number, without probabilities: 19.2, 22.5 and 31.2.)
   static std::atomic<int> held[kMaxDevices][kMostBlocks + 1] = {};
   auto places = [&](int n) { return paged::clusters_at_once(held[device_ordinal()][n], verify_kernel<T>, kVerifyThreads, kRingBytes, n); };
   p.cluster = paged::most_blocks_at_once(places, kMostBlocks, batch);

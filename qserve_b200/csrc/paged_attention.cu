@@ -1922,11 +1922,11 @@ Plan plan_shared(int batch, int shared_blocks, int heads, int kv_heads) {
   return plan_tiles(rows, 1, rows, kv_heads, shared_blocks, false);
 }
 
-
 // Portions of up to 16 rows are the row kernel's, but for few long sequences, which the tile kernel cuts into more parts than a cluster has blocks.  (INT4, 4 rows of 4
 // heads, us, tile and row kernel, of one sequence and kv head behind 8000 positions 10.0 and 9.2, behind 60000 16 and 38; of eight in all 12.8 and 12.4, 40 and 52; of
 // twelve 15.4 and 12.4, 60 and 54; of 32 25 and 19, 146 and 99.)
-// Those of more, whose pages it reads once for every 16, in small calls: by their half pages in all.  (32 heads over 8, INT4: 13 rows of one sequence behind 100 6.3 and
+// Those of more, whose pages it reads once for every 16, in small calls: by the pages of all its blocks, up to where it takes a twentieth longer than the tile kernel, for
+// its results are off by half as much.  (32 heads over 8, INT4: 13 rows of one sequence behind 100 6.3 and
 // 4.9, behind 500 8.5 and 7.4, of four 10.2 and 10.7, of eight 12.1 and 12.3, of 16 13.3 and 23; 5 rows, which is twice 16, of eight behind 500 9.8 and 9.6, behind 2000
 // 20.1 and 19.7, behind 4000 28 and 32; 26 of 16 behind 100, more blocks than places, 7.2 and 18.)
 bool rows_few(int batch, int max_seqlen, int max_length, int heads, int kv_heads) {
