@@ -431,6 +431,7 @@ def verify_drafts(logits, draft_tokens, cu_seqlens: Optional[torch.Tensor], max_
     probabilities p exceeds the row's coin is taken, otherwise the sequence ends with a token drawn from the others.  Chains drawn at random from draft_probs fp32
     [T, vocab] (row i: what row i + 1's token was drawn from): a token x is taken where coin q(x) < p(x), otherwise the sequence ends with one drawn from max(p - q, 0).
     Returns tokens int64 [B, max_seqlen], rows int32 [B, max_seqlen] and counts int32 [B]: the rows taken, from row 0 on, the token behind each, and how many; -1 beyond.
+    A row's child that is no token (outside the vocabulary) counts as one that was refused, so a chain that ends early ends its portion, or has zeros for q there.
     Logits of -inf or NaN are no tokens; a row with nothing else gives -1.  max_seqlen <= 256.  Decisions and draws are those of 64-bit sums, but for max(p - q, 0): tokens
     whose p and q differ by less than a 32-bit sum's error may count with up to that error, no more than 1e-4 of what is drawn from in all."""
     return _bind.verify_drafts(logits, draft_tokens, cu_seqlens, max_seqlen, coins, draws, parents, draft_probs, temperatures)

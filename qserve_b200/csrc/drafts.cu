@@ -322,34 +322,35 @@ __device__ __forceinline__ void meet_of(int cluster) {
   }
 }
 
-// A token drawn from max(e - S q, 0), number by number, S = `all` the row's sum of 64 bits; where that leaves nothing, from the weights e.  The row's words are shared
-// out over the cluster's threads, a run each, gone through for its sum and, the one that the threshold falls into, again.  `of_warps`, `of_blocks`: places for sums, the
-// blocks' twice.  (A function of its own, with nothing to come back to but the end: the pass above once more, in a loop or called again, held registers that made 64 chains
-// of 6, 128256 tokens, 1 to 3 us longer where none needs it.)
+// A token drawn from max(e - S q, 0), number by number, S = `all` the row's sum of 64 bits; where that leaves nothing, from the weights e.  A run of the row for each of
+// the cluster's warps; the one that the threshold falls into shared out over its block's lanes.  `of_warps`, `of_blocks`: places for sums, the blocks' twice.  (A function
+// of its own, with nothing to come back to but the end: the pass above once more, in a loop or called again, held registers that made 64 chains of 6, 128256 tokens, 1 to
+// 3 us longer where none needs it.  Where all do, 64 rows of 128256 tokens and their q take 64 us, 32 without it; one row of 32000 15, 12.4 without.  A run of the row for
+// each thread of the cluster, in place of the two steps: 123 us, for loads that lie apart.)
 template <typename T>
 __device__ __noinline__ void draw_exactly(const T* p, int vocab, const float* q, double all, Weigh weigh, float draw, double* of_warps, double* of_blocks0, double* of_blocks1, int cluster, int rank,
                                           long long* out) {
   constexpr int kN = Row<T>::kN;
   const Row<T> row(p, vocab);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, me = rank * kVerifyThreads + threadIdx.x, threads = cluster * kVerifyThreads;
-  const int c0 = static_cast<int>(static_cast<long long>(row.words) * me / threads), c1 = static_cast<int>(static_cast<long long>(row.words) * (me + 1) / threads);
-  // the run's sum; or its first number with which the sum from `ahead` on is past the threshold, the last with any weight if none is
-  auto go_through = [&](bool search, double ahead, double threshold, int& found) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // the sum over words c0, c0 + step, .. ahead of c1; or the first number with which the sum from `ahead` on is past the threshold, the last with any weight if none is
+  auto go_through = [&](int c0, int c1, int step, bool search, double ahead, double threshold, int& found) {
     double sum = 0.0;
 #pragma unroll 1
-    for (int c = c0; c < c1; ++c) {
-      float x[kN];
+    for (int c = c0; c < c1; c += step) {
+      float x[kN], qs[kN];
+      const int first = row.first(c);
+#pragma unroll
+      for (int k = 0; k < kN; ++k) qs[k] = q && static_cast<unsigned>(first + k) < static_cast<unsigned>(vocab) ? __ldcg(q + first + k) : 0.f;
       numbers_of<T>(row.word(c), x);
 #pragma unroll
       for (int k = 0; k < kN; ++k) {
-        const int token = row.first(c) + k;
         double w = weigh(x[k]);
+        if (q) w = w > 0.0 ? fma(-all, static_cast<double>(qs[k]), w) : 0.0;
         if (!(w > 0.0)) continue;  // (what lies outside the row among them)
-        if (q) w = fma(-all, static_cast<double>(__ldcg(q + token)), w);
-        if (!(w > 0.0)) continue;
         sum += w;
         if (!search) continue;
-        found = token;
+        found = first + k;
         if (ahead + sum > threshold) return sum;
       }
     }
@@ -363,13 +364,16 @@ __device__ __noinline__ void draw_exactly(const T* p, int vocab, const float* q,
     }
     return x;
   };
+  const int per_warp = (row.words + kVerifyWarps * cluster - 1) / (kVerifyWarps * cluster);
+  auto begin_of = [&](int w) { return static_cast<int>(min(static_cast<long long>(row.words), static_cast<long long>(per_warp) * w)); };
   int found = -1;
 #pragma unroll 1
   for (int pass = 0; pass < 2; ++pass) {
-    const double of_mine = go_through(false, 0.0, 0.0, found), run = run_of(of_mine);
+    const int mine = rank * kVerifyWarps + warp;
+    const double of_mine = run_of(go_through(begin_of(mine) + lane, begin_of(mine + 1), 32, false, 0.0, 0.0, found));
     double* const of_blocks = pass == 0 ? of_blocks0 : of_blocks1;
     __syncthreads();  // what lay in the places has been read
-    if (lane == 31) of_warps[warp] = run;
+    if (lane == 31) of_warps[warp] = of_mine;
     __syncthreads();
     const double of_warp = lane < kVerifyWarps ? of_warps[lane] : 0.0, run_warps = run_of(of_warp);
     if (warp == 0) {
@@ -385,14 +389,22 @@ __device__ __noinline__ void draw_exactly(const T* p, int vocab, const float* q,
     }
     const double threshold = static_cast<double>(draw) * whole;
     double ahead = 0.0;
-    auto choose = [&](double mine, double run_to) {
-      const unsigned any = __ballot_sync(0xffffffffu, mine > 0.0), past = __ballot_sync(0xffffffffu, mine > 0.0 && ahead + run_to > threshold);
+    auto choose = [&](double share, double run) {
+      const unsigned any = __ballot_sync(0xffffffffu, share > 0.0), past = __ballot_sync(0xffffffffu, share > 0.0 && ahead + run > threshold);
       const int chosen = past ? __ffs(past) - 1 : 31 - __clz(any);
-      ahead += __shfl_sync(0xffffffffu, run_to - mine, chosen & 31);
+      ahead += __shfl_sync(0xffffffffu, run - share, chosen & 31);
       return chosen;
     };
-    if (choose(of_block, run_blocks) == rank && choose(of_warp, run_warps) == warp && choose(of_mine, run) == lane) {
-      go_through(true, ahead, threshold, found);
+    if (choose(of_block, run_blocks) != rank) return;  // the whole block
+    const int in = rank * kVerifyWarps + choose(of_warp, run_warps), w0 = begin_of(in), len = begin_of(in + 1) - w0;
+    const int c0 = w0 + static_cast<int>(static_cast<long long>(len) * threadIdx.x / kVerifyThreads), c1 = w0 + static_cast<int>(static_cast<long long>(len) * (threadIdx.x + 1) / kVerifyThreads);
+    const double of_lane = go_through(c0, c1, 1, false, 0.0, 0.0, found), run_lanes = run_of(of_lane);
+    __syncthreads();  // of_warps has been read
+    if (lane == 31) of_warps[warp] = run_lanes;
+    __syncthreads();
+    const double of_run = lane < kVerifyWarps ? of_warps[lane] : 0.0;
+    if (choose(of_run, run_of(of_run)) == warp && choose(of_lane, run_lanes) == lane) {
+      go_through(c0, c1, 1, true, ahead, threshold, found);
       *out = found;
     }
     return;
