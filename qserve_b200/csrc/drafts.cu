@@ -64,10 +64,10 @@ __global__ void __launch_bounds__(kMostDrafted) tree_kernel(int* positions, unsi
 // bits could get wrong is taken again with a sum of 64 bits.  The token that the sequence ends with is drawn with weights and sums of 64 bits: among 10^5 tokens one
 // border or another lies within 32 bits' error of one draw in a hundred.  For that the last row is read once more, out of L2.
 //
-// 64 chains of up to 6 rows with the draft's probabilities, 128256 tokens, fp16, two blocks a chain: 45.2 us, of which maxima and sums take 19 (77 MB, 4.1 TB/s of 128
+// 64 chains of up to 6 rows with the draft's probabilities, 128256 tokens, fp16, two blocks a chain: 45.5 us, of which maxima and sums take 19 (77 MB, 4.1 TB/s of 128
 // multiprocessors' copies), the second reading of a row and its probabilities 14 (48 MB; 46 cycles of the 64-bit pipe for a warp's 32 numbers), exchanges and decisions 4,
 // the search for the drawn token 3.5, start and end 4; over all of it issue slots are at 0.47, the 64-bit pipe at 0.14.  Few sequences wait for one another's blocks
-// instead: one chain of 5, 32000 tokens, 13.3, a quarter of it for instructions.  Blocks of 8 warps, two on a multiprocessor, 51.7 (of 46.5 then).
+// instead: one chain of 5, 32000 tokens, 13.4, a quarter of it for instructions.  Blocks of 8 warps, two on a multiprocessor, 51.7 (of 46.5 then).
 // ------------------------------------------------------------------------------------------------------------------------
 constexpr int kVerifyWarps = 16, kVerifyThreads = 32 * kVerifyWarps, kMostBlocks = 16;
 constexpr int kMostWindow = 8;
